@@ -168,7 +168,18 @@ int rbln_paged_prefill_workspace_size(const rbln_paged_attn_params_t* p, size_t*
  * (p->causal = 1) or t < seq[b] + S_q (p->causal = 0, "is_bidirectional");
  * p->mask, when set, is an extra [B, L] keep-mask over keys.
  * bf16/f16 only, q and caches of one dtype, D in {64, 128}, block_size in
- * {8, 16, 32, 64, 128} or a multiple of 128. No workspace. */
+ * {8, 16, 32, 64, 128} or a multiple of 128. No workspace.
+ *
+ * kv_dtype FP8_E4M3 (q bf16 or f16, k_scale / v_scale required, D and
+ * block_size as above, any S_q from one token up): the new rows are written by
+ * the rule of rbln_paged_kv_write, which finds the scales of the touched
+ * blocks anew (a sequence whose rows would pass the table's span is not
+ * written), and attention reads them back with the rest. k_new / v_new NULL:
+ * the rows [seq[b], seq[b] + S_q) are in the cache already
+ * (rbln_rotary_paged_kv_write). A key in a block outside the pool, at or past
+ * the span, or not kept by the mask is not seen, whatever its bytes hold; a
+ * query that sees no key gives NaN. sinks are not supported. The workspace
+ * (rbln_paged_prefill_workspace_size) is required. */
 int rbln_paged_causal_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stream);
 
 /* rbln_custom_ops::paged_attn_prefill
@@ -192,6 +203,58 @@ int rbln_paged_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stre
  * as they are.
  * No reference counterpart as a separate entry point. */
 int rbln_paged_kv_write(const rbln_paged_attn_params_t* p, cudaStream_t stream);
+
+/* Rotary positions. Pair i of a row at position p turns by the angle
+ * p * inv_freq[i] (the exact product, whatever the position):
+ *   y1 = mscale (x1 cos - x2 sin),  y2 = mscale (x2 cos + x1 sin),
+ * (x1, x2) = (x[i], x[i + rotary_dim / 2]), or (x[2 i], x[2 i + 1]) when
+ * interleaved; dimensions from rotary_dim on are copied. inverse: sin negated,
+ * the transposed map, which takes the gradient of y to that of x.
+ * No reference counterpart as a separate entry point. */
+typedef struct {
+  int32_t batch, q_heads, k_heads, seq_len, head_dim; /* either head count may be 0; head_dim <= 1024 */
+  int32_t rotary_dim;       /* even, <= head_dim */
+  int32_t dtype;            /* F32, F16 or BF16, shared by q, k and the outputs */
+  const void* q;            /* [B, Hq, S, D]; strides in elements: b, h, s (d contiguous) */
+  int64_t q_stride[3];
+  void* q_out;              /* may be q itself, with the same strides */
+  int64_t q_out_stride[3];
+  const void* k;            /* [B, Hk, S, D] */
+  int64_t k_stride[3];
+  void* k_out;
+  int64_t k_out_stride[3];
+  const void* positions;    /* [B, S], I32 or I64; strides b, s in elements (0 broadcasts) */
+  int32_t positions_dtype;
+  int64_t positions_stride[2];
+  const float* inv_freq;    /* [rotary_dim / 2] */
+  int32_t interleaved;
+  int32_t inverse;
+  float mscale;
+} rbln_rotary_params_t;
+
+size_t rbln_rotary_params_sizeof(void);
+int rbln_rotary(const rbln_rotary_params_t* p, cudaStream_t stream);
+
+/* rbln_rotary on q and k_new at positions seq[b] + s, the rotated q to p->out
+ * and the rotated keys and the values to the paged cache as
+ * rbln_paged_kv_write puts them there, in one launch. Of r, rotary_dim,
+ * inv_freq, interleaved and mscale are read. q / out strides as for the paged
+ * ops; D in {64, 128}, rotary_dim a multiple of 16. An fp8 cache is quantised
+ * from the float32 rotated keys. q is rotated for every sequence; rows are
+ * written where rbln_paged_kv_write would write them. */
+int rbln_rotary_paged_kv_write(const rbln_paged_attn_params_t* p, const rbln_rotary_params_t* r,
+                               cudaStream_t stream);
+
+/* Reads the paged cache back: rows [0, seq[b]) (seq: lengths here, cut to
+ * [0, span], RBLN_DEVERR_SEQ_RANGE raised outside it) of every sequence to
+ * dense k_out / v_out [B, Hkv, q_len, D] (out_stride: b, h, t in elements,
+ * both outputs alike), an fp8 cache's codes times their scale in float32,
+ * rounded once to q_dtype (BF16, F16 or F32). Rows from the length on, and of
+ * blocks outside the pool, are zeros; rows past q_len are not read. Of p:
+ * shapes (q_len = rows returned a sequence), q_dtype, caches, scales, seq,
+ * block table and error_flags. D in {64, 128}. */
+int rbln_paged_kv_read(const rbln_paged_attn_params_t* p, void* k_out, void* v_out, const int64_t* out_stride,
+                       cudaStream_t stream);
 
 /* Dense scaled dot-product attention, forward. */
 typedef struct {

@@ -41,6 +41,11 @@
 #include "tma_map.cuh"
 
 namespace rbln {
+
+// fp8 caches (paged_attn_fp8.cu)
+size_t fp8_prefill_ws_bytes(const rbln_paged_attn_params_t* p);
+int run_prefill_fp8(const rbln_paged_attn_params_t* p, cudaStream_t st);
+
 namespace {
 
 using namespace sm100;
@@ -2137,11 +2142,12 @@ extern "C" {
 
 int rbln_paged_prefill_workspace_size(const rbln_paged_attn_params_t* p, size_t* bytes) {
   if (!p || !bytes) return RBLN_ERR_INVALID_ARGUMENT;
-  *bytes = (size_t)rbln::prefill_ws_bytes(p);
+  *bytes = p->kv_dtype == RBLN_DT_FP8_E4M3 ? rbln::fp8_prefill_ws_bytes(p) : (size_t)rbln::prefill_ws_bytes(p);
   return RBLN_OK;
 }
 
 int rbln_paged_causal_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stream) {
+  if (p && p->kv_dtype == RBLN_DT_FP8_E4M3) return rbln::run_prefill_fp8(p, stream);
   return rbln::run_prefill(p, stream, /*keep_mask_op=*/false);
 }
 

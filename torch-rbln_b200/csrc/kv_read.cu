@@ -1,0 +1,194 @@
+// Paged KV-cache read-back (rbln_paged_kv_read): rows [0, len[b]) of every
+// sequence gathered through the block table into dense k / v
+// [B, Hkv, T, D], an fp8 cache's rows times their block's scale, zeros past
+// the length.
+//
+// Bound by HBM: 1 or 2 bytes an element in, 2 or 4 out. A thread moves eight
+// elements of a row at a time, so that a warp's stores are whole lines; a CTA
+// takes 4 x 256 such pieces of one (sequence, head) and both caches, whose
+// eight loads a thread are issued before any is used, behind the one
+// dependent look-up of the block table.
+
+#include "common.cuh"
+
+namespace rbln {
+namespace {
+
+constexpr int kReadThreads = 256;
+constexpr int kReadSteps = 4;  // pieces a thread, of each cache
+
+struct ReadArgs {
+  const char* kcache;
+  const char* vcache;
+  int64_t cs_block, cs_head, cs_tok;  // elements
+  const float* k_scale;
+  const float* v_scale;
+  int64_t ss_block, ss_head;
+  const int32_t* len;
+  int64_t len_stride;
+  const void* bt;
+  int bt_dtype;
+  int64_t bt_stride;
+  char* k_out;
+  char* v_out;
+  int64_t os_b, os_h, os_t;  // elements
+  int B, Hkv, T, D, bs, max_blocks, num_blocks, ctas_per_head;
+  uint32_t* err;
+};
+
+enum { R_BF16 = 0, R_F16 = 1, R_FP8 = 2, R_F32 = 3 };
+
+// Eight cache elements as floats, times `s` for fp8.
+template <int KV>
+__device__ __forceinline__ void widen8(uint4 w, float s, float (&x)[8]) {
+  if constexpr (KV == R_FP8) {
+    uint32_t h[4];
+    e4m3x4_to_f16x2x2(w.x, h[0], h[1]);
+    e4m3x4_to_f16x2x2(w.y, h[2], h[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<false>(h[i]);
+      x[2 * i] = f.x * s;
+      x[2 * i + 1] = f.y * s;
+    }
+  } else {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<KV == R_BF16>(u[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+template <int OUT>
+__device__ __forceinline__ void store8(char* p, const float (&x)[8]) {
+  if constexpr (OUT == R_F32) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    constexpr bool BF = OUT == R_BF16;
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]), pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7]));
+  }
+}
+
+template <int KV, int OUT>
+__global__ void __launch_bounds__(kReadThreads) paged_kv_read_kernel(const ReadArgs a) {
+  constexpr int SZ = KV == R_FP8 ? 1 : 2, OSZ = OUT == R_F32 ? 4 : 2;
+  const int64_t unit = blockIdx.x / a.ctas_per_head;
+  const int part = (int)(blockIdx.x - unit * a.ctas_per_head);
+  const int b = (int)(unit / a.Hkv), h = (int)(unit - (int64_t)b * a.Hkv);
+  const int64_t span = (int64_t)a.max_blocks * a.bs;
+  int len = a.len[b * a.len_stride];
+  if (len < 0 || len > span) {
+    if (a.err && threadIdx.x == 0) atomicOr(a.err, RBLN_DEVERR_SEQ_RANGE);
+    len = len < 0 ? 0 : (int)span;
+  }
+  const int cpr = a.D / 8;
+  uint4 kw[kReadSteps], vw[kReadSteps];
+  float ks[kReadSteps], vs[kReadSteps];
+#pragma unroll
+  for (int u = 0; u < kReadSteps; ++u) {
+    const int64_t i = ((int64_t)part * kReadSteps + u) * kReadThreads + threadIdx.x;
+    const int64_t t = i / cpr;
+    const int c = (int)(i - t * cpr);
+    kw[u] = vw[u] = make_uint4(0, 0, 0, 0);
+    ks[u] = vs[u] = 0.f;
+    if (t >= a.T || t >= len) continue;
+    const int64_t blk = load_index(a.bt, a.bt_dtype, b * a.bt_stride + t / a.bs);
+    if (blk < 0 || blk >= a.num_blocks) {
+      if (a.err) atomicOr(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
+      continue;
+    }
+    const int64_t at = (blk * a.cs_block + h * a.cs_head + (t % a.bs) * a.cs_tok + c * 8) * SZ;
+    if constexpr (KV == R_FP8) {
+      const uint2 x = ld_stream_v2(a.kcache + at), y = ld_stream_v2(a.vcache + at);
+      kw[u] = make_uint4(x.x, x.y, 0, 0);
+      vw[u] = make_uint4(y.x, y.y, 0, 0);
+      ks[u] = a.k_scale[blk * a.ss_block + h * a.ss_head];
+      vs[u] = a.v_scale[blk * a.ss_block + h * a.ss_head];
+    } else {
+      kw[u] = ld_stream_v4(a.kcache + at);
+      vw[u] = ld_stream_v4(a.vcache + at);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kReadSteps; ++u) {
+    const int64_t i = ((int64_t)part * kReadSteps + u) * kReadThreads + threadIdx.x;
+    const int64_t t = i / cpr;
+    const int c = (int)(i - t * cpr);
+    if (t >= a.T) continue;
+    const int64_t to = (b * a.os_b + h * a.os_h + t * a.os_t + c * 8) * OSZ;
+    if constexpr (KV == OUT) {
+      *reinterpret_cast<uint4*>(a.k_out + to) = kw[u];
+      *reinterpret_cast<uint4*>(a.v_out + to) = vw[u];
+    } else {
+      float x[8];
+      widen8<KV>(kw[u], ks[u], x);
+      store8<OUT>(a.k_out + to, x);
+      widen8<KV>(vw[u], vs[u], x);
+      store8<OUT>(a.v_out + to, x);
+    }
+  }
+}
+
+template <int KV>
+int launch_read(const ReadArgs& a, int out, unsigned grid, cudaStream_t st) {
+  if (out == RBLN_DT_BF16) paged_kv_read_kernel<KV, R_BF16><<<grid, kReadThreads, 0, st>>>(a);
+  else if (out == RBLN_DT_F16) paged_kv_read_kernel<KV, R_F16><<<grid, kReadThreads, 0, st>>>(a);
+  else paged_kv_read_kernel<KV, R_F32><<<grid, kReadThreads, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace rbln
+
+extern "C" int rbln_paged_kv_read(const rbln_paged_attn_params_t* p, void* k_out, void* v_out,
+                                  const int64_t* out_stride, cudaStream_t stream) {
+  using namespace rbln;
+  if (!p || !out_stride || p->batch < 0 || p->num_kv_heads <= 0 || p->q_len < 0 || p->block_size <= 0 ||
+      p->max_blocks <= 0 || p->num_blocks <= 0)
+    return RBLN_ERR_INVALID_ARGUMENT;
+  if (p->batch == 0 || p->q_len == 0) return RBLN_OK;
+  if (p->head_dim != 64 && p->head_dim != 128) return RBLN_ERR_UNSUPPORTED;
+  if (p->q_dtype != RBLN_DT_BF16 && p->q_dtype != RBLN_DT_F16 && p->q_dtype != RBLN_DT_F32)
+    return RBLN_ERR_UNSUPPORTED;
+  const bool fp8 = p->kv_dtype == RBLN_DT_FP8_E4M3;
+  if (!fp8 && p->kv_dtype != RBLN_DT_BF16 && p->kv_dtype != RBLN_DT_F16) return RBLN_ERR_UNSUPPORTED;
+  if (p->block_table_dtype != RBLN_DT_I16 && p->block_table_dtype != RBLN_DT_I32 &&
+      p->block_table_dtype != RBLN_DT_I64)
+    return RBLN_ERR_UNSUPPORTED;
+  if ((int64_t)p->max_blocks * p->block_size > (1 << 30)) return RBLN_ERR_UNSUPPORTED;
+  if (!k_out || !v_out || !p->kcache || !p->vcache || !p->seq || !p->block_table || (fp8 && (!p->k_scale || !p->v_scale)))
+    return RBLN_ERR_INVALID_ARGUMENT;
+  {  // 8 elements at a time: 8 or 16 bytes in, 16 out
+    auto al = [](const void* q, unsigned m) { return (reinterpret_cast<uintptr_t>(q) & m) == 0; };
+    const unsigned cm = fp8 ? 7u : 15u;
+    if (!al(k_out, 15u) || !al(v_out, 15u) || !al(p->kcache, cm) || !al(p->vcache, cm)) return RBLN_ERR_INVALID_ARGUMENT;
+    for (int i = 0; i < 3; ++i)
+      if (out_stride[i] % 8 || p->cache_stride[i] % 8) return RBLN_ERR_INVALID_ARGUMENT;
+  }
+  ReadArgs a{};
+  a.kcache = static_cast<const char*>(p->kcache);
+  a.vcache = static_cast<const char*>(p->vcache);
+  a.cs_block = p->cache_stride[0]; a.cs_head = p->cache_stride[1]; a.cs_tok = p->cache_stride[2];
+  a.k_scale = p->k_scale; a.v_scale = p->v_scale;
+  a.ss_block = p->scale_stride[0]; a.ss_head = p->scale_stride[1];
+  a.len = p->seq; a.len_stride = p->seq_stride;
+  a.bt = p->block_table; a.bt_dtype = p->block_table_dtype; a.bt_stride = p->block_table_stride;
+  a.k_out = static_cast<char*>(k_out); a.v_out = static_cast<char*>(v_out);
+  a.os_b = out_stride[0]; a.os_h = out_stride[1]; a.os_t = out_stride[2];
+  a.B = p->batch; a.Hkv = p->num_kv_heads; a.T = p->q_len; a.D = p->head_dim; a.bs = p->block_size;
+  a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
+  a.err = p->error_flags;
+  const int64_t pieces = (int64_t)a.T * (a.D / 8);
+  const int64_t per = (pieces + kReadThreads * kReadSteps - 1) / (kReadThreads * kReadSteps);
+  const int64_t grid = per * a.B * a.Hkv;
+  if (grid > INT32_MAX) return RBLN_ERR_UNSUPPORTED;
+  a.ctas_per_head = (int)per;
+  if (fp8) return launch_read<R_FP8>(a, p->q_dtype, (unsigned)grid, stream);
+  return p->kv_dtype == RBLN_DT_BF16 ? launch_read<R_BF16>(a, p->q_dtype, (unsigned)grid, stream)
+                                     : launch_read<R_F16>(a, p->q_dtype, (unsigned)grid, stream);
+}

@@ -16,6 +16,9 @@
 #include <ATen/ops/_fused_sdp_choice_native.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -183,6 +186,16 @@ void fill_paged(Common& c, const char* op, const at::Tensor& q_in, const at::Ten
   }
 }
 
+// The scales of an fp8 cache: float32 [num_blocks, Hkv], alike, beside it.
+void check_scales(const char* op, const at::Tensor& kcache, const at::Tensor& k_scale, const at::Tensor& v_scale) {
+  TORCH_CHECK(k_scale.scalar_type() == at::kFloat && v_scale.scalar_type() == at::kFloat && k_scale.dim() == 2 &&
+                  k_scale.size(0) == kcache.size(0) && k_scale.size(1) == kcache.size(1) &&
+                  v_scale.sizes() == k_scale.sizes() && v_scale.strides() == k_scale.strides(),
+              op, ": k_scale/v_scale must be float32 [num_blocks, Hkv], alike");
+  TORCH_CHECK(k_scale.device() == kcache.device() && v_scale.device() == kcache.device(), op,
+              ": scales must be on the caches' device");
+}
+
 void check_rc(int rc, const char* op) {
   TORCH_CHECK(rc == RBLN_OK, op, ": ", status_name(rc), " (status ", rc, ")");
 }
@@ -304,6 +317,277 @@ at::Tensor paged_causal_attn_prefill_cuda(const at::Tensor& q, const at::Tensor&
   fill_paged(c, op, q, k, v, kcache, vcache, seq, scale, block_table, block_size, mask, false);
   c.p.causal = is_bidirectional ? 0 : 1;
   return run_prefill(c, op, false);
+}
+
+// rbln_custom_ops::paged_causal_attn_prefill_kvfp8: paged_causal_attn_prefill
+// over an fp8-e4m3 cache with one fp32 dequant scale per (block, KV head). No
+// counterpart in the reference's op set; k and v absent: their rows are in the
+// cache already (rotary_paged_kv_write).
+at::Tensor paged_causal_attn_prefill_kvfp8_cuda(const at::Tensor& q, const std::optional<at::Tensor>& k,
+                                                const std::optional<at::Tensor>& v, at::Tensor& kcache,
+                                                at::Tensor& vcache, at::Tensor& k_scale, at::Tensor& v_scale,
+                                                const at::Tensor& seq, const at::Tensor& scale,
+                                                const at::Tensor& block_table, int64_t block_size,
+                                                bool is_bidirectional, const std::optional<at::Tensor>& mask) {
+  const char* op = "paged_causal_attn_prefill_kvfp8";
+  TORCH_CHECK(kcache.scalar_type() == at::kFloat8_e4m3fn, op, ": caches must be float8_e4m3fn");
+  const bool rows = k.has_value() && k->defined();
+  TORCH_CHECK(rows == (v.has_value() && v->defined()), op, ": k and v go together");
+  TORCH_CHECK(q.dim() == 5, op, ": q must be 5-D [B, Hkv, G, S, D]");
+  check_scales(op, kcache, k_scale, v_scale);
+  Common c;
+  // without k and v, q's first query heads stand in for their checks
+  const at::Tensor qk = rows ? at::Tensor() : q.slice(2, 0, 1);
+  fill_paged(c, op, q, rows ? *k : qk, rows ? *v : qk, kcache, vcache, seq, scale, block_table, block_size, mask,
+             false);
+  if (c.mask.defined())
+    TORCH_CHECK(c.mask.dim() == 2 && (c.mask.size(0) == 1 || c.mask.size(0) == q.size(0)), op,
+                ": mask must be a position mask [B, L], got ", c.mask.sizes());
+  if (!rows) c.p.k_new = c.p.v_new = nullptr;
+  c.p.k_scale = k_scale.data_ptr<float>();
+  c.p.v_scale = v_scale.data_ptr<float>();
+  c.p.scale_stride[0] = k_scale.stride(0);
+  c.p.scale_stride[1] = k_scale.stride(1);
+  c.p.causal = is_bidirectional ? 0 : 1;
+  return run_prefill(c, op, false);
+}
+
+// ---------------------------------------------------------------------------
+// Rotary positions (rotary.cu)
+// ---------------------------------------------------------------------------
+bool is_float16or32(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf || t == at::kFloat; }
+
+at::Tensor check_inv_freq(const char* op, const at::Tensor& inv_freq, const at::Tensor& like) {
+  TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.scalar_type() == at::kFloat && inv_freq.numel() > 0, op,
+              ": inv_freq must be float32 [rotary_dim / 2], got ", inv_freq.sizes(), " of ", inv_freq.scalar_type());
+  TORCH_CHECK(2 * inv_freq.numel() <= like.size(-1), op, ": rotary_dim ", 2 * inv_freq.numel(),
+              " exceeds the head dimension ", like.size(-1));
+  return on_device(inv_freq, like).contiguous();
+}
+
+// rbln_attn::rotary: q [B, Hq, S, D] and k [B, Hk, S, D] turned by their
+// positions [B, S] (or [S]); the outputs keep the inputs' layout.
+std::tuple<at::Tensor, at::Tensor> rotary_cuda(const at::Tensor& q_in, const at::Tensor& k_in,
+                                               const at::Tensor& positions, const at::Tensor& inv_freq_in,
+                                               bool interleaved, double mscale, bool inverse) {
+  const char* op = "rotary";
+  TORCH_CHECK(q_in.is_cuda() && k_in.device() == q_in.device(), op, ": q and k must be on one CUDA device");
+  TORCH_CHECK(q_in.dim() == 4 && k_in.dim() == 4 && k_in.size(0) == q_in.size(0) && k_in.size(2) == q_in.size(2) &&
+                  k_in.size(3) == q_in.size(3),
+              op, ": q and k must be [B, H, S, D] alike but for H, got ", q_in.sizes(), " and ", k_in.sizes());
+  const auto dt = q_in.scalar_type();
+  TORCH_CHECK(is_float16or32(dt) && k_in.scalar_type() == dt, op,
+              ": q and k must share one of bfloat16, float16 and float32, got ", dt, " and ", k_in.scalar_type());
+  const int64_t B = q_in.size(0), S = q_in.size(2), D = q_in.size(3);
+  at::Tensor inv_freq = check_inv_freq(op, inv_freq_in, q_in);
+  at::Tensor pos = on_device(positions, q_in);
+  TORCH_CHECK(pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong, op,
+              ": positions must be int32 or int64, got ", pos.scalar_type());
+  if (pos.dim() == 1) pos = pos.unsqueeze(0);
+  TORCH_CHECK(pos.dim() == 2 && (pos.size(0) == B || pos.size(0) == 1) && pos.size(1) == S, op,
+              ": positions must be [B, S] or [S], got ", positions.sizes(), " for ", q_in.sizes());
+  c10::cuda::CUDAGuard guard(q_in.device());
+  auto inner = [](const at::Tensor& t) { return t.stride(-1) == 1 || t.numel() == 0 ? t : t.contiguous(); };
+  at::Tensor q = inner(q_in), k = inner(k_in);
+  at::Tensor qo = at::empty_like(q_in), ko = at::empty_like(k_in);
+  if (qo.stride(-1) != 1) qo = at::empty_like(q_in, at::MemoryFormat::Contiguous);
+  if (ko.stride(-1) != 1) ko = at::empty_like(k_in, at::MemoryFormat::Contiguous);
+  rbln_rotary_params_t p{};
+  p.batch = (int32_t)B;
+  p.q_heads = (int32_t)q.size(1);
+  p.k_heads = (int32_t)k.size(1);
+  p.seq_len = (int32_t)S;
+  p.head_dim = (int32_t)D;
+  p.rotary_dim = (int32_t)(2 * inv_freq.numel());
+  p.dtype = to_rbln_dtype(dt);
+  p.q = q.data_ptr();
+  p.q_out = qo.data_ptr();
+  p.k = k.data_ptr();
+  p.k_out = ko.data_ptr();
+  for (int i = 0; i < 3; ++i) {
+    p.q_stride[i] = q.stride(i);
+    p.q_out_stride[i] = qo.stride(i);
+    p.k_stride[i] = k.stride(i);
+    p.k_out_stride[i] = ko.stride(i);
+  }
+  p.positions = pos.data_ptr();
+  p.positions_dtype = to_rbln_dtype(pos.scalar_type());
+  p.positions_stride[0] = pos.size(0) == 1 ? 0 : pos.stride(0);
+  p.positions_stride[1] = pos.stride(1);
+  p.inv_freq = inv_freq.data_ptr<float>();
+  p.interleaved = interleaved;
+  p.inverse = inverse;
+  p.mscale = (float)mscale;
+  check_rc(rbln_rotary(&p, at::cuda::getCurrentCUDAStream(q.device().index()).stream()), op);
+  return {qo, ko};
+}
+
+using RotaryOp = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                    const at::Tensor&, bool, double, bool);
+std::tuple<at::Tensor, at::Tensor> call_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                                               const at::Tensor& inv_freq, bool interleaved, double mscale,
+                                               bool inverse) {
+  static auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("rbln_attn::rotary", "").typed<RotaryOp>();
+  return op.call(q, k, positions, inv_freq, interleaved, mscale, inverse);
+}
+
+// The map is linear: the gradient is the transposed map of the outputs'
+// gradients, the same op (so it can be differentiated again).
+struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                                                const at::Tensor& k, const at::Tensor& positions,
+                                                const at::Tensor& inv_freq, bool interleaved, double mscale,
+                                                bool inverse) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [qo, ko] = call_rotary(q, k, positions, inv_freq, interleaved, mscale, inverse);
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["mscale"] = mscale;
+    ctx->saved_data["inverse"] = inverse;
+    return {qo, ko};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad) {
+    const auto saved = ctx->get_saved_variables();
+    auto [dq, dk] = call_rotary(grad[0], grad[1], saved[0], saved[1], ctx->saved_data["interleaved"].toBool(),
+                                ctx->saved_data["mscale"].toDouble(), !ctx->saved_data["inverse"].toBool());
+    return {dq, dk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k,
+                                                   const at::Tensor& positions, const at::Tensor& inv_freq,
+                                                   bool interleaved, double mscale, bool inverse) {
+  TORCH_CHECK(!inv_freq.requires_grad(), "rotary: inv_freq has no gradient (detach it)");
+  // A leaf of a graph that still lives has its gradient node on the stream of
+  // that graph; a backward pass captured on another stream would make the
+  // engine wait for it, which breaks the capture. Refused before that.
+  if (at::cuda::currentStreamCaptureStatus() != at::cuda::CaptureStatus::None) {
+    const c10::Stream now = at::cuda::getCurrentCUDAStream(q.device().index());
+    for (const at::Tensor* t : {&q, &k}) {
+      if (!t->requires_grad() || !t->is_leaf()) continue;
+      const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+      const auto at = node ? node->stream() : std::nullopt;
+      TORCH_CHECK(!at.has_value() || *at == now, "rotary: an input belongs to a graph that lives on another stream; "
+                  "free that graph before capturing, or capture with inputs of their own");
+    }
+  }
+  auto out = RotaryFunction::apply(q, k, positions, inv_freq, interleaved, mscale, inverse);
+  return {out[0], out[1]};
+}
+
+// rbln_attn::rotary_paged_kv_write: q [B, Hkv, G, S, D] rotated and returned,
+// k rotated and v as it is written into the paged cache, as paged_kv_write
+// writes them; positions seq[b] + s.
+at::Tensor rotary_paged_kv_write_cuda(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                                      at::Tensor& kcache, at::Tensor& vcache, const at::Tensor& seq_in,
+                                      const at::Tensor& block_table_in, int64_t block_size,
+                                      const at::Tensor& inv_freq_in, bool interleaved, double mscale,
+                                      const std::optional<at::Tensor>& k_scale,
+                                      const std::optional<at::Tensor>& v_scale) {
+  const char* op = "rotary_paged_kv_write";
+  TORCH_CHECK(q_in.is_cuda() && q_in.dim() == 5, op, ": q must be CUDA [B, Hkv, G, S, D]");
+  const bool fp8 = kcache.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(fp8 || kcache.scalar_type() == q_in.scalar_type(), op, ": cache dtype must be q's or float8_e4m3fn");
+  TORCH_CHECK(kcache.size(-1) == q_in.size(-1), op, ": cache head_dim differs from q's");
+  Common c;
+  fill_paged(c, op, q_in, k_in, v_in, kcache, vcache, seq_in, at::scalar_tensor(1.0, at::kFloat), block_table_in,
+             block_size, std::nullopt, false);
+  at::Tensor inv_freq = check_inv_freq(op, inv_freq_in, q_in);
+  if (fp8) {
+    TORCH_CHECK(k_scale.has_value() && v_scale.has_value(), op, ": fp8 caches need k_scale and v_scale");
+    check_scales(op, kcache, *k_scale, *v_scale);
+    c.p.k_scale = k_scale->data_ptr<float>();
+    c.p.v_scale = v_scale->data_ptr<float>();
+    c.p.scale_stride[0] = k_scale->stride(0);
+    c.p.scale_stride[1] = k_scale->stride(1);
+  }
+  rbln_rotary_params_t r{};
+  r.rotary_dim = (int32_t)(2 * inv_freq.numel());
+  r.inv_freq = inv_freq.data_ptr<float>();
+  r.interleaved = interleaved;
+  r.mscale = (float)mscale;
+  c10::cuda::CUDAGuard guard(c.q.device());
+  check_rc(rbln_rotary_paged_kv_write(&c.p, &r, at::cuda::getCurrentCUDAStream(c.q.device().index()).stream()), op);
+  check_device_flags(c, op);
+  return c.out;
+}
+
+// rbln_attn::paged_kv_read: rows [0, lengths[b]) of every sequence as dense
+// k, v [B, Hkv, 1, max_len, D], zeros behind them.
+std::tuple<at::Tensor, at::Tensor> paged_kv_read_cuda(const at::Tensor& kcache, const at::Tensor& vcache,
+                                                      const at::Tensor& lengths_in, const at::Tensor& block_table_in,
+                                                      int64_t block_size, int64_t max_len,
+                                                      const std::optional<at::Tensor>& k_scale,
+                                                      const std::optional<at::Tensor>& v_scale,
+                                                      std::optional<at::ScalarType> dtype) {
+  const char* op = "paged_kv_read";
+  TORCH_CHECK(kcache.is_cuda() && kcache.dim() == 5 && kcache.sizes() == vcache.sizes() &&
+                  kcache.strides() == vcache.strides() && kcache.scalar_type() == vcache.scalar_type() &&
+                  vcache.device() == kcache.device() && kcache.stride(-1) == 1 && kcache.size(2) == 1,
+              op, ": caches must be CUDA [num_blocks, Hkv, 1, block_size, D], alike, with a contiguous last dim");
+  TORCH_CHECK(kcache.size(3) == block_size, op, ": block_size ", block_size,
+              " does not match the cache's block dimension ", kcache.size(3));
+  const auto ct = kcache.scalar_type();
+  const bool fp8 = ct == at::kFloat8_e4m3fn;
+  TORCH_CHECK(fp8 || ct == at::kBFloat16 || ct == at::kHalf, op,
+              ": caches must be bfloat16, float16 or float8_e4m3fn, got ", ct);
+  const auto dt = dtype.has_value() ? *dtype : fp8 ? at::kBFloat16 : ct;
+  TORCH_CHECK(is_float16or32(dt), op, ": dtype must be bfloat16, float16 or float32, got ", dt);
+  TORCH_CHECK(max_len >= 0 && max_len <= INT32_MAX, op, ": max_len must be in [0, 2^31)");
+  at::Tensor len = on_device(lengths_in, kcache).reshape({-1}).to(at::kInt).contiguous();
+  const int64_t B = len.numel(), Hkv = kcache.size(1), D = kcache.size(-1);
+  at::Tensor bt = on_device(block_table_in, kcache);
+  if (bt.dim() == 1) bt = bt.unsqueeze(0);
+  TORCH_CHECK(bt.dim() == 2 && (bt.size(0) == B || bt.size(0) == 1), op, ": block_table must be [B, max_blocks]");
+  TORCH_CHECK(bt.scalar_type() == at::kShort || bt.scalar_type() == at::kInt || bt.scalar_type() == at::kLong, op,
+              ": block_table must be int16/int32/int64");
+  if (bt.stride(1) != 1) bt = bt.contiguous();
+  rbln_paged_attn_params_t p{};
+  p.batch = (int32_t)B;
+  p.num_kv_heads = (int32_t)Hkv;
+  p.group = 1;
+  p.q_len = (int32_t)max_len;
+  p.head_dim = (int32_t)D;
+  p.num_blocks = (int32_t)kcache.size(0);
+  p.block_size = (int32_t)block_size;
+  p.max_blocks = (int32_t)bt.size(1);
+  p.q_dtype = to_rbln_dtype(dt);
+  p.kcache = kcache.data_ptr();
+  p.vcache = vcache.data_ptr();
+  p.kv_dtype = to_rbln_dtype(ct);
+  p.cache_stride[0] = kcache.stride(0); p.cache_stride[1] = kcache.stride(1); p.cache_stride[2] = kcache.stride(3);
+  if (fp8) {
+    TORCH_CHECK(k_scale.has_value() && v_scale.has_value(), op, ": fp8 caches need k_scale and v_scale");
+    check_scales(op, kcache, *k_scale, *v_scale);
+    p.k_scale = k_scale->data_ptr<float>();
+    p.v_scale = v_scale->data_ptr<float>();
+    p.scale_stride[0] = k_scale->stride(0);
+    p.scale_stride[1] = k_scale->stride(1);
+  }
+  p.seq = len.data_ptr<int32_t>();
+  p.seq_stride = 1;
+  p.block_table = bt.data_ptr();
+  p.block_table_dtype = to_rbln_dtype(bt.scalar_type());
+  p.block_table_stride = bt.size(0) == 1 ? 0 : bt.stride(0);
+  c10::cuda::CUDAGuard guard(kcache.device());
+  at::Tensor err;
+  if (debug_checks()) {
+    err = at::zeros({1}, kcache.options().dtype(at::kInt));
+    p.error_flags = reinterpret_cast<uint32_t*>(err.data_ptr<int32_t>());
+  }
+  at::Tensor k = at::empty({B, Hkv, 1, max_len, D}, kcache.options().dtype(dt));
+  at::Tensor v = at::empty({B, Hkv, 1, max_len, D}, kcache.options().dtype(dt));
+  const int64_t os[3] = {k.stride(0), k.stride(1), k.stride(3)};
+  check_rc(rbln_paged_kv_read(&p, k.data_ptr(), v.data_ptr(), os,
+                              at::cuda::getCurrentCUDAStream(kcache.device().index()).stream()),
+           op);
+  if (err.defined()) {
+    const int flags = err.item<int>();
+    TORCH_CHECK(flags == 0, op, ": device-side input check failed (flags 0x", std::hex, flags, ")");
+  }
+  return {k, v};
 }
 
 // rbln_attn::paged_kv_write: the paged ops' append step on its own (k, v
@@ -709,9 +993,26 @@ TORCH_LIBRARY(rbln_attn, m) {
   m.def(
       "paged_kv_write(Tensor k, Tensor v, Tensor(a!) kcache, Tensor(b!) vcache, Tensor seq, Tensor block_table, "
       "SymInt block_size, Tensor(c!)? k_scale=None, Tensor(d!)? v_scale=None) -> ()");
+  m.def(
+      "rotary(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, bool interleaved=False, float mscale=1.0, "
+      "bool inverse=False) -> (Tensor, Tensor)");
+  m.def(
+      "rotary_paged_kv_write(Tensor q, Tensor k, Tensor v, Tensor(a!) kcache, Tensor(b!) vcache, Tensor seq, "
+      "Tensor block_table, SymInt block_size, Tensor inv_freq, bool interleaved=False, float mscale=1.0, "
+      "Tensor(c!)? k_scale=None, Tensor(d!)? v_scale=None) -> Tensor");
+  m.def(
+      "paged_kv_read(Tensor kcache, Tensor vcache, Tensor lengths, Tensor block_table, SymInt block_size, "
+      "SymInt max_len, Tensor? k_scale=None, Tensor? v_scale=None, ScalarType? dtype=None) -> (Tensor, Tensor)");
 }
 
-TORCH_LIBRARY_IMPL(rbln_attn, CUDA, m) { m.impl("paged_kv_write", &paged_kv_write_cuda); }
+TORCH_LIBRARY_IMPL(rbln_attn, CUDA, m) {
+  m.impl("paged_kv_write", &paged_kv_write_cuda);
+  m.impl("rotary", &rotary_cuda);
+  m.impl("rotary_paged_kv_write", &rotary_paged_kv_write_cuda);
+  m.impl("paged_kv_read", &paged_kv_read_cuda);
+}
+
+TORCH_LIBRARY_IMPL(rbln_attn, AutogradCUDA, m) { m.impl("rotary", &rotary_autograd); }
 
 TORCH_LIBRARY_IMPL(rbln_attn, CompositeExplicitAutograd, m) {
   m.impl("set_sdpa_route", &set_sdpa_route);
@@ -736,6 +1037,10 @@ TORCH_LIBRARY(rbln_custom_ops, m) {
       "Tensor seq, Tensor scale, Tensor block_table, SymInt block_size, bool is_bidirectional, "
       "Tensor? mask=None) -> Tensor");
   m.def(
+      "paged_causal_attn_prefill_kvfp8(Tensor q, Tensor? k, Tensor? v, Tensor(a3!) kcache, Tensor(a4!) vcache, "
+      "Tensor(a5!) k_scale, Tensor(a6!) v_scale, Tensor seq, Tensor scale, Tensor block_table, SymInt block_size, "
+      "bool is_bidirectional, Tensor? mask=None) -> Tensor");
+  m.def(
       "paged_causal_attn_decode(Tensor q, Tensor k, Tensor v, Tensor(a3!) kcache, Tensor(a4!) vcache, "
       "Tensor seq, Tensor scale, Tensor block_table, SymInt block_size, Tensor? mask=None) -> Tensor");
   m.def(
@@ -753,6 +1058,7 @@ TORCH_LIBRARY(rbln_custom_ops, m) {
 TORCH_LIBRARY_IMPL(rbln_custom_ops, CUDA, m) {
   m.impl("paged_attn_prefill", &paged_attn_prefill_cuda);
   m.impl("paged_causal_attn_prefill", &paged_causal_attn_prefill_cuda);
+  m.impl("paged_causal_attn_prefill_kvfp8", &paged_causal_attn_prefill_kvfp8_cuda);
   m.impl("paged_attn_decode", &paged_attn_decode_cuda);
   m.impl("paged_causal_attn_decode", &paged_causal_attn_decode_cuda);
   m.impl("paged_causal_attn_decode_kvfp8", &paged_causal_attn_decode_kvfp8_cuda);

@@ -43,7 +43,9 @@ from .ops import (  # noqa: E402,F401
     paged_causal_attn_decode,
     paged_causal_attn_decode_kvfp8,
     paged_causal_attn_prefill,
+    paged_causal_attn_prefill_kvfp8,
 )
+from .rotary import rotary_frequencies  # noqa: E402,F401
 
 __all__ = [
     "flash_attention_naive_decode",
@@ -53,6 +55,8 @@ __all__ = [
     "paged_causal_attn_decode",
     "paged_causal_attn_decode_kvfp8",
     "paged_causal_attn_prefill",
+    "paged_causal_attn_prefill_kvfp8",
+    "rotary_frequencies",
     "CABI_LIBRARY",
     "TORCH_LIBRARY",
 ]

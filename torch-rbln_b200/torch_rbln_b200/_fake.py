@@ -10,6 +10,7 @@ _NAMES = (
     "paged_attn_prefill",
     "paged_attn_decode",
     "paged_causal_attn_prefill",
+    "paged_causal_attn_prefill_kvfp8",
     "paged_causal_attn_decode",
     "paged_causal_attn_decode_kvfp8",
     "flash_attention_naive_prefill",
@@ -32,3 +33,25 @@ def _writes_only(*args, **kwargs):
 
 
 torch.library.register_fake("rbln_attn::paged_kv_write", _writes_only)
+
+
+@torch.library.register_fake("rbln_attn::rotary")
+def _rotary(q, k, positions, inv_freq, interleaved=False, mscale=1.0, inverse=False):
+    def like(x):  # x's layout, unless that would leave the head dimension strided
+        y = torch.empty_like(x)
+        return y if y.stride(-1) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+    return like(q), like(k)
+
+
+@torch.library.register_fake("rbln_attn::rotary_paged_kv_write")
+def _rotary_paged_kv_write(q, *args, **kwargs):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
+@torch.library.register_fake("rbln_attn::paged_kv_read")
+def _paged_kv_read(kcache, vcache, lengths, block_table, block_size, max_len, k_scale=None, v_scale=None, dtype=None):
+    if dtype is None:
+        dtype = torch.bfloat16 if kcache.dtype == torch.float8_e4m3fn else kcache.dtype
+    shape = [lengths.numel(), kcache.shape[1], 1, max_len, kcache.shape[-1]]
+    return kcache.new_empty(shape, dtype=dtype), kcache.new_empty(shape, dtype=dtype)

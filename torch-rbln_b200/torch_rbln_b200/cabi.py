@@ -104,6 +104,17 @@ class SdpaBwdParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("q_heads", c_i32), ("k_heads", c_i32), ("seq_len", c_i32), ("head_dim", c_i32),
+        ("rotary_dim", c_i32), ("dtype", c_i32),
+        ("q", c_vp), ("q_stride", c_i64 * 3), ("q_out", c_vp), ("q_out_stride", c_i64 * 3),
+        ("k", c_vp), ("k_stride", c_i64 * 3), ("k_out", c_vp), ("k_out_stride", c_i64 * 3),
+        ("positions", c_vp), ("positions_dtype", c_i32), ("positions_stride", c_i64 * 2),
+        ("inv_freq", c_vp), ("interleaved", c_i32), ("inverse", c_i32), ("mscale", ctypes.c_float),
+    ]
+
+
 class PeerOut(ctypes.Structure):
     """rbln_peer_out_t: every rank's output buffer and flag array, as mapped on this GPU."""
     _fields_ = [("out", c_vp), ("flags", c_vp), ("n", c_i32), ("rank", c_i32), ("head0", c_i32),
@@ -126,6 +137,10 @@ ENTRY_POINTS = {
     "rbln_paged_causal_attn_prefill": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), c_vp]),
     "rbln_paged_attn_prefill": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), c_vp]),
     "rbln_paged_kv_write": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), c_vp]),
+    "rbln_rotary_params_sizeof": (ctypes.c_size_t, []),
+    "rbln_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryParams), c_vp]),
+    "rbln_rotary_paged_kv_write": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), ctypes.POINTER(RotaryParams), c_vp]),
+    "rbln_paged_kv_read": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), c_vp, c_vp, ctypes.POINTER(c_i64), c_vp]),
     "rbln_sdpa_fwd": (ctypes.c_int, [ctypes.POINTER(SdpaParams), c_vp]),
     "rbln_sdpa_bwd_workspace_size": (ctypes.c_int, [ctypes.POINTER(SdpaBwdParams), ctypes.POINTER(ctypes.c_size_t)]),
     "rbln_sdpa_bwd": (ctypes.c_int, [ctypes.POINTER(SdpaBwdParams), c_vp]),
@@ -156,6 +171,8 @@ def lib() -> ctypes.CDLL:
             raise RuntimeError("rbln_paged_attn_params_t layout mismatch between ctypes and the library")
         if L.rbln_peer_out_sizeof() != ctypes.sizeof(PeerOut):
             raise RuntimeError("rbln_peer_out_t layout mismatch between ctypes and the library")
+        if L.rbln_rotary_params_sizeof() != ctypes.sizeof(RotaryParams):
+            raise RuntimeError("rbln_rotary_params_t layout mismatch between ctypes and the library")
         _lib = L
     return _lib
 
@@ -263,6 +280,28 @@ def sdpa_bwd_params(q, k, v, out, dout, lse, dq=None, dk=None, dv=None, causal=T
             st[i] = t.stride(i)
     p.causal = 1 if causal else 0
     p.scale = scale if scale is not None else 1.0 / (q.shape[-1] ** 0.5)
+    return p
+
+
+def rotary_params(q, k, q_out, k_out, positions, inv_freq, interleaved=False, mscale=1.0, inverse=False):
+    """Fills RotaryParams for q [B, Hq, S, D], k [B, Hk, S, D] (inner dim contiguous), positions [B, S]."""
+    p = RotaryParams()
+    p.batch, p.q_heads, p.seq_len, p.head_dim = q.shape
+    p.k_heads = 0 if k is None else k.shape[1]
+    p.rotary_dim = 2 * inv_freq.numel()
+    p.dtype = _DT[q.dtype]
+    for name, t in (("q", q), ("q_out", q_out), ("k", k), ("k_out", k_out)):
+        if t is None:
+            continue
+        setattr(p, name, t.data_ptr())
+        st = getattr(p, name + "_stride")
+        for i in range(3):
+            st[i] = t.stride(i)
+    p.positions = positions.data_ptr()
+    p.positions_dtype = _DT[positions.dtype]
+    p.positions_stride[0], p.positions_stride[1] = positions.stride(0), positions.stride(1)
+    p.inv_freq = inv_freq.data_ptr()
+    p.interleaved, p.inverse, p.mscale = int(interleaved), int(inverse), mscale
     return p
 
 

@@ -34,6 +34,13 @@ def paged_causal_attn_prefill(*args):
     return _ops.paged_causal_attn_prefill(*args)
 
 
+def paged_causal_attn_prefill_kvfp8(*args):
+    """S_q new tokens a sequence over an fp8-e4m3 cache: paged_causal_attn_prefill's arguments with k_scale and
+    v_scale [num_blocks, Hkv] after the caches; k and v None when their rows are in the cache already."""
+    _count("paged_causal_attn_prefill_kvfp8", args, 12, 13)
+    return _ops.paged_causal_attn_prefill_kvfp8(*args)
+
+
 def paged_causal_attn_decode(*args):
     _count("paged_causal_attn_decode", args, 9, 10)
     return _ops.paged_causal_attn_decode(*args)
