@@ -23,6 +23,8 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "sm100.cuh"
+#include "tma_map.cuh"
 
 namespace rbln {
 namespace {
@@ -77,6 +79,17 @@ __device__ __forceinline__ float pow2_above(float x) {
   return __uint_as_float((__float_as_uint(x) + 0x007fffffu) & 0x7f800000u);
 }
 
+// Power of two that brings a row's largest magnitude m to [2^14, 2^15), and
+// its inverse; 1 for rows of zeros, infinities or NaN.
+__device__ __forceinline__ float f16_factor(float m, float& undo) {
+  undo = 1.f;
+  if (!(m > 0.f && m < 3e38f)) return 1.f;
+  const int e = (int)(__float_as_uint(m) >> 23) - 127;  // m in [2^e, 2^(e+1)), or subnormal
+  const int k = min(max(14 - e, -120), 120);
+  undo = __uint_as_float((uint32_t)(127 - k) << 23);
+  return __uint_as_float((uint32_t)(127 + k) << 23);
+}
+
 // Keys [0, L) that some row of item's row tile may see; `last` is the tile's last token.
 __device__ __forceinline__ int item_keys(const Fp8Args& a, int b, int last) {
   const int pos = a.seq[b * a.seq_stride];
@@ -85,18 +98,16 @@ __device__ __forceinline__ int item_keys(const Fp8Args& a, int b, int last) {
   return (int)min(end, (int64_t)a.span);
 }
 
-// Exclusive prefix P[0..items] of the items' costs (keys rounded up to 16
-// plus kSegCost), by the whole CTA. rows: rows of a row tile.
-template <int THREADS>
-__device__ __forceinline__ void cost_prefix(const Fp8Args& a, int rows, int* P) {
-  __shared__ int wsum[THREADS / 32];
+// Exclusive prefix P[0..items] of the items' costs, by the whole CTA: keys
+// rounded up to a multiple of `unit`, in units of it, plus `seg` for the
+// unit's start. keys(i): keys of item i.
+template <int THREADS, typename Keys>
+__device__ __forceinline__ void cost_prefix(const Fp8Args& a, int unit, int scale, int seg, Keys keys, int* wsum,
+                                            int* P) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.items + THREADS - 1) / THREADS;
   const int first = tid * per;
-  auto cost = [&](int i) {
-    const int b = i / a.tiles, t = i - b * a.tiles;
-    return ((item_keys(a, b, (int)(((int64_t)(t + 1) * rows - 1) / a.G)) + 15) & ~15) + kSegCost;
-  };
+  auto cost = [&](int i) { return (keys(i) + unit - 1) / unit * scale + seg; };
   int sum = 0;
   for (int i = 0; i < per; ++i)
     if (first + i < a.items) sum += cost(first + i);
@@ -184,13 +195,7 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
       if constexpr (BF16) {
         qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, 1));
         qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, 2));
-        float up = 1.f;
-        if (qmax > 0.f && qmax < 3e38f) {
-          const int e = (int)(__float_as_uint(qmax) >> 23) - 127;  // qmax in [2^e, 2^(e+1))
-          const int k = min(max(14 - e, -120), 120);
-          up = __uint_as_float((uint32_t)(127 + k) << 23);
-          undo[nt] = __uint_as_float((uint32_t)(127 - k) << 23);
-        }
+        const float up = f16_factor(qmax, undo[nt]);
 #pragma unroll
         for (int k = 0; k < KR; ++k) {
           const float2 f = unpack2<true>(qf[nt][k]);
@@ -420,7 +425,6 @@ template <typename Keys, typename Seg>
 __device__ __forceinline__ void walk_share(const Fp8Args& a, const int* P, int64_t lo, int64_t hi, Keys keys, Seg seg) {
   const int64_t T = P[a.items];
   int cont = -1, start = -1;
-  const int64_t first = lo;
   while (lo < hi) {
     const int h = (int)(lo / T);
     const int x = (int)(lo - h * T);
@@ -434,7 +438,7 @@ __device__ __forceinline__ void walk_share(const Fp8Args& a, const int* P, int64
     const bool starts = lo == u0 - kSegCost;
     const int L = keys(i);
     const int unit = h * a.items + i;
-    lo = seg_hi > lo ? seg_hi : (hi < u1 ? hi : u1);
+    lo = seg_hi;  // hi or u1: past lo either way
     if (L == 0) {
       if (starts) seg(h, i, 0, 0, 0, true, 0);
       continue;
@@ -447,7 +451,6 @@ __device__ __forceinline__ void walk_share(const Fp8Args& a, const int* P, int64
     }
     seg(h, i, L, t0, t1, whole, 2 * (int)blockIdx.x + (head ? 1 : 0));
   }
-  (void)first;
   if (threadIdx.x == 0) {
     a.desc[2 * blockIdx.x] = cont;
     a.desc[2 * blockIdx.x + 1] = start;
@@ -480,12 +483,772 @@ __global__ void __launch_bounds__(kMqThreads, NT == 1 ? 4 : 2) paged_attn_fp8_ro
     return;
   }
   int* P = reinterpret_cast<int*>(dsm + kMqWarps * NC * (D * 4 + 8));
-  cost_prefix<kMqThreads>(a, NC, P);
+  __shared__ int wsum[kMqWarps];
+  cost_prefix<kMqThreads>(a, 16, 16, kSegCost, keys, wsum, P);  // counted in keys
   const int64_t total = (int64_t)P[a.items] * a.Hkv;
   int64_t W = ((total + gridDim.x - 1) / gridDim.x + 15) & ~(int64_t)15;
   if (W < kMinW) W = kMinW;
   const int64_t lo = min(W * blockIdx.x, total);
   walk_share(a, P, lo, min(lo + W, total), keys, seg);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: bound by the tensor cores, or by HBM behind a long context.
+// One persistent CTA an SM on tcgen05; a unit is one KV head's G query heads x
+// NX row tiles of 128 rows (rows = G heads x QT = 128 / G tokens), key tiles
+// are 128 keys. Roles:
+//   softmax     NX warpgroups, thread = row: scores from TMEM, times the
+//               block's K scale, online softmax, probabilities times the
+//               block's relative V scale, as f16 over the scores in TMEM;
+//   producer    one warp: the codes' tiles by TMA through the block table into
+//               a ring of raw tiles (16 KB at D = 128), and Q;
+//   scales      one warp: each tile's 16 K and V scales (one for 8 keys, the
+//               smallest block) and 128 keep bits, into a ring of four;
+//   convert     four warps: codes to f16 in the 128-byte-swizzled operand
+//               layout, V rows that no query may see as zeros;
+//   MMA         one thread: S = Q K^T, O += P V, accumulators in TMEM.
+// f16 operands take every code exactly, so no scale enters the operands and
+// the conversion is one instruction for two codes; reading codes instead of
+// 16-bit rows halves HBM and L2 traffic. Shared memory (D = 128, NX = 2):
+// Q 64 KB, K and V 2 x 32 KB each, raw 2 x 16 KB.
+//
+// The key tiles of all units, head-major, are cut into equal shares, one a
+// CTA, so that there is one wave without a tail however unequal the
+// sequences; the units that shares cut are joined by the merge kernel.
+// NX = 2: one score buffer a row tile, PV(j - 1) before QK(j), so that one
+// tile's softmax runs under the other's products. NX = 1: two score buffers,
+// QK(j) before PV(j - 1), so that they run under the only softmax.
+// Every wait is bounded; on expiry the CTA raises RBLN_DEVERR_TIMEOUT, lets
+// its copies and products finish, frees TMEM and returns.
+// ---------------------------------------------------------------------------
+using namespace sm100;
+
+constexpr int kPanel = 128 * 128;  // 128 rows of 64 f16
+constexpr int kTcSegCost = 2;      // key tiles charged to a unit's start
+constexpr int kMetaRing = 4;
+
+struct TileMeta {
+  float ks[16], vs[16];  // scale of keys [8 g, 8 g + 8)
+  uint32_t keep[4];
+  float vmax;
+  float pad[3];
+};
+
+template <int D, int NX>
+struct TcSmem {
+  static constexpr int NP = D / 64;
+  static constexpr int TILE = NP * kPanel;  // 128 rows x D of f16
+  static constexpr int RAW = 128 * D;       // 128 rows x D codes
+  static constexpr int NRAW = (D == 128 && NX == 2) ? 2 : 4;
+  static constexpr int Q = 0;
+  static constexpr int K0 = Q + NX * TILE;
+  static constexpr int V0 = K0 + 2 * TILE;
+  static constexpr int R0 = V0 + 2 * TILE;
+  static constexpr int META = R0 + NRAW * RAW;
+  static constexpr int BAR = META + kMetaRing * (int)sizeof(TileMeta);
+  static constexpr int MISC = BAR + 40 * 8;  // TMEM slot, abort, share start (5 ints), prefix sums (16 ints)
+  static constexpr int TOTAL = MISC + 32 * 4;
+  static constexpr int ALLOC = TOTAL + 1024;
+  static_assert(ALLOC <= 232448, "shared memory");
+};
+
+template <int NX>
+struct TcCfg {
+  static constexpr int THREADS = 128 * NX + 256;
+  // registers a thread after the split: softmax, control, convert. The
+  // launch has 128 (512 threads) or 168 (384 threads) each.
+  static constexpr uint32_t RS = NX == 2 ? 200 : 216, RC = NX == 2 ? 48 : 64, RV = NX == 2 ? 64 : 104;
+  static constexpr uint32_t LAUNCH = NX == 2 ? 128 : 168;
+  static_assert(128 * (NX * RS + RC + RV) <= THREADS * LAUNCH, "register split exceeds the launch");
+};
+
+enum TcBar {
+  T_RF = 0, T_RE = 4,    // raw ring
+  T_KF = 8, T_KE = 10,   // f16 K stages
+  T_VF = 12, T_VE = 14,  // f16 V stages
+  T_MF = 16, T_ME = 20,  // scales and keep bits
+  T_QF = 24, T_QE = 25,
+  T_SF = 26,   // scores (NX = 2: of row tile x; NX = 1: of buffer T & 1)
+  T_PF = 28,   // probabilities written (NX = 2: of row tile x; NX = 1: one)
+  T_PV = 30,   // NX = 1: a PV complete
+  T_O = 31,    // last PV of a segment complete, row tile x
+  T_OE = 33,   // O read
+  T_DONE = 35, T_COUNT = 36
+};
+
+// A CTA's share as every role walks it: `left` positions from position `off`
+// of unit (h, i) on; each unit has kTcSegCost positions and then one a key tile.
+struct Share {
+  int h, i, off, left;
+};
+struct Segment {
+  int h, i, b, tile, keys, j0, j1;
+  bool head, whole;
+};
+template <int NX>
+__device__ __forceinline__ int tc_keys(const Fp8Args& a, int qt, int i) {
+  const int b = i / a.tiles, t = i - b * a.tiles;
+  return item_keys(a, b, (int)min((int64_t)(t + 1) * NX * qt - 1, (int64_t)a.S));
+}
+template <int NX>
+__device__ __forceinline__ bool next_segment(const Fp8Args& a, int qt, Share& sh, Segment& g) {
+  while (sh.left > 0) {
+    if (!a.balanced && sh.i >= a.items) return false;
+    const int keys = tc_keys<NX>(a, qt, sh.i);
+    const int nt = (keys + 127) / 128, cost = nt + kTcSegCost;
+    g.h = sh.h;
+    g.i = sh.i;
+    const int from = sh.off, to = a.balanced ? min(from + sh.left, cost) : cost;
+    if (a.balanced) {
+      sh.left -= to - from;
+      sh.off = to;
+      if (to == cost) {
+        sh.off = 0;
+        if (++sh.i == a.items) {
+          sh.i = 0;
+          ++sh.h;
+        }
+      }
+    } else {  // whole units, every gridDim.x-th of item-major order
+      const int64_t u = (int64_t)sh.i * a.Hkv + sh.h + gridDim.x;
+      sh.i = (int)(u / a.Hkv);
+      sh.h = (int)(u - (int64_t)sh.i * a.Hkv);
+    }
+    g.b = g.i / a.tiles;
+    g.tile = g.i - g.b * a.tiles;
+    g.keys = keys;
+    g.j0 = max(from - kTcSegCost, 0);
+    g.j1 = max(to - kTcSegCost, 0);
+    g.head = g.j0 == 0;
+    g.whole = g.head && g.j1 == nt;
+    if (nt == 0 ? from == 0 : g.j1 > g.j0) return true;
+  }
+  return false;
+}
+
+// Block (-1: none) of the key that starts group `key` of sequence b.
+__device__ __forceinline__ int block_of(const Fp8Args& a, int b, int key, int keys) {
+  if (key >= keys) return -1;
+  const int64_t v = load_index(a.bt, a.bt_dtype, b * a.bt_stride + key / a.bs);
+  if (v >= 0 && v < a.num_blocks) return (int)v;
+  if (a.err) atomicOr(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
+  return -1;
+}
+
+template <int D, bool BF16, int NX>
+__global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
+    paged_attn_fp8_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                                const __grid_constant__ CUtensorMap tm_v, const Fp8Args a, const int qt,
+                                const float* q_undo) {
+  using L = TcSmem<D, NX>;
+  using C = TcCfg<NX>;
+  constexpr int NP = L::NP, NRAW = L::NRAW;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* sgen = smem_raw + (sbase - smem_u32(smem_raw));
+  int* misc = reinterpret_cast<int*>(sgen + L::MISC);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
+  volatile int* abort = misc + 1;
+  TileMeta* meta = reinterpret_cast<TileMeta*>(sgen + L::META);
+  auto bar = [&](int i) { return sbase + L::BAR + 8u * i; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int W0 = 4 * NX;  // first control warp: producer, MMA, scales, -; then four converters
+
+  if (threadIdx.x == 0) {
+    *abort = 0;
+    for (int i = 0; i < T_COUNT; ++i) {
+      uint32_t n = 1;
+      if (i >= T_RE && i < T_KF) n = 4;                                          // converters
+      if ((i >= T_KF && i < T_KE) || (i >= T_VF && i < T_VE)) n = 4;             // converters
+      if (i >= T_ME && i < T_QF) n = 4 + 4 * NX;                                 // converters and softmax warps
+      if ((i >= T_PF && i < T_PV) || i == T_OE || i == T_OE + 1) n = 4;          // a row tile's softmax warps
+      mbar_init(bar(i), n);
+    }
+    fence_mbar_init();
+  }
+  if (warp == W0 + 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  dependents_enter();
+  // this CTA's share
+  if (a.balanced) {
+    int* P = reinterpret_cast<int*>(sgen + L::K0);  // before any copy or conversion uses it
+    auto keys = [&](int i) { return tc_keys<NX>(a, qt, i); };
+    cost_prefix<C::THREADS>(a, 128, 1, kTcSegCost, keys, misc + 8, P);
+    if (threadIdx.x == 0) {
+      const int64_t T = P[a.items], total = T * a.Hkv;
+      // at least four tiles a CTA; fewer CTAs work then
+      const int64_t W = max((total + gridDim.x - 1) / gridDim.x, (int64_t)(4 + kTcSegCost));
+      const int64_t lo = min(W * blockIdx.x, total), hi = min(lo + W, total);
+      int i = 0;
+      int64_t h = 0;
+      if (lo < hi) {
+        h = lo / T;
+        const int x = (int)(lo - h * T);
+        int j = a.items - 1;
+        while (i < j) {
+          const int mid = (i + j + 1) >> 1;
+          if (P[mid] <= x) i = mid; else j = mid - 1;
+        }
+        misc[4] = x - P[i];
+      }
+      misc[2] = (int)h;
+      misc[3] = i;
+      misc[5] = (int)(hi - lo);
+    }
+    fence_proxy_async_smem();  // the prefix's area is written by TMA next
+  } else if (threadIdx.x == 0) {
+    misc[2] = (int)(blockIdx.x % a.Hkv);
+    misc[3] = (int)(blockIdx.x / a.Hkv);
+    misc[4] = 0;
+    misc[5] = 1;
+  }
+  if (blockIdx.x == 0 && a.err)
+    for (int b = threadIdx.x; b < a.B; b += C::THREADS)
+      if (a.seq[b * a.seq_stride] < 0) atomicOr(a.err, RBLN_DEVERR_SEQ_RANGE);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Share sh{misc[2], misc[3], misc[4], misc[5]};
+  Segment g;
+  auto t_o = [&](int x) { return tmem + 256 + x * 128; };
+  // score buffer of row tile x at running tile T
+  auto t_s = [&](int x, int T) { return tmem + (NX == 2 ? x : (T & 1)) * 128; };
+  // row tiles of a segment with tokens in the chunk
+  auto active = [&](const Segment& s) { return NX == 1 || (s.tile * NX + 1) * qt >= a.S ? 1 : 2; };
+
+  if (warp >= W0 + 4) {
+    // ---------------------------------------------------------- convert
+    setmaxnreg_dec<C::RV>();
+    const int cw = warp - W0 - 4;
+    constexpr int LPR = D / 16;          // lanes a row
+    constexpr int RPI = 32 / LPR;        // rows a warp and step
+    constexpr int STEPS = 128 / (4 * RPI);
+    const int c16 = lane % LPR;
+    const uint32_t dst_panel = (uint32_t)(c16 >> 2) * kPanel;
+    const int chunk = 2 * (c16 & 3);
+    // the upper panel's lanes store their chunks in the other order, so that
+    // eight lanes of one row cover all banks
+    const int swap = (D == 128) ? (c16 >> 2) : 0;
+    int T = 0;
+    bool ok = true;
+    while (ok && next_segment<NX>(a, qt, sh, g)) {
+      for (int j = g.j0; ok && j < g.j1; ++j, ++T) {
+        const int ms = T % kMetaRing;
+        uint32_t kw[4];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const int n = 2 * T + part, rs = n % NRAW, st = T & 1;
+          const int full = (part ? T_VF : T_KF) + st, empty = (part ? T_VE : T_KE) + st;
+          ok = mbar_wait(bar(T_RF + rs), (n / NRAW) & 1, abort);
+          if (ok && T >= 2) ok = mbar_wait(bar(empty), ((T >> 1) - 1) & 1, abort);
+          bool all = true;
+          if (part == 1 && ok) {
+            ok = mbar_wait(bar(T_MF + ms), (T / kMetaRing) & 1, abort);
+            const uint4 k = *reinterpret_cast<const uint4*>(meta[ms].keep);
+            kw[0] = k.x; kw[1] = k.y; kw[2] = k.z; kw[3] = k.w;
+            all = (k.x & k.y & k.z & k.w) == 0xffffffffu;
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint8_t* raw = sgen + L::R0 + rs * L::RAW;
+          uint8_t* dst = sgen + (part ? L::V0 : L::K0) + st * L::TILE + dst_panel;
+          // unroll 4: four 16-byte loads in flight a lane
+#pragma unroll 4
+          for (int k = 0; k < STEPS; ++k) {
+            const int r = (k * 4 + cw) * RPI + lane / LPR;
+            uint4 w = *reinterpret_cast<const uint4*>(raw + r * D + c16 * 16);
+            if (part == 1 && !all) {
+              // 0 x NaN would reach every row's sum: what no query may see is zeros
+              const uint32_t word = r < 64 ? (r < 32 ? kw[0] : kw[1]) : (r < 96 ? kw[2] : kw[3]);
+              if (!((word >> (r & 31)) & 1u)) w = make_uint4(0, 0, 0, 0);
+            }
+            uint4 lo, hi;
+            e4m3x4_to_f16x2x2(w.x, lo.x, lo.y);
+            e4m3x4_to_f16x2x2(w.y, lo.z, lo.w);
+            e4m3x4_to_f16x2x2(w.z, hi.x, hi.y);
+            e4m3x4_to_f16x2x2(w.w, hi.z, hi.w);
+            uint8_t* row = dst + r * 128;
+            const int x0 = (chunk + swap) ^ (r & 7), x1 = (chunk + 1 - swap) ^ (r & 7);
+            *reinterpret_cast<uint4*>(row + x0 * 16) = swap ? hi : lo;
+            *reinterpret_cast<uint4*>(row + x1 * 16) = swap ? lo : hi;
+          }
+          fence_proxy_async_smem();  // read by the MMA; and the raw slot is rewritten by TMA
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bar(full));
+            mbar_arrive(bar(T_RE + rs));
+            if (part == 1) mbar_arrive(bar(T_ME + ms));
+          }
+        }
+      }
+    }
+  } else if (warp >= W0) {
+    setmaxnreg_dec<C::RC>();
+    if (warp == W0) {
+      // -------------------------------------------------------- producer
+      if (lane == 0) {
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+      }
+      const int rpb = min(a.bs, 128), nbox = 128 / rpb;  // nbox <= 16
+      int T = 0, act = 0, issued = 0;
+      bool ok = true;
+      while (ok && next_segment<NX>(a, qt, sh, g)) {
+        if (g.j1 == g.j0) continue;  // an empty unit
+        const int nx = active(g);
+        int blk = lane < nbox ? block_of(a, g.b, g.j0 * 128 + lane * rpb, g.keys) : -1;
+        for (int j = g.j0; ok && j < g.j1; ++j, ++T) {
+          const int row = (j * 128 + lane * rpb) % a.bs;
+          const int now = blk < 0 ? a.num_blocks : blk;  // out of range: zeros
+          if (j + 1 < g.j1 && lane < nbox) blk = block_of(a, g.b, (j + 1) * 128 + lane * rpb, g.keys);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const int n = 2 * T + part, rs = n % NRAW;
+            if (n >= NRAW && !__all_sync(0xffffffffu, mbar_wait(bar(T_RE + rs), ((n / NRAW) - 1) & 1, abort))) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(bar(T_RF + rs), L::RAW);
+            __syncwarp();
+            if (lane < nbox)
+              tma_load_4d(sbase + L::R0 + rs * L::RAW + lane * rpb * D, part ? &tm_v : &tm_k, bar(T_RF + rs), 0, row,
+                          g.h, now);
+            issued = n + 1;
+          }
+          if (ok && j == g.j0) {
+            // Q behind the first codes: the previous segment's QKs must be done
+            if (act >= 1 && !__all_sync(0xffffffffu, mbar_wait(bar(T_QE), (act - 1) & 1, abort))) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) {
+              mbar_arrive_expect_tx(bar(T_QF), nx * NP * qt * a.G * 128);
+              for (int x = 0; x < nx; ++x)
+                for (int p = 0; p < NP; ++p)
+                  tma_load_5d(sbase + L::Q + x * L::TILE + p * kPanel, &tm_q, bar(T_QF), p * 64,
+                              (g.tile * NX + x) * qt, 0, g.h, g.b);
+            }
+            __syncwarp();
+          }
+        }
+        ++act;
+      }
+      if (*abort) {  // let the copies in flight land before the CTA exits
+        const long long t0 = clock64();
+        for (int n = max(0, issued - NRAW); n < issued; ++n)
+          while (!mbar_try_wait(bar(T_RF + n % NRAW), (n / NRAW) & 1) && clock64() - t0 < 4000000) {
+          }
+        if (act >= 0)
+          while (!mbar_try_wait(bar(T_QF), (act > 0 ? act - 1 : 0) & 1) && clock64() - t0 < 8000000) {
+          }
+      }
+    } else if (warp == W0 + 1) {
+      // ------------------------------------------------------------- MMA
+      if (lane == 0) {
+        const uint32_t id_qk = idesc_f16(false, 128, 128, false);
+        const uint32_t id_pv = idesc_f16(false, 128, D, true);
+        int T = 0, act = 0, actx[2] = {0, 0}, segx[2] = {0, 0};  // tiles, segments; of each row tile
+        bool ok = true;
+        auto qk = [&](int x, int Tj) {
+          const uint32_t qb = sbase + L::Q + x * L::TILE, kb = sbase + L::K0 + (Tj & 1) * L::TILE;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t ad = sw128_desc(qb + (kk >> 2) * kPanel + (kk & 3) * 32, 16, 1024);
+            const uint64_t bd = sw128_desc(kb + (kk >> 2) * kPanel + (kk & 3) * 32, 16, 1024);
+            umma_f16_ss(t_s(x, Tj), ad, bd, id_qk, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(bar(T_SF + (NX == 2 ? x : (Tj & 1))));
+        };
+        auto pv = [&](int x, int Tj, bool first) {
+          const uint32_t vb = sbase + L::V0 + (Tj & 1) * L::TILE;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint64_t bd = sw128_desc(vb + kk * 16 * 128, kPanel, 1024);
+            umma_f16_ts(t_o(x), t_s(x, Tj) + kk * 8, bd, id_pv, (!first || kk > 0) ? 1u : 0u);
+          }
+        };
+        while (ok && next_segment<NX>(a, qt, sh, g)) {
+          const int nt = g.j1 - g.j0;
+          if (nt == 0) continue;
+          const int nx = active(g);
+          ok = mbar_wait(bar(T_QF), act & 1, abort);
+          for (int j = 0; ok && j <= nt; ++j) {
+            const int Tj = T + j;
+            if (j < nt && !mbar_wait(bar(T_KF + (Tj & 1)), (Tj >> 1) & 1, abort)) {
+              ok = false;
+              break;
+            }
+            if constexpr (NX == 1) {
+              if (j < nt) {
+                tc_fence_after();
+                qk(0, Tj);
+                umma_commit(bar(T_KE + (Tj & 1)));
+                if (j == nt - 1) umma_commit(bar(T_QE));
+              }
+            }
+            if (j >= 1 && !mbar_wait(bar(T_VF + ((Tj - 1) & 1)), ((Tj - 1) >> 1) & 1, abort)) {
+              ok = false;
+              break;
+            }
+            for (int x = 0; x < nx; ++x) {
+              if (j >= 1) {
+                // the row tile's P; its first PV overwrites O once the last segment's is read
+                const int ph = NX == 2 ? actx[x] + j - 1 : Tj - 1;
+                if (!mbar_wait(bar(T_PF + x), ph & 1, abort) ||
+                    (j == 1 && segx[x] >= 1 && !mbar_wait(bar(T_OE + x), (segx[x] - 1) & 1, abort))) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+                pv(x, Tj - 1, j == 1);
+                if (NX == 1) umma_commit(bar(T_PV));
+                if (j == nt) umma_commit(bar(T_O + x));
+              }
+              if (NX == 2 && j < nt) {
+                tc_fence_after();
+                qk(x, Tj);
+              }
+            }
+            if (!ok) break;
+            if (NX == 2 && j < nt) {
+              umma_commit(bar(T_KE + (Tj & 1)));
+              if (j == nt - 1) umma_commit(bar(T_QE));
+            }
+            if (j >= 1) umma_commit(bar(T_VE + ((Tj - 1) & 1)));
+          }
+          T += nt;
+          ++act;
+          for (int x = 0; x < nx; ++x) {
+            actx[x] += nt;
+            ++segx[x];
+          }
+        }
+        if (!ok) {
+          umma_commit(bar(T_DONE));
+          const long long t0 = clock64();
+          while (!mbar_try_wait(bar(T_DONE), 0) && clock64() - t0 < 4000000) {
+          }
+        }
+      }
+    } else if (warp == W0 + 2) {
+      // ---------------------------------------------------------- scales
+      int T = 0;
+      bool ok = true;
+      while (ok && next_segment<NX>(a, qt, sh, g)) {
+        if (g.j1 == g.j0) continue;
+        const int grp = lane & 15;
+        int blk = block_of(a, g.b, g.j0 * 128 + grp * 8, g.keys);
+        for (int j = g.j0; j < g.j1; ++j, ++T) {
+          const int ms = T % kMetaRing, t0 = j * 128;
+          const int now = blk;
+          float ks = 1.f, vs = 0.f;
+          if (now >= 0) {
+            ks = a.k_scale[now * a.ss_block + g.h * a.ss_head];
+            vs = a.v_scale[now * a.ss_block + g.h * a.ss_head];
+          }
+          if (j + 1 < g.j1) blk = block_of(a, g.b, t0 + 128 + grp * 8, g.keys);
+          uint32_t kw[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int key = t0 + 32 * w + lane;
+            bool keep = __shfl_sync(0xffffffffu, now, 4 * w + (lane >> 3)) >= 0 && key < g.keys;
+            if (keep && a.mask)
+              keep = key < a.mask_len && load_keep(a.mask, a.mask_dtype, g.b * a.mask_stride + key);
+            kw[w] = __ballot_sync(0xffffffffu, keep);
+          }
+          // a scale of zero stands for zeros: kept above zero so that a masked -inf stays -inf
+          ks = fmaxf(ks, 1e-30f);
+          const uint32_t vmax = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.f)));
+          if (T >= kMetaRing &&
+              !__all_sync(0xffffffffu, mbar_wait(bar(T_ME + ms), ((T / kMetaRing) - 1) & 1, abort))) {
+            ok = false;
+            break;
+          }
+          if (lane < 16) {
+            meta[ms].ks[lane] = ks;
+            meta[ms].vs[lane] = vs;
+          }
+          if (lane == 0) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) meta[ms].keep[w] = kw[w];
+            meta[ms].vmax = __uint_as_float(vmax);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(T_MF + ms));
+        }
+      }
+    }
+  } else {
+    setmaxnreg_inc<C::RS>();
+    // ----------------------------------------------------------- softmax
+    const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const int gq = r / qt, i = r - gq * qt;
+    const float mult = (a.scale_dev ? *a.scale_dev : a.scale) * kLog2e;
+    int T = 0, act = 0, TX = 0;  // tiles of the CTA; segments and tiles of this row tile
+    int cont = -1, start = -1;
+    bool ok = true;
+    while (ok && next_segment<NX>(a, qt, sh, g)) {
+      const int unit = g.h * a.items + g.i;
+      const int nt = g.j1 - g.j0;
+      if (!g.whole) {
+        if (g.head) start = unit; else cont = unit;
+      }
+      if (x >= active(g)) {  // no tokens in this row tile: only pass the ring on
+        for (int j = 0; j < nt; ++j, ++T) {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(T_MF + T % kMetaRing), (T / kMetaRing) & 1, abort))) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive(bar(T_ME + T % kMetaRing));
+        }
+        continue;
+      }
+      const int s = (g.tile * NX + x) * qt + i;
+      const bool row_ok = gq < a.G && s < a.S;
+      const int pos = a.seq[g.b * a.seq_stride];
+      const int lim = a.causal ? (int)min((int64_t)pos + s + 1, (int64_t)g.keys) : g.keys;
+      const int first_lim = a.causal ? pos + (g.tile * NX + x) * qt + 1 : g.keys;  // of the tile's first token
+      float qmult = mult;
+      if (BF16 && row_ok) qmult *= q_undo[(((int64_t)g.b * a.Hkv + g.h) * a.G + gq) * a.S + s];
+      const float base = qmult > 0.f ? qmult : 1.f;
+      float m_run = neg_inf(), l_run = 0.f, vref = 0.f, inv_vref = 0.f;
+      for (int j = 0; j < nt; ++j, ++T, ++TX) {
+        const int ms = T % kMetaRing, t0 = (g.j0 + j) * 128;
+        const int sfb = NX == 2 ? x : (T & 1), sfp = NX == 2 ? TX & 1 : (T >> 1) & 1;
+        ok = mbar_wait(bar(T_MF + ms), (T / kMetaRing) & 1, abort) && mbar_wait(bar(T_SF + sfb), sfp, abort);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        __syncwarp();
+        float xv[128];
+        {
+          uint32_t r0[32], r1[32], r2[32], r3[32];
+          const uint32_t ts = t_s(x, T) + lane_off;
+          tmem_ld32(ts + 0, r0);
+          tmem_ld32(ts + 32, r1);
+          tmem_ld32(ts + 64, r2);
+          tmem_ld32(ts + 96, r3);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            xv[e] = __uint_as_float(r0[e]);
+            xv[32 + e] = __uint_as_float(r1[e]);
+            xv[64 + e] = __uint_as_float(r2[e]);
+            xv[96 + e] = __uint_as_float(r3[e]);
+          }
+        }
+        // a multiplier that is not positive would turn the order round: taken in first
+        if (!(qmult > 0.f)) {
+#pragma unroll
+          for (int e = 0; e < 128; e += 2) mul2(xv[e], xv[e + 1], qmult, qmult);
+        }
+        const uint4 kwv = *reinterpret_cast<const uint4*>(meta[ms].keep);
+        if ((kwv.x & kwv.y & kwv.z & kwv.w) != 0xffffffffu || t0 + 128 > first_lim) {
+          uint32_t kw[4] = {kwv.x, kwv.y, kwv.z, kwv.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int n = lim - (t0 + 32 * w);  // keys of the word before the row's limit
+            kw[w] &= n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+          }
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (!((kw[e >> 5] >> (e & 31)) & 1u)) xv[e] = neg_inf();
+        }
+        // maximum of the scaled scores: each group's raw maximum times its scale
+        float mt = neg_inf();
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const float4 ks = *reinterpret_cast<const float4*>(meta[ms].ks + 4 * q4);
+          const float k4[4] = {ks.x, ks.y, ks.z, ks.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float* p = xv + (4 * q4 + u) * 8;
+            const float mg = fmaxf(max3(max3(p[0], p[1], p[2]), p[3], p[4]), max3(p[5], p[6], p[7]));
+            mt = fmaxf(mt, mg * (k4[u] * base));
+          }
+        }
+        const float m_new = fmaxf(m_run, mt);
+        const bool grow = m_new > m_run + 8.f;
+        float factor = 1.f;
+        if (grow) {
+          factor = exp2_approx(m_run - m_new);
+          l_run *= factor;
+          m_run = m_new;
+        }
+        const float vm = meta[ms].vmax;
+        if (vm > vref) {  // the same for every row
+          const float now = pow2_above(vm);
+          inv_vref = 1.f / now;
+          factor *= vref * inv_vref;
+          vref = now;
+        }
+        if (j >= 1 && __any_sync(0xffffffffu, factor != 1.f)) {
+          // NX = 2: the scores come after PV(j - 1) in issue order; NX = 1: wait for it
+          if (NX == 1 && !__all_sync(0xffffffffu, mbar_wait(bar(T_PV), (T - 1) & 1, abort))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o(x) + lane_off + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st32(t_o(x) + lane_off + c * 32, o);
+          }
+          tmem_wait_st();
+        }
+        const float nmu = (m_run == neg_inf()) ? 0.f : -m_run;
+        float sa0 = 0.f, sa1 = 0.f, sb0 = 0.f, sb1 = 0.f;
+        uint32_t pk[64];
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const float4 ks = *reinterpret_cast<const float4*>(meta[ms].ks + 4 * q4);
+          const float4 vs = *reinterpret_cast<const float4*>(meta[ms].vs + 4 * q4);
+          const float k4[4] = {ks.x, ks.y, ks.z, ks.w}, v4[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            float* p = xv + (4 * q4 + u) * 8;
+            const float km = k4[u] * base, vr = v4[u] * inv_vref;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              fma2(p[e], p[e + 1], km, km, nmu, nmu);
+              p[e] = exp2_approx(p[e]);
+              p[e + 1] = exp2_approx(p[e + 1]);
+            }
+            add2(sa0, sa1, p[0], p[1]);
+            add2(sb0, sb1, p[2], p[3]);
+            add2(sa0, sa1, p[4], p[5]);
+            add2(sb0, sb1, p[6], p[7]);
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              mul2(p[e], p[e + 1], vr, vr);
+              pk[(4 * q4 + u) * 4 + e / 2] = pack2<false>(p[e], p[e + 1]);
+            }
+          }
+        }
+        l_run += (sa0 + sa1) + (sb0 + sb1);
+        __syncwarp();
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4)
+          tmem_st16(t_s(x, T) + lane_off + c4 * 16, *reinterpret_cast<const uint32_t(*)[16]>(pk + 16 * c4));
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(T_PF + x));
+          mbar_arrive(bar(T_ME + ms));
+        }
+      }
+      if (!ok) break;
+      if (nt > 0 && !__all_sync(0xffffffffu, mbar_wait(bar(T_O + x), act & 1, abort))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const float up = g.whole ? vref / l_run : vref;  // a row that sees no key: 0 / 0
+      const int64_t slot = ((int64_t)(2 * blockIdx.x + (g.head ? 1 : 0)) * NX + x) * 128 + r;
+      char* orow = a.out + g.b * a.os_b + g.h * a.os_h + gq * a.os_g + (int64_t)s * a.os_s;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (nt > 0) {
+          __syncwarp();
+          tmem_ld32(t_o(x) + lane_off + c * 32, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (!row_ok) continue;
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]) * up;
+        if (g.whole) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+            *reinterpret_cast<uint4*>(orow + (c * 32 + q4 * 8) * 2) =
+                make_uint4(pack2<BF16>(f[q4 * 8], f[q4 * 8 + 1]), pack2<BF16>(f[q4 * 8 + 2], f[q4 * 8 + 3]),
+                           pack2<BF16>(f[q4 * 8 + 4], f[q4 * 8 + 5]), pack2<BF16>(f[q4 * 8 + 6], f[q4 * 8 + 7]));
+        } else {
+#pragma unroll
+          for (int q4 = 0; q4 < 8; ++q4)
+            *reinterpret_cast<float4*>(a.part_o + slot * D + c * 32 + q4 * 4) =
+                make_float4(f[q4 * 4], f[q4 * 4 + 1], f[q4 * 4 + 2], f[q4 * 4 + 3]);
+        }
+      }
+      if (!g.whole && row_ok) a.part_ml[slot] = make_float2(m_run, l_run);
+      if (nt > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(T_OE + x));
+        ++act;
+      }
+    }
+    if (a.balanced && threadIdx.x == 0) {
+      a.desc[2 * blockIdx.x] = cont;
+      a.desc[2 * blockIdx.x + 1] = start;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort && threadIdx.x == 0 && a.err) atomicOr(a.err, RBLN_DEVERR_TIMEOUT);
+  if (warp == W0 + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// bf16 queries as f16 [B, Hkv, G, S, D] with a power of two of each row, and
+// the factors that undo it: D / 8 lanes a row.
+template <int D>
+__global__ void __launch_bounds__(256) query_f16_kernel(const Fp8Args a, char* qh, float* undo) {
+  dependents_enter();
+  constexpr int LPR = D / 8;
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  const int c = threadIdx.x % LPR;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.G * a.S;
+  const bool in = row < rows;
+  uint4 w = make_uint4(0, 0, 0, 0);
+  if (in) {
+    const int s = (int)(row % a.S);
+    int64_t t = row / a.S;
+    const int g = (int)(t % a.G);
+    t /= a.G;
+    const int h = (int)(t % a.Hkv), b = (int)(t / a.Hkv);
+    w = *reinterpret_cast<const uint4*>(a.q + b * a.qs_b + h * a.qs_h + g * a.qs_g + (int64_t)s * a.qs_s + c * 16);
+  }
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  float m = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = unpack2<true>(u[k]);
+    m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+  }
+#pragma unroll
+  for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float down;
+  const float up = f16_factor(m, down);
+  uint32_t v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = unpack2<true>(u[k]);
+    v[k] = pack2<false>(f.x * up, f.y * up);
+  }
+  if (!in) return;
+  *reinterpret_cast<uint4*>(qh + row * D * 2 + c * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+  if (c == 0) undo[row] = down;
 }
 
 // Joins the partial results of the units that several CTAs share. CTA (c, y):
@@ -592,12 +1355,14 @@ __global__ void __launch_bounds__(256) paged_attn_fp8_merge_kernel(const Fp8Args
 // host side
 // ---------------------------------------------------------------------------
 struct Fp8Plan {
+  int nx;       // row tiles of 128 of the tile kernel; 0: the row kernel
   int nt;       // 8-column groups of the row kernel
-  int rows;     // rows of a row tile
+  int qt;       // tokens of a 128-row tile
+  int rows;     // rows of a unit
   int tiles, items;
   bool balanced;
   int ctas;
-  size_t desc, ml, o, total;  // workspace regions
+  size_t desc, ml, o, qh, undo, total;  // workspace regions
 };
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
@@ -605,18 +1370,23 @@ size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 int plan_fp8(const rbln_paged_attn_params_t* p, Fp8Plan* pl) {
   const int64_t span = (int64_t)p->max_blocks * p->block_size;
   const int64_t rows = (int64_t)p->q_len * p->group;
+  // Up to 16 rows of a KV head the row kernel reads the codes once; more
+  // rows would read them again for each 16, so they go to 128-row tiles.
+  pl->nx = rows <= 16 ? 0 : rows <= 128 ? 1 : 2;
   pl->nt = rows <= 8 ? 1 : 2;
-  pl->rows = 8 * pl->nt;
-  const int64_t tiles = (rows + pl->rows - 1) / pl->rows;
+  pl->qt = 128 / p->group;
+  pl->rows = pl->nx ? 128 * pl->nx : 8 * pl->nt;
+  const int64_t tiles = pl->nx ? (p->q_len + (int64_t)pl->nx * pl->qt - 1) / (pl->nx * pl->qt)
+                               : (rows + pl->rows - 1) / pl->rows;
   if (tiles * p->batch * p->num_kv_heads > INT32_MAX) return RBLN_ERR_UNSUPPORTED;
   pl->tiles = (int)tiles;
   pl->items = (int)(tiles * p->batch);
-  const int64_t slots = 148LL * (pl->nt == 1 ? 4 : 2);
+  const int64_t slots = pl->nx ? 148LL : 148LL * (pl->nt == 1 ? 4 : 2);
   // the prefix fits shared memory and counts in 32 bits; with more items than
   // that there are enough whole units for every CTA
   pl->balanced = pl->items <= kMaxItems && (int64_t)pl->items * (span + 16 + kSegCost) < INT32_MAX;
   const int64_t units = (int64_t)pl->items * p->num_kv_heads;
-  pl->ctas = (int)(pl->balanced ? slots : std::min<int64_t>(units, slots * 8));
+  pl->ctas = (int)(pl->balanced ? slots : std::min<int64_t>(units, pl->nx ? slots : slots * 8));
   size_t off = 0;
   if (pl->balanced) {
     pl->desc = off;
@@ -626,12 +1396,19 @@ int plan_fp8(const rbln_paged_attn_params_t* p, Fp8Plan* pl) {
     pl->o = off;
     off += round256((size_t)2 * pl->ctas * pl->rows * p->head_dim * sizeof(float));
   }
+  if (pl->nx && p->q_dtype == RBLN_DT_BF16) {
+    const size_t n = (size_t)p->batch * p->num_kv_heads * rows;
+    pl->qh = off;
+    off += round256(n * p->head_dim * 2);
+    pl->undo = off;
+    off += round256(n * sizeof(float));
+  }
   pl->total = off ? off + 256 : 0;
   return RBLN_OK;
 }
 
-template <typename... A>
-int launch_after(void (*kernel)(A...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+template <typename... A, typename... B>
+int launch_after(void (*kernel)(A...), dim3 grid, int threads, size_t smem, cudaStream_t st, const B&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -642,7 +1419,7 @@ int launch_after(void (*kernel)(A...), dim3 grid, int threads, size_t smem, cuda
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<A>(args)...) == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
 }
 
 template <int D, bool BF16, int NT>
@@ -657,8 +1434,71 @@ int launch_rows(const Fp8Args& a, const Fp8Plan& pl, cudaStream_t st) {
   return launch_after(paged_attn_fp8_merge_kernel<D, BF16, 8 * NT, 4>, dim3(pl.ctas, 2 * NT), 256, 0, st, a, pl.ctas, 0);
 }
 
+// cache [NB, Hkv, bs, D] of codes -> 4-D map of bytes, box {D, rpb, 1, 1}, not swizzled
+bool map_codes(CUtensorMap* m, const rbln_paged_attn_params_t* p, const void* cache) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->block_size, (cuuint64_t)p->num_kv_heads,
+                              (cuuint64_t)p->num_blocks};
+  const cuuint64_t str[3] = {(cuuint64_t)p->cache_stride[2], (cuuint64_t)p->cache_stride[1],
+                             (cuuint64_t)p->cache_stride[0]};
+  const cuuint32_t box[4] = {(cuuint32_t)p->head_dim, (cuuint32_t)std::min(p->block_size, 128), 1, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(cache), dims, str, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16, int NX>
+int launch_tiles(const rbln_paged_attn_params_t* p, const Fp8Args& a, const Fp8Plan& pl, char* base, cudaStream_t st) {
+  using L = TcSmem<D, NX>;
+  using C = TcCfg<NX>;
+  auto kernel = paged_attn_fp8_tiles_kernel<D, BF16, NX>;
+  // the register split assumes the launch's count; with fewer a warpgroup
+  // that raises its own would never be served
+  static const bool regs_ok = [kernel] {
+    cudaFuncAttributes fa{};
+    return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess &&
+           128 * (NX * C::RS + C::RC + C::RV) <= (uint32_t)fa.numRegs * C::THREADS;
+  }();
+  if (!regs_ok) return RBLN_ERR_LAUNCH;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC) != cudaSuccess)
+    return RBLN_ERR_LAUNCH;
+  CUtensorMap tq, tk, tv;
+  if (!map_codes(&tk, p, p->kcache) || !map_codes(&tv, p, p->vcache)) return RBLN_ERR_LAUNCH;
+  const void* q = p->q;
+  int64_t qs[4] = {p->q_stride[0], p->q_stride[1], p->q_stride[2], p->q_stride[3]};
+  float* undo = nullptr;
+  if (BF16) {
+    char* qh = base + pl.qh;
+    undo = reinterpret_cast<float*>(base + pl.undo);
+    const int64_t rows = (int64_t)a.B * a.Hkv * a.G * a.S;
+    const int64_t grid = (rows * (D / 8) + 255) / 256;
+    if (grid > INT32_MAX) return RBLN_ERR_UNSUPPORTED;
+    const int rc = launch_after(query_f16_kernel<D>, dim3((unsigned)grid), 256, 0, st, a, qh, undo);
+    if (rc != RBLN_OK) return rc;
+    q = qh;
+    qs[3] = D;
+    qs[2] = (int64_t)a.S * D;
+    qs[1] = a.G * qs[2];
+    qs[0] = a.Hkv * qs[1];
+  }
+  {  // [B, Hkv, G, S, D] -> 5-D map, box {64, QT, G, 1, 1}
+    const uint64_t dims[5] = {(uint64_t)D, (uint64_t)a.S, (uint64_t)a.G, (uint64_t)a.Hkv, (uint64_t)a.B};
+    const uint64_t str[4] = {(uint64_t)qs[3] * 2, (uint64_t)qs[2] * 2, (uint64_t)qs[1] * 2, (uint64_t)qs[0] * 2};
+    const uint32_t box[5] = {64, (uint32_t)pl.qt, (uint32_t)a.G, 1, 1};
+    if (!make_map(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(q), dims, str, box)) return RBLN_ERR_LAUNCH;
+  }
+  int rc = launch_after(kernel, dim3(pl.ctas), C::THREADS, L::ALLOC, st, tq, tk, tv, a, pl.qt, (const float*)undo);
+  if (rc != RBLN_OK || !pl.balanced) return rc;
+  return launch_after(paged_attn_fp8_merge_kernel<D, BF16, 128 * NX, 8>, dim3(pl.ctas, 16 * NX), 256, 0, st, a, pl.ctas,
+                      pl.qt);
+}
+
 template <int D, bool BF16>
-int launch_fp8(const Fp8Args& a, const Fp8Plan& pl, cudaStream_t st) {
+int launch_fp8(const rbln_paged_attn_params_t* p, const Fp8Args& a, const Fp8Plan& pl, char* base, cudaStream_t st) {
+  if (pl.nx == 2) return launch_tiles<D, BF16, 2>(p, a, pl, base, st);
+  if (pl.nx == 1) return launch_tiles<D, BF16, 1>(p, a, pl, base, st);
   return pl.nt == 1 ? launch_rows<D, BF16, 1>(a, pl, st) : launch_rows<D, BF16, 2>(a, pl, st);
 }
 
@@ -732,8 +1572,8 @@ int run_prefill_fp8(const rbln_paged_attn_params_t* p, cudaStream_t st) {
   a.causal = p->causal;
   a.tiles = pl.tiles; a.items = pl.items;
   a.balanced = pl.balanced;
+  char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p->workspace) + 255) & ~uintptr_t(255));
   if (pl.balanced) {
-    char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p->workspace) + 255) & ~uintptr_t(255));
     a.desc = reinterpret_cast<int*>(base + pl.desc);
     a.part_ml = reinterpret_cast<float2*>(base + pl.ml);
     a.part_o = reinterpret_cast<float*>(base + pl.o);
@@ -741,8 +1581,10 @@ int run_prefill_fp8(const rbln_paged_attn_params_t* p, cudaStream_t st) {
   a.err = p->error_flags;
   if (p->prof_events[0]) cudaEventRecord(static_cast<cudaEvent_t>(p->prof_events[0]), st);
   const bool bf = p->q_dtype == RBLN_DT_BF16;
-  if (p->head_dim == 128) rc = bf ? launch_fp8<128, true>(a, pl, st) : launch_fp8<128, false>(a, pl, st);
-  else rc = bf ? launch_fp8<64, true>(a, pl, st) : launch_fp8<64, false>(a, pl, st);
+  if (p->head_dim == 128)
+    rc = bf ? launch_fp8<128, true>(p, a, pl, base, st) : launch_fp8<128, false>(p, a, pl, base, st);
+  else
+    rc = bf ? launch_fp8<64, true>(p, a, pl, base, st) : launch_fp8<64, false>(p, a, pl, base, st);
   if (p->prof_events[1]) cudaEventRecord(static_cast<cudaEvent_t>(p->prof_events[1]), st);
   return rc;
 }
