@@ -523,6 +523,26 @@ __global__ void __launch_bounds__(kMqThreads, NT == 1 ? 4 : 2) paged_attn_fp8_ro
 // ---------------------------------------------------------------------------
 using namespace sm100;
 
+// sm100's bounded wait with a time for the hardware to suspend the warp in:
+// two dozen warps that poll take issue slots from those at work.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort) {
+  const long long t0 = clock64();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(100000u)  // nanoseconds
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+    if (clock64() - t0 > kWaitLimitCycles) {
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
 constexpr int kPanel = 128 * 128;  // 128 rows of 64 f16
 constexpr int kTcSegCost = 2;      // key tiles charged to a unit's start
 constexpr int kMetaRing = 4;
@@ -557,7 +577,7 @@ struct TcCfg {
   static constexpr int THREADS = 128 * NX + 256;
   // registers a thread after the split: softmax, control, convert. The
   // launch has 128 (512 threads) or 168 (384 threads) each.
-  static constexpr uint32_t RS = NX == 2 ? 200 : 216, RC = NX == 2 ? 48 : 64, RV = NX == 2 ? 64 : 104;
+  static constexpr uint32_t RS = NX == 2 ? 152 : 216, RC = NX == 2 ? 96 : 64, RV = NX == 2 ? 112 : 104;
   static constexpr uint32_t LAUNCH = NX == 2 ? 128 : 168;
   static_assert(128 * (NX * RS + RC + RV) <= THREADS * LAUNCH, "register split exceeds the launch");
 };
@@ -575,6 +595,21 @@ enum TcBar {
   T_OE = 33,   // O read
   T_DONE = 35, T_COUNT = 36
 };
+
+// What a group's raw scores are multiplied by, above zero also where a scale
+// is zero, so that -inf stays -inf.
+__device__ __forceinline__ float score_mult(float ks, float mult) { return fmaxf(ks * mult, 1.2e-38f); }
+
+// Eight f16 that stand for codes as bf16, exact: a code has four bits.
+__device__ __forceinline__ uint4 f16_to_bf16(uint4 w) {
+  uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<false>(u[i]);
+    u[i] = pack2<true>(f.x, f.y);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
 
 // A CTA's share as every role walks it: `left` positions from position `off`
 // of unit (h, i) on; each unit has kTcSegCost positions and then one a key tile.
@@ -638,8 +673,7 @@ __device__ __forceinline__ int block_of(const Fp8Args& a, int b, int key, int ke
 template <int D, bool BF16, int NX>
 __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
     paged_attn_fp8_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                                const __grid_constant__ CUtensorMap tm_v, const Fp8Args a, const int qt,
-                                const float* q_undo) {
+                                const __grid_constant__ CUtensorMap tm_v, const Fp8Args a, const int qt) {
   using L = TcSmem<D, NX>;
   using C = TcCfg<NX>;
   constexpr int NP = L::NP, NRAW = L::NRAW;
@@ -728,52 +762,61 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
     constexpr int STEPS = 128 / (4 * RPI);
     const int c16 = lane % LPR;
     const uint32_t dst_panel = (uint32_t)(c16 >> 2) * kPanel;
-    const int chunk = 2 * (c16 & 3);
-    // the upper panel's lanes store their chunks in the other order, so that
-    // eight lanes of one row cover all banks
-    const int swap = (D == 128) ? (c16 >> 2) : 0;
+    const int row0 = cw * RPI + lane / LPR;  // first row; then every 4 RPI-th, of the same swizzle
+    // The upper panel's lanes take their two chunks in the other order, so
+    // that eight lanes of one row cover all banks.
+    const int swap = (D == 128 && c16 >= 4) ? 8 : 0;
+    const int chunk = 2 * (c16 & 3) + swap / 8;
+    const int x0 = (chunk ^ (row0 & 7)) * 16, x1 = ((chunk ^ 1) ^ (row0 & 7)) * 16;
+    // a negative softmax scale turns the order of the scores round: its sign goes into the keys
+    const uint32_t flip = (a.scale_dev ? *a.scale_dev : a.scale) < 0.f ? 0x80808080u : 0u;
     int T = 0;
     bool ok = true;
     while (ok && next_segment<NX>(a, qt, sh, g)) {
       for (int j = g.j0; ok && j < g.j1; ++j, ++T) {
         const int ms = T % kMetaRing;
         uint32_t kw[4];
-#pragma unroll
+#pragma unroll 1
         for (int part = 0; part < 2; ++part) {
           const int n = 2 * T + part, rs = n % NRAW, st = T & 1;
           const int full = (part ? T_VF : T_KF) + st, empty = (part ? T_VE : T_KE) + st;
-          ok = mbar_wait(bar(T_RF + rs), (n / NRAW) & 1, abort);
-          if (ok && T >= 2) ok = mbar_wait(bar(empty), ((T >> 1) - 1) & 1, abort);
+          ok = wait_for(bar(T_RF + rs), (n / NRAW) & 1, abort);
+          if (ok && T >= 2) ok = wait_for(bar(empty), ((T >> 1) - 1) & 1, abort);
           bool all = true;
           if (part == 1 && ok) {
-            ok = mbar_wait(bar(T_MF + ms), (T / kMetaRing) & 1, abort);
+            ok = wait_for(bar(T_MF + ms), (T / kMetaRing) & 1, abort);
             const uint4 k = *reinterpret_cast<const uint4*>(meta[ms].keep);
             kw[0] = k.x; kw[1] = k.y; kw[2] = k.z; kw[3] = k.w;
             all = (k.x & k.y & k.z & k.w) == 0xffffffffu;
           }
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const uint8_t* raw = sgen + L::R0 + rs * L::RAW;
-          uint8_t* dst = sgen + (part ? L::V0 : L::K0) + st * L::TILE + dst_panel;
-          // unroll 4: four 16-byte loads in flight a lane
+          const uint32_t turn = part == 0 ? flip : 0u;
+          const uint8_t* src = sgen + L::R0 + rs * L::RAW + row0 * D + c16 * 16;
+          uint8_t* dst = sgen + (part ? L::V0 : L::K0) + st * L::TILE + row0 * 128 + dst_panel;
 #pragma unroll 4
           for (int k = 0; k < STEPS; ++k) {
-            const int r = (k * 4 + cw) * RPI + lane / LPR;
-            uint4 w = *reinterpret_cast<const uint4*>(raw + r * D + c16 * 16);
-            if (part == 1 && !all) {
-              // 0 x NaN would reach every row's sum: what no query may see is zeros
-              const uint32_t word = r < 64 ? (r < 32 ? kw[0] : kw[1]) : (r < 96 ? kw[2] : kw[3]);
-              if (!((word >> (r & 31)) & 1u)) w = make_uint4(0, 0, 0, 0);
+            uint2 w0 = *reinterpret_cast<const uint2*>(src + k * 4 * RPI * D + swap);
+            uint2 w1 = *reinterpret_cast<const uint2*>(src + k * 4 * RPI * D + 8 - swap);
+            if (turn) {
+              w0.x ^= turn; w0.y ^= turn; w1.x ^= turn; w1.y ^= turn;
             }
-            uint4 lo, hi;
-            e4m3x4_to_f16x2x2(w.x, lo.x, lo.y);
-            e4m3x4_to_f16x2x2(w.y, lo.z, lo.w);
-            e4m3x4_to_f16x2x2(w.z, hi.x, hi.y);
-            e4m3x4_to_f16x2x2(w.w, hi.z, hi.w);
-            uint8_t* row = dst + r * 128;
-            const int x0 = (chunk + swap) ^ (r & 7), x1 = (chunk + 1 - swap) ^ (r & 7);
-            *reinterpret_cast<uint4*>(row + x0 * 16) = swap ? hi : lo;
-            *reinterpret_cast<uint4*>(row + x1 * 16) = swap ? lo : hi;
+            if (!all) {
+              const int r = row0 + k * 4 * RPI;
+              const uint32_t word = r < 64 ? (r < 32 ? kw[0] : kw[1]) : (r < 96 ? kw[2] : kw[3]);
+              if (!((word >> (r & 31)) & 1u)) w0 = w1 = make_uint2(0, 0);
+            }
+            uint4 o0, o1;
+            e4m3x4_to_f16x2x2(w0.x, o0.x, o0.y);
+            e4m3x4_to_f16x2x2(w0.y, o0.z, o0.w);
+            e4m3x4_to_f16x2x2(w1.x, o1.x, o1.y);
+            e4m3x4_to_f16x2x2(w1.y, o1.z, o1.w);
+            if (BF16 && part == 0) {
+              o0 = f16_to_bf16(o0);
+              o1 = f16_to_bf16(o1);
+            }
+            *reinterpret_cast<uint4*>(dst + k * 4 * RPI * 128 + x0) = o0;
+            *reinterpret_cast<uint4*>(dst + k * 4 * RPI * 128 + x1) = o1;
           }
           fence_proxy_async_smem();  // read by the MMA; and the raw slot is rewritten by TMA
           __syncwarp();
@@ -808,7 +851,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
             const int n = 2 * T + part, rs = n % NRAW;
-            if (n >= NRAW && !__all_sync(0xffffffffu, mbar_wait(bar(T_RE + rs), ((n / NRAW) - 1) & 1, abort))) {
+            if (n >= NRAW && !__all_sync(0xffffffffu, wait_for(bar(T_RE + rs), ((n / NRAW) - 1) & 1, abort))) {
               ok = false;
               break;
             }
@@ -821,7 +864,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           }
           if (ok && j == g.j0) {
             // Q behind the first codes: the previous segment's QKs must be done
-            if (act >= 1 && !__all_sync(0xffffffffu, mbar_wait(bar(T_QE), (act - 1) & 1, abort))) {
+            if (act >= 1 && !__all_sync(0xffffffffu, wait_for(bar(T_QE), (act - 1) & 1, abort))) {
               ok = false;
               break;
             }
@@ -849,36 +892,40 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
     } else if (warp == W0 + 1) {
       // ------------------------------------------------------------- MMA
       if (lane == 0) {
-        const uint32_t id_qk = idesc_f16(false, 128, 128, false);
+        const uint32_t id_qk = idesc_f16(BF16, 128, 128, false);
         const uint32_t id_pv = idesc_f16(false, 128, D, true);
         int T = 0, act = 0, actx[2] = {0, 0}, segx[2] = {0, 0};  // tiles, segments; of each row tile
         bool ok = true;
+        // A descriptor's address field counts 16-byte units and no operand
+        // passes its 14 bits, so an offset within shared memory is one add.
+        const uint32_t hi = (uint32_t)(sw128_desc(0, 16, 1024) >> 32);
+        const uint32_t lo_k = (uint32_t)sw128_desc(sbase, 16, 1024), lo_v = (uint32_t)sw128_desc(sbase, kPanel, 1024);
+        auto desc = [&](uint32_t lo) { return ((uint64_t)hi << 32) | lo; };
         auto qk = [&](int x, int Tj) {
-          const uint32_t qb = sbase + L::Q + x * L::TILE, kb = sbase + L::K0 + (Tj & 1) * L::TILE;
+          const uint32_t qb = lo_k + (L::Q + x * L::TILE) / 16, kb = lo_k + (L::K0 + (Tj & 1) * L::TILE) / 16;
+          const uint32_t to = t_s(x, Tj);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t ad = sw128_desc(qb + (kk >> 2) * kPanel + (kk & 3) * 32, 16, 1024);
-            const uint64_t bd = sw128_desc(kb + (kk >> 2) * kPanel + (kk & 3) * 32, 16, 1024);
-            umma_f16_ss(t_s(x, Tj), ad, bd, id_qk, kk > 0 ? 1u : 0u);
+            const uint32_t off = ((kk >> 2) * kPanel + (kk & 3) * 32) / 16;
+            umma_f16_ss(to, desc(qb + off), desc(kb + off), id_qk, kk > 0 ? 1u : 0u);
           }
           umma_commit(bar(T_SF + (NX == 2 ? x : (Tj & 1))));
         };
         auto pv = [&](int x, int Tj, bool first) {
-          const uint32_t vb = sbase + L::V0 + (Tj & 1) * L::TILE;
+          const uint32_t vb = lo_v + (L::V0 + (Tj & 1) * L::TILE) / 16;
+          const uint32_t to = t_o(x), from = t_s(x, Tj);
+          umma_f16_ts(to, from, desc(vb), id_pv, first ? 0u : 1u);
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t bd = sw128_desc(vb + kk * 16 * 128, kPanel, 1024);
-            umma_f16_ts(t_o(x), t_s(x, Tj) + kk * 8, bd, id_pv, (!first || kk > 0) ? 1u : 0u);
-          }
+          for (int kk = 1; kk < 8; ++kk) umma_f16_ts(to, from + kk * 8, desc(vb + kk * 16 * 128 / 16), id_pv, 1u);
         };
         while (ok && next_segment<NX>(a, qt, sh, g)) {
           const int nt = g.j1 - g.j0;
           if (nt == 0) continue;
           const int nx = active(g);
-          ok = mbar_wait(bar(T_QF), act & 1, abort);
+          ok = wait_for(bar(T_QF), act & 1, abort);
           for (int j = 0; ok && j <= nt; ++j) {
             const int Tj = T + j;
-            if (j < nt && !mbar_wait(bar(T_KF + (Tj & 1)), (Tj >> 1) & 1, abort)) {
+            if (j < nt && !wait_for(bar(T_KF + (Tj & 1)), (Tj >> 1) & 1, abort)) {
               ok = false;
               break;
             }
@@ -890,7 +937,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
                 if (j == nt - 1) umma_commit(bar(T_QE));
               }
             }
-            if (j >= 1 && !mbar_wait(bar(T_VF + ((Tj - 1) & 1)), ((Tj - 1) >> 1) & 1, abort)) {
+            if (j >= 1 && !wait_for(bar(T_VF + ((Tj - 1) & 1)), ((Tj - 1) >> 1) & 1, abort)) {
               ok = false;
               break;
             }
@@ -898,8 +945,8 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
               if (j >= 1) {
                 // the row tile's P; its first PV overwrites O once the last segment's is read
                 const int ph = NX == 2 ? actx[x] + j - 1 : Tj - 1;
-                if (!mbar_wait(bar(T_PF + x), ph & 1, abort) ||
-                    (j == 1 && segx[x] >= 1 && !mbar_wait(bar(T_OE + x), (segx[x] - 1) & 1, abort))) {
+                if (!wait_for(bar(T_PF + x), ph & 1, abort) ||
+                    (j == 1 && segx[x] >= 1 && !wait_for(bar(T_OE + x), (segx[x] - 1) & 1, abort))) {
                   ok = false;
                   break;
                 }
@@ -960,11 +1007,9 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
               keep = key < a.mask_len && load_keep(a.mask, a.mask_dtype, g.b * a.mask_stride + key);
             kw[w] = __ballot_sync(0xffffffffu, keep);
           }
-          // a scale of zero stands for zeros: kept above zero so that a masked -inf stays -inf
-          ks = fmaxf(ks, 1e-30f);
           const uint32_t vmax = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.f)));
           if (T >= kMetaRing &&
-              !__all_sync(0xffffffffu, mbar_wait(bar(T_ME + ms), ((T / kMetaRing) - 1) & 1, abort))) {
+              !__all_sync(0xffffffffu, wait_for(bar(T_ME + ms), ((T / kMetaRing) - 1) & 1, abort))) {
             ok = false;
             break;
           }
@@ -988,7 +1033,8 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
     const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const int gq = r / qt, i = r - gq * qt;
-    const float mult = (a.scale_dev ? *a.scale_dev : a.scale) * kLog2e;
+    // the sign of a negative softmax scale is in the converted keys
+    const float mult = fabsf(a.scale_dev ? *a.scale_dev : a.scale) * kLog2e;
     int T = 0, act = 0, TX = 0;  // tiles of the CTA; segments and tiles of this row tile
     int cont = -1, start = -1;
     bool ok = true;
@@ -1000,7 +1046,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
       }
       if (x >= active(g)) {  // no tokens in this row tile: only pass the ring on
         for (int j = 0; j < nt; ++j, ++T) {
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(T_MF + T % kMetaRing), (T / kMetaRing) & 1, abort))) {
+          if (!__all_sync(0xffffffffu, wait_for(bar(T_MF + T % kMetaRing), (T / kMetaRing) & 1, abort))) {
             ok = false;
             break;
           }
@@ -1013,66 +1059,64 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
       const int pos = a.seq[g.b * a.seq_stride];
       const int lim = a.causal ? (int)min((int64_t)pos + s + 1, (int64_t)g.keys) : g.keys;
       const int first_lim = a.causal ? pos + (g.tile * NX + x) * qt + 1 : g.keys;  // of the tile's first token
-      float qmult = mult;
-      if (BF16 && row_ok) qmult *= q_undo[(((int64_t)g.b * a.Hkv + g.h) * a.G + gq) * a.S + s];
-      const float base = qmult > 0.f ? qmult : 1.f;
       float m_run = neg_inf(), l_run = 0.f, vref = 0.f, inv_vref = 0.f;
       for (int j = 0; j < nt; ++j, ++T, ++TX) {
         const int ms = T % kMetaRing, t0 = (g.j0 + j) * 128;
         const int sfb = NX == 2 ? x : (T & 1), sfp = NX == 2 ? TX & 1 : (T >> 1) & 1;
-        ok = mbar_wait(bar(T_MF + ms), (T / kMetaRing) & 1, abort) && mbar_wait(bar(T_SF + sfb), sfp, abort);
+        ok = wait_for(bar(T_MF + ms), (T / kMetaRing) & 1, abort) && wait_for(bar(T_SF + sfb), sfp, abort);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
         __syncwarp();
-        float xv[128];
-        {
-          uint32_t r0[32], r1[32], r2[32], r3[32];
-          const uint32_t ts = t_s(x, T) + lane_off;
-          tmem_ld32(ts + 0, r0);
-          tmem_ld32(ts + 32, r1);
-          tmem_ld32(ts + 64, r2);
-          tmem_ld32(ts + 96, r3);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            xv[e] = __uint_as_float(r0[e]);
-            xv[32 + e] = __uint_as_float(r1[e]);
-            xv[64 + e] = __uint_as_float(r2[e]);
-            xv[96 + e] = __uint_as_float(r3[e]);
-          }
-        }
-        // a multiplier that is not positive would turn the order round: taken in first
-        if (!(qmult > 0.f)) {
-#pragma unroll
-          for (int e = 0; e < 128; e += 2) mul2(xv[e], xv[e + 1], qmult, qmult);
-        }
+        // Two passes over the row's 128 scores, 32 at a time in rolled loops:
+        // the roles share one instruction cache, and the code of a whole row
+        // unrolled, masks in it, took three times as long, waiting for
+        // instructions.
+        const uint32_t ts = t_s(x, T) + lane_off;
+        uint32_t v[32];
+        float* const p = reinterpret_cast<float*>(v);
         const uint4 kwv = *reinterpret_cast<const uint4*>(meta[ms].keep);
         if ((kwv.x & kwv.y & kwv.z & kwv.w) != 0xffffffffu || t0 + 128 > first_lim) {
-          uint32_t kw[4] = {kwv.x, kwv.y, kwv.z, kwv.w};
+          // some key is not for some row: -inf over those scores first
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const int n = lim - (t0 + 32 * c);  // keys of the chunk before the row's limit
+            const uint32_t kw = meta[ms].keep[c] & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u);
+            tmem_ld32(ts + c * 32, v);
+            tmem_wait_ld32(v);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int n = lim - (t0 + 32 * w);  // keys of the word before the row's limit
-            kw[w] &= n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+            for (int e = 0; e < 32; ++e)
+              if (!((kw >> e) & 1u)) v[e] = 0xff800000u;
+            tmem_st32(ts + c * 32, v);
           }
-#pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (!((kw[e >> 5] >> (e & 31)) & 1u)) xv[e] = neg_inf();
+          tmem_wait_st();
         }
         // maximum of the scaled scores: each group's raw maximum times its scale
         float mt = neg_inf();
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const float4 ks = *reinterpret_cast<const float4*>(meta[ms].ks + 4 * q4);
+        uint32_t v2[32];
+        auto max_of = [&](int c, const uint32_t (&r)[32]) {
+          const float* q = reinterpret_cast<const float*>(r);
+          const float4 ks = *reinterpret_cast<const float4*>(meta[ms].ks + 4 * c);
           const float k4[4] = {ks.x, ks.y, ks.z, ks.w};
+          float mg[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float* p = xv + (4 * q4 + u) * 8;
-            const float mg = fmaxf(max3(max3(p[0], p[1], p[2]), p[3], p[4]), max3(p[5], p[6], p[7]));
-            mt = fmaxf(mt, mg * (k4[u] * base));
+            const float* w = q + u * 8;
+            mg[u] = fmaxf(max3(max3(w[0], w[1], w[2]), w[3], w[4]), max3(w[5], w[6], w[7])) * score_mult(k4[u], mult);
           }
+          mt = fmaxf(mt, max3(mg[0], mg[1], fmaxf(mg[2], mg[3])));
+        };
+        tmem_ld32(ts, v);
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_wait_ld32(v);
+          tmem_ld32(ts + c * 32 + 32, v2);
+          max_of(c, v);
+          tmem_wait_ld32(v2);
+          if (c == 0) tmem_ld32(ts + 64, v);
+          max_of(c + 1, v2);
         }
         const float m_new = fmaxf(m_run, mt);
         const bool grow = m_new > m_run + 8.f;
@@ -1091,7 +1135,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
         }
         if (j >= 1 && __any_sync(0xffffffffu, factor != 1.f)) {
           // NX = 2: the scores come after PV(j - 1) in issue order; NX = 1: wait for it
-          if (NX == 1 && !__all_sync(0xffffffffu, mbar_wait(bar(T_PV), (T - 1) & 1, abort))) {
+          if (NX == 1 && !__all_sync(0xffffffffu, wait_for(bar(T_PV), (T - 1) & 1, abort))) {
             ok = false;
             break;
           }
@@ -1110,38 +1154,37 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
         }
         const float nmu = (m_run == neg_inf()) ? 0.f : -m_run;
         float sa0 = 0.f, sa1 = 0.f, sb0 = 0.f, sb1 = 0.f;
-        uint32_t pk[64];
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const float4 ks = *reinterpret_cast<const float4*>(meta[ms].ks + 4 * q4);
-          const float4 vs = *reinterpret_cast<const float4*>(meta[ms].vs + 4 * q4);
+        // P of a chunk is 16 columns of f16 pairs over scores that are done with
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld32(ts + c * 32, v);
+          const float4 ks = *reinterpret_cast<const float4*>(meta[ms].ks + 4 * c);
+          const float4 vs = *reinterpret_cast<const float4*>(meta[ms].vs + 4 * c);
           const float k4[4] = {ks.x, ks.y, ks.z, ks.w}, v4[4] = {vs.x, vs.y, vs.z, vs.w};
+          uint32_t pk[16];
+          tmem_wait_ld32(v);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            float* p = xv + (4 * q4 + u) * 8;
-            const float km = k4[u] * base, vr = v4[u] * inv_vref;
+            const float km = score_mult(k4[u], mult), vr = v4[u] * inv_vref;
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
+            for (int e = 8 * u; e < 8 * u + 8; e += 2) {
               fma2(p[e], p[e + 1], km, km, nmu, nmu);
               p[e] = exp2_approx(p[e]);
               p[e + 1] = exp2_approx(p[e + 1]);
             }
-            add2(sa0, sa1, p[0], p[1]);
-            add2(sb0, sb1, p[2], p[3]);
-            add2(sa0, sa1, p[4], p[5]);
-            add2(sb0, sb1, p[6], p[7]);
+            add2(sa0, sa1, p[8 * u], p[8 * u + 1]);
+            add2(sb0, sb1, p[8 * u + 2], p[8 * u + 3]);
+            add2(sa0, sa1, p[8 * u + 4], p[8 * u + 5]);
+            add2(sb0, sb1, p[8 * u + 6], p[8 * u + 7]);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
+            for (int e = 8 * u; e < 8 * u + 8; e += 2) {
               mul2(p[e], p[e + 1], vr, vr);
-              pk[(4 * q4 + u) * 4 + e / 2] = pack2<false>(p[e], p[e + 1]);
+              pk[e / 2] = pack2<false>(p[e], p[e + 1]);
             }
           }
+          tmem_st16(ts + c * 16, pk);
         }
         l_run += (sa0 + sa1) + (sb0 + sb1);
-        __syncwarp();
-#pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4)
-          tmem_st16(t_s(x, T) + lane_off + c4 * 16, *reinterpret_cast<const uint32_t(*)[16]>(pk + 16 * c4));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -1151,7 +1194,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
         }
       }
       if (!ok) break;
-      if (nt > 0 && !__all_sync(0xffffffffu, mbar_wait(bar(T_O + x), act & 1, abort))) {
+      if (nt > 0 && !__all_sync(0xffffffffu, wait_for(bar(T_O + x), act & 1, abort))) {
         ok = false;
         break;
       }
@@ -1210,54 +1253,16 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
   }
 }
 
-// bf16 queries as f16 [B, Hkv, G, S, D] with a power of two of each row, and
-// the factors that undo it: D / 8 lanes a row.
-template <int D>
-__global__ void __launch_bounds__(256) query_f16_kernel(const Fp8Args a, char* qh, float* undo) {
-  dependents_enter();
-  constexpr int LPR = D / 8;
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
-  const int c = threadIdx.x % LPR;
-  const int64_t rows = (int64_t)a.B * a.Hkv * a.G * a.S;
-  const bool in = row < rows;
-  uint4 w = make_uint4(0, 0, 0, 0);
-  if (in) {
-    const int s = (int)(row % a.S);
-    int64_t t = row / a.S;
-    const int g = (int)(t % a.G);
-    t /= a.G;
-    const int h = (int)(t % a.Hkv), b = (int)(t / a.Hkv);
-    w = *reinterpret_cast<const uint4*>(a.q + b * a.qs_b + h * a.qs_h + g * a.qs_g + (int64_t)s * a.qs_s + c * 16);
-  }
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-  float m = 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 f = unpack2<true>(u[k]);
-    m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
-  }
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float down;
-  const float up = f16_factor(m, down);
-  uint32_t v[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 f = unpack2<true>(u[k]);
-    v[k] = pack2<false>(f.x * up, f.y * up);
-  }
-  if (!in) return;
-  *reinterpret_cast<uint4*>(qh + row * D * 2 + c * 16) = make_uint4(v[0], v[1], v[2], v[3]);
-  if (c == 0) undo[row] = down;
-}
-
 // Joins the partial results of the units that several CTAs share. CTA (c, y):
 // the chain that CTA c of the attention kernel starts, in parts c, c + 1, ...
-// while those continue the same unit; 8 warps = RPC rows x KS slices of the
-// chain, a lane holding 4 (D = 128) or 2 dimensions of its row.
-template <int D, bool BF16, int ROWS, int RPC>
+// while those continue the same unit. 8 warps = RPC rows x KS slices of the
+// chain, PASSES times over, a lane holding 4 (D = 128) or 2 dimensions of its
+// row; the next four parts' loads are issued before any is used. Bound by the
+// parts' bytes in L2, and by its launch where there are few.
+template <int D, bool BF16, int ROWS, int RPC, int PASSES>
 __global__ void __launch_bounds__(256) paged_attn_fp8_merge_kernel(const Fp8Args a, int n_cta, int qt) {
-  constexpr int KS = 8 / RPC, E = D / 32;
+  constexpr int KS = 8 / RPC, E = D / 32, U = 4;
+  static_assert(KS == 1 || PASSES == 1, "slices meet once");
   __shared__ float so[8][D];
   __shared__ float2 sml[8];
   __shared__ int s_len;
@@ -1274,81 +1279,83 @@ __global__ void __launch_bounds__(256) paged_attn_fp8_merge_kernel(const Fp8Args
     }
   __syncthreads();
   const int parts = s_len + 1;  // the chain's start and the parts that follow
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.y * RPC + warp % RPC, slice = warp / RPC;
-  float M = neg_inf(), L = 0.f, acc[E];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slice = warp / RPC;
+  const int h = unit / a.items, item = unit - h * a.items;
+  const int b = item / a.tiles, tile = item - b * a.tiles;
+#pragma unroll 1
+  for (int pass = 0; pass < PASSES; ++pass) {
+    const int row = (blockIdx.y * PASSES + pass) * RPC + warp % RPC;
+    int s, g;
+    if (qt == 0) {  // rows in the order s G + g
+      const int cg = tile * ROWS + row;
+      s = cg / a.G;
+      g = cg - s * a.G;
+    } else {  // 128-row tiles of G heads x qt tokens
+      const int r = row & 127;
+      g = r / qt;
+      s = (tile * (ROWS / 128) + (row >> 7)) * qt + r - g * qt;
+    }
+    const bool live = g < a.G && s < a.S;
+    float M = neg_inf(), L = 0.f, acc[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  constexpr int U = 4;
-  for (int i0 = slice; i0 < parts; i0 += U * KS) {
-    float2 ml[U];
-    float o[U][E];
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int i0 = slice; live && i0 < parts; i0 += U * KS) {
+      float2 ml[U];
+      float o[U][E];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * KS;
-      ml[u] = make_float2(neg_inf(), 0.f);
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * KS;
+        ml[u] = make_float2(neg_inf(), 0.f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[u][e] = 0.f;
-      if (i < parts) {
-        const int64_t at = ((int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * ROWS + row);
-        ml[u] = a.part_ml[at];
-        if constexpr (E == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(a.part_o + at * D + lane * 4);
-          o[u][0] = v.x; o[u][1] = v.y; o[u][2] = v.z; o[u][3] = v.w;
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(a.part_o + at * D + lane * 2);
-          o[u][0] = v.x; o[u][1] = v.y;
+        for (int e = 0; e < E; ++e) o[u][e] = 0.f;
+        if (i < parts) {
+          const int64_t at = ((int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * ROWS + row);
+          ml[u] = a.part_ml[at];
+          if constexpr (E == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(a.part_o + at * D + lane * 4);
+            o[u][0] = v.x; o[u][1] = v.y; o[u][2] = v.z; o[u][3] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(a.part_o + at * D + lane * 2);
+            o[u][0] = v.x; o[u][1] = v.y;
+          }
         }
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (ml[u].x == neg_inf()) continue;
+        const float mn = fmaxf(M, ml[u].x);
+        const float f0 = exp2_approx(M - mn), f1 = exp2_approx(ml[u].x - mn);
+        M = mn;
+        L = L * f0 + ml[u].y * f1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + o[u][e] * f1;
+      }
     }
+    if (KS > 1) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (ml[u].x == neg_inf()) continue;
-      const float mn = fmaxf(M, ml[u].x);
-      const float f0 = exp2_approx(M - mn), f1 = exp2_approx(ml[u].x - mn);
-      M = mn;
-      L = L * f0 + ml[u].y * f1;
+      for (int e = 0; e < E; ++e) so[warp][lane * E + e] = acc[e];
+      if (lane == 0) sml[warp] = make_float2(M, L);
+      __syncthreads();
+      for (int k = 1; slice == 0 && k < KS; ++k) {
+        const float2 ml = sml[warp + k * RPC];
+        if (ml.x == neg_inf()) continue;
+        const float mn = fmaxf(M, ml.x);
+        const float f0 = exp2_approx(M - mn), f1 = exp2_approx(ml.x - mn);
+        M = mn;
+        L = L * f0 + ml.y * f1;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + o[u][e] * f1;
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + so[warp + k * RPC][lane * E + e] * f1;
+      }
     }
+    if (!live || slice != 0) continue;
+    const float inv = 1.f / L;
+    char* to = a.out + b * a.os_b + h * a.os_h + g * a.os_g + (int64_t)s * a.os_s + lane * E * 2;
+    if constexpr (E == 4)
+      *reinterpret_cast<uint2*>(to) =
+          make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(to) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
   }
-  if (KS > 1) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = acc[e];
-    if (lane == 0) sml[warp] = make_float2(M, L);
-    __syncthreads();
-    if (slice != 0) return;
-    for (int k = 1; k < KS; ++k) {
-      const float2 ml = sml[warp + k * RPC];
-      if (ml.x == neg_inf()) continue;
-      const float mn = fmaxf(M, ml.x);
-      const float f0 = exp2_approx(M - mn), f1 = exp2_approx(ml.x - mn);
-      M = mn;
-      L = L * f0 + ml.y * f1;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + so[warp + k * RPC][lane * E + e] * f1;
-    }
-  }
-  const int h = unit / a.items, i = unit - h * a.items;
-  const int b = i / a.tiles, tile = i - b * a.tiles;
-  int s, g;
-  if (qt == 0) {  // rows in the order s G + g
-    const int cg = tile * ROWS + row;
-    s = cg / a.G;
-    g = cg - s * a.G;
-  } else {  // 128-row tiles of G heads x qt tokens
-    const int r = row & 127;
-    g = r / qt;
-    s = (tile * (ROWS / 128) + (row >> 7)) * qt + r - g * qt;
-  }
-  if (g >= a.G || s >= a.S) return;
-  const float inv = 1.f / L;
-  char* to = a.out + b * a.os_b + h * a.os_h + g * a.os_g + s * a.os_s + lane * E * 2;
-  if constexpr (E == 4)
-    *reinterpret_cast<uint2*>(to) =
-        make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(to) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
 }
 
 // ---------------------------------------------------------------------------
@@ -1362,7 +1369,7 @@ struct Fp8Plan {
   int tiles, items;
   bool balanced;
   int ctas;
-  size_t desc, ml, o, qh, undo, total;  // workspace regions
+  size_t desc, ml, o, total;  // workspace regions
 };
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
@@ -1396,13 +1403,6 @@ int plan_fp8(const rbln_paged_attn_params_t* p, Fp8Plan* pl) {
     pl->o = off;
     off += round256((size_t)2 * pl->ctas * pl->rows * p->head_dim * sizeof(float));
   }
-  if (pl->nx && p->q_dtype == RBLN_DT_BF16) {
-    const size_t n = (size_t)p->batch * p->num_kv_heads * rows;
-    pl->qh = off;
-    off += round256(n * p->head_dim * 2);
-    pl->undo = off;
-    off += round256(n * sizeof(float));
-  }
   pl->total = off ? off + 256 : 0;
   return RBLN_OK;
 }
@@ -1431,7 +1431,7 @@ int launch_rows(const Fp8Args& a, const Fp8Plan& pl, cudaStream_t st) {
     return RBLN_ERR_LAUNCH;
   int rc = launch_after(paged_attn_fp8_rows_kernel<D, BF16, NT>, dim3(pl.ctas), kMqThreads, smem, st, a);
   if (rc != RBLN_OK || !pl.balanced) return rc;
-  return launch_after(paged_attn_fp8_merge_kernel<D, BF16, 8 * NT, 4>, dim3(pl.ctas, 2 * NT), 256, 0, st, a, pl.ctas, 0);
+  return launch_after(paged_attn_fp8_merge_kernel<D, BF16, 8 * NT, 4, 1>, dim3(pl.ctas, 2 * NT), 256, 0, st, a, pl.ctas, 0);
 }
 
 // cache [NB, Hkv, bs, D] of codes -> 4-D map of bytes, box {D, rpb, 1, 1}, not swizzled
@@ -1450,7 +1450,7 @@ bool map_codes(CUtensorMap* m, const rbln_paged_attn_params_t* p, const void* ca
 }
 
 template <int D, bool BF16, int NX>
-int launch_tiles(const rbln_paged_attn_params_t* p, const Fp8Args& a, const Fp8Plan& pl, char* base, cudaStream_t st) {
+int launch_tiles(const rbln_paged_attn_params_t* p, const Fp8Args& a, const Fp8Plan& pl, cudaStream_t st) {
   using L = TcSmem<D, NX>;
   using C = TcCfg<NX>;
   auto kernel = paged_attn_fp8_tiles_kernel<D, BF16, NX>;
@@ -1466,39 +1466,22 @@ int launch_tiles(const rbln_paged_attn_params_t* p, const Fp8Args& a, const Fp8P
     return RBLN_ERR_LAUNCH;
   CUtensorMap tq, tk, tv;
   if (!map_codes(&tk, p, p->kcache) || !map_codes(&tv, p, p->vcache)) return RBLN_ERR_LAUNCH;
-  const void* q = p->q;
-  int64_t qs[4] = {p->q_stride[0], p->q_stride[1], p->q_stride[2], p->q_stride[3]};
-  float* undo = nullptr;
-  if (BF16) {
-    char* qh = base + pl.qh;
-    undo = reinterpret_cast<float*>(base + pl.undo);
-    const int64_t rows = (int64_t)a.B * a.Hkv * a.G * a.S;
-    const int64_t grid = (rows * (D / 8) + 255) / 256;
-    if (grid > INT32_MAX) return RBLN_ERR_UNSUPPORTED;
-    const int rc = launch_after(query_f16_kernel<D>, dim3((unsigned)grid), 256, 0, st, a, qh, undo);
-    if (rc != RBLN_OK) return rc;
-    q = qh;
-    qs[3] = D;
-    qs[2] = (int64_t)a.S * D;
-    qs[1] = a.G * qs[2];
-    qs[0] = a.Hkv * qs[1];
-  }
   {  // [B, Hkv, G, S, D] -> 5-D map, box {64, QT, G, 1, 1}
     const uint64_t dims[5] = {(uint64_t)D, (uint64_t)a.S, (uint64_t)a.G, (uint64_t)a.Hkv, (uint64_t)a.B};
-    const uint64_t str[4] = {(uint64_t)qs[3] * 2, (uint64_t)qs[2] * 2, (uint64_t)qs[1] * 2, (uint64_t)qs[0] * 2};
+    const uint64_t str[4] = {(uint64_t)a.qs_s, (uint64_t)a.qs_g, (uint64_t)a.qs_h, (uint64_t)a.qs_b};
     const uint32_t box[5] = {64, (uint32_t)pl.qt, (uint32_t)a.G, 1, 1};
-    if (!make_map(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(q), dims, str, box)) return RBLN_ERR_LAUNCH;
+    if (!make_map(&tq, tmap_dtype(p->q_dtype), 5, const_cast<void*>(p->q), dims, str, box)) return RBLN_ERR_LAUNCH;
   }
-  int rc = launch_after(kernel, dim3(pl.ctas), C::THREADS, L::ALLOC, st, tq, tk, tv, a, pl.qt, (const float*)undo);
+  int rc = launch_after(kernel, dim3(pl.ctas), C::THREADS, L::ALLOC, st, tq, tk, tv, a, pl.qt);
   if (rc != RBLN_OK || !pl.balanced) return rc;
-  return launch_after(paged_attn_fp8_merge_kernel<D, BF16, 128 * NX, 8>, dim3(pl.ctas, 16 * NX), 256, 0, st, a, pl.ctas,
+  return launch_after(paged_attn_fp8_merge_kernel<D, BF16, 128 * NX, 8, 4>, dim3(pl.ctas, 4 * NX), 256, 0, st, a, pl.ctas,
                       pl.qt);
 }
 
 template <int D, bool BF16>
-int launch_fp8(const rbln_paged_attn_params_t* p, const Fp8Args& a, const Fp8Plan& pl, char* base, cudaStream_t st) {
-  if (pl.nx == 2) return launch_tiles<D, BF16, 2>(p, a, pl, base, st);
-  if (pl.nx == 1) return launch_tiles<D, BF16, 1>(p, a, pl, base, st);
+int launch_fp8(const rbln_paged_attn_params_t* p, const Fp8Args& a, const Fp8Plan& pl, cudaStream_t st) {
+  if (pl.nx == 2) return launch_tiles<D, BF16, 2>(p, a, pl, st);
+  if (pl.nx == 1) return launch_tiles<D, BF16, 1>(p, a, pl, st);
   return pl.nt == 1 ? launch_rows<D, BF16, 1>(a, pl, st) : launch_rows<D, BF16, 2>(a, pl, st);
 }
 
@@ -1582,9 +1565,9 @@ int run_prefill_fp8(const rbln_paged_attn_params_t* p, cudaStream_t st) {
   if (p->prof_events[0]) cudaEventRecord(static_cast<cudaEvent_t>(p->prof_events[0]), st);
   const bool bf = p->q_dtype == RBLN_DT_BF16;
   if (p->head_dim == 128)
-    rc = bf ? launch_fp8<128, true>(p, a, pl, base, st) : launch_fp8<128, false>(p, a, pl, base, st);
+    rc = bf ? launch_fp8<128, true>(p, a, pl, st) : launch_fp8<128, false>(p, a, pl, st);
   else
-    rc = bf ? launch_fp8<64, true>(p, a, pl, base, st) : launch_fp8<64, false>(p, a, pl, base, st);
+    rc = bf ? launch_fp8<64, true>(p, a, pl, st) : launch_fp8<64, false>(p, a, pl, st);
   if (p->prof_events[1]) cudaEventRecord(static_cast<cudaEvent_t>(p->prof_events[1]), st);
   return rc;
 }
