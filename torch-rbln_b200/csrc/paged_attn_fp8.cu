@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kMqWarps = 4;
 constexpr int kMqThreads = kMqWarps * 32;
-constexpr int kMqTile = 16;     // keys a warp's tile
+constexpr int kMqTile = 32;     // keys a warp's tile
 constexpr int kSegCost = 128;   // virtual keys charged to each unit's start
 constexpr int kMinW = 256;      // smallest share of a CTA, in keys
 constexpr int kMaxItems = 4096; // (sequence, row tile) items whose prefix a CTA holds in shared memory
@@ -57,6 +57,7 @@ struct Fp8Args {
   float scale;
   const float* scale_dev;
   int B, Hkv, G, S, num_blocks, bs, max_blocks, span;
+  uint32_t bs_mul, bs_shift;  // n / bs = (mulhi(n, bs_mul) + n) >> bs_shift
   int causal;
   int tiles, items;  // row tiles a sequence; items = B * tiles
   int balanced;      // 1: the keys of all units cut into equal shares; 0: whole units, grid-strided
@@ -67,6 +68,10 @@ struct Fp8Args {
   float2* part_ml; // [2 nCTA][rows]: (m, l)
   uint32_t* err;
 };
+
+__device__ __forceinline__ int div_bs(const Fp8Args& a, int n) {
+  return (int)((__umulhi((uint32_t)n, a.bs_mul) + (uint32_t)n) >> a.bs_shift);  // n < 2^30: no carry
+}
 
 __device__ __forceinline__ void dependents_enter() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -140,6 +145,38 @@ __device__ __forceinline__ void cost_prefix(const Fp8Args& a, int unit, int scal
 // take 16-key tiles round-robin and are joined in shared memory. The keys of
 // all (head, sequence) units are cut into equal shares, one CTA each.
 // ---------------------------------------------------------------------------
+// A warp's ring of tiles in shared memory, filled by cp.async. Rows are
+// swizzled by 16-byte chunks so that the fragments' loads meet no bank twice:
+// K fragments take rows gid and gid + 8, four neighbouring chunks at once, V
+// fragments rows 2 tig (+ 1, + 8, + 9), one piece of each.
+template <int D>
+struct MqRing {
+  static constexpr int STAGES = 2;
+  static constexpr int K = 0, V = kMqTile * D, KS = 2 * kMqTile * D, VS = KS + 4 * kMqTile, MASK = VS + 4 * kMqTile;
+  static constexpr int STAGE = MASK + 32;
+  static constexpr int WARP = STAGES * STAGE;
+  static __device__ __forceinline__ int k_at(int row, int chunk) {
+    return row * D + ((D == 128 ? chunk ^ ((row & 1) << 2) : chunk) << 4);
+  }
+  static __device__ __forceinline__ int v_at(int row, int chunk) {
+    if (D == 128) return row * D + ((chunk ^ (((row >> 1) & 3) << 1)) << 4);
+    const int slot = (row & 16) + (row & 1) * 8 + ((row & 15) >> 1);
+    return slot * D + ((chunk ^ (((slot >> 1) & 1) << 1)) << 4);
+  }
+};
+// 16 (or 4) bytes global -> shared in the background; zeros when not `valid`.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 template <int D, bool BF16, int NT>
 __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm, int b, int h, int tile, int t0,
                                            int t1, bool whole, int slot) {
@@ -149,20 +186,66 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
   const int c0 = tile * NC, cols = min(NC, a.S * a.G - c0);
   const int pos = a.seq[b * a.seq_stride];
 
+  // Row offset, in 16-byte units, of this lane's key ts + lane and its place
+  // in the scales; at = -1 for a key that is not seen.
   struct Entry {
-    int blk;
-    bool keep;
+    uint32_t off;
+    int at;
   };
   auto entry = [&](int ts, Entry& e) {
-    const int t = ts + (lane & 15);
-    const bool in = t < t1;
-    e.keep = in && (a.mask == nullptr ||
-                    (t < a.mask_len && load_keep(a.mask, a.mask_dtype, b * a.mask_stride + t)));
-    const int64_t blk = in ? load_index(a.bt, a.bt_dtype, b * a.bt_stride + t / a.bs) : -1;
-    e.blk = (blk >= 0 && blk < a.num_blocks) ? (int)blk : -1;
+    const int t = ts + lane;
+    e.at = -1;
+    if (t < t1) {
+      const int bi = div_bs(a, t);
+      const int64_t blk = load_index(a.bt, a.bt_dtype, b * a.bt_stride + bi);
+      const bool keep =
+          a.mask == nullptr || (t < a.mask_len && load_keep(a.mask, a.mask_dtype, b * a.mask_stride + t));
+      if (blk >= 0 && blk < a.num_blocks) {
+        if (keep) e.at = (int)blk;
+        e.off = (uint32_t)((blk * a.cs_block + h * a.cs_head + (t - bi * a.bs) * a.cs_tok) >> 4);
+      } else if (a.err) {
+        atomicOr(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
+      }
+    }
   };
+  using R = MqRing<D>;
+  unsigned char* ring = dsm + warp * R::WARP;
+  const uint32_t ring_s = smem_u32(ring);
+  // issues the copies of the tile of entry e into stage st
+  auto issue = [&](int st, const Entry& e) {
+    const uint32_t to = ring_s + st * R::STAGE;
+    const bool valid = e.at >= 0;
+    const uint32_t vmask = __ballot_sync(0xffffffffu, valid);
+    if (lane == 0) *reinterpret_cast<uint32_t*>(ring + st * R::STAGE + R::MASK) = vmask;
+    if (vmask != 0) {
+      const int64_t so = valid ? e.at * a.ss_block + h * a.ss_head : 0;
+      copy4(to + R::KS + lane * 4, a.k_scale + so, valid);
+      copy4(to + R::VS + lane * 4, a.v_scale + so, valid);
+      constexpr int CPR = D / 16, RPI = 32 / CPR;  // chunks a row, rows a step
+      const int c = lane % CPR;
+#pragma unroll
+      for (int k = 0; k < kMqTile / RPI; ++k) {
+        const int row = k * RPI + lane / CPR;
+        const uint32_t ro = __shfl_sync(0xffffffffu, e.off, row);
+        const bool ok = (vmask >> row) & 1;
+        const size_t at = ok ? (size_t)ro * 16 + c * 16 : 0;
+        copy16(to + R::K + R::k_at(row, c), a.kcache + at, ok);
+        copy16(to + R::V + R::v_at(row, c), a.vcache + at, ok);
+      }
+    }
+    copy_commit();
+  };
+  // the first tiles on their way before the queries are looked at
+  const int step = kMqWarps * kMqTile, first = t0 + warp * kMqTile;
   Entry ent;
-  entry(t0 + warp * kMqTile, ent);
+  entry(first, ent);
+#pragma unroll
+  for (int st = 0; st < R::STAGES - 1; ++st) {
+    const int ts = first + st * step;
+    if (ts < t1) issue(st, ent);
+    else copy_commit();
+    entry(ts + step, ent);
+  }
 
   // query fragments (B operand: k = head_dim, n = column gid + 8 nt) in f16
   uint32_t qf[NT][KR];
@@ -228,79 +311,43 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
     m_run[nt][0] = m_run[nt][1] = neg_inf();
     l_run[nt][0] = l_run[nt][1] = 0.f;
   }
+  // keys below this are every live row's (their columns' limits)
+  const int all_lim = a.causal ? (int)min((int64_t)pos + c0 / a.G + 1, (int64_t)t1) : t1;
   float vref = 0.f, inv_vref = 0.f;  // power of two at or above every V scale met, and its reciprocal
-  const int tv[4] = {2 * tig, 2 * tig + 1, 2 * tig + 8, 2 * tig + 9};
 
-  struct Tile {
-    uint4 kraw[2][KCH];
-    uint32_t vraw[4][NVW];
-    uint32_t vmask;
-    float ksc, vsc;
-  };
-  auto fetch = [&](int ts, Tile& T, const Entry& e) {
-    const int t = ts + (lane & 15);
-    bool valid = e.keep;
-    int64_t off = 0;
-    T.ksc = 1.f;
-    T.vsc = 0.f;
-    if (valid) {
-      if (e.blk < 0) {
-        valid = false;
-        if (a.err) atomicOr(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
-      } else {
-        off = e.blk * a.cs_block + h * a.cs_head + (t % a.bs) * a.cs_tok;
-        T.ksc = a.k_scale[e.blk * a.ss_block + h * a.ss_head];
-        T.vsc = a.v_scale[e.blk * a.ss_block + h * a.ss_head];
+  auto consume = [&](int ts, int st) {
+    const unsigned char* stage = ring + st * R::STAGE;
+    const uint32_t vmask = *reinterpret_cast<const uint32_t*>(stage + R::MASK);
+    if (vmask == 0) return;  // the same for the whole warp
+    const float* ks = reinterpret_cast<const float*>(stage + R::KS);
+    const float* vs = reinterpret_cast<const float*>(stage + R::VS);
+    // scores of keys gid + 8 r (r = 0..3): s[nt][2 r + k], column 2 tig + k
+    float s[NT][8];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[nt][k] = 0.f;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int i = 0; i < KCH; ++i) {
+        const uint4 k0 = *reinterpret_cast<const uint4*>(stage + R::K + R::k_at(16 * sub + gid, 4 * i + tig));
+        const uint4 k1 = *reinterpret_cast<const uint4*>(stage + R::K + R::k_at(16 * sub + gid + 8, 4 * i + tig));
+        const uint32_t r0[4] = {k0.x, k0.y, k0.z, k0.w}, r1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_to_f16x2x2(r0[w], a0, a2);
+          e4m3x4_to_f16x2x2(r1[w], a1, a3);
+          const int kk = 4 * i + w;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816<false>(reinterpret_cast<float(&)[4]>(s[nt][4 * sub]), a0, a1, a2, a3, qf[nt][2 * kk],
+                            qf[nt][2 * kk + 1]);
+        }
       }
-    }
-    T.vmask = __ballot_sync(0xffffffffu, valid) & 0xffffu;
-    if (T.vmask == 0) return;
-    const int64_t ok0 = __shfl_sync(0xffffffffu, off, gid);
-    const int64_t ok1 = __shfl_sync(0xffffffffu, off, gid + 8);
-    const bool vk0 = (T.vmask >> gid) & 1, vk1 = (T.vmask >> (gid + 8)) & 1;
-#pragma unroll
-    for (int i = 0; i < KCH; ++i) {
-      T.kraw[0][i] = vk0 ? ld_stream_v4(a.kcache + ok0 + (4 * i + tig) * 16) : make_uint4(0, 0, 0, 0);
-      T.kraw[1][i] = vk1 ? ld_stream_v4(a.kcache + ok1 + (4 * i + tig) * 16) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t ov = __shfl_sync(0xffffffffu, off, tv[j]);
-      const bool vv = (T.vmask >> tv[j]) & 1;
-      const char* row = a.vcache + ov + gid * VSEG;
-      if constexpr (NVW == 4) {
-        const uint4 x = vv ? ld_stream_v4(row) : make_uint4(0, 0, 0, 0);
-        T.vraw[j][0] = x.x; T.vraw[j][1] = x.y; T.vraw[j][2] = x.z; T.vraw[j][3] = x.w;
-      } else {
-        const uint2 x = vv ? ld_stream_v2(row) : make_uint2(0, 0);
-        T.vraw[j][0] = x.x; T.vraw[j][1] = x.y;
-      }
-    }
-  };
-
-  auto consume = [&](int ts, const Tile& T) {
-    if (T.vmask == 0) return;  // warp-uniform (ballot)
-    const bool vk0 = (T.vmask >> gid) & 1, vk1 = (T.vmask >> (gid + 8)) & 1;
-    float s[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-    for (int i = 0; i < KCH; ++i) {
-      const uint32_t* r0 = reinterpret_cast<const uint32_t*>(&T.kraw[0][i]);
-      const uint32_t* r1 = reinterpret_cast<const uint32_t*>(&T.kraw[1][i]);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t a0, a1, a2, a3;
-        e4m3x4_to_f16x2x2(r0[w], a0, a2);
-        e4m3x4_to_f16x2x2(r1[w], a1, a3);
-        const int kk = 4 * i + w;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma16816<false>(s[nt], a0, a1, a2, a3, qf[nt][2 * kk], qf[nt][2 * kk + 1]);
-      }
-    }
     // V scales relative to vref; positive floats order as their bits
-    const uint32_t vmaxb = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(T.vsc, 0.f)));
+    const uint32_t vmaxb = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs[lane], 0.f)));
     if (__uint_as_float(vmaxb) > vref) {
       const float now = pow2_above(__uint_as_float(vmaxb));
       const float inv = 1.f / now;  // a power of two: exact
@@ -316,62 +363,106 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
       vref = now;
       inv_vref = inv;
     }
-    const float ks0 = __shfl_sync(0xffffffffu, T.ksc, gid), ks1 = __shfl_sync(0xffffffffu, T.ksc, gid + 8);
-    const float vs0 = __shfl_sync(0xffffffffu, T.vsc, gid) * inv_vref;
-    const float vs1 = __shfl_sync(0xffffffffu, T.vsc, gid + 8) * inv_vref;
-    uint32_t pb0[NT], pb1[NT];
+    float ksc[4], vsc[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      ksc[r] = ks[gid + 8 * r];
+      vsc[r] = vs[gid + 8 * r] * inv_vref;
+    }
+    const bool whole_tile = vmask == 0xffffffffu && ts + kMqTile <= all_lim;
+    uint32_t pb[2][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r0 = ts + gid, r1 = r0 + 8;
-      const float x0 = vk0 && r0 < lim[nt][0] ? s[nt][0] * (colmul[nt][0] * ks0) : neg_inf();
-      const float x1 = vk0 && r0 < lim[nt][1] ? s[nt][1] * (colmul[nt][1] * ks0) : neg_inf();
-      const float x2 = vk1 && r1 < lim[nt][0] ? s[nt][2] * (colmul[nt][0] * ks1) : neg_inf();
-      const float x3 = vk1 && r1 < lim[nt][1] ? s[nt][3] * (colmul[nt][1] * ks1) : neg_inf();
-      const float mn0 = fmaxf(m_run[nt][0], warp_max_xor_rows(fmaxf(x0, x2)));
-      const float mn1 = fmaxf(m_run[nt][1], warp_max_xor_rows(fmaxf(x1, x3)));
-      const float ms0 = (mn0 == neg_inf()) ? 0.f : mn0;
-      const float ms1 = (mn1 == neg_inf()) ? 0.f : mn1;
-      const float al0 = exp2_approx(m_run[nt][0] - ms0), al1 = exp2_approx(m_run[nt][1] - ms1);
-      const float p0 = exp2_approx(x0 - ms0), p2 = exp2_approx(x2 - ms0);
-      const float p1 = exp2_approx(x1 - ms1), p3 = exp2_approx(x3 - ms1);
-      l_run[nt][0] = l_run[nt][0] * al0 + p0 + p2;
-      l_run[nt][1] = l_run[nt][1] * al1 + p1 + p3;
-      m_run[nt][0] = mn0;
-      m_run[nt][1] = mn1;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) s[nt][2 * r + k] *= colmul[nt][k] * ksc[r];
+      if (!whole_tile) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (!((vmask >> (gid + 8 * r)) & 1u) || ts + gid + 8 * r >= lim[nt][k]) s[nt][2 * r + k] = neg_inf();
+      }
+      float al[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float mx = fmaxf(fmaxf(s[nt][k], s[nt][2 + k]), fmaxf(s[nt][4 + k], s[nt][6 + k]));
+        const float mn = fmaxf(m_run[nt][k], warp_max_xor_rows(mx));
+        const float ms = (mn == neg_inf()) ? 0.f : mn;
+        al[k] = exp2_approx(m_run[nt][k] - ms);
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[nt][2 * r + k] = exp2_approx(s[nt][2 * r + k] - ms);
+          sum += s[nt][2 * r + k];
+        }
+        l_run[nt][k] = l_run[nt][k] * al[k] + sum;
+        m_run[nt][k] = mn;
+      }
       // the factors are exactly 1 once the maxima settle
-      if (__any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {
+      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          o_acc[nt][mt][0] *= al0; o_acc[nt][mt][2] *= al0;
-          o_acc[nt][mt][1] *= al1; o_acc[nt][mt][3] *= al1;
+          o_acc[nt][mt][0] *= al[0]; o_acc[nt][mt][2] *= al[0];
+          o_acc[nt][mt][1] *= al[1]; o_acc[nt][mt][3] *= al[1];
         }
       }
-      pb0[nt] = movmatrix_trans(pack2<false>(p0 * vs0, p1 * vs0));
-      pb1[nt] = movmatrix_trans(pack2<false>(p2 * vs1, p3 * vs1));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        pb[r >> 1][nt][r & 1] =
+            movmatrix_trans(pack2<false>(s[nt][2 * r] * vsc[r], s[nt][2 * r + 1] * vsc[r]));
     }
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int w = mt >> 1;
-      const uint32_t sel = (mt & 1) ? 0x7362u : 0x5140u;
-      uint32_t a0, a1, a2, a3;
-      e4m3x4_to_f16x2x2(prmt(T.vraw[0][w], T.vraw[1][w], sel), a0, a1);
-      e4m3x4_to_f16x2x2(prmt(T.vraw[2][w], T.vraw[3][w], sel), a2, a3);
+    for (int sub = 0; sub < 2; ++sub) {
+      uint32_t vraw[4][NVW];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma16816<false>(o_acc[nt][mt], a0, a1, a2, a3, pb0[nt], pb1[nt]);
+      for (int j = 0; j < 4; ++j) {
+        const int row = 16 * sub + 2 * tig + (j & 1) + (j >> 1) * 8;
+        if constexpr (NVW == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(stage + R::V + R::v_at(row, gid));
+          vraw[j][0] = x.x; vraw[j][1] = x.y; vraw[j][2] = x.z; vraw[j][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(stage + R::V + R::v_at(row, gid >> 1) + (gid & 1) * 8);
+          vraw[j][0] = x.x; vraw[j][1] = x.y;
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int w = mt >> 1;
+        const uint32_t sel = (mt & 1) ? 0x7362u : 0x5140u;
+        uint32_t a0, a1, a2, a3;
+        e4m3x4_to_f16x2x2(prmt(vraw[0][w], vraw[1][w], sel), a0, a1);
+        e4m3x4_to_f16x2x2(prmt(vraw[2][w], vraw[3][w], sel), a2, a3);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma16816<false>(o_acc[nt][mt], a0, a1, a2, a3, pb[sub][nt][0], pb[sub][nt][1]);
+      }
     }
   };
 
-  for (int ts = t0 + warp * kMqTile; ts < t1; ts += kMqWarps * kMqTile) {
-    Tile T;
-    fetch(ts, T, ent);
-    entry(ts + kMqWarps * kMqTile, ent);  // the next tile's look-up overlaps this tile's loads and math
-    consume(ts, T);
+  int st = 0;
+  for (int ts = first; ts < t1; ts += step) {
+    const int ahead = ts + (R::STAGES - 1) * step;
+    const int to = st == 0 ? R::STAGES - 1 : st - 1;  // the stage used last
+    if (ahead < t1) issue(to, ent);
+    else copy_commit();
+    entry(ahead + step, ent);  // the look-up of the tile after it
+    copy_wait<R::STAGES - 1>();
+    __syncwarp();
+    consume(ts, st);
+    __syncwarp();
+    st = st == R::STAGES - 1 ? 0 : st + 1;
   }
+  copy_wait<0>();
+  __syncwarp();
 
   // ---- join the four warps ------------------------------------------------
-  auto sO = reinterpret_cast<float(*)[NC][D]>(dsm);
-  auto sM = reinterpret_cast<float(*)[NC]>(dsm + kMqWarps * NC * D * 4);
-  auto sL = reinterpret_cast<float(*)[NC]>(dsm + kMqWarps * NC * D * 4 + kMqWarps * NC * 4);
+  // a warp's O lies over its own ring; the maxima and sums behind all rings
+  static_assert(NC * D * 4 <= R::WARP, "O over the ring");
+  auto sO = [&](int w) { return reinterpret_cast<float(*)[D]>(dsm + w * R::WARP); };
+  auto sM = reinterpret_cast<float(*)[NC]>(dsm + kMqWarps * R::WARP);
+  auto sL = reinterpret_cast<float(*)[NC]>(dsm + kMqWarps * R::WARP + kMqWarps * NC * 4);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const float l0 = warp_sum_xor_rows(l_run[nt][0]), l1 = warp_sum_xor_rows(l_run[nt][1]);
@@ -383,10 +474,10 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int d0 = gid * VSEG + 2 * mt, d1 = d0 + 1;
-      sO[warp][c][d0] = o_acc[nt][mt][0] * vref;
-      sO[warp][c + 1][d0] = o_acc[nt][mt][1] * vref;
-      sO[warp][c][d1] = o_acc[nt][mt][2] * vref;
-      sO[warp][c + 1][d1] = o_acc[nt][mt][3] * vref;
+      sO(warp)[c][d0] = o_acc[nt][mt][0] * vref;
+      sO(warp)[c + 1][d0] = o_acc[nt][mt][1] * vref;
+      sO(warp)[c][d1] = o_acc[nt][mt][2] * vref;
+      sO(warp)[c + 1][d1] = o_acc[nt][mt][3] * vref;
     }
   }
   __syncthreads();
@@ -401,7 +492,7 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
     for (int w = 0; w < kMqWarps; ++w) {
       const float f = (sM[w][c] == neg_inf()) ? 0.f : exp2_approx(sM[w][c] - M);
       L += f * sL[w][c];
-      const float4 o = *reinterpret_cast<const float4*>(&sO[w][c][d4]);
+      const float4 o = *reinterpret_cast<const float4*>(&sO(w)[c][d4]);
       acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
     }
     if (whole) {
@@ -457,8 +548,9 @@ __device__ __forceinline__ void walk_share(const Fp8Args& a, const int* P, int64
   }
 }
 
+constexpr int kMqCtas = 3;  // CTAs an SM: their rings fill its shared memory
 template <int D, bool BF16, int NT>
-__global__ void __launch_bounds__(kMqThreads, NT == 1 ? 4 : 2) paged_attn_fp8_rows_kernel(const Fp8Args a) {
+__global__ void __launch_bounds__(kMqThreads, kMqCtas) paged_attn_fp8_rows_kernel(const Fp8Args a) {
   extern __shared__ __align__(16) unsigned char dsm[];
   constexpr int NC = 8 * NT;
   dependents_enter();
@@ -482,11 +574,12 @@ __global__ void __launch_bounds__(kMqThreads, NT == 1 ? 4 : 2) paged_attn_fp8_ro
     }
     return;
   }
-  int* P = reinterpret_cast<int*>(dsm + kMqWarps * NC * (D * 4 + 8));
+  int* P = reinterpret_cast<int*>(dsm + kMqWarps * (MqRing<D>::WARP + NC * 8));
   __shared__ int wsum[kMqWarps];
-  cost_prefix<kMqThreads>(a, 16, 16, kSegCost, keys, wsum, P);  // counted in keys
+  cost_prefix<kMqThreads>(a, kMqTile, kMqTile, kSegCost, keys, wsum, P);  // counted in keys
   const int64_t total = (int64_t)P[a.items] * a.Hkv;
-  int64_t W = ((total + gridDim.x - 1) / gridDim.x + 15) & ~(int64_t)15;
+  int64_t W = (total + gridDim.x - 1) / gridDim.x;
+  W = (W + kMqTile - 1) / kMqTile * kMqTile;
   if (W < kMinW) W = kMinW;
   const int64_t lo = min(W * blockIdx.x, total);
   walk_share(a, P, lo, min(lo + W, total), keys, seg);
@@ -1374,12 +1467,20 @@ struct Fp8Plan {
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
+// Dynamic shared memory of the row kernel: rings, maxima and sums, prefix.
+size_t rows_smem(int D, int rows, int items) {
+  const int ring = D == 128 ? MqRing<128>::WARP : MqRing<64>::WARP;
+  return (size_t)kMqWarps * (ring + rows * 8) + (items + 1) * sizeof(int);
+}
+
 int plan_fp8(const rbln_paged_attn_params_t* p, Fp8Plan* pl) {
   const int64_t span = (int64_t)p->max_blocks * p->block_size;
   const int64_t rows = (int64_t)p->q_len * p->group;
   // Up to 16 rows of a KV head the row kernel reads the codes once; more
   // rows would read them again for each 16, so they go to 128-row tiles.
-  pl->nx = rows <= 16 ? 0 : rows <= 128 ? 1 : 2;
+  // (which also takes pools of over 64 GB: the row kernel's offsets are 32 bits of 16 bytes)
+  const int64_t pool = (int64_t)p->num_blocks * p->cache_stride[0];
+  pl->nx = rows <= 16 && pool >> 4 <= (int64_t)UINT32_MAX ? 0 : rows <= 128 ? 1 : 2;
   pl->nt = rows <= 8 ? 1 : 2;
   pl->qt = 128 / p->group;
   pl->rows = pl->nx ? 128 * pl->nx : 8 * pl->nt;
@@ -1388,10 +1489,12 @@ int plan_fp8(const rbln_paged_attn_params_t* p, Fp8Plan* pl) {
   if (tiles * p->batch * p->num_kv_heads > INT32_MAX) return RBLN_ERR_UNSUPPORTED;
   pl->tiles = (int)tiles;
   pl->items = (int)(tiles * p->batch);
-  const int64_t slots = pl->nx ? 148LL : 148LL * (pl->nt == 1 ? 4 : 2);
+  // CTAs that run at once: a long prefix leaves room for fewer
+  const int64_t fit = 232448 / (int64_t)(rows_smem(p->head_dim, pl->rows, std::min(pl->items, kMaxItems)) + 1024);
+  const int64_t slots = 148LL * (pl->nx ? 1 : std::min<int64_t>(kMqCtas, fit));
   // the prefix fits shared memory and counts in 32 bits; with more items than
   // that there are enough whole units for every CTA
-  pl->balanced = pl->items <= kMaxItems && (int64_t)pl->items * (span + 16 + kSegCost) < INT32_MAX;
+  pl->balanced = pl->items <= kMaxItems && (int64_t)pl->items * (span + kMqTile + kSegCost) < INT32_MAX;
   const int64_t units = (int64_t)pl->items * p->num_kv_heads;
   pl->ctas = (int)(pl->balanced ? slots : std::min<int64_t>(units, pl->nx ? slots : slots * 8));
   size_t off = 0;
@@ -1424,7 +1527,7 @@ int launch_after(void (*kernel)(A...), dim3 grid, int threads, size_t smem, cuda
 
 template <int D, bool BF16, int NT>
 int launch_rows(const Fp8Args& a, const Fp8Plan& pl, cudaStream_t st) {
-  const size_t smem = (size_t)kMqWarps * pl.rows * (D * 4 + 8) + (pl.balanced ? (pl.items + 1) * sizeof(int) : 0);
+  const size_t smem = rows_smem(D, pl.rows, pl.balanced ? pl.items : -1);
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(paged_attn_fp8_rows_kernel<D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            (int)smem) != cudaSuccess)
@@ -1552,6 +1655,9 @@ int run_prefill_fp8(const rbln_paged_attn_params_t* p, cudaStream_t st) {
   a.B = p->batch; a.Hkv = p->num_kv_heads; a.G = p->group; a.S = p->q_len;
   a.num_blocks = p->num_blocks; a.bs = p->block_size; a.max_blocks = p->max_blocks;
   a.span = p->max_blocks * p->block_size;
+  for (a.bs_shift = 0; (1u << a.bs_shift) < (uint32_t)a.bs; ++a.bs_shift) {
+  }
+  a.bs_mul = (uint32_t)(((uint64_t)((1u << a.bs_shift) - (uint32_t)a.bs) << 32) / (uint32_t)a.bs + 1);
   a.causal = p->causal;
   a.tiles = pl.tiles; a.items = pl.items;
   a.balanced = pl.balanced;
