@@ -32,7 +32,8 @@ struct ReadArgs {
   char* k_out;
   char* v_out;
   int64_t os_b, os_h, os_t;  // elements
-  int B, Hkv, T, D, bs, max_blocks, num_blocks, ctas_per_head;
+  int B, Hkv, T, cshift, bs, max_blocks, num_blocks, ctas_per_head;  // 2^cshift pieces of 8 elements a row
+  uint32_t bs_mul, bs_shift;  // n / bs = (mulhi(n, bs_mul) + n) >> bs_shift, n < 2^30
   uint32_t* err;
 };
 
@@ -86,41 +87,51 @@ __global__ void __launch_bounds__(kReadThreads) paged_kv_read_kernel(const ReadA
     if (a.err && threadIdx.x == 0) atomicOr(a.err, RBLN_DEVERR_SEQ_RANGE);
     len = len < 0 ? 0 : (int)span;
   }
-  const int cpr = a.D / 8;
+  // this thread's pieces: one column, rows t0 + u rstep
+  const int c = threadIdx.x & ((1 << a.cshift) - 1), rstep = kReadThreads >> a.cshift;
+  const int t0 = part * kReadSteps * rstep + (threadIdx.x >> a.cshift);
+  const char* kc = a.kcache + ((int64_t)h * a.cs_head + c * 8) * SZ;
+  const char* vc = a.vcache + ((int64_t)h * a.cs_head + c * 8) * SZ;
+  int64_t blk[kReadSteps];
+  int row[kReadSteps];
+#pragma unroll
+  for (int u = 0; u < kReadSteps; ++u) {
+    const int t = t0 + u * rstep;
+    blk[u] = -1;
+    if (t >= a.T || t >= len) continue;
+    const int bi = (int)((__umulhi((uint32_t)t, a.bs_mul) + (uint32_t)t) >> a.bs_shift);
+    row[u] = t - bi * a.bs;
+    blk[u] = load_index(a.bt, a.bt_dtype, b * a.bt_stride + bi);
+    if (blk[u] < 0 || blk[u] >= a.num_blocks) {
+      if (a.err) atomicOr(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
+      blk[u] = -1;
+    }
+  }
   uint4 kw[kReadSteps], vw[kReadSteps];
   float ks[kReadSteps], vs[kReadSteps];
 #pragma unroll
   for (int u = 0; u < kReadSteps; ++u) {
-    const int64_t i = ((int64_t)part * kReadSteps + u) * kReadThreads + threadIdx.x;
-    const int64_t t = i / cpr;
-    const int c = (int)(i - t * cpr);
     kw[u] = vw[u] = make_uint4(0, 0, 0, 0);
     ks[u] = vs[u] = 0.f;
-    if (t >= a.T || t >= len) continue;
-    const int64_t blk = load_index(a.bt, a.bt_dtype, b * a.bt_stride + t / a.bs);
-    if (blk < 0 || blk >= a.num_blocks) {
-      if (a.err) atomicOr(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
-      continue;
-    }
-    const int64_t at = (blk * a.cs_block + h * a.cs_head + (t % a.bs) * a.cs_tok + c * 8) * SZ;
+    if (blk[u] < 0) continue;
+    const int64_t at = (blk[u] * a.cs_block + row[u] * a.cs_tok) * SZ;
     if constexpr (KV == R_FP8) {
-      const uint2 x = ld_stream_v2(a.kcache + at), y = ld_stream_v2(a.vcache + at);
+      const uint2 x = ld_stream_v2(kc + at), y = ld_stream_v2(vc + at);
       kw[u] = make_uint4(x.x, x.y, 0, 0);
       vw[u] = make_uint4(y.x, y.y, 0, 0);
-      ks[u] = a.k_scale[blk * a.ss_block + h * a.ss_head];
-      vs[u] = a.v_scale[blk * a.ss_block + h * a.ss_head];
+      ks[u] = a.k_scale[blk[u] * a.ss_block + h * a.ss_head];
+      vs[u] = a.v_scale[blk[u] * a.ss_block + h * a.ss_head];
     } else {
-      kw[u] = ld_stream_v4(a.kcache + at);
-      vw[u] = ld_stream_v4(a.vcache + at);
+      kw[u] = ld_stream_v4(kc + at);
+      vw[u] = ld_stream_v4(vc + at);
     }
   }
+  const int64_t to0 = (b * a.os_b + h * a.os_h + c * 8) * OSZ;
 #pragma unroll
   for (int u = 0; u < kReadSteps; ++u) {
-    const int64_t i = ((int64_t)part * kReadSteps + u) * kReadThreads + threadIdx.x;
-    const int64_t t = i / cpr;
-    const int c = (int)(i - t * cpr);
+    const int t = t0 + u * rstep;
     if (t >= a.T) continue;
-    const int64_t to = (b * a.os_b + h * a.os_h + t * a.os_t + c * 8) * OSZ;
+    const int64_t to = to0 + t * a.os_t * OSZ;
     if constexpr (KV == OUT) {
       *reinterpret_cast<uint4*>(a.k_out + to) = kw[u];
       *reinterpret_cast<uint4*>(a.v_out + to) = vw[u];
@@ -160,7 +171,7 @@ extern "C" int rbln_paged_kv_read(const rbln_paged_attn_params_t* p, void* k_out
   if (p->block_table_dtype != RBLN_DT_I16 && p->block_table_dtype != RBLN_DT_I32 &&
       p->block_table_dtype != RBLN_DT_I64)
     return RBLN_ERR_UNSUPPORTED;
-  if ((int64_t)p->max_blocks * p->block_size > (1 << 30)) return RBLN_ERR_UNSUPPORTED;
+  if ((int64_t)p->max_blocks * p->block_size > (1 << 30) || p->q_len > (1 << 30)) return RBLN_ERR_UNSUPPORTED;
   if (!k_out || !v_out || !p->kcache || !p->vcache || !p->seq || !p->block_table || (fp8 && (!p->k_scale || !p->v_scale)))
     return RBLN_ERR_INVALID_ARGUMENT;
   {  // 8 elements at a time: 8 or 16 bytes in, 16 out
@@ -180,10 +191,14 @@ extern "C" int rbln_paged_kv_read(const rbln_paged_attn_params_t* p, void* k_out
   a.bt = p->block_table; a.bt_dtype = p->block_table_dtype; a.bt_stride = p->block_table_stride;
   a.k_out = static_cast<char*>(k_out); a.v_out = static_cast<char*>(v_out);
   a.os_b = out_stride[0]; a.os_h = out_stride[1]; a.os_t = out_stride[2];
-  a.B = p->batch; a.Hkv = p->num_kv_heads; a.T = p->q_len; a.D = p->head_dim; a.bs = p->block_size;
+  a.B = p->batch; a.Hkv = p->num_kv_heads; a.T = p->q_len; a.cshift = p->head_dim == 128 ? 4 : 3;
+  a.bs = p->block_size;
+  for (a.bs_shift = 0; (1u << a.bs_shift) < (uint32_t)a.bs; ++a.bs_shift) {
+  }
+  a.bs_mul = (uint32_t)(((uint64_t)((1u << a.bs_shift) - (uint32_t)a.bs) << 32) / (uint32_t)a.bs + 1);
   a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
   a.err = p->error_flags;
-  const int64_t pieces = (int64_t)a.T * (a.D / 8);
+  const int64_t pieces = (int64_t)a.T << a.cshift;
   const int64_t per = (pieces + kReadThreads * kReadSteps - 1) / (kReadThreads * kReadSteps);
   const int64_t grid = per * a.B * a.Hkv;
   if (grid > INT32_MAX) return RBLN_ERR_UNSUPPORTED;

@@ -74,7 +74,7 @@ __device__ __forceinline__ double position(const RotaryArgs& a, int b, int s) {
 // grid (ceil(tokens / tpb), head groups), 256 threads: thread = (token,
 // item, head lane), item fastest, so that 8 neighbours cover a 256-byte row.
 template <typename T>
-__global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotThreads, 4) rotary_vec_kernel(const RotaryArgs a) {
   constexpr int V = Vec<T>::N;
   extern __shared__ float2 table[];  // [tpb][R/2]
   const int half = a.R / 2;
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(const RotaryArg
     for (int i = 0; i < V; ++i) cs[i] = table[t * half + c * V + i];
   }
   const int step = a.hp * (int)gridDim.y;
-  constexpr int U = 4;  // heads whose loads are in flight together
+  constexpr int U = 2;  // heads whose loads are in flight together
   for (int h0 = blockIdx.y * a.hp + hl; h0 < a.heads; h0 += U * step) {
     uint4 w0[U], w1[U];
 #pragma unroll

@@ -27,7 +27,7 @@ namespace {
 constexpr int kRwThreads = 256;
 constexpr int kRwWarps = kRwThreads / 32;
 constexpr int kTileRows = 16;
-constexpr int kTableRows = 128;  // rows whose angles a CTA keeps; rows past them find theirs again (blocks > 128)
+constexpr int kTableRows = 128;  // rows whose angles are kept at once
 
 struct RotWriteArgs {
   const char* q;
@@ -95,11 +95,17 @@ __device__ __forceinline__ void decode8(uint2 w, float s, float (&x)[8]) {
   }
 }
 
-template <int D, bool BF16, bool FP8>
+// MULTI: blocks of more than 16 rows. Their rows are taken 128 at a time (the
+// angles kept in shared memory), an fp8 cache's twice: for the amax, then for
+// the codes. Blocks of up to 16 rows stay in registers in between.
+template <int D, bool BF16, bool FP8, bool MULTI>
 __global__ void __launch_bounds__(kRwThreads, FP8 && D == 128 ? 2 : 3) rotary_write_kernel(const RotWriteArgs a) {
   constexpr int V = 8, NI = D / 16;           // items a row
   constexpr int PER = kTileRows * NI / 32;    // items a lane of a 16-row tile
-  extern __shared__ float2 table[];           // [min(rows, kTableRows)][R/2]
+  // [rows][V][R / 16] pairs, a row padded so that the lanes of neighbouring
+  // rows meet other banks: pair c V + i of a row at i R/16 + c
+  extern __shared__ float2 table[];
+  __shared__ float unit_max[MULTI ? 64 : 1];  // an fp8 block's amax so far, of each (head, K or V)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = blockIdx.x % a.slots, b = blockIdx.x / a.slots;
   const int h0 = blockIdx.y * a.hg, h1 = min(h0 + a.hg, a.Hkv);
@@ -108,7 +114,6 @@ __global__ void __launch_bounds__(kRwThreads, FP8 && D == 128 ? 2 : 3) rotary_wr
   const int p0 = ((s0 % a.bs) + a.bs) % a.bs;
   const int lo = max(j * a.bs - p0, 0), hi = (int)min((int64_t)(j + 1) * a.bs - p0, (int64_t)a.S);
   if (lo >= hi) return;  // tokens [lo, hi) fall in this block
-  const int rows = hi - lo;
 
   // write target: the block's pool index, or none
   bool write = true;
@@ -124,163 +129,251 @@ __global__ void __launch_bounds__(kRwThreads, FP8 && D == 128 ? 2 : 3) rotary_wr
       if (threadIdx.x == 0 && a.err) atomicOr(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
     }
   }
-  const int row0 = j == 0 ? p0 : 0;        // block row of token lo
+  const int row0 = j == 0 ? p0 : 0;            // block row of token lo
   const int held = j == 0 && s0 > 0 ? p0 : 0;  // block rows the sequence holds already
+  const int units = FP8 && write ? 2 * (h1 - h0) : 0;  // (head, K or V) of an fp8 cache, one a warp
 
-  const int half = a.R / 2;
-  for (int i = threadIdx.x; i < min(rows, kTableRows) * half; i += kRwThreads) {
-    const int r = i / half, p = i - r * half;
-    table[i] = rotary_cos_sin((double)((int64_t)s0 + lo + r), a.inv_freq[p], a.mscale);
-  }
-  __syncthreads();
-  // x: the two vectors of item c of token lo + r
+  const int half = a.R / 2, groups = a.R / 16, stride = half + groups;
+  auto fill_table = [&](int from, int rows) {  // angles of tokens [from, from + rows)
+    for (int i = threadIdx.x; i < rows * half; i += kRwThreads) {
+      const int r = i / half, p = i - r * half;
+      table[r * stride + (p % V) * groups + p / V] =
+          rotary_cos_sin((double)((int64_t)s0 + from + r), a.inv_freq[p], a.mscale);
+    }
+    __syncthreads();
+  };
+  // x: the two vectors of item c of the table's row r
   auto turn = [&](int r, int c, float (&x)[16]) {
     float2 cs[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      cs[i] = r < kTableRows ? table[r * half + c * V + i]
-                             : rotary_cos_sin((double)((int64_t)s0 + lo + r), a.inv_freq[c * V + i], a.mscale);
+    for (int i = 0; i < V; ++i) cs[i] = table[r * stride + i * groups + c];
     rotary_turn<V>(x, cs, a.interleaved);
   };
+  // where unit u's rows come from and go to
+  struct Unit {
+    const char* src;
+    int64_t src_s;
+    float* scale;
+    uint8_t* codes;
+    int R;  // rotated dimensions (values: none)
+  };
+  auto unit_of = [&](int u) {
+    const int h = h0 + (u >> 1), part = u & 1;
+    Unit t;
+    t.src = part == 0 ? a.k_new + b * a.kn_b + h * a.kn_h : a.v_new + b * a.vn_b + h * a.vn_h;
+    t.src_s = part == 0 ? a.kn_s : a.vn_s;
+    t.scale = (part == 0 ? a.k_scale : a.v_scale) + phys * a.ss_block + (int64_t)h * a.ss_head;
+    t.codes = reinterpret_cast<uint8_t*>(part == 0 ? a.kcache : a.vcache) + phys * a.cs_block + (int64_t)h * a.cs_head;
+    t.R = part == 0 ? a.R : 0;
+    return t;
+  };
+  // tokens [from, from + n) of the unit, n <= 16, the first at the table's row `at`
+  auto load_tile = [&](const Unit& t, int from, int n, int at, float (&x)[PER][16]) {
+    uint4 w0[PER], w1[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = lane + 32 * k, r = i / NI;
+      const RotaryItem it = rotary_item(i % NI, V, t.R, a.interleaved);
+      w0[k] = w1[k] = make_uint4(0, 0, 0, 0);
+      if (r < n) {
+        const char* p = t.src + (int64_t)(from + r) * t.src_s;
+        w0[k] = *reinterpret_cast<const uint4*>(p + it.e0 * 2);
+        w1[k] = *reinterpret_cast<const uint4*>(p + it.e1 * 2);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = lane + 32 * k, r = i / NI;
+      widen16<BF16>(w0[k], w1[k], x[k]);
+      if (r < n && rotary_item(i % NI, V, t.R, a.interleaved).turned) turn(at + r, i % NI, x[k]);
+    }
+  };
+  auto tile_max = [&](const float (&x)[PER][16], float m) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[k][e]));
+    return m;
+  };
+  auto held_max = [&](const Unit& t, float old) {
+    float m = 0.f;
+#pragma unroll 1
+    for (int i = lane; i < held * (D / 8); i += 32) {
+      float y[8];
+      decode8(*reinterpret_cast<const uint2*>(t.codes + (int64_t)(i / (D / 8)) * a.cs_tok + (i % (D / 8)) * 8), old, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(y[e]));
+    }
+    return m;
+  };
+  auto recode_held = [&](const Unit& t, float old, float inv) {
+#pragma unroll 1
+    for (int i = lane; i < held * (D / 8); i += 32) {
+      uint2* w = reinterpret_cast<uint2*>(t.codes + (int64_t)(i / (D / 8)) * a.cs_tok + (i % (D / 8)) * 8);
+      float y[8];
+      decode8(*w, old, y);
+      *w = codes8(y, inv);
+    }
+  };
+  auto store_tile = [&](const Unit& t, int row, int n, const float (&x)[PER][16], float inv) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = lane + 32 * k, r = i / NI;
+      const RotaryItem it = rotary_item(i % NI, V, t.R, a.interleaved);
+      if (r < n) {
+        uint8_t* w = t.codes + (int64_t)(row + r) * a.cs_tok;
+        *reinterpret_cast<uint2*>(w + it.e0) = codes8(x[k], inv);
+        *reinterpret_cast<uint2*>(w + it.e1) = codes8(x[k] + 8, inv);
+      }
+    }
+  };
+  auto warp_max = [](float m) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+  };
+  // the query heads, and the rows of a 16-bit cache, tokens [from, from + rows): items one by one
+  auto stream_rows = [&](int from, int rows) {
+    const int nq = (h1 - h0) * a.G, heads = nq + (FP8 || !write ? 0 : 2 * (h1 - h0));
+    const int total = heads * rows * NI;
+    constexpr int U = 2;
+#pragma unroll 1
+    for (int i0 = threadIdx.x; i0 < total; i0 += U * kRwThreads) {
+      uint4 w0[U], w1[U];
+      char* to[U];
+      RotaryItem it[U];
+      int rc[U];  // table row x NI + item
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kRwThreads;
+        to[u] = nullptr;
+        if (i >= total) continue;
+        const int q = i / NI, c = i % NI, hh = q / rows, r = q - hh * rows;
+        rc[u] = r * NI + c;
+        const char* src;
+        int turned = a.R;
+        if (FP8 || hh < nq) {
+          const int hk = hh / a.G, h = h0 + hk, g = hh - hk * a.G;
+          src = a.q + b * a.qs_b + h * a.qs_h + g * a.qs_g + (int64_t)(from + r) * a.qs_s;
+          to[u] = a.out + b * a.os_b + h * a.os_h + g * a.os_g + (int64_t)(from + r) * a.os_s;
+        } else {
+          const int part = (hh - nq) & 1, h = h0 + ((hh - nq) >> 1);
+          src = part == 0 ? a.k_new + b * a.kn_b + h * a.kn_h + (int64_t)(from + r) * a.kn_s
+                          : a.v_new + b * a.vn_b + h * a.vn_h + (int64_t)(from + r) * a.vn_s;
+          to[u] = (part == 0 ? a.kcache : a.vcache) +
+                  (phys * a.cs_block + (int64_t)h * a.cs_head + (int64_t)(row0 + from - lo + r) * a.cs_tok) * 2;
+          if (part == 1) turned = 0;
+        }
+        it[u] = rotary_item(c, V, turned, a.interleaved);
+        w0[u] = *reinterpret_cast<const uint4*>(src + it[u].e0 * 2);
+        w1[u] = *reinterpret_cast<const uint4*>(src + it[u].e1 * 2);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (to[u] == nullptr) continue;
+        if (it[u].turned) {
+          float x[16];
+          widen16<BF16>(w0[u], w1[u], x);
+          turn(rc[u] / NI, rc[u] % NI, x);
+          w0[u] = narrow8<BF16>(x);
+          w1[u] = narrow8<BF16>(x + 8);
+        }
+        *reinterpret_cast<uint4*>(to[u] + it[u].e0 * 2) = w0[u];
+        *reinterpret_cast<uint4*>(to[u] + it[u].e1 * 2) = w1[u];
+      }
+    }
+  };
 
-  if constexpr (FP8) {
-    // one warp per (head, K or V): amax, scale, held rows, codes
-    for (int u = warp; write && u < 2 * (h1 - h0); u += kRwWarps) {
-      const int h = h0 + (u >> 1), part = u & 1;
-      const char* src = part == 0 ? a.k_new + b * a.kn_b + h * a.kn_h : a.v_new + b * a.vn_b + h * a.vn_h;
-      const int64_t src_s = part == 0 ? a.kn_s : a.vn_s;
-      float* sp = (part == 0 ? a.k_scale : a.v_scale) + phys * a.ss_block + (int64_t)h * a.ss_head;
-      uint8_t* c8 = reinterpret_cast<uint8_t*>(part == 0 ? a.kcache : a.vcache) + phys * a.cs_block +
-                    (int64_t)h * a.cs_head;
-      const float old = *sp;
-      const int ntile = (rows + kTileRows - 1) / kTileRows;
+  if constexpr (!MULTI) {
+    fill_table(lo, hi - lo);
+#pragma unroll 1
+    for (int u = warp; u < units; u += kRwWarps) {
+      const Unit t = unit_of(u);
+      const float old = *t.scale;
       float x[PER][16];
-      auto load_tile = [&](int t) {
-        uint4 w0[PER], w1[PER];
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const int i = lane + 32 * k, r = t * kTileRows + i / NI;
-          const RotaryItem it = rotary_item(i % NI, V, part == 0 ? a.R : 0, a.interleaved);
-          if (r < rows) {
-            const char* p = src + (int64_t)(lo + r) * src_s;
-            w0[k] = *reinterpret_cast<const uint4*>(p + it.e0 * 2);
-            w1[k] = *reinterpret_cast<const uint4*>(p + it.e1 * 2);
-          } else {
-            w0[k] = w1[k] = make_uint4(0, 0, 0, 0);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const int i = lane + 32 * k, r = t * kTileRows + i / NI;
-          widen16<BF16>(w0[k], w1[k], x[k]);
-          if (r < rows && rotary_item(i % NI, V, part == 0 ? a.R : 0, a.interleaved).turned) turn(r, i % NI, x[k]);
-        }
-      };
-      float m = 0.f;
-      for (int i = lane; i < held * (D / 8); i += 32) {
-        const int r = i / (D / 8), c = i % (D / 8);
-        float y[8];
-        decode8(*reinterpret_cast<const uint2*>(c8 + (int64_t)r * a.cs_tok + c * 8), old, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(y[e]));
-      }
-      for (int t = 0; t < ntile; ++t) {
-        load_tile(t);
-#pragma unroll
-        for (int k = 0; k < PER; ++k)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[k][e]));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      load_tile(t, lo, hi - lo, 0, x);
+      const float m = warp_max(tile_max(x, held_max(t, old)));
       const float scale = __fdiv_rn(fmaxf(m, 1e-6f), 448.f);
       const float inv = __frcp_rn(scale);
-      if (held > 0 && scale != old) {
-        for (int i = lane; i < held * (D / 8); i += 32) {
-          const int r = i / (D / 8), c = i % (D / 8);
-          uint2* w = reinterpret_cast<uint2*>(c8 + (int64_t)r * a.cs_tok + c * 8);
-          float y[8];
-          decode8(*w, old, y);
-          *w = codes8(y, inv);
-        }
-      }
-      for (int t = ntile - 1; t >= 0; --t) {  // the last tile is still in registers
-        if (t != ntile - 1) load_tile(t);
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const int i = lane + 32 * k, r = t * kTileRows + i / NI;
-          const RotaryItem it = rotary_item(i % NI, V, part == 0 ? a.R : 0, a.interleaved);
-          if (r < rows) {
-            uint8_t* w = c8 + (int64_t)(row0 + r) * a.cs_tok;
-            *reinterpret_cast<uint2*>(w + it.e0) = codes8(x[k], inv);
-            *reinterpret_cast<uint2*>(w + it.e1) = codes8(x[k] + 8, inv);
-          }
-        }
-      }
+      if (scale != old) recode_held(t, old, inv);
+      store_tile(t, row0, hi - lo, x, inv);
       __syncwarp();  // every lane has read `old` before it is replaced
-      if (lane == 0) *sp = scale;
+      if (lane == 0) *t.scale = scale;
     }
-  }
-
-  // the query heads, and the rows of a 16-bit cache: items one by one
-  const int nq = (h1 - h0) * a.G, heads = nq + (FP8 ? 0 : 2 * (h1 - h0));
-  const int total = heads * rows * NI;  // rows <= S, bounded on the host
-  constexpr int U = 4;
-  for (int i0 = threadIdx.x; i0 < total; i0 += U * kRwThreads) {
-    uint4 w0[U], w1[U];
-    char* to[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kRwThreads;
-      to[u] = nullptr;
-      if (i >= total) continue;
-      const int c = i % NI, r = (i / NI) % rows, hh = i / (NI * rows);
-      const char* src;
-      int turned = a.R;
-      if (hh < nq) {
-        const int h = h0 + hh / a.G, g = hh % a.G;
-        src = a.q + b * a.qs_b + h * a.qs_h + g * a.qs_g + (int64_t)(lo + r) * a.qs_s;
-        to[u] = a.out + b * a.os_b + h * a.os_h + g * a.os_g + (int64_t)(lo + r) * a.os_s;
-      } else {
-        const int part = (hh - nq) & 1, h = h0 + ((hh - nq) >> 1);
-        if (!write) continue;
-        src = part == 0 ? a.k_new + b * a.kn_b + h * a.kn_h + (int64_t)(lo + r) * a.kn_s
-                        : a.v_new + b * a.vn_b + h * a.vn_h + (int64_t)(lo + r) * a.vn_s;
-        to[u] = (part == 0 ? a.kcache : a.vcache) +
-                (phys * a.cs_block + (int64_t)h * a.cs_head + (int64_t)(row0 + r) * a.cs_tok) * 2;
-        if (part == 1) turned = 0;
+    stream_rows(lo, hi - lo);
+  } else {
+    const bool again = hi - lo > kTableRows;  // the angles do not fit at once
+    if (!again || units == 0) fill_table(lo, min(hi - lo, kTableRows));
+    if (units > 0) {
+#pragma unroll 1
+      for (int from = lo; from < hi; from += kTableRows) {
+        const int rows = min(hi - from, kTableRows);
+        if (again) {
+          __syncthreads();
+          fill_table(from, rows);
+        }
+#pragma unroll 1
+        for (int u = warp; u < units; u += kRwWarps) {
+          const Unit t = unit_of(u);
+          float m = from == lo ? held_max(t, *t.scale) : unit_max[u];
+#pragma unroll 1
+          for (int r = 0; r < rows; r += kTileRows) {
+            float x[PER][16];
+            load_tile(t, from + r, min(rows - r, kTileRows), r, x);
+            m = tile_max(x, m);
+          }
+          m = warp_max(m);
+          __syncwarp();
+          if (lane == 0) unit_max[u] = m;
+          __syncwarp();
+        }
       }
-      const RotaryItem it = rotary_item(c, V, turned, a.interleaved);
-      w0[u] = *reinterpret_cast<const uint4*>(src + it.e0 * 2);
-      w1[u] = *reinterpret_cast<const uint4*>(src + it.e1 * 2);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (to[u] == nullptr) continue;
-      const int i = i0 + u * kRwThreads;
-      const int c = i % NI, r = (i / NI) % rows, hh = i / (NI * rows);
-      const RotaryItem it = rotary_item(c, V, hh >= nq && ((hh - nq) & 1) ? 0 : a.R, a.interleaved);
-      if (it.turned) {
-        float x[16];
-        widen16<BF16>(w0[u], w1[u], x);
-        turn(r, c, x);
-        w0[u] = narrow8<BF16>(x);
-        w1[u] = narrow8<BF16>(x + 8);
+#pragma unroll 1
+    for (int from = lo; from < hi; from += kTableRows) {
+      const int rows = min(hi - from, kTableRows);
+      if (again && (units > 0 || from > lo)) {
+        __syncthreads();
+        fill_table(from, rows);
       }
-      *reinterpret_cast<uint4*>(to[u] + it.e0 * 2) = w0[u];
-      *reinterpret_cast<uint4*>(to[u] + it.e1 * 2) = w1[u];
+#pragma unroll 1
+      for (int u = warp; u < units; u += kRwWarps) {
+        const Unit t = unit_of(u);
+        const float old = *t.scale;
+        const float scale = __fdiv_rn(fmaxf(unit_max[u], 1e-6f), 448.f);
+        const float inv = __frcp_rn(scale);
+        if (from == lo && scale != old) recode_held(t, old, inv);
+#pragma unroll 1
+        for (int r = 0; r < rows; r += kTileRows) {
+          float x[PER][16];
+          load_tile(t, from + r, min(rows - r, kTileRows), r, x);
+          store_tile(t, row0 + from - lo + r, min(rows - r, kTileRows), x, inv);
+        }
+        __syncwarp();  // every lane has read `old` before it is replaced
+        if (lane == 0) *t.scale = scale;
+        __syncwarp();
+      }
+      stream_rows(from, rows);
     }
   }
 }
 
+template <int D, bool BF16, bool FP8, bool MULTI>
+int launch_rotary_write(const RotWriteArgs& a, dim3 grid, size_t smem, cudaStream_t st) {
+  auto kernel = rotary_write_kernel<D, BF16, FP8, MULTI>;
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return RBLN_ERR_LAUNCH;
+  kernel<<<grid, kRwThreads, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
+}
 template <int D, bool BF16>
 int launch_rotary_write(const RotWriteArgs& a, bool fp8, dim3 grid, size_t smem, cudaStream_t st) {
-  const void* fn = fp8 ? (const void*)rotary_write_kernel<D, BF16, true> : (const void*)rotary_write_kernel<D, BF16, false>;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return RBLN_ERR_LAUNCH;
-  if (fp8) rotary_write_kernel<D, BF16, true><<<grid, kRwThreads, smem, st>>>(a);
-  else rotary_write_kernel<D, BF16, false><<<grid, kRwThreads, smem, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
+  if (a.bs > kTileRows)
+    return fp8 ? launch_rotary_write<D, BF16, true, true>(a, grid, smem, st)
+               : launch_rotary_write<D, BF16, false, true>(a, grid, smem, st);
+  return fp8 ? launch_rotary_write<D, BF16, true, false>(a, grid, smem, st)
+             : launch_rotary_write<D, BF16, false, false>(a, grid, smem, st);
 }
 
 }  // namespace
@@ -348,11 +441,11 @@ extern "C" int rbln_rotary_paged_kv_write(const rbln_paged_attn_params_t* p, con
   a.slots = (int)slots;
   // All heads of a block in one CTA, unless that leaves the GPU short of CTAs
   // (about four an SM): then groups of KV heads, each finding the angles anew.
-  a.hg = a.Hkv;
+  a.hg = a.Hkv < 32 ? a.Hkv : 32;  // unit_max holds 64
   while (a.hg > 1 && slots * a.B * ((a.Hkv + a.hg - 1) / a.hg) < 4 * 148) a.hg = (a.hg + 1) / 2;
   const int gy = (a.Hkv + a.hg - 1) / a.hg;
   if (gy > 65535) return RBLN_ERR_UNSUPPORTED;
-  const size_t smem = (size_t)(block_rows < kTableRows ? block_rows : kTableRows) * (a.R / 2) * sizeof(float2);
+  const size_t smem = (size_t)(block_rows < kTableRows ? block_rows : kTableRows) * (a.R / 2 + a.R / 16) * sizeof(float2);
   const dim3 grid((unsigned)(slots * a.B), (unsigned)gy);
   const bool bf = p->q_dtype == RBLN_DT_BF16;
   if (p->head_dim == 128)

@@ -17,7 +17,9 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
@@ -434,25 +436,24 @@ std::tuple<at::Tensor, at::Tensor> call_rotary(const at::Tensor& q, const at::Te
 
 // The map is linear: the gradient is the transposed map of the outputs'
 // gradients, the same op (so it can be differentiated again).
-struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
-                                                const at::Tensor& k, const at::Tensor& positions,
-                                                const at::Tensor& inv_freq, bool interleaved, double mscale,
-                                                bool inverse) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto [qo, ko] = call_rotary(q, k, positions, inv_freq, interleaved, mscale, inverse);
-    ctx->save_for_backward({positions, inv_freq});
-    ctx->saved_data["interleaved"] = interleaved;
-    ctx->saved_data["mscale"] = mscale;
-    ctx->saved_data["inverse"] = inverse;
-    return {qo, ko};
+struct RotaryBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable positions, inv_freq;
+  at::TensorOptions options;
+  std::vector<int64_t> q_size, k_size;
+  bool interleaved, inverse;
+  double mscale;
+
+  std::string name() const override { return "RotaryBackward"; }
+  void release_variables() override {
+    positions.reset_data();
+    inv_freq.reset_data();
   }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
-                                                 torch::autograd::variable_list grad) {
-    const auto saved = ctx->get_saved_variables();
-    auto [dq, dk] = call_rotary(grad[0], grad[1], saved[0], saved[1], ctx->saved_data["interleaved"].toBool(),
-                                ctx->saved_data["mscale"].toDouble(), !ctx->saved_data["inverse"].toBool());
-    return {dq, dk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grad) override {
+    // an output that nothing used has no gradient: zeros stand for it
+    const at::Tensor gq = grad[0].defined() ? grad[0] : at::zeros(q_size, options);
+    const at::Tensor gk = grad[1].defined() ? grad[1] : at::zeros(k_size, options);
+    auto [dq, dk] = call_rotary(gq, gk, positions.unpack(), inv_freq.unpack(), interleaved, mscale, !inverse);
+    return {task_should_compute_output(0) ? dq : at::Tensor(), task_should_compute_output(1) ? dk : at::Tensor()};
   }
 };
 
@@ -460,10 +461,11 @@ std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at
                                                    const at::Tensor& positions, const at::Tensor& inv_freq,
                                                    bool interleaved, double mscale, bool inverse) {
   TORCH_CHECK(!inv_freq.requires_grad(), "rotary: inv_freq has no gradient (detach it)");
+  const bool graph = c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad());
   // A leaf of a graph that still lives has its gradient node on the stream of
   // that graph; a backward pass captured on another stream would make the
   // engine wait for it, which breaks the capture. Refused before that.
-  if (at::cuda::currentStreamCaptureStatus() != at::cuda::CaptureStatus::None) {
+  if (graph && at::cuda::currentStreamCaptureStatus() != at::cuda::CaptureStatus::None) {
     const c10::Stream now = at::cuda::getCurrentCUDAStream(q.device().index());
     for (const at::Tensor* t : {&q, &k}) {
       if (!t->requires_grad() || !t->is_leaf()) continue;
@@ -473,8 +475,26 @@ std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at
                   "free that graph before capturing, or capture with inputs of their own");
     }
   }
-  auto out = RotaryFunction::apply(q, k, positions, inv_freq, interleaved, mscale, inverse);
-  return {out[0], out[1]};
+  std::shared_ptr<RotaryBackward> node;
+  if (graph) {
+    node = std::shared_ptr<RotaryBackward>(new RotaryBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(q, k));
+    node->positions = torch::autograd::SavedVariable(positions, false);
+    node->inv_freq = torch::autograd::SavedVariable(inv_freq, false);
+    node->options = q.options();
+    node->q_size = q.sizes().vec();
+    node->k_size = k.sizes().vec();
+    node->interleaved = interleaved;
+    node->inverse = inverse;
+    node->mscale = mscale;
+  }
+  at::Tensor qo, ko;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    std::tie(qo, ko) = call_rotary(q, k, positions, inv_freq, interleaved, mscale, inverse);
+  }
+  if (node) torch::autograd::set_history(torch::autograd::variable_list{qo, ko}, node);
+  return {qo, ko};
 }
 
 // rbln_attn::rotary_paged_kv_write: q [B, Hkv, G, S, D] rotated and returned,
