@@ -73,62 +73,75 @@ __device__ __forceinline__ double position(const RotaryArgs& a, int b, int s) {
 
 // grid (ceil(tokens / tpb), head groups), 256 threads: thread = (token,
 // item, head lane), item fastest, so that 8 neighbours cover a 256-byte row.
+// The first heads' loads are issued before the angles are found, and each
+// step's next ones before its own are turned.
 template <typename T>
-__global__ void __launch_bounds__(kRotThreads, 4) rotary_vec_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotThreads, 3) rotary_vec_kernel(const RotaryArgs a) {
   constexpr int V = Vec<T>::N;
   extern __shared__ float2 table[];  // [tpb][R/2]
   const int half = a.R / 2;
   const int64_t tok0 = (int64_t)blockIdx.x * a.tpb;
+  const int c = threadIdx.x % a.items;
+  const int rest = threadIdx.x / a.items;
+  const int t = rest % a.tpb, hl = rest / a.tpb;
+  const bool live = hl < a.hp && tok0 + t < a.tokens;
+  const int b = live ? (int)((tok0 + t) / a.S) : 0, s = live ? (int)(tok0 + t - (int64_t)b * a.S) : 0;
+  const RotaryItem it = rotary_item(c, V, a.R, a.interleaved);
+  const int step = a.hp * (int)gridDim.y, first = live ? blockIdx.y * a.hp + hl : a.heads;
+  const T* qb = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + s * a.qs[2];
+  const T* kb = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + s * a.ks[2];
+  T* qo = reinterpret_cast<T*>(a.qo) + b * a.qos[0] + s * a.qos[2];
+  T* ko = reinterpret_cast<T*>(a.ko) + b * a.kos[0] + s * a.kos[2];
+  constexpr int U = 2;  // heads a step
+  struct Heads {
+    uint4 w[U][2];
+  };
+  auto load = [&](int h0, Heads& x) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * step;
+      if (h >= a.heads) break;
+      const T* src = h < a.H ? qb + h * a.qs[1] : kb + (h - a.H) * a.ks[1];
+      x.w[u][0] = *reinterpret_cast<const uint4*>(src + it.e0);
+      x.w[u][1] = *reinterpret_cast<const uint4*>(src + it.e1);
+    }
+  };
+  Heads now, next;
+  load(first, now);
+
   for (int i = threadIdx.x; i < a.tpb * half; i += kRotThreads) {
-    const int t = i / half, p = i - t * half;
-    if (tok0 + t >= a.tokens) break;
-    const int b = (int)((tok0 + t) / a.S), s = (int)(tok0 + t - (int64_t)b * a.S);
-    float2 cs = rotary_cos_sin(position(a, b, s), a.inv_freq[p], a.mscale);
+    const int r = i / half, p = i - r * half;
+    if (tok0 + r >= a.tokens) break;
+    const int rb = (int)((tok0 + r) / a.S), rs = (int)(tok0 + r - (int64_t)rb * a.S);
+    float2 cs = rotary_cos_sin(position(a, rb, rs), a.inv_freq[p], a.mscale);
     cs.y *= a.sin_sign;
     table[i] = cs;
   }
   __syncthreads();
-  const int c = threadIdx.x % a.items;
-  const int rest = threadIdx.x / a.items;
-  const int t = rest % a.tpb, hl = rest / a.tpb;
-  if (hl >= a.hp || tok0 + t >= a.tokens) return;
-  const int b = (int)((tok0 + t) / a.S), s = (int)(tok0 + t - (int64_t)b * a.S);
-  const RotaryItem it = rotary_item(c, V, a.R, a.interleaved);
   float2 cs[V];
   if (it.turned) {
 #pragma unroll
     for (int i = 0; i < V; ++i) cs[i] = table[t * half + c * V + i];
   }
-  const int step = a.hp * (int)gridDim.y;
-  constexpr int U = 2;  // heads whose loads are in flight together
-  for (int h0 = blockIdx.y * a.hp + hl; h0 < a.heads; h0 += U * step) {
-    uint4 w0[U], w1[U];
+  for (int h0 = first; h0 < a.heads; h0 += U * step) {
+    load(h0 + U * step, next);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int h = h0 + u * step;
       if (h >= a.heads) break;
-      const T* src = h < a.H ? reinterpret_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[1] + s * a.qs[2]
-                             : reinterpret_cast<const T*>(a.k) + b * a.ks[0] + (h - a.H) * a.ks[1] + s * a.ks[2];
-      w0[u] = *reinterpret_cast<const uint4*>(src + it.e0);
-      w1[u] = *reinterpret_cast<const uint4*>(src + it.e1);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * step;
-      if (h >= a.heads) break;
-      T* dst = h < a.H ? reinterpret_cast<T*>(a.qo) + b * a.qos[0] + h * a.qos[1] + s * a.qos[2]
-                       : reinterpret_cast<T*>(a.ko) + b * a.kos[0] + (h - a.H) * a.kos[1] + s * a.kos[2];
+      T* dst = h < a.H ? qo + h * a.qos[1] : ko + (h - a.H) * a.kos[1];
       if (it.turned) {
         float x[2 * V];
-        Vec<T>::load(w0[u], x);
-        Vec<T>::load(w1[u], x + V);
+        Vec<T>::load(now.w[u][0], x);
+        Vec<T>::load(now.w[u][1], x + V);
         rotary_turn<V>(x, cs, a.interleaved);
-        w0[u] = Vec<T>::store(x);
-        w1[u] = Vec<T>::store(x + V);
+        now.w[u][0] = Vec<T>::store(x);
+        now.w[u][1] = Vec<T>::store(x + V);
       }
-      *reinterpret_cast<uint4*>(dst + it.e0) = w0[u];
-      *reinterpret_cast<uint4*>(dst + it.e1) = w1[u];
+      *reinterpret_cast<uint4*>(dst + it.e0) = now.w[u][0];
+      *reinterpret_cast<uint4*>(dst + it.e1) = now.w[u][1];
     }
+    now = next;
   }
 }
 

@@ -15,9 +15,7 @@
 // block) and a group of KV heads with their query heads: the angles depend on
 // the token alone, so their sines and cosines are found once for the block,
 // in shared memory. q (and the rows of a 16-bit cache) stream through all
-// threads; a warp takes one (head, K or V) of an fp8 cache, 16 rows at a
-// time, in registers from the amax to the codes: a block of 16 rows is read
-// once, a larger one twice (its last 16 rows once).
+// threads, two 16-byte loads and stores an item.
 
 #include "rotary.cuh"
 
@@ -26,8 +24,8 @@ namespace {
 
 constexpr int kRwThreads = 256;
 constexpr int kRwWarps = kRwThreads / 32;
-constexpr int kTileRows = 16;
-constexpr int kTableRows = 128;  // rows whose angles are kept at once
+constexpr int kTableRows = 128;  // rows whose angles a streaming CTA keeps at once
+constexpr int kStageRows = 16;   // rows a quantising CTA holds in shared memory
 
 struct RotWriteArgs {
   const char* q;
@@ -48,7 +46,9 @@ struct RotWriteArgs {
   int bt_dtype;
   int64_t bt_stride;
   const float* inv_freq;
-  int B, Hkv, G, S, R, bs, max_blocks, num_blocks, slots, hg;  // hg: KV heads a CTA
+  int B, Hkv, G, S, R, bs, max_blocks, num_blocks, slots;
+  int hg, kv_groups, sg;  // KV heads a quantising CTA, its groups; KV heads a streaming CTA
+  uint32_t g_mul, g_shift;  // n / G = (mulhi(n, g_mul) + n) >> g_shift, n < 2^30
   bool interleaved;
   float mscale;
   uint32_t* err;
@@ -95,29 +95,40 @@ __device__ __forceinline__ void decode8(uint2 w, float s, float (&x)[8]) {
   }
 }
 
-// MULTI: blocks of more than 16 rows. Their rows are taken 128 at a time (the
-// angles kept in shared memory), an fp8 cache's twice: for the amax, then for
-// the codes. Blocks of up to 16 rows stay in registers in between.
-template <int D, bool BF16, bool FP8, bool MULTI>
-__global__ void __launch_bounds__(kRwThreads, FP8 && D == 128 ? 2 : 3) rotary_write_kernel(const RotWriteArgs a) {
-  constexpr int V = 8, NI = D / 16;           // items a row
-  constexpr int PER = kTileRows * NI / 32;    // items a lane of a 16-row tile
-  // [rows][V][R / 16] pairs, a row padded so that the lanes of neighbouring
-  // rows meet other banks: pair c V + i of a row at i R/16 + c
-  extern __shared__ float2 table[];
-  __shared__ float unit_max[MULTI ? 64 : 1];  // an fp8 block's amax so far, of each (head, K or V)
+// 16 bytes global -> shared in the background.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// grid (blocks touched x sequences, kv_groups + stream_groups): the first
+// kv_groups CTAs of a block quantise groups of KV heads of an fp8 cache, the
+// others stream groups of query heads (and a 16-bit cache's rows).
+//
+// A quantising CTA copies 16 rows of its heads' keys and values into shared
+// memory, all of them on their way at once, finds the angles meanwhile, and
+// then works out of shared memory, one warp a (head, K or V): the amax, held
+// rows among it, then the codes. A block of more than 16 rows passes twice.
+// The loops are rolled: most launches are a few microseconds long, and a
+// 16-row tile unrolled in registers spent them fetching instructions.
+template <int D, bool BF16, bool FP8>
+__global__ void __launch_bounds__(kRwThreads, 4) rotary_write_kernel(const RotWriteArgs a) {
+  constexpr int V = 8, NI = D / 16;  // items a row
+  extern __shared__ __align__(16) unsigned char dsm[];
+  // (cos, sin) of two pairs a float4: pairs c V + 2 i and c V + 2 i + 1 of a
+  // row at i R/16 + c, so that the eight items of a row meet all banks once
+  float4* table = reinterpret_cast<float4*>(dsm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int j = blockIdx.x % a.slots, b = blockIdx.x / a.slots;
-  const int h0 = blockIdx.y * a.hg, h1 = min(h0 + a.hg, a.Hkv);
   const int s0 = a.seq[b * a.seq_stride];
   // row of the first token in its block (s0 may be negative: refused below)
   const int p0 = ((s0 % a.bs) + a.bs) % a.bs;
   const int lo = max(j * a.bs - p0, 0), hi = (int)min((int64_t)(j + 1) * a.bs - p0, (int64_t)a.S);
   if (lo >= hi) return;  // tokens [lo, hi) fall in this block
+  const bool quantise = FP8 && (int)blockIdx.y < a.kv_groups;
 
   // write target: the block's pool index, or none
-  bool write = true;
-  if (s0 < 0 || (int64_t)s0 + a.S > (int64_t)a.max_blocks * a.bs) {
+  bool write = quantise || !FP8;
+  if (write && (s0 < 0 || (int64_t)s0 + a.S > (int64_t)a.max_blocks * a.bs)) {
     write = false;
     if (threadIdx.x == 0 && a.err) atomicOr(a.err, RBLN_DEVERR_SEQ_RANGE);
   }
@@ -129,144 +140,194 @@ __global__ void __launch_bounds__(kRwThreads, FP8 && D == 128 ? 2 : 3) rotary_wr
       if (threadIdx.x == 0 && a.err) atomicOr(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
     }
   }
-  const int row0 = j == 0 ? p0 : 0;            // block row of token lo
-  const int held = j == 0 && s0 > 0 ? p0 : 0;  // block rows the sequence holds already
-  const int units = FP8 && write ? 2 * (h1 - h0) : 0;  // (head, K or V) of an fp8 cache, one a warp
+  const int row0 = j == 0 ? p0 : 0;  // block row of token lo
 
-  const int half = a.R / 2, groups = a.R / 16, stride = half + groups;
+  const int half = a.R / 2, groups = a.R / 16, stride = a.R / 4;
   auto fill_table = [&](int from, int rows) {  // angles of tokens [from, from + rows)
+#pragma unroll 1
     for (int i = threadIdx.x; i < rows * half; i += kRwThreads) {
       const int r = i / half, p = i - r * half;
-      table[r * stride + (p % V) * groups + p / V] =
+      float4* to = table + r * stride + (p % V) / 2 * groups + p / V;
+      reinterpret_cast<float2*>(to)[p & 1] =
           rotary_cos_sin((double)((int64_t)s0 + from + r), a.inv_freq[p], a.mscale);
     }
-    __syncthreads();
   };
   // x: the two vectors of item c of the table's row r
   auto turn = [&](int r, int c, float (&x)[16]) {
     float2 cs[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) cs[i] = table[r * stride + i * groups + c];
+    for (int i = 0; i < V / 2; ++i) {
+      const float4 w = table[r * stride + i * groups + c];
+      cs[2 * i] = make_float2(w.x, w.y);
+      cs[2 * i + 1] = make_float2(w.z, w.w);
+    }
     rotary_turn<V>(x, cs, a.interleaved);
   };
-  // where unit u's rows come from and go to
-  struct Unit {
-    const char* src;
-    int64_t src_s;
-    float* scale;
-    uint8_t* codes;
-    int R;  // rotated dimensions (values: none)
-  };
-  auto unit_of = [&](int u) {
-    const int h = h0 + (u >> 1), part = u & 1;
-    Unit t;
-    t.src = part == 0 ? a.k_new + b * a.kn_b + h * a.kn_h : a.v_new + b * a.vn_b + h * a.vn_h;
-    t.src_s = part == 0 ? a.kn_s : a.vn_s;
-    t.scale = (part == 0 ? a.k_scale : a.v_scale) + phys * a.ss_block + (int64_t)h * a.ss_head;
-    t.codes = reinterpret_cast<uint8_t*>(part == 0 ? a.kcache : a.vcache) + phys * a.cs_block + (int64_t)h * a.cs_head;
-    t.R = part == 0 ? a.R : 0;
-    return t;
-  };
-  // tokens [from, from + n) of the unit, n <= 16, the first at the table's row `at`
-  auto load_tile = [&](const Unit& t, int from, int n, int at, float (&x)[PER][16]) {
-    uint4 w0[PER], w1[PER];
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int i = lane + 32 * k, r = i / NI;
-      const RotaryItem it = rotary_item(i % NI, V, t.R, a.interleaved);
-      w0[k] = w1[k] = make_uint4(0, 0, 0, 0);
-      if (r < n) {
-        const char* p = t.src + (int64_t)(from + r) * t.src_s;
-        w0[k] = *reinterpret_cast<const uint4*>(p + it.e0 * 2);
-        w1[k] = *reinterpret_cast<const uint4*>(p + it.e1 * 2);
+
+  if (quantise) {
+    if (!write) return;
+    const int h0 = blockIdx.y * a.hg, h1 = min(h0 + a.hg, a.Hkv), units = 2 * (h1 - h0);
+    const int held = j == 0 && s0 > 0 ? p0 : 0;  // block rows the sequence holds already
+    // rows [unit][16][D] after the angles of 16 rows; each unit's amax
+    unsigned char* stage = dsm + kStageRows * stride * sizeof(float4);
+    float* unit_max = reinterpret_cast<float*>(stage + a.hg * 2 * kStageRows * D * 2);
+    auto fetch = [&](int from, int rows) {
+      constexpr int C = D / 8;  // 16-byte pieces a row
+      for (int i = threadIdx.x; i < units * rows * C; i += kRwThreads) {
+        const int c = i % C, z = i / C, u = z / rows, r = z - u * rows, h = h0 + (u >> 1);
+        const char* src = u & 1 ? a.v_new + b * a.vn_b + h * a.vn_h + (int64_t)(from + r) * a.vn_s
+                                : a.k_new + b * a.kn_b + h * a.kn_h + (int64_t)(from + r) * a.kn_s;
+        copy16(stage + ((u * kStageRows + r) * C + c) * 16, src + c * 16);
       }
-    }
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int i = lane + 32 * k, r = i / NI;
-      widen16<BF16>(w0[k], w1[k], x[k]);
-      if (r < n && rotary_item(i % NI, V, t.R, a.interleaved).turned) turn(at + r, i % NI, x[k]);
-    }
-  };
-  auto tile_max = [&](const float (&x)[PER][16], float m) {
-#pragma unroll
-    for (int k = 0; k < PER; ++k)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[k][e]));
-    return m;
-  };
-  auto held_max = [&](const Unit& t, float old) {
-    float m = 0.f;
+      fill_table(from, rows);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncthreads();
+    };
+    // item i of unit u's rows in shared memory: its 16 values, turned
+    auto item = [&](int u, int i, RotaryItem& it, float (&x)[16]) {
+      const int r = i / NI, c = i % NI;
+      it = rotary_item(c, V, u & 1 ? 0 : a.R, a.interleaved);
+      const unsigned char* p = stage + (u * kStageRows + r) * D * 2;
+      widen16<BF16>(*reinterpret_cast<const uint4*>(p + it.e0 * 2), *reinterpret_cast<const uint4*>(p + it.e1 * 2), x);
+      if (it.turned) turn(r, c, x);
+    };
+    auto scale_of = [&](int u) {
+      return (u & 1 ? a.v_scale : a.k_scale) + phys * a.ss_block + (int64_t)(h0 + (u >> 1)) * a.ss_head;
+    };
+    auto codes_of = [&](int u) {
+      return reinterpret_cast<uint8_t*>(u & 1 ? a.vcache : a.kcache) + phys * a.cs_block +
+             (int64_t)(h0 + (u >> 1)) * a.cs_head;
+    };
+    auto held_piece = [&](uint8_t* codes, int i) {
+      return reinterpret_cast<uint2*>(codes + (int64_t)(i / (D / 8)) * a.cs_tok + (i % (D / 8)) * 8);
+    };
+    auto amax = [&](int from, int rows) {
 #pragma unroll 1
-    for (int i = lane; i < held * (D / 8); i += 32) {
-      float y[8];
-      decode8(*reinterpret_cast<const uint2*>(t.codes + (int64_t)(i / (D / 8)) * a.cs_tok + (i % (D / 8)) * 8), old, y);
+      for (int u = warp; u < units; u += kRwWarps) {
+        float m = from == lo ? 0.f : unit_max[u];
+        if (from == lo) {
+          const float old = *scale_of(u);
+          uint8_t* codes = codes_of(u);
+#pragma unroll 4
+          for (int i = lane; i < held * (D / 8); i += 32) {
+            float y[8];
+            decode8(*held_piece(codes, i), old, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(y[e]));
-    }
-    return m;
-  };
-  auto recode_held = [&](const Unit& t, float old, float inv) {
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(y[e]));
+          }
+        }
 #pragma unroll 1
-    for (int i = lane; i < held * (D / 8); i += 32) {
-      uint2* w = reinterpret_cast<uint2*>(t.codes + (int64_t)(i / (D / 8)) * a.cs_tok + (i % (D / 8)) * 8);
-      float y[8];
-      decode8(*w, old, y);
-      *w = codes8(y, inv);
-    }
-  };
-  auto store_tile = [&](const Unit& t, int row, int n, const float (&x)[PER][16], float inv) {
+        for (int i = lane; i < rows * NI; i += 32) {
+          RotaryItem it;
+          float x[16];
+          item(u, i, it, x);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int i = lane + 32 * k, r = i / NI;
-      const RotaryItem it = rotary_item(i % NI, V, t.R, a.interleaved);
-      if (r < n) {
-        uint8_t* w = t.codes + (int64_t)(row + r) * a.cs_tok;
-        *reinterpret_cast<uint2*>(w + it.e0) = codes8(x[k], inv);
-        *reinterpret_cast<uint2*>(w + it.e1) = codes8(x[k] + 8, inv);
+          for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        __syncwarp();
+        if (lane == 0) unit_max[u] = m;
+        __syncwarp();
       }
-    }
-  };
-  auto warp_max = [](float m) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
-  };
-  // the query heads, and the rows of a 16-bit cache, tokens [from, from + rows): items one by one
-  auto stream_rows = [&](int from, int rows) {
-    const int nq = (h1 - h0) * a.G, heads = nq + (FP8 || !write ? 0 : 2 * (h1 - h0));
-    const int total = heads * rows * NI;
-    constexpr int U = 2;
+    };
+    auto encode = [&](int from, int rows) {
 #pragma unroll 1
-    for (int i0 = threadIdx.x; i0 < total; i0 += U * kRwThreads) {
+      for (int u = warp; u < units; u += kRwWarps) {
+        uint8_t* codes = codes_of(u);
+        const float old = *scale_of(u);
+        const float scale = __fdiv_rn(fmaxf(unit_max[u], 1e-6f), 448.f);
+        const float inv = __frcp_rn(scale);
+        if (from == lo && scale != old) {
+#pragma unroll 4
+          for (int i = lane; i < held * (D / 8); i += 32) {
+            float y[8];
+            decode8(*held_piece(codes, i), old, y);
+            *held_piece(codes, i) = codes8(y, inv);
+          }
+        }
+#pragma unroll 1
+        for (int i = lane; i < rows * NI; i += 32) {
+          RotaryItem it;
+          float x[16];
+          item(u, i, it, x);
+          uint8_t* w = codes + (int64_t)(row0 + from - lo + i / NI) * a.cs_tok;
+          *reinterpret_cast<uint2*>(w + it.e0) = codes8(x, inv);
+          *reinterpret_cast<uint2*>(w + it.e1) = codes8(x + 8, inv);
+        }
+        __syncwarp();  // every lane has read `old` before it is replaced
+        if (lane == 0) *scale_of(u) = scale;
+        __syncwarp();
+      }
+    };
+#pragma unroll 1
+    for (int from = lo; from < hi; from += kStageRows) {
+      if (from > lo) __syncthreads();  // the rows before have been read
+      fetch(from, min(hi - from, kStageRows));
+      amax(from, min(hi - from, kStageRows));
+    }
+#pragma unroll 1
+    for (int from = lo; from < hi; from += kStageRows) {
+      if (hi - lo > kStageRows) {
+        __syncthreads();
+        fetch(from, min(hi - from, kStageRows));
+      }
+      encode(from, min(hi - from, kStageRows));
+    }
+    return;
+  }
+
+  // The query heads, and the rows of a 16-bit cache: a thread keeps its item
+  // of a row and walks (head, row), row fastest.
+  const int h0 = (blockIdx.y - a.kv_groups) * a.sg, h1 = min(h0 + a.sg, a.Hkv);
+  const int nq = (h1 - h0) * a.G, heads = nq + (write ? 2 * (h1 - h0) : 0);
+  constexpr int STEP = kRwThreads / NI, U = 2;  // rows a step; steps whose loads are in flight
+  const int c = threadIdx.x % NI, z = threadIdx.x / NI;
+  const RotaryItem turned = rotary_item(c, V, a.R, a.interleaved), passed = rotary_item(c, V, 0, false);
+#pragma unroll 1
+  for (int from = lo; from < hi; from += kTableRows) {
+    const int rows = min(hi - from, kTableRows);
+    if (from > lo) __syncthreads();
+    fill_table(from, rows);
+    __syncthreads();
+    const int dh = STEP / rows, dr = STEP - dh * rows;
+    const char* qb = a.q + b * a.qs_b + h0 * a.qs_h + (int64_t)from * a.qs_s;
+    char* ob = a.out + b * a.os_b + h0 * a.os_h + (int64_t)from * a.os_s;
+    int hh = z / rows, r = z - hh * rows;
+#pragma unroll 1
+    while (hh < heads) {
       uint4 w0[U], w1[U];
       char* to[U];
       RotaryItem it[U];
-      int rc[U];  // table row x NI + item
+      int row[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * kRwThreads;
         to[u] = nullptr;
-        if (i >= total) continue;
-        const int q = i / NI, c = i % NI, hh = q / rows, r = q - hh * rows;
-        rc[u] = r * NI + c;
-        const char* src;
-        int turned = a.R;
-        if (FP8 || hh < nq) {
-          const int hk = hh / a.G, h = h0 + hk, g = hh - hk * a.G;
-          src = a.q + b * a.qs_b + h * a.qs_h + g * a.qs_g + (int64_t)(from + r) * a.qs_s;
-          to[u] = a.out + b * a.os_b + h * a.os_h + g * a.os_g + (int64_t)(from + r) * a.os_s;
-        } else {
-          const int part = (hh - nq) & 1, h = h0 + ((hh - nq) >> 1);
-          src = part == 0 ? a.k_new + b * a.kn_b + h * a.kn_h + (int64_t)(from + r) * a.kn_s
-                          : a.v_new + b * a.vn_b + h * a.vn_h + (int64_t)(from + r) * a.vn_s;
-          to[u] = (part == 0 ? a.kcache : a.vcache) +
-                  (phys * a.cs_block + (int64_t)h * a.cs_head + (int64_t)(row0 + from - lo + r) * a.cs_tok) * 2;
-          if (part == 1) turned = 0;
+        row[u] = r;
+        it[u] = turned;
+        if (hh < heads) {
+          const char* src;
+          if (FP8 || hh < nq) {
+            const int hk = (int)((__umulhi((uint32_t)hh, a.g_mul) + (uint32_t)hh) >> a.g_shift), g = hh - hk * a.G;
+            src = qb + hk * a.qs_h + g * a.qs_g + r * a.qs_s;
+            to[u] = ob + hk * a.os_h + g * a.os_g + r * a.os_s;
+          } else {
+            const int part = (hh - nq) & 1, h = h0 + ((hh - nq) >> 1);
+            src = part == 0 ? a.k_new + b * a.kn_b + h * a.kn_h + (int64_t)(from + r) * a.kn_s
+                            : a.v_new + b * a.vn_b + h * a.vn_h + (int64_t)(from + r) * a.vn_s;
+            to[u] = (part == 0 ? a.kcache : a.vcache) +
+                    (phys * a.cs_block + (int64_t)h * a.cs_head + (int64_t)(row0 + from - lo + r) * a.cs_tok) * 2;
+            if (part == 1) it[u] = passed;
+          }
+          w0[u] = *reinterpret_cast<const uint4*>(src + it[u].e0 * 2);
+          w1[u] = *reinterpret_cast<const uint4*>(src + it[u].e1 * 2);
+          hh += dh;
+          r += dr;
+          if (r >= rows) {
+            r -= rows;
+            ++hh;
+          }
         }
-        it[u] = rotary_item(c, V, turned, a.interleaved);
-        w0[u] = *reinterpret_cast<const uint4*>(src + it[u].e0 * 2);
-        w1[u] = *reinterpret_cast<const uint4*>(src + it[u].e1 * 2);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -274,7 +335,7 @@ __global__ void __launch_bounds__(kRwThreads, FP8 && D == 128 ? 2 : 3) rotary_wr
         if (it[u].turned) {
           float x[16];
           widen16<BF16>(w0[u], w1[u], x);
-          turn(rc[u] / NI, rc[u] % NI, x);
+          turn(row[u], c, x);
           w0[u] = narrow8<BF16>(x);
           w1[u] = narrow8<BF16>(x + 8);
         }
@@ -282,98 +343,17 @@ __global__ void __launch_bounds__(kRwThreads, FP8 && D == 128 ? 2 : 3) rotary_wr
         *reinterpret_cast<uint4*>(to[u] + it[u].e1 * 2) = w1[u];
       }
     }
-  };
-
-  if constexpr (!MULTI) {
-    fill_table(lo, hi - lo);
-#pragma unroll 1
-    for (int u = warp; u < units; u += kRwWarps) {
-      const Unit t = unit_of(u);
-      const float old = *t.scale;
-      float x[PER][16];
-      load_tile(t, lo, hi - lo, 0, x);
-      const float m = warp_max(tile_max(x, held_max(t, old)));
-      const float scale = __fdiv_rn(fmaxf(m, 1e-6f), 448.f);
-      const float inv = __frcp_rn(scale);
-      if (scale != old) recode_held(t, old, inv);
-      store_tile(t, row0, hi - lo, x, inv);
-      __syncwarp();  // every lane has read `old` before it is replaced
-      if (lane == 0) *t.scale = scale;
-    }
-    stream_rows(lo, hi - lo);
-  } else {
-    const bool again = hi - lo > kTableRows;  // the angles do not fit at once
-    if (!again || units == 0) fill_table(lo, min(hi - lo, kTableRows));
-    if (units > 0) {
-#pragma unroll 1
-      for (int from = lo; from < hi; from += kTableRows) {
-        const int rows = min(hi - from, kTableRows);
-        if (again) {
-          __syncthreads();
-          fill_table(from, rows);
-        }
-#pragma unroll 1
-        for (int u = warp; u < units; u += kRwWarps) {
-          const Unit t = unit_of(u);
-          float m = from == lo ? held_max(t, *t.scale) : unit_max[u];
-#pragma unroll 1
-          for (int r = 0; r < rows; r += kTileRows) {
-            float x[PER][16];
-            load_tile(t, from + r, min(rows - r, kTileRows), r, x);
-            m = tile_max(x, m);
-          }
-          m = warp_max(m);
-          __syncwarp();
-          if (lane == 0) unit_max[u] = m;
-          __syncwarp();
-        }
-      }
-    }
-#pragma unroll 1
-    for (int from = lo; from < hi; from += kTableRows) {
-      const int rows = min(hi - from, kTableRows);
-      if (again && (units > 0 || from > lo)) {
-        __syncthreads();
-        fill_table(from, rows);
-      }
-#pragma unroll 1
-      for (int u = warp; u < units; u += kRwWarps) {
-        const Unit t = unit_of(u);
-        const float old = *t.scale;
-        const float scale = __fdiv_rn(fmaxf(unit_max[u], 1e-6f), 448.f);
-        const float inv = __frcp_rn(scale);
-        if (from == lo && scale != old) recode_held(t, old, inv);
-#pragma unroll 1
-        for (int r = 0; r < rows; r += kTileRows) {
-          float x[PER][16];
-          load_tile(t, from + r, min(rows - r, kTileRows), r, x);
-          store_tile(t, row0 + from - lo + r, min(rows - r, kTileRows), x, inv);
-        }
-        __syncwarp();  // every lane has read `old` before it is replaced
-        if (lane == 0) *t.scale = scale;
-        __syncwarp();
-      }
-      stream_rows(from, rows);
-    }
   }
 }
 
-template <int D, bool BF16, bool FP8, bool MULTI>
-int launch_rotary_write(const RotWriteArgs& a, dim3 grid, size_t smem, cudaStream_t st) {
-  auto kernel = rotary_write_kernel<D, BF16, FP8, MULTI>;
+template <int D, bool BF16>
+int launch_rotary_write(const RotWriteArgs& a, bool fp8, dim3 grid, size_t smem, cudaStream_t st) {
+  auto kernel = fp8 ? rotary_write_kernel<D, BF16, true> : rotary_write_kernel<D, BF16, false>;
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return RBLN_ERR_LAUNCH;
   kernel<<<grid, kRwThreads, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
-}
-template <int D, bool BF16>
-int launch_rotary_write(const RotWriteArgs& a, bool fp8, dim3 grid, size_t smem, cudaStream_t st) {
-  if (a.bs > kTileRows)
-    return fp8 ? launch_rotary_write<D, BF16, true, true>(a, grid, smem, st)
-               : launch_rotary_write<D, BF16, false, true>(a, grid, smem, st);
-  return fp8 ? launch_rotary_write<D, BF16, true, false>(a, grid, smem, st)
-             : launch_rotary_write<D, BF16, false, false>(a, grid, smem, st);
 }
 
 }  // namespace
@@ -430,6 +410,9 @@ extern "C" int rbln_rotary_paged_kv_write(const rbln_paged_attn_params_t* p, con
   a.B = p->batch; a.Hkv = p->num_kv_heads; a.G = p->group; a.S = p->q_len; a.R = r->rotary_dim; a.bs = p->block_size;
   a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
   a.interleaved = r->interleaved != 0;
+  for (a.g_shift = 0; (1u << a.g_shift) < (uint32_t)a.G; ++a.g_shift) {
+  }
+  a.g_mul = (uint32_t)(((uint64_t)((1u << a.g_shift) - (uint32_t)a.G) << 32) / (uint32_t)a.G + 1);
   a.mscale = r->mscale;
   a.err = p->error_flags;
   // blocks a sequence's tokens can touch: S rows from anywhere in a block
@@ -439,13 +422,20 @@ extern "C" int rbln_rotary_paged_kv_write(const rbln_paged_attn_params_t* p, con
   // a CTA's items are counted in 32 bits
   if ((int64_t)a.Hkv * (a.G + 2) * block_rows * (p->head_dim / 16) > (1 << 30)) return RBLN_ERR_UNSUPPORTED;
   a.slots = (int)slots;
-  // All heads of a block in one CTA, unless that leaves the GPU short of CTAs
-  // (about four an SM): then groups of KV heads, each finding the angles anew.
-  a.hg = a.Hkv < 32 ? a.Hkv : 32;  // unit_max holds 64
-  while (a.hg > 1 && slots * a.B * ((a.Hkv + a.hg - 1) / a.hg) < 4 * 148) a.hg = (a.hg + 1) / 2;
-  const int gy = (a.Hkv + a.hg - 1) / a.hg;
+  const int64_t work = ((int64_t)a.S + a.bs - 1) / a.bs * a.B;  // blocks that are touched, about
+  // Four KV heads a quantising CTA: one (head, K or V) a warp, 32 KB of rows.
+  // A streaming CTA takes all heads of a block, or a group of them where that
+  // leaves the GPU short of CTAs (three an SM), down to one KV head.
+  a.hg = a.Hkv < 4 ? a.Hkv : 4;
+  a.kv_groups = fp8 ? (a.Hkv + a.hg - 1) / a.hg : 0;
+  a.sg = a.Hkv;
+  while (a.sg > 1 && work * ((a.Hkv + a.sg - 1) / a.sg) < 3 * 148) a.sg = (a.sg + 1) / 2;
+  const int64_t gy = a.kv_groups + (a.Hkv + a.sg - 1) / a.sg;
   if (gy > 65535) return RBLN_ERR_UNSUPPORTED;
-  const size_t smem = (size_t)(block_rows < kTableRows ? block_rows : kTableRows) * (a.R / 2 + a.R / 16) * sizeof(float2);
+  const size_t angles = (size_t)(a.R / 4) * sizeof(float4);
+  const size_t stream_smem = angles * (block_rows < kTableRows ? block_rows : kTableRows);
+  const size_t quant_smem = fp8 ? angles * kStageRows + (size_t)a.hg * 2 * (kStageRows * p->head_dim * 2 + sizeof(float)) : 0;
+  const size_t smem = stream_smem > quant_smem ? stream_smem : quant_smem;
   const dim3 grid((unsigned)(slots * a.B), (unsigned)gy);
   const bool bf = p->q_dtype == RBLN_DT_BF16;
   if (p->head_dim == 128)
