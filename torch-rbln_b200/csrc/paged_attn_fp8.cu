@@ -32,7 +32,7 @@ namespace {
 constexpr int kMqWarps = 4;
 constexpr int kMqThreads = kMqWarps * 32;
 constexpr int kMqTile = 32;     // keys a warp's tile
-constexpr int kSegCost = 128;   // virtual keys charged to each unit's start
+constexpr int kSegCost = 256;   // virtual keys charged to each unit's start
 constexpr int kMinW = 256;      // smallest share of a CTA, in keys
 constexpr int kMaxItems = 4096; // (sequence, row tile) items whose prefix a CTA holds in shared memory
 
@@ -237,15 +237,12 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
   };
   // the first tiles on their way before the queries are looked at
   const int step = kMqWarps * kMqTile, first = t0 + warp * kMqTile;
-  Entry ent;
-  entry(first, ent);
-#pragma unroll
-  for (int st = 0; st < R::STAGES - 1; ++st) {
-    const int ts = first + st * step;
-    if (ts < t1) issue(st, ent);
-    else copy_commit();
-    entry(ts + step, ent);
-  }
+  static_assert(R::STAGES == 2, "one tile ahead");
+  Entry e0, ent;
+  entry(first, e0);
+  entry(first + step, ent);  // both look-ups at once
+  if (first < t1) issue(0, e0);
+  else copy_commit();
 
   // query fragments (B operand: k = head_dim, n = column gid + 8 nt) in f16
   uint32_t qf[NT][KR];
@@ -328,24 +325,26 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
 #pragma unroll
       for (int k = 0; k < 8; ++k) s[nt][k] = 0.f;
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
+    for (int i = 0; i < KCH; ++i) {
+      uint4 kr[4];
 #pragma unroll
-      for (int i = 0; i < KCH; ++i) {
-        const uint4 k0 = *reinterpret_cast<const uint4*>(stage + R::K + R::k_at(16 * sub + gid, 4 * i + tig));
-        const uint4 k1 = *reinterpret_cast<const uint4*>(stage + R::K + R::k_at(16 * sub + gid + 8, 4 * i + tig));
-        const uint32_t r0[4] = {k0.x, k0.y, k0.z, k0.w}, r1[4] = {k1.x, k1.y, k1.z, k1.w};
+      for (int r = 0; r < 4; ++r)
+        kr[r] = *reinterpret_cast<const uint4*>(stage + R::K + R::k_at(8 * r + gid, 4 * i + tig));
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 4; ++w) {
+        const int kk = 4 * i + w;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
           uint32_t a0, a1, a2, a3;
-          e4m3x4_to_f16x2x2(r0[w], a0, a2);
-          e4m3x4_to_f16x2x2(r1[w], a1, a3);
-          const int kk = 4 * i + w;
+          e4m3x4_to_f16x2x2(reinterpret_cast<const uint32_t*>(&kr[2 * sub])[w], a0, a2);
+          e4m3x4_to_f16x2x2(reinterpret_cast<const uint32_t*>(&kr[2 * sub + 1])[w], a1, a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
             mma16816<false>(reinterpret_cast<float(&)[4]>(s[nt][4 * sub]), a0, a1, a2, a3, qf[nt][2 * kk],
                             qf[nt][2 * kk + 1]);
         }
       }
+    }
     // V scales relative to vref; positive floats order as their bits
     const uint32_t vmaxb = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs[lane], 0.f)));
     if (__uint_as_float(vmaxb) > vref) {
@@ -443,16 +442,14 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
 
   int st = 0;
   for (int ts = first; ts < t1; ts += step) {
-    const int ahead = ts + (R::STAGES - 1) * step;
-    const int to = st == 0 ? R::STAGES - 1 : st - 1;  // the stage used last
-    if (ahead < t1) issue(to, ent);
+    if (ts + step < t1) issue(st ^ 1, ent);
     else copy_commit();
-    entry(ahead + step, ent);  // the look-up of the tile after it
-    copy_wait<R::STAGES - 1>();
+    entry(ts + 2 * step, ent);  // the look-up of the tile after it
+    copy_wait<1>();
     __syncwarp();
     consume(ts, st);
     __syncwarp();
-    st = st == R::STAGES - 1 ? 0 : st + 1;
+    st ^= 1;
   }
   copy_wait<0>();
   __syncwarp();
@@ -805,8 +802,8 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
     cost_prefix<C::THREADS>(a, 128, 1, kTcSegCost, keys, misc + 8, P);
     if (threadIdx.x == 0) {
       const int64_t T = P[a.items], total = T * a.Hkv;
-      // at least four tiles a CTA; fewer CTAs work then
-      const int64_t W = max((total + gridDim.x - 1) / gridDim.x, (int64_t)(4 + kTcSegCost));
+      // at least a tile a CTA; fewer CTAs work then
+      const int64_t W = max((total + gridDim.x - 1) / gridDim.x, (int64_t)(1 + kTcSegCost));
       const int64_t lo = min(W * blockIdx.x, total), hi = min(lo + W, total);
       int i = 0;
       int64_t h = 0;
