@@ -171,10 +171,14 @@ int rbln_paged_prefill_workspace_size(const rbln_paged_attn_params_t* p, size_t*
  * {8, 16, 32, 64, 128} or a multiple of 128. No workspace.
  *
  * kv_dtype FP8_E4M3 (q bf16 or f16, k_scale / v_scale required, D and
- * block_size as above, any S_q from one token up): the new rows are written by
- * the rule of rbln_paged_kv_write, which finds the scales of the touched
- * blocks anew (a sequence whose rows would pass the table's span is not
- * written), and attention reads them back with the rest. k_new / v_new NULL:
+ * block_size as above, any S_q from one token up): the new rows are written as
+ * rbln_paged_kv_write writes them, with the scales of the touched blocks found
+ * anew (a sequence whose rows would pass the table's span is not written), and
+ * attention reads them back with the rest. The scale here is
+ * max(amax, 1e-6) * (1 / 448) with the reciprocal rounded to float32, as torch
+ * computes `amax / 448.0` on the GPU, so a cache filled by this call holds bit
+ * for bit what one quantised by torch there holds; rbln_paged_kv_write divides,
+ * and its scales differ from these by at most one unit in the last place. k_new / v_new NULL:
  * the rows [seq[b], seq[b] + S_q) are in the cache already
  * (rbln_rotary_paged_kv_write). A key in a block outside the pool, at or past
  * the span, or not kept by the mask is not seen, whatever its bytes hold; a

@@ -78,3 +78,38 @@ def assert_within(got, ref, bound, what=""):
 def fp8_values(cache, scale):
     """Codes times scales, float64, [num_blocks, Hkv, 1, bs, D]."""
     return cache.double() * scale.double()[:, :, None, None, None]
+
+
+def write_reciprocal(k, v, kcache, vcache, seq, table, bs, k_scale, v_scale):
+    """The fp8 write of paged_causal_attn_prefill_kvfp8, in place: oracle.paged_attention.kv_write with
+    scale = max(amax, 1e-6) * (1 / 448), the reciprocal rounded to float32 (what torch computes on the GPU for
+    amax / 448.0). A sequence whose start is negative or whose rows pass the span is left."""
+    B, Hkv, _, S, D = k.shape
+    third = torch.tensor(1.0) / torch.tensor(448.0)
+    for b in range(B):
+        n = int(seq.reshape(-1)[b])
+        if n < 0 or n + S > table.shape[1] * bs:
+            continue
+        for j in range(n // bs, (n + S - 1) // bs + 1):
+            p = int(table[b, j])
+            if not 0 <= p < kcache.shape[0]:
+                continue
+            lo, hi = max(n, j * bs), min(n + S, (j + 1) * bs)
+            held = max(0, min(n - j * bs, bs))
+            for cache, new, scales in ((kcache, k, k_scale), (vcache, v, v_scale)):
+                rows = new[b, :, 0, lo - n: hi - n].float()  # [Hkv, rows, D]
+                old = scales[p].clone()
+                was = cache[p, :, 0, :held, :D].float() * old[:, None, None]
+                amax = torch.cat([was, rows], 1).abs().amax((1, 2))
+                scale = amax.clamp_min(1e-6) * third
+                inv = (1.0 / scale)[:, None, None]
+
+                def codes(x):
+                    return (x * inv).clamp(-448, 448).to(torch.float8_e4m3fn)
+
+                moved = (scale != old)[:, None, None]
+                if held:
+                    keep = cache[p, :, 0, :held, :D].view(torch.uint8)
+                    cache.view(torch.uint8)[p, :, 0, :held, :D] = torch.where(moved, codes(was).view(torch.uint8), keep)
+                cache.view(torch.uint8)[p, :, 0, lo - j * bs: hi - j * bs, :D] = codes(rows).view(torch.uint8)
+                scales[p] = scale

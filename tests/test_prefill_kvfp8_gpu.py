@@ -1,4 +1,4 @@
-"""paged_causal_attn_prefill_kvfp8: caches and scales bit for bit the oracle's
+"""paged_causal_attn_prefill_kvfp8: caches and scales bit for bit the plain
 write, the output within the bounds of tests/operator_refs.py of float64
 attention over what the cache then holds."""
 
@@ -7,7 +7,6 @@ import math
 import pytest
 import torch
 
-from oracle import paged_attention as opa
 from tests import operator_refs as R
 
 pytestmark = pytest.mark.gpu
@@ -66,10 +65,7 @@ def reference(d, both=False, mask=None, rows=True):
     bs, bt = d["bs"], d["bt"].long()
     span = bt.shape[1] * bs
     if rows:
-        for b in range(B):
-            if 0 <= int(d["seq"][b]) and int(d["seq"][b]) + S <= span:
-                opa.kv_write(d["k"][b:b + 1], d["v"][b:b + 1], d["kc"], d["vc"], d["seq"][b:b + 1], bt[b:b + 1], bs,
-                             d["ks"], d["vs"])
+        R.write_reciprocal(d["k"], d["v"], d["kc"], d["vc"], d["seq"], bt, bs, d["ks"], d["vs"])
     outs, bounds = [], []
     t = torch.arange(span)
     for b in range(B):
@@ -394,3 +390,22 @@ def test_a_served_prompt():
             want, size = R.rotary(q[b].cpu().reshape(1, Hkv * G, S, D), pos, f.cpu(), False, m)
             R.assert_within(rq[b].reshape(1, Hkv * G, S, D), want, R.rotary_bound(want, size, torch.bfloat16))
         seq = seq + S
+
+
+def test_scales_are_those_of_torch_and_near_the_cache_writes():
+    """The scales are what torch computes on the GPU for amax / 448.0, and within one unit in the last place of
+    paged_kv_write's, which divides."""
+    d = setup([0, 0, 0], 64, 4, 2, 64, 16, seed=11)
+    x, y = dev(d), dev(d)
+    run(x)
+    torch.ops.rbln_attn.paged_kv_write(y["k"], y["v"], y["kc"], y["vc"], y["seq"], y["bt"], y["bs"], y["ks"], y["vs"])
+    differ = 0
+    for b in range(3):
+        for j in range(4):
+            p = int(d["bt"][b, j])
+            amax = x["k"][b, :, 0, 16 * j: 16 * j + 16].float().abs().amax((1, 2))
+            assert torch.equal(x["ks"][p], amax.clamp_min(1e-6) / 448.0)
+            bits = (x["ks"][p].view(torch.int32) - y["ks"][p].view(torch.int32)).abs()
+            assert int(bits.max()) <= 1
+            differ += int(bits.sum())
+    assert differ > 0

@@ -52,8 +52,17 @@ struct WriteArgs {
   int bt_dtype;
   int64_t bt_stride;
   int B, Hkv, S, D, bs, max_blocks, num_blocks;
+  int reciprocal;  // see block_scale
   uint32_t* err;
 };
+
+// A block's scale from its amax: amax / 448, or, for the prefill over an fp8
+// cache, amax * (1 / 448) with the reciprocal rounded to float32, which is
+// what torch computes on the GPU for `amax / 448.0`.
+__device__ __forceinline__ float block_scale(const WriteArgs& a, float amax) {
+  const float m = fmaxf(amax, 1e-6f);
+  return a.reciprocal ? m * (1.f / kFp8Max) : __fdiv_rn(m, kFp8Max);
+}
 
 __device__ __forceinline__ float from_e4m3(uint8_t q) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)q, __NV_E4M3);
@@ -190,7 +199,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_kv_write_kernel(const Wri
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
     }
-    const float scale = __fdiv_rn(fmaxf(warp_max(m), 1e-6f), kFp8Max);
+    const float scale = block_scale(a, warp_max(m));
     const float inv = __frcp_rn(scale);
     if (held > 0 && scale != old) {
       for (int i = lane; i < held * cpr; i += 32) {
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_kv_write_staged_kernel(co
     const float2 f = unpack2<IN_BF16>(am);
     m = fmaxf(m, fmaxf(f.x, f.y));
   }
-  const float scale = __fdiv_rn(fmaxf(warp_max(m), 1e-6f), kFp8Max);
+  const float scale = block_scale(a, warp_max(m));
   const float inv = __frcp_rn(scale);
   if (held > 0 && scale != old) {
     for (int i = lane; i < held * cpr; i += 32) {
@@ -327,10 +336,10 @@ __global__ void __launch_bounds__(kWriteThreads) paged_kv_write_staged_kernel(co
 }
 
 }  // namespace
-}  // namespace rbln
 
-extern "C" int rbln_paged_kv_write(const rbln_paged_attn_params_t* p, cudaStream_t stream) {
-  using namespace rbln;
+// rbln_paged_kv_write, and the write of the prefill over an fp8 cache
+// (paged_attn_fp8.cu), which finds its scales by the reciprocal.
+int kv_write(const rbln_paged_attn_params_t* p, cudaStream_t stream, bool reciprocal) {
   if (!p || p->batch < 0 || p->num_kv_heads <= 0 || p->q_len < 0 || p->block_size <= 0 || p->max_blocks <= 0 ||
       p->num_blocks <= 0)
     return RBLN_ERR_INVALID_ARGUMENT;
@@ -370,6 +379,7 @@ extern "C" int rbln_paged_kv_write(const rbln_paged_attn_params_t* p, cudaStream
   a.bt = p->block_table; a.bt_dtype = p->block_table_dtype; a.bt_stride = p->block_table_stride;
   a.B = p->batch; a.Hkv = p->num_kv_heads; a.S = p->q_len; a.D = p->head_dim; a.bs = p->block_size;
   a.max_blocks = p->max_blocks; a.num_blocks = p->num_blocks;
+  a.reciprocal = reciprocal;
   a.err = p->error_flags;
   // blocks one sequence's write can touch: S rows starting anywhere in a block
   const int slots = (p->q_len + p->block_size - 1) / p->block_size + 1;
@@ -389,4 +399,10 @@ extern "C" int rbln_paged_kv_write(const rbln_paged_attn_params_t* p, cudaStream
     else paged_kv_write_kernel<false, false><<<grid, kWriteThreads, 0, stream>>>(a, slots);
   }
   return cudaGetLastError() == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
+}
+
+}  // namespace rbln
+
+extern "C" int rbln_paged_kv_write(const rbln_paged_attn_params_t* p, cudaStream_t stream) {
+  return rbln::kv_write(p, stream, false);
 }

@@ -1,8 +1,8 @@
 // Attention of S_q new tokens a sequence over an fp8-e4m3 paged KV cache with
 // one fp32 scale for each (block, KV head): the kv_dtype FP8_E4M3 form of
-// rbln_paged_causal_attn_prefill. The new rows are written first, by the rule
-// of rbln_paged_kv_write (scales of touched blocks found anew), and read back
-// with the rest.
+// rbln_paged_causal_attn_prefill. The new rows are written first, as
+// rbln_paged_kv_write writes them (scales of touched blocks found anew, but as
+// amax * (1 / 448)), and read back with the rest.
 //
 //   out[s] = sum_t p_st v_t / sum_t p_st,  p_st = exp(scale q_s . k_t)
 // over the keys t <= seq[b] + s (causal) or t < seq[b] + S_q (both ways) that
@@ -27,6 +27,9 @@
 #include "tma_map.cuh"
 
 namespace rbln {
+
+int kv_write(const rbln_paged_attn_params_t* p, cudaStream_t stream, bool reciprocal);  // kv_write.cu
+
 namespace {
 
 constexpr int kMqWarps = 4;
@@ -1632,7 +1635,7 @@ int run_prefill_fp8(const rbln_paged_attn_params_t* p, cudaStream_t st) {
   if (rc != RBLN_OK) return rc;
   if (pl.total > 0 && (!p->workspace || p->workspace_bytes < pl.total)) return RBLN_ERR_WORKSPACE;
   if (p->k_new) {
-    rc = rbln_paged_kv_write(p, st);
+    rc = kv_write(p, st, /*reciprocal=*/true);
     if (rc != RBLN_OK) return rc;
   }
   Fp8Args a{};
