@@ -409,3 +409,38 @@ def test_scales_are_those_of_torch_and_near_the_cache_writes():
             assert int(bits.max()) <= 1
             differ += int(bits.sum())
     assert differ > 0
+
+
+@pytest.mark.parametrize("S", [1, 4, 40])
+def test_scales_that_are_not_numbers(S):
+    """A NaN scale of a block that is seen gives NaN, for K and for V; of a block that the mask drops, nothing."""
+    for name in ("ks", "vs"):
+        d = setup([200, 90], S, 2, 4, 64, 16)
+        d[name][d["bt"][0, 2].item()] = float("nan")  # keys 32 to 47 of sequence 0
+        x = dev(d)
+        out = run(x)
+        assert torch.isnan(out[0]).all() and not torch.isnan(out[1]).any()
+        mask = torch.ones([2, 300], dtype=torch.bool)
+        mask[0, 32:48] = False
+        out = run(x, mask=mask.to(DEV), rows=False)
+        assert not torch.isnan(out).any()
+
+
+@pytest.mark.parametrize("S", [1, 4, 40])
+def test_bad_query_rows_stay_alone(S):
+    """Inf and NaN in one query row: NaN in its output, no other touched. And the largest finite bf16 queries."""
+    d = setup([150], S, 2, 4, 64, 16)
+    clean = run(dev(d))
+    d["q"][0, 1, 2, S - 1, 5] = float("inf")
+    d["q"][0, 0, 1, 0, 7] = float("nan")
+    x = dev(d)
+    out = run(x)
+    assert torch.isnan(out[0, 0, 1, 0]).all()
+    keep = torch.ones([1, 2, 4, S], dtype=torch.bool)
+    keep[0, 1, 2, S - 1] = keep[0, 0, 1, 0] = False
+    assert torch.equal(out[keep.to(DEV)], clean[keep.to(DEV)])
+    d = setup([90], S, 2, 4, 64, 16)
+    big = torch.finfo(torch.bfloat16).max
+    d["q"] = (d["q"].float() / 8 * big).clamp(-big, big).to(torch.bfloat16)
+    d["scale"] = torch.tensor(0.25 * 2.0 ** -126)
+    assert not torch.isnan(run(dev(d))).any()

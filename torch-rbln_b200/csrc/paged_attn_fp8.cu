@@ -91,7 +91,7 @@ __device__ __forceinline__ float pow2_above(float x) {
 // its inverse; 1 for rows of zeros, infinities or NaN.
 __device__ __forceinline__ float f16_factor(float m, float& undo) {
   undo = 1.f;
-  if (!(m > 0.f && m < 3e38f)) return 1.f;
+  if (!(m > 0.f && m <= 3.4028235e38f)) return 1.f;
   const int e = (int)(__float_as_uint(m) >> 23) - 127;  // m in [2^e, 2^(e+1)), or subnormal
   const int k = min(max(14 - e, -120), 120);
   undo = __uint_as_float((uint32_t)(127 - k) << 23);
@@ -689,17 +689,29 @@ enum TcBar {
   T_DONE = 35, T_COUNT = 36
 };
 
-// What a group's raw scores are multiplied by, above zero also where a scale
-// is zero, so that -inf stays -inf.
-__device__ __forceinline__ float score_mult(float ks, float mult) { return fmaxf(ks * mult, 1.2e-38f); }
+// Keys of bf16 queries are multiplied by 2^-17: then no sum of D <= 256
+// products of a code (at most 448) and a finite bf16 reaches 2^128.
+constexpr float kKeyUp = 131072.f;
 
-// Eight f16 that stand for codes as bf16, exact: a code has four bits.
+// What raw scores are multiplied by besides their key's scale. The sign of a
+// negative softmax scale is in the converted keys; and it is above zero, so
+// that -inf stays -inf.
+template <bool BF16>
+__device__ __forceinline__ float score_mult(const Fp8Args& a) {
+  return fmaxf(fabsf(a.scale_dev ? *a.scale_dev : a.scale) * (BF16 ? kKeyUp * kLog2e : kLog2e), 1.2e-38f);
+}
+
+// Eight f16 that stand for codes as bf16 times 2^-17, exact: a code has four
+// bits. One packed product: f32 products before the rounding take the same
+// time (389 us against 387 for 8 sequences of 512 queries behind 512 to 7680
+// keys, 32 heads of 128 over 8 KV heads).
 __device__ __forceinline__ uint4 f16_to_bf16(uint4 w) {
   uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = unpack2<false>(u[i]);
     u[i] = pack2<true>(f.x, f.y);
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(u[i]) : "r"(0x37003700u));
   }
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
@@ -887,7 +899,10 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           const uint32_t turn = part == 0 ? flip : 0u;
           const uint8_t* src = sgen + L::R0 + rs * L::RAW + row0 * D + c16 * 16;
           uint8_t* dst = sgen + (part ? L::V0 : L::K0) + st * L::TILE + row0 * 128 + dst_panel;
-#pragma unroll 4
+          // two steps a turn: instruction fetch bounds this kernel (one, two, four steps:
+          // 386, 387, 404 us for 8 sequences of 512 queries behind 512 to 7680 keys, 251, 250,
+          // 257 for 4 of 48 queries behind 18432 to 30720; eight: a third slower than two)
+#pragma unroll 2
           for (int k = 0; k < STEPS; ++k) {
             uint2 w0 = *reinterpret_cast<const uint2*>(src + k * 4 * RPI * D + swap);
             uint2 w1 = *reinterpret_cast<const uint2*>(src + k * 4 * RPI * D + 8 - swap);
@@ -1076,6 +1091,10 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
       }
     } else if (warp == W0 + 2) {
       // ---------------------------------------------------------- scales
+      // K scales leave here between these two, so that their product with
+      // `mult` is above zero, and finite where the scale is
+      const float mult = score_mult<BF16>(a);
+      const float klo = 1.2e-38f / mult, khi = 3.4e38f / mult;
       int T = 0;
       bool ok = true;
       while (ok && next_segment<NX>(a, qt, sh, g)) {
@@ -1100,6 +1119,12 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
               keep = key < a.mask_len && load_keep(a.mask, a.mask_dtype, g.b * a.mask_stride + key);
             kw[w] = __ballot_sync(0xffffffffu, keep);
           }
+          // a group none of whose keys is kept: its scales may be anything
+          const uint32_t word = grp < 8 ? (grp < 4 ? kw[0] : kw[1]) : (grp < 12 ? kw[2] : kw[3]);
+          if (((word >> (8 * (grp & 3))) & 0xffu) == 0) {
+            ks = 1.f;
+            vs = 0.f;
+          }
           const uint32_t vmax = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.f)));
           if (T >= kMetaRing &&
               !__all_sync(0xffffffffu, wait_for(bar(T_ME + ms), ((T / kMetaRing) - 1) & 1, abort))) {
@@ -1107,7 +1132,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
             break;
           }
           if (lane < 16) {
-            meta[ms].ks[lane] = ks;
+            meta[ms].ks[lane] = ks < klo ? klo : (ks > khi && ks <= 3.4028235e38f) ? khi : ks;
             meta[ms].vs[lane] = vs;
           }
           if (lane == 0) {
@@ -1126,8 +1151,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
     const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const int gq = r / qt, i = r - gq * qt;
-    // the sign of a negative softmax scale is in the converted keys
-    const float mult = fabsf(a.scale_dev ? *a.scale_dev : a.scale) * kLog2e;
+    const float mult = score_mult<BF16>(a);
     int T = 0, act = 0, TX = 0;  // tiles of the CTA; segments and tiles of this row tile
     int cont = -1, start = -1;
     bool ok = true;
@@ -1197,7 +1221,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const float* w = q + u * 8;
-            mg[u] = fmaxf(max3(max3(w[0], w[1], w[2]), w[3], w[4]), max3(w[5], w[6], w[7])) * score_mult(k4[u], mult);
+            mg[u] = fmaxf(max3(max3(w[0], w[1], w[2]), w[3], w[4]), max3(w[5], w[6], w[7])) * (k4[u] * mult);
           }
           mt = fmaxf(mt, max3(mg[0], mg[1], fmaxf(mg[2], mg[3])));
         };
@@ -1258,7 +1282,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           tmem_wait_ld32(v);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float km = score_mult(k4[u], mult), vr = v4[u] * inv_vref;
+            const float km = k4[u] * mult, vr = v4[u] * inv_vref;
 #pragma unroll
             for (int e = 8 * u; e < 8 * u + 8; e += 2) {
               fma2(p[e], p[e + 1], km, km, nmu, nmu);
