@@ -10,8 +10,9 @@
 // v_t = vs d_t, c and d the e4m3 codes of a block and ks, vs its scales, the
 // products run on the codes: every code is exact in f16, ks multiplies the
 // score in float32 and vs the probability, which is rounded to f16 once.
-// A bf16 query goes to f16 with a power of two of its row, so that its largest
-// magnitude lies in [2^14, 2^15): exact down to 2^-28 of the row's largest.
+// Few rows: a bf16 query goes to f16 with a power of two of its row, so that
+// its largest magnitude lies in [2^14, 2^15): exact down to 2^-28 of the row's
+// largest. Many rows: the keys go to bf16 instead, exact too.
 // The probabilities' vs is taken relative to a running power of two (vref) at
 // or above the largest scale seen, so a cache of small values keeps all of
 // f16's bits and one of large values cannot overflow; the accumulator is
@@ -35,7 +36,9 @@ namespace {
 constexpr int kMqWarps = 4;
 constexpr int kMqThreads = kMqWarps * 32;
 constexpr int kMqTile = 32;     // keys a warp's tile
-constexpr int kSegCost = 256;   // virtual keys charged to each unit's start
+// Virtual keys charged to each unit's start: 64, 128, 256, 384, 512 took 111,
+// 108, 103, 103, 103 us for 64 sequences of 4 tokens behind 128 to 4096 keys.
+constexpr int kSegCost = 256;
 constexpr int kMinW = 256;      // smallest share of a CTA, in keys
 constexpr int kMaxItems = 4096; // (sequence, row tile) items whose prefix a CTA holds in shared memory
 
@@ -141,12 +144,16 @@ __device__ __forceinline__ void cost_prefix(const Fp8Args& a, int unit, int scal
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (S_q G up to 16 of a KV head a tile): bound by HBM, one read of
-// the cached bytes. As in the one-token decode, tokens are the M side of
-// mma.m16n8k16 and the rows (token s, head g), s G + g, the N side, so that a
-// tile's codes go from 16-byte loads to f16 fragments in registers; four warps
-// take 16-key tiles round-robin and are joined in shared memory. The keys of
-// all (head, sequence) units are cut into equal shares, one CTA each.
+// Few rows (S_q G up to 16 of a KV head): one read of the cached bytes. As in
+// the one-token decode, tokens are the M side of mma.m16n8k16 and the rows
+// (token s, head g), s G + g, the N side, so that a tile's codes go from
+// shared memory to f16 fragments in registers; four warps take 32-key tiles
+// round-robin, each with a ring of two filled by cp.async, and are joined in
+// shared memory. The keys of all (head, sequence) units are cut into equal
+// shares, one CTA each, three CTAs an SM (two: 110 us against 102 for 64
+// sequences of 4 tokens, G = 4, 8 KV heads, behind 128 to 4096 keys). There it
+// reads 2.7 TB/s, 42 % of the copy rate: latency of 12 warps an SM and the
+// segments' starts bound it (copies alone 82 us, products alone 77).
 // ---------------------------------------------------------------------------
 // A warp's ring of tiles in shared memory, filled by cp.async. Rows are
 // swizzled by 16-byte chunks so that the fragments' loads meet no bank twice:
@@ -600,10 +607,14 @@ __global__ void __launch_bounds__(kMqThreads, kMqCtas) paged_attn_fp8_rows_kerne
 //   convert     four warps: codes to f16 in the 128-byte-swizzled operand
 //               layout, V rows that no query may see as zeros;
 //   MMA         one thread: S = Q K^T, O += P V, accumulators in TMEM.
-// f16 operands take every code exactly, so no scale enters the operands and
-// the conversion is one instruction for two codes; reading codes instead of
-// 16-bit rows halves HBM and L2 traffic. Shared memory (D = 128, NX = 2):
-// Q 64 KB, K and V 2 x 32 KB each, raw 2 x 16 KB.
+// Both 16-bit types take every code exactly, so no scale enters the operands;
+// V and the keys of f16 queries are f16 (one instruction for two codes), the
+// keys of bf16 queries bf16. Reading codes instead of 16-bit rows halves HBM
+// and L2 traffic. Shared memory (D = 128, NX = 2): Q 64 KB, K and V 2 x 32 KB
+// each, raw 2 x 16 KB. Loops are rolled: instruction fetch bounds the kernel
+// (the chunk below took 633 us unrolled). It measures 387 us, 754 TFLOP/s, for
+// 8 sequences of 512 queries behind 512 to 7680 keys: the chain from a row
+// tile's scores through its softmax to its product bounds it.
 //
 // The key tiles of all units, head-major, are cut into equal shares, one a
 // CTA, so that there is one wave without a tail however unequal the
@@ -637,7 +648,7 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile
 }
 
 constexpr int kPanel = 128 * 128;  // 128 rows of 64 f16
-constexpr int kTcSegCost = 2;      // key tiles charged to a unit's start
+constexpr int kTcSegCost = 2;      // key tiles charged to a unit's start (1, 2, 3: 395, 390, 391 us for that chunk)
 constexpr int kMetaRing = 4;
 
 struct TileMeta {
@@ -836,7 +847,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
       misc[3] = i;
       misc[5] = (int)(hi - lo);
     }
-    fence_proxy_async_smem();  // the prefix's area is written by TMA next
+    fence_proxy_async_smem();  // the prefix lay where the keys go, which the MMA reads
   } else if (threadIdx.x == 0) {
     misc[2] = (int)(blockIdx.x % a.Hkv);
     misc[3] = (int)(blockIdx.x / a.Hkv);
@@ -1500,9 +1511,14 @@ size_t rows_smem(int D, int rows, int items) {
 int plan_fp8(const rbln_paged_attn_params_t* p, Fp8Plan* pl) {
   const int64_t span = (int64_t)p->max_blocks * p->block_size;
   const int64_t rows = (int64_t)p->q_len * p->group;
-  // Up to 16 rows of a KV head the row kernel reads the codes once; more
-  // rows would read them again for each 16, so they go to 128-row tiles.
-  // (which also takes pools of over 64 GB: the row kernel's offsets are 32 bits of 16 bytes)
+  // Up to 16 rows of a KV head the row kernel reads the codes once; more rows
+  // would read them again for each 16, so they go to 128-row tiles. 16
+  // sequences behind 4096 keys, row kernel against tiles: 62 to 99 us at 8
+  // rows, 74 to 99 at 16, 101 to 99 at 20, 134 to 101 at 48.
+  // (Pools of over 64 GB take the tiles too: the row kernel's offsets are 32 bits of 16 bytes.)
+  // Two row tiles share a key tile's conversion where there are over 128 rows:
+  // one tile against two, same sequences: 105 to 111 us at 128 rows, 169 to
+  // 124 at 160, 310 to 216 at 512.
   const int64_t pool = (int64_t)p->num_blocks * p->cache_stride[0];
   pl->nx = rows <= 16 && pool >> 4 <= (int64_t)UINT32_MAX ? 0 : rows <= 128 ? 1 : 2;
   pl->nt = rows <= 8 ? 1 : 2;

@@ -15,7 +15,11 @@
 // block) and a group of KV heads with their query heads: the angles depend on
 // the token alone, so their sines and cosines are found once for the block,
 // in shared memory. q (and the rows of a 16-bit cache) stream through all
-// threads, two 16-byte loads and stores an item.
+// threads, two 16-byte loads and stores an item; the rows that are quantised
+// wait in shared memory between their amax and their codes (held in registers
+// by an unrolled tile: 65.7 us against 26.6 for 8 sequences of 512 tokens, and
+// 16.4 against 10.3 for 256 of one; instruction fetch bounded that). The 512
+// tokens run at 3.5 TB/s, 53 % of the copy rate.
 
 #include "rotary.cuh"
 
@@ -423,9 +427,14 @@ extern "C" int rbln_rotary_paged_kv_write(const rbln_paged_attn_params_t* p, con
   if ((int64_t)a.Hkv * (a.G + 2) * block_rows * (p->head_dim / 16) > (1 << 30)) return RBLN_ERR_UNSUPPORTED;
   a.slots = (int)slots;
   const int64_t work = ((int64_t)a.S + a.bs - 1) / a.bs * a.B;  // blocks that are touched, about
-  // Four KV heads a quantising CTA: one (head, K or V) a warp, 32 KB of rows.
+  // Four KV heads a quantising CTA: one (head, K or V) a warp, 32 KB of rows
+  // (one, two, four heads: 128, 100, 90 us for 32 sequences of 512 tokens, 32
+  // query heads over 8 KV heads of 128; equal for a step of one token).
   // A streaming CTA takes all heads of a block, or a group of them where that
-  // leaves the GPU short of CTAs (three an SM), down to one KV head.
+  // leaves the GPU short of CTAs (three an SM), down to one KV head. Same
+  // heads, all against this rule against one head: 17.2, 12.3, 13.2 us for 1
+  // sequence of 512 tokens, 34.8, 31.6, 36.8 for 8 of them, 88.8, 90.0, 117
+  // for 32, and 14.3, 16.3, 22.5 for 256 of one token.
   a.hg = a.Hkv < 4 ? a.Hkv : 4;
   a.kv_groups = fp8 ? (a.Hkv + a.hg - 1) / a.hg : 0;
   a.sg = a.Hkv;
