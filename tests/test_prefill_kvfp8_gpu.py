@@ -444,3 +444,34 @@ def test_bad_query_rows_stay_alone(S):
     d["q"] = (d["q"].float() / 8 * big).clamp(-big, big).to(torch.bfloat16)
     d["scale"] = torch.tensor(0.25 * 2.0 ** -126)
     assert not torch.isnan(run(dev(d))).any()
+
+
+@pytest.mark.parametrize("S", [1, 4, 40])
+def test_softmax_scales_at_the_ends(S):
+    """NaN gives NaN; zero the mean of the keys, for the largest finite queries too."""
+    d = setup([150], S, 2, 4, 64, 16)
+    d["scale"] = torch.tensor(float("nan"))
+    assert torch.isnan(run(dev(d))).all()
+    for big in (False, True):
+        d = setup([150], S, 2, 4, 64, 16)
+        d["scale"] = torch.tensor(0.0)
+        x = dev(d)
+        if big:
+            x["q"] = torch.full_like(x["q"], torch.finfo(torch.bfloat16).max)
+        out = run(x)
+        d["q"].zero_()
+        want, bound = reference(d)
+        assert ((out.double().cpu() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("S", [1, 4, 40])
+@pytest.mark.parametrize("both", [False, True])
+def test_lengths_past_the_table(S, both):
+    """Rows that are there already and a length of up to 2^31 - 1: every key of the table is seen, none behind it."""
+    d = setup([100, 100], S, 2, 4, 64, 16)
+    x = dev(d)
+    span = x["bt"].shape[1] * 16
+    x["seq"] = torch.full_like(x["seq"], span)
+    want = run(x, both, rows=False)
+    x["seq"] = torch.full_like(x["seq"], 2**31 - 1)
+    assert torch.equal(run(x, both, rows=False), want)

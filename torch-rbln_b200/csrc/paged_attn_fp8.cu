@@ -705,11 +705,14 @@ enum TcBar {
 constexpr float kKeyUp = 131072.f;
 
 // What raw scores are multiplied by besides their key's scale. The sign of a
-// negative softmax scale is in the converted keys; and it is above zero, so
-// that -inf stays -inf.
+// negative softmax scale is in the converted keys; and it is above zero (the
+// smallest float, which no finite score makes more than 5e-7), so that -inf
+// stays -inf. NaN stays NaN.
+constexpr float kLeast = 1.4e-45f;
 template <bool BF16>
 __device__ __forceinline__ float score_mult(const Fp8Args& a) {
-  return fmaxf(fabsf(a.scale_dev ? *a.scale_dev : a.scale) * (BF16 ? kKeyUp * kLog2e : kLog2e), 1.2e-38f);
+  const float m = fabsf(a.scale_dev ? *a.scale_dev : a.scale) * (BF16 ? kKeyUp * kLog2e : kLog2e);
+  return m < kLeast ? kLeast : m;
 }
 
 // Eight f16 that stand for codes as bf16 times 2^-17, exact: a code has four
@@ -1105,7 +1108,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
       // K scales leave here between these two, so that their product with
       // `mult` is above zero, and finite where the scale is
       const float mult = score_mult<BF16>(a);
-      const float klo = 1.2e-38f / mult, khi = 3.4e38f / mult;
+      const float klo = kLeast / mult, khi = 3.4e38f / mult;
       int T = 0;
       bool ok = true;
       while (ok && next_segment<NX>(a, qt, sh, g)) {
@@ -1186,7 +1189,8 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
       const bool row_ok = gq < a.G && s < a.S;
       const int pos = a.seq[g.b * a.seq_stride];
       const int lim = a.causal ? (int)min((int64_t)pos + s + 1, (int64_t)g.keys) : g.keys;
-      const int first_lim = a.causal ? pos + (g.tile * NX + x) * qt + 1 : g.keys;  // of the tile's first token
+      // of the tile's first token
+      const int first_lim = a.causal ? (int)min((int64_t)pos + (g.tile * NX + x) * qt + 1, (int64_t)g.keys) : g.keys;
       float m_run = neg_inf(), l_run = 0.f, vref = 0.f, inv_vref = 0.f;
       for (int j = 0; j < nt; ++j, ++T, ++TX) {
         const int ms = T % kMetaRing, t0 = (g.j0 + j) * 128;
