@@ -229,3 +229,25 @@ def test_through_sdpa():
     # bf16 in four places on the way (turned q and k, P, dS): 2^-8 each of the tensors' largest values
     for a, b in zip((out,) + grads, (ref,) + want):
         assert (a.detach().cpu().double() - b).abs().max() <= 4 * 2.0 ** -8 * b.abs().max()
+
+
+@pytest.mark.parametrize("dtype,H,D", [(torch.bfloat16, 40, 128), (torch.float32, 3, 1024)])
+@pytest.mark.parametrize("tokens", [147, 148, 149, 601])
+def test_tokens_around_the_choice_of_tokens_a_cta(dtype, H, D, tokens):
+    q, k, pos = inputs(1, H, 1, tokens, D, dtype, seed=tokens)
+    check(q, k, pos, freqs(D), False)
+
+
+def test_one_tensor_as_queries_and_keys():
+    """The gradient of a leaf that is both is the sum; an expanded gradient of a sum too."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn([2, 3, 9, 64], generator=g)
+    pos, f = torch.arange(9), freqs(64)
+    leaf = x.to(DEV).requires_grad_()
+    a, b = op(leaf, leaf, pos.to(DEV), f.to(DEV))
+    assert torch.equal(a, b)
+    (d,) = torch.autograd.grad(a.sum() + b.sum(), leaf)
+    ref, size = R.rotary(torch.ones_like(x), pos[None], f, False, 1.0, inverse=True)
+    bound = R.rotary_bound(ref, size, torch.float32)
+    # twice one gradient: the sum of two equal floats is exact
+    R.assert_within(d, 2 * ref, 2 * bound)

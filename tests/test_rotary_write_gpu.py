@@ -282,3 +282,53 @@ def test_captured_step_on_another_stream():
             assert torch.equal(g, w)
     for n in ("kc", "vc", "ks", "vs"):
         same(x[n], e[n], n)
+
+
+@pytest.mark.parametrize("cache", [FP8, torch.bfloat16])
+def test_nothing_to_write(cache):
+    """No tokens, and no sequences: empty queries, the cache left."""
+    d = setup([4, 9], 1, 2, 3, 64, 16, torch.bfloat16, cache)
+    x = dev(d)
+    for q, k, x["seq"], x["bt"] in ((x["q"][:, :, :, :0], x["k"][:, :, :, :0], x["seq"], x["bt"]),
+                                    (x["q"][:0], x["k"][:0], x["seq"][:0], x["bt"][:0])):
+        assert write(x, freqs(64).to(DEV), q=q, k=k, v=k).shape == q.shape
+    for n in ("kc", "vc"):
+        same(x[n], d[n], n)
+
+
+@pytest.mark.parametrize("Hkv,G", [(1, 71), (5, 40), (17, 1)])
+@pytest.mark.parametrize("S", [1, 37])
+def test_odd_heads_are_the_rotation_and_the_write(Hkv, G, S):
+    """Queries bit for bit the rotary op's; a 16-bit cache's rows those of its keys and the plain write."""
+    d = setup([11, 0], S, Hkv, G, 64, 16, torch.bfloat16, torch.bfloat16)
+    a, b = dev(d), dev(d)
+    f = freqs(32).to(DEV)
+    out = write(a, f)
+    pos = b["seq"].long()[:, None] + torch.arange(S, device=DEV)
+    q, k = torch.ops.rbln_attn.rotary(b["q"].flatten(1, 2), b["k"].flatten(1, 2), pos, f)
+    assert torch.equal(out.flatten(1, 2), q)
+    b["k"] = k.reshape(b["k"].shape)
+    plain_write(b)
+    for n in ("kc", "vc"):
+        same(a[n], b[n], n)
+
+
+def test_expanded_inputs_and_two_streams_at_once():
+    """Inputs that broadcast one row, and two pools written and read on two streams: as one after the other."""
+    f = freqs(128).to(DEV)
+    pools = [setup([7, 300], 200, 2, 4, 128, 16, torch.bfloat16, FP8, seed=s) for s in (1, 2)]
+    first, then = [dev(d) for d in pools], [dev(d) for d in pools]
+    for x in first + then:
+        x["q"] = x["q"][:, :, :1].expand(-1, -1, 4, -1, -1)
+        x["v"] = x["v"][:, :1].expand(-1, 2, -1, -1, -1)
+    lens = [x["seq"] + 200 for x in first]
+    want = [(write(x, f), *read(x, n, 500)) for x, n in zip(first, lens)]
+    streams = [torch.cuda.Stream() for _ in pools]
+    torch.cuda.synchronize()
+    got = []
+    for x, n, s in zip(then, lens, streams):
+        with torch.cuda.stream(s):
+            got.append((write(x, f), *read(x, n, 500)))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(w, g))
