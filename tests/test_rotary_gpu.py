@@ -232,7 +232,7 @@ def test_through_sdpa():
 
 
 @pytest.mark.parametrize("dtype,H,D", [(torch.bfloat16, 40, 128), (torch.float32, 3, 1024)])
-@pytest.mark.parametrize("tokens", [147, 148, 149, 601])
+@pytest.mark.parametrize("tokens", [147, 149, 295, 296, 601, 1183, 1187])
 def test_tokens_around_the_choice_of_tokens_a_cta(dtype, H, D, tokens):
     q, k, pos = inputs(1, H, 1, tokens, D, dtype, seed=tokens)
     check(q, k, pos, freqs(D), False)

@@ -7,15 +7,17 @@
 // once, in shared memory, one per thread, and applies them to all heads of q
 // and k: a thread keeps the pairs of its (token, item) in registers and walks
 // the heads with two 16-byte loads and stores each. Forward and gradient of 4
-// sequences of 4096 tokens, 32 + 8 heads of 128 in bf16, take 135 us: 5.0 TB/s,
-// 76 % of the copy rate.
+// sequences of 4096 tokens, 32 + 8 heads of 128 in bf16, take 122 us: 5.5 TB/s,
+// 84 % of the copy rate. CTAs of 128 threads, six an SM, so that one's angles
+// run under others' copies (256 threads, three: 135; 128, seven: 126; three
+// heads a step and fewer CTAs: 141).
 
 #include "rotary.cuh"
 
 namespace rbln {
 namespace {
 
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
 
 struct RotaryArgs {
   const char* q;
@@ -73,12 +75,12 @@ __device__ __forceinline__ double position(const RotaryArgs& a, int b, int s) {
   return (double)load_index(a.pos, a.pos_dtype, b * a.pos_b + s * a.pos_s);
 }
 
-// grid (ceil(tokens / tpb), head groups), 256 threads: thread = (token,
+// grid (ceil(tokens / tpb), head groups), 128 threads: thread = (token,
 // item, head lane), item fastest, so that 8 neighbours cover a 256-byte row.
 // The first heads' loads are issued before the angles are found, and each
 // step's next ones before its own are turned.
 template <typename T>
-__global__ void __launch_bounds__(kRotThreads, 3) rotary_vec_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotThreads, 6) rotary_vec_kernel(const RotaryArgs a) {
   constexpr int V = Vec<T>::N;
   extern __shared__ float2 table[];  // [tpb][R/2]
   const int half = a.R / 2;
@@ -185,12 +187,13 @@ int launch_rotary(RotaryArgs a, bool vec, cudaStream_t st) {
   constexpr int V = Vec<T>::N;
   if (vec) {
     a.items = a.D / (2 * V);
-    // Four tokens a CTA share its angles' latency when there are enough of
-    // them; with few, one token a CTA and its heads spread over CTAs, so that
-    // every thread has one head. 32 + 8 heads of 128, four against one: 10.2
-    // to 8.2 us at 64 tokens, 10.2 to 12.3 at 296, 12.3 to 22.5 at 1184, 72 to
-    // 205 at 16384 (two a CTA: 98).
-    a.tpb = a.tokens >= 148 ? 4 : 1;
+    // Tokens of a CTA share the latency of its angles, where there are enough
+    // to fill the GPU; with fewer, one token a CTA and its heads spread over
+    // CTAs, so that every thread has one head. 32 + 8 heads of 128, one, two,
+    // four tokens a CTA: 8.2, 10.2, 12.3 us at 148 tokens, 10.2, 10.2, 12.3 at
+    // 296, 12.3, 10.2, 12.3 at 592, 18.4, 14.4, 14.3 at 1184, 29, 18, 17 at
+    // 2368, 145, 72, 66 at 16384 (eight: 68).
+    a.tpb = a.tokens >= 8 * 148 ? 4 : a.tokens >= 2 * 148 ? 2 : 1;
     while (a.tpb > 1 && a.tpb * a.items > kRotThreads) a.tpb /= 2;
     a.hp = kRotThreads / (a.tpb * a.items);
     const int64_t gx = (a.tokens + a.tpb - 1) / a.tpb;
