@@ -915,7 +915,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           uint8_t* dst = sgen + (part ? L::V0 : L::K0) + st * L::TILE + row0 * 128 + dst_panel;
           // two steps a turn: instruction fetch bounds this kernel (one, two, four steps:
           // 386, 387, 404 us for 8 sequences of 512 queries behind 512 to 7680 keys, 251, 250,
-          // 257 for 4 of 48 queries behind 18432 to 30720; eight: a third slower than two)
+          // 257 for 4 of 48 queries behind some 18000 to 31000; eight: a third slower than two)
 #pragma unroll 2
           for (int k = 0; k < STEPS; ++k) {
             uint2 w0 = *reinterpret_cast<const uint2*>(src + k * 4 * RPI * D + swap);
