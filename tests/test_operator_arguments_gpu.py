@@ -1,0 +1,52 @@
+"""Calls of the paged and rotary operators that are refused, or that take an unusual argument, on the GPU."""
+
+import pytest
+import torch
+
+from tests import test_prefill_kvfp8_gpu as P
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _ext():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    import torch_rbln_b200  # noqa: F401
+
+
+def freqs(rot):
+    return (10000.0 ** (-2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)).float()
+
+
+@pytest.mark.parametrize("name", ["k", "v", "vc"])
+def test_tensors_of_another_device(name):
+    """Keys, values or one of the caches left on the host: refused by every paged op, before any launch."""
+    import torch_rbln_b200 as tr
+
+    f = freqs(64).to(DEV)
+    for S in (1, 5):
+        x = P.dev(P.setup([20, 3], S, 2, 4, 64, 16))
+        wide = {n: x[n].to(torch.bfloat16) for n in ("kc", "vc")}  # a 16-bit cache
+        x[name] = x[name].cpu()
+        if name == "vc":
+            wide["vc"] = wide["vc"].cpu()
+        new, at = (x["q"], x["k"], x["v"]), (x["seq"], x["scale"], x["bt"], x["bs"])
+        fp8, scales = (x["kc"], x["vc"]), (x["ks"], x["vs"])
+        b16 = (wide["kc"], wide["vc"])
+        calls = [lambda: tr.paged_causal_attn_prefill_kvfp8(*new, *fp8, *scales, *at, False),
+                 lambda: tr.paged_causal_attn_prefill(*new, *b16, *at, False),
+                 lambda: torch.ops.rbln_attn.rotary_paged_kv_write(*new, *fp8, x["seq"], x["bt"], x["bs"], f, False, 1.0,
+                                                                   *scales),
+                 lambda: torch.ops.rbln_attn.paged_kv_write(*new[1:], *fp8, x["seq"], x["bt"], x["bs"], *scales)]
+        if S == 1:
+            calls += [lambda: tr.paged_causal_attn_decode_kvfp8(*new, *fp8, *scales, *at),
+                      lambda: tr.paged_causal_attn_decode(*new, *b16, *at)]
+        if name == "vc":
+            calls.append(lambda: torch.ops.rbln_attn.paged_kv_read(*fp8, x["seq"], x["bt"], x["bs"], 20, *scales))
+        for i, call in enumerate(calls):
+            with pytest.raises(RuntimeError, match="device|must be"):
+                call()
+                pytest.fail(f"call {i} was taken")
+    torch.cuda.synchronize()

@@ -96,7 +96,10 @@ void fill_paged(Common& c, const char* op, const at::Tensor& q_in, const at::Ten
   TORCH_CHECK(kcache.sizes() == vcache.sizes() && kcache.strides() == vcache.strides() &&
                   kcache.scalar_type() == vcache.scalar_type(),
               op, ": kcache and vcache must match in shape, strides and dtype");
-  TORCH_CHECK(kcache.is_cuda() && kcache.device() == q_in.device(), op, ": caches must be on q's device");
+  // k, v or a cache of another device would be read through a pointer that q's GPU does not have
+  TORCH_CHECK(kcache.device() == q_in.device() && vcache.device() == q_in.device(), op,
+              ": caches must be on q's device");
+  TORCH_CHECK(k_in.device() == q_in.device() && v_in.device() == q_in.device(), op, ": k and v must be on q's device");
   TORCH_CHECK(kcache.stride(-1) == 1 && kcache.size(2) == 1, op,
               ": caches must be [num_blocks, Hkv, 1, block_size, D] with a contiguous last dim");
   const auto dt = q_in.scalar_type();
@@ -177,7 +180,7 @@ void fill_paged(Common& c, const char* op, const at::Tensor& q_in, const at::Ten
   }
 
   if (scale.is_cuda()) {
-    c.scale_dev = scale.scalar_type() == at::kFloat ? scale : scale.to(at::kFloat);
+    c.scale_dev = on_device(scale, c.q).to(at::kFloat);
     p.scale_dev = c.scale_dev.data_ptr<float>();
   } else {
     p.scale = scale.item<float>();
@@ -621,8 +624,9 @@ void paged_kv_write_cuda(const at::Tensor& k_in, const at::Tensor& v_in, at::Ten
   TORCH_CHECK(k_in.is_cuda() && k_in.dim() == 5 && v_in.sizes() == k_in.sizes() && k_in.size(2) == 1, op,
               ": k/v must be CUDA [B, Hkv, 1, S, D]");
   TORCH_CHECK(kcache.dim() == 5 && kcache.sizes() == vcache.sizes() && kcache.strides() == vcache.strides() &&
-                  kcache.stride(-1) == 1 && kcache.size(3) == block_size && kcache.device() == k_in.device(),
-              op, ": caches must be [num_blocks, Hkv, 1, block_size, D] on k's device, alike");
+                  kcache.stride(-1) == 1 && kcache.size(3) == block_size && kcache.device() == k_in.device() &&
+                  vcache.device() == k_in.device() && v_in.device() == k_in.device(),
+              op, ": caches must be [num_blocks, Hkv, 1, block_size, D] on k's and v's device, alike");
   const auto dt = k_in.scalar_type();
   TORCH_CHECK((dt == at::kBFloat16 || dt == at::kHalf) && v_in.scalar_type() == dt, op, ": k/v bf16 or f16");
   const bool fp8 = kcache.scalar_type() == at::kFloat8_e4m3fn;
