@@ -1,0 +1,35 @@
+"""Derivatives of torch.ops.rbln_attn.rotary as the tracer sees them: fake CUDA tensors, no GPU."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _ext():
+    import torch_rbln_b200  # noqa: F401
+
+
+def inputs():
+    q, k = (torch.empty(2, h, 3, 64, device="cuda", dtype=torch.bfloat16) for h in (4, 2))
+    return q, k, torch.empty(2, 3, device="cuda", dtype=torch.int64), torch.empty(32, device="cuda")
+
+
+def op(*args):
+    return torch.ops.rbln_attn.rotary(*args)
+
+
+def test_forward_mode_tangents():
+    """A dual input gives a dual output, on either side alone too; the other side has none."""
+    with FakeTensorMode():
+        q, k, p, f = inputs()
+        with fwd.dual_level():
+            dq, dk = (fwd.make_dual(x, torch.empty_like(x)) for x in (q, k))
+            for a, b in ((dq, dk), (dq, k), (q, dk), (q, k)):
+                for x, y in zip((a, b), op(a, b, p, f)):
+                    t = fwd.unpack_dual(y).tangent
+                    assert (t is None) == (fwd.unpack_dual(x).tangent is None)
+                    assert t is None or (t.shape == x.shape and t.dtype == x.dtype)
+            with pytest.raises(RuntimeError, match="inv_freq has no gradient"):
+                op(q, k, p, fwd.make_dual(f, torch.empty_like(f)))

@@ -463,7 +463,8 @@ struct RotaryBackward : public torch::autograd::Node {
 std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k,
                                                    const at::Tensor& positions, const at::Tensor& inv_freq,
                                                    bool interleaved, double mscale, bool inverse) {
-  TORCH_CHECK(!inv_freq.requires_grad(), "rotary: inv_freq has no gradient (detach it)");
+  TORCH_CHECK(!inv_freq.requires_grad() && !inv_freq._fw_grad(0).defined(),
+              "rotary: inv_freq has no gradient (detach it)");
   const bool graph = c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad());
   // A leaf of a graph that still lives has its gradient node on the stream of
   // that graph; a backward pass captured on another stream would make the
@@ -497,6 +498,15 @@ std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at
     std::tie(qo, ko) = call_rotary(q, k, positions, inv_freq, interleaved, mscale, inverse);
   }
   if (node) torch::autograd::set_history(torch::autograd::variable_list{qo, ko}, node);
+  // Forward mode: the map is linear, so it takes the tangents as it takes the tensors.
+  const at::Tensor qt = q._fw_grad(0), kt = k._fw_grad(0);
+  if (qt.defined() || kt.defined()) {
+    auto zeros = [](const at::Tensor& t) { return at::zeros_symint(t.sym_sizes(), t.options()); };
+    auto [dq, dk] = call_rotary(qt.defined() ? qt : zeros(q), kt.defined() ? kt : zeros(k), positions, inv_freq,
+                                interleaved, mscale, inverse);
+    if (qt.defined()) qo._set_fw_grad(dq, 0, false);
+    if (kt.defined()) ko._set_fw_grad(dk, 0, false);
+  }
   return {qo, ko};
 }
 
