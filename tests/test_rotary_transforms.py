@@ -33,3 +33,13 @@ def test_forward_mode_tangents():
                     assert t is None or (t.shape == x.shape and t.dtype == x.dtype)
             with pytest.raises(RuntimeError, match="inv_freq has no gradient"):
                 op(q, k, p, fwd.make_dual(f, torch.empty_like(f)))
+
+
+def test_a_training_step_is_traced():
+    """The forward pass with gradients, leaves used once and twice: no CUDA runtime is asked for anything."""
+    with FakeTensorMode():
+        q, k, p, f = inputs()
+        q.requires_grad_(), k.requires_grad_()
+        for _ in range(2):
+            a, b = op(q, k, p, f)
+            assert a.requires_grad and b.requires_grad and a.shape == q.shape and b.shape == k.shape

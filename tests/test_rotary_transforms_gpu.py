@@ -62,3 +62,17 @@ def test_forward_over_reverse():
     d, t = torch.func.jvp(grad, (x[0], x[2]), (x[2], x[0]))
     near(d, tq, pos, f, False, 1.0, inverse=True)
     near(t, q, pos, f, False, 1.0, inverse=True)
+
+
+def test_functional_gradient():
+    """torch.func.grad, and under vmap a gradient for each of several cotangents."""
+    q, k, tq, tk, pos, f = case(5)
+    x = [t.to(DEV) for t in (q, k, tq, tk, pos, f)]
+    got = torch.func.grad(lambda a, b: sum((y * t).sum() for y, t in zip(op(a, b, x[4], x[5]), (x[2], x[3]))),
+                          argnums=(0, 1))(x[0], x[1])
+    near(got[0], tq, pos, f, False, 1.0, inverse=True)
+    near(got[1], tk, pos, f, False, 1.0, inverse=True)
+    _, pull = torch.func.vjp(lambda a: op(a, x[1], x[4], x[5])[0], x[0])
+    many = torch.func.vmap(pull)(torch.stack([x[2], x[0]]))[0]
+    near(many[0], tq, pos, f, False, 1.0, inverse=True)
+    near(many[1], q, pos, f, False, 1.0, inverse=True)

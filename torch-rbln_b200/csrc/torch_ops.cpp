@@ -16,7 +16,6 @@
 #include <ATen/ops/_fused_sdp_choice_native.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -460,25 +459,33 @@ struct RotaryBackward : public torch::autograd::Node {
   }
 };
 
+// A leaf of a graph that still lives has its gradient node on the stream of
+// that graph; a backward pass captured on another stream would make the
+// engine wait for it, which breaks the capture. Refused before that. Only a
+// leaf that has such a node makes the CUDA runtime be asked, and a traced one
+// on a machine without a GPU does not.
+void check_capture(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors) {
+    if (!t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto at = node ? node->stream() : std::nullopt;
+    if (!at.has_value() || c10::cuda::device_count() == 0) continue;
+    const auto now = at::cuda::getCurrentCUDAStream(t->device().index());
+    if (*at == now.unwrap()) continue;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    C10_CUDA_CHECK(cudaStreamIsCapturing(now.stream(), &status));
+    TORCH_CHECK(status == cudaStreamCaptureStatusNone, "rotary: an input belongs to a graph that lives on another "
+                "stream; free that graph before capturing, or capture with inputs of their own");
+  }
+}
+
 std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k,
                                                    const at::Tensor& positions, const at::Tensor& inv_freq,
                                                    bool interleaved, double mscale, bool inverse) {
   TORCH_CHECK(!inv_freq.requires_grad() && !inv_freq._fw_grad(0).defined(),
               "rotary: inv_freq has no gradient (detach it)");
   const bool graph = c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad());
-  // A leaf of a graph that still lives has its gradient node on the stream of
-  // that graph; a backward pass captured on another stream would make the
-  // engine wait for it, which breaks the capture. Refused before that.
-  if (graph && at::cuda::currentStreamCaptureStatus() != at::cuda::CaptureStatus::None) {
-    const c10::Stream now = at::cuda::getCurrentCUDAStream(q.device().index());
-    for (const at::Tensor* t : {&q, &k}) {
-      if (!t->requires_grad() || !t->is_leaf()) continue;
-      const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-      const auto at = node ? node->stream() : std::nullopt;
-      TORCH_CHECK(!at.has_value() || *at == now, "rotary: an input belongs to a graph that lives on another stream; "
-                  "free that graph before capturing, or capture with inputs of their own");
-    }
-  }
+  if (graph) check_capture({&q, &k});
   std::shared_ptr<RotaryBackward> node;
   if (graph) {
     node = std::shared_ptr<RotaryBackward>(new RotaryBackward(), torch::autograd::deleteNode);
