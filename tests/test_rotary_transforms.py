@@ -43,3 +43,20 @@ def test_a_training_step_is_traced():
         for _ in range(2):
             a, b = op(q, k, p, f)
             assert a.requires_grad and b.requires_grad and a.shape == q.shape and b.shape == k.shape
+
+
+def test_symbolic_sizes_are_traced():
+    """A sequence length that is a symbol, with and without gradients."""
+    from torch._dynamo.source import ConstantSource
+    from torch.fx.experimental.symbolic_shapes import ShapeEnv
+
+    env = ShapeEnv()
+    symbol = env.create_symbol(7, source=ConstantSource("S"))
+    with FakeTensorMode(shape_env=env):
+        S = env.create_symintnode(symbol, hint=7)
+        q, k = (torch.empty(2, h, S, 64, device="cuda") for h in (4, 2))
+        p, f = torch.empty(2, S, device="cuda", dtype=torch.int64), torch.empty(32, device="cuda")
+        for grad in (False, True):
+            a, b = op(q.requires_grad_(grad), k, p, f)
+            assert a.shape == q.shape and b.shape == k.shape and a.requires_grad == grad
+            assert not env.guards, f"the length was made a constant: {env.guards}"

@@ -76,3 +76,31 @@ def test_functional_gradient():
     many = torch.func.vmap(pull)(torch.stack([x[2], x[0]]))[0]
     near(many[0], tq, pos, f, False, 1.0, inverse=True)
     near(many[1], q, pos, f, False, 1.0, inverse=True)
+
+
+def test_compiled_for_any_length():
+    """A function traced once for every length, gradients with it."""
+    f = freqs(32)
+    seen = []
+
+    def backend(gm, args):
+        from torch._dynamo.backends.common import aot_autograd
+
+        seen.append(1)
+        return aot_autograd(fw_compiler=lambda g, _: g, bw_compiler=lambda g, _: g)(gm, args)
+
+    @torch.compile(backend=backend, dynamic=True, fullgraph=True)
+    def turn(q, k, pos, f):
+        a, b = op(q * 1.0, k * 1.0, pos, f)
+        return a, b
+
+    for S in (5, 9, 17):
+        q, k, pos = inputs(2, 4, 2, S, 64, torch.float32, seed=S)
+        x = [q.to(DEV).requires_grad_(), k.to(DEV).requires_grad_()]
+        a, b = turn(*x, pos.to(DEV), f.to(DEV))
+        near(a, q, pos, f, False)
+        near(b, k, pos, f, False)
+        dq, dk = torch.autograd.grad((a, b), x, (torch.ones_like(a), torch.ones_like(b)))
+        near(dq, torch.ones_like(q), pos, f, False, 1.0, inverse=True)
+        near(dk, torch.ones_like(k), pos, f, False, 1.0, inverse=True)
+    assert len(seen) == 1

@@ -441,7 +441,7 @@ std::tuple<at::Tensor, at::Tensor> call_rotary(const at::Tensor& q, const at::Te
 struct RotaryBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable positions, inv_freq;
   at::TensorOptions options;
-  std::vector<int64_t> q_size, k_size;
+  std::vector<c10::SymInt> q_size, k_size;  // symbols in a trace
   bool interleaved, inverse;
   double mscale;
 
@@ -452,8 +452,8 @@ struct RotaryBackward : public torch::autograd::Node {
   }
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grad) override {
     // an output that nothing used has no gradient: zeros stand for it
-    const at::Tensor gq = grad[0].defined() ? grad[0] : at::zeros(q_size, options);
-    const at::Tensor gk = grad[1].defined() ? grad[1] : at::zeros(k_size, options);
+    const at::Tensor gq = grad[0].defined() ? grad[0] : at::zeros_symint(q_size, options);
+    const at::Tensor gk = grad[1].defined() ? grad[1] : at::zeros_symint(k_size, options);
     auto [dq, dk] = call_rotary(gq, gk, positions.unpack(), inv_freq.unpack(), interleaved, mscale, !inverse);
     return {task_should_compute_output(0) ? dq : at::Tensor(), task_should_compute_output(1) ? dk : at::Tensor()};
   }
@@ -493,8 +493,8 @@ std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at
     node->positions = torch::autograd::SavedVariable(positions, false);
     node->inv_freq = torch::autograd::SavedVariable(inv_freq, false);
     node->options = q.options();
-    node->q_size = q.sizes().vec();
-    node->k_size = k.sizes().vec();
+    node->q_size = q.sym_sizes().vec();
+    node->k_size = k.sym_sizes().vec();
     node->interleaved = interleaved;
     node->inverse = inverse;
     node->mscale = mscale;
