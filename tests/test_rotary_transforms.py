@@ -60,3 +60,17 @@ def test_symbolic_sizes_are_traced():
             a, b = op(q.requires_grad_(grad), k, p, f)
             assert a.shape == q.shape and b.shape == k.shape and a.requires_grad == grad
             assert not env.guards, f"the length was made a constant: {env.guards}"
+
+
+def test_frequencies_that_are_a_parameter():
+    """Taken where no gradient is asked for, refused where one is."""
+    with FakeTensorMode():
+        q, k, p, f = inputs()
+        f.requires_grad_()
+        with torch.no_grad():
+            assert op(q, k, p, f)[0].shape == q.shape
+        with torch.inference_mode():
+            assert op(q, k, p, f)[0].shape == q.shape
+        assert op(q, k, p, f.detach())[0].shape == q.shape
+        with pytest.raises(RuntimeError, match="inv_freq has no gradient"):
+            op(q, k, p, f)

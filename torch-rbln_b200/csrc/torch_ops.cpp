@@ -482,9 +482,10 @@ void check_capture(std::initializer_list<const at::Tensor*> tensors) {
 std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k,
                                                    const at::Tensor& positions, const at::Tensor& inv_freq,
                                                    bool interleaved, double mscale, bool inverse) {
-  TORCH_CHECK(!inv_freq.requires_grad() && !inv_freq._fw_grad(0).defined(),
+  const bool grads = c10::GradMode::is_enabled();
+  TORCH_CHECK(!(grads && inv_freq.requires_grad()) && !inv_freq._fw_grad(0).defined(),
               "rotary: inv_freq has no gradient (detach it)");
-  const bool graph = c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad());
+  const bool graph = grads && (q.requires_grad() || k.requires_grad());
   if (graph) check_capture({&q, &k});
   std::shared_ptr<RotaryBackward> node;
   if (graph) {
