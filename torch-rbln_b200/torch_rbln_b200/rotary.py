@@ -13,7 +13,7 @@ import torch
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
-                       original_length: int = 0, low: float = 1.0, high: float = 32.0,
+                       original_length: int = 0, low: float = 1.0, high: Optional[float] = None,
                        device=None) -> Tuple[torch.Tensor, float]:
     """(inv_freq, mscale) of rotary positions: inv_freq fp32 [rotary_dim / 2], inv_freq[i] = base^(-2 i / rotary_dim).
 
@@ -26,7 +26,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
                 between the two blended linearly in the pair's index (between the indices where r = high, rounded
                 down, and r = low, rounded up); mscale = 0.1 ln(factor) + 1;
       "llama3"  the same with the blend linear in r.
-    The values are computed in float64 and rounded once.
+    low is 1 turn unless given, high 32 for yarn and 4 for llama3. The values are computed in float64 and rounded once.
     """
     R = int(rotary_dim)
     if R <= 0 or R % 2:
@@ -48,6 +48,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     elif scaling == "linear":
         inv = inv / factor
     elif scaling in ("yarn", "llama3"):
+        if high is None:
+            high = 32.0 if scaling == "yarn" else 4.0
         if original_length <= 0 or not 0 < low < high:
             raise ValueError(f"rotary_frequencies: {scaling} needs original_length > 0 and 0 < low < high")
         if scaling == "llama3":
