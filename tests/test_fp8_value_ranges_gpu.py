@@ -1,0 +1,63 @@
+"""paged_causal_attn_prefill_kvfp8 where the scales of the blocks differ by much: zero, not numbers, at the ends of
+float32, or of other sizes before and behind a row's limit. Bounds as in tests/operator_refs.py, but each row's own:
+the largest value is taken over the blocks that the row sees."""
+
+import pytest
+import torch
+
+from tests import operator_refs as R
+from tests import test_prefill_kvfp8_gpu as P
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _ext():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    import torch_rbln_b200  # noqa: F401
+
+
+def reference(d, mask=None, rows=True):
+    """(out, bound) in float64; a probability is rounded relative to a power of two at most twice the largest V scale
+    that its row sees, so 448 of that scale stands for the bound's largest value."""
+    B, Hkv, G, S, D = d["q"].shape
+    bs, bt = d["bs"], d["bt"].long()
+    if rows:
+        R.write_reciprocal(d["k"], d["v"], d["kc"], d["vc"], d["seq"], bt, bs, d["ks"], d["vs"])
+    t = torch.arange(bt.shape[1] * bs)
+    outs, bounds = [], []
+    for b in range(B):
+        blk = bt[b][t // bs]
+        K, V = ((c[blk, :, 0, t % bs].double() * s[blk].double()[:, :, None]).transpose(0, 1)
+                for c, s in ((d["kc"], d["ks"]), (d["vc"], d["vs"])))
+        keep = t < int(d["seq"][b]) + 1 + torch.arange(S)[:, None]
+        if mask is not None:
+            keep = keep & mask[b, : t.numel()]
+        out, A, e = R.attention(d["q"][b], K, V, keep, float(d["scale"]))
+        seen = d["vs"][blk].double().t()[:, None].expand(Hkv, S, -1).masked_fill(~keep, 0.0)
+        vmax = 448 * seen.amax(-1)[:, None, :, None]
+        outs.append(out)
+        bounds.append(R.attention_bound(out, A, e, t.numel(), vmax, d["q"].dtype))
+    return torch.stack(outs), torch.stack(bounds)
+
+
+def check(d, mask=None, rows=True):
+    out = P.run(P.dev(d), mask=None if mask is None else mask.to(DEV), rows=rows)
+    torch.cuda.synchronize()
+    ref, bound = reference(d, mask, rows)
+    R.assert_within(out, ref, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("S", [4, 40, 200])
+def test_key_scales_of_zero(S, dtype):
+    """A block whose keys are all zeros, its scale too, and only some of its keys kept: scores of zero, no NaN."""
+    d = P.setup([200, 90], S, 2, 4, 64, 16, dtype)
+    for b, j in ((0, 2), (0, 5), (1, 1)):
+        d["ks"][d["bt"][b, j].item()] = 0.0
+    mask = torch.ones([2, d["bt"].shape[1] * 16], dtype=torch.bool)
+    mask[0, 33:45:2] = False
+    mask[1, 18:21] = False
+    check(d, mask, rows=False)

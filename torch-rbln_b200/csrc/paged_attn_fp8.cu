@@ -652,7 +652,7 @@ constexpr int kTcSegCost = 2;      // key tiles charged to a unit's start (1, 2,
 constexpr int kMetaRing = 4;
 
 struct TileMeta {
-  float ks[16], vs[16];  // scale of keys [8 g, 8 g + 8)
+  float ks[16], vs[16];  // of keys [8 g, 8 g + 8): key_factor, V scale
   uint32_t keep[4];
   float vmax;
   float pad[3];
@@ -705,14 +705,20 @@ enum TcBar {
 constexpr float kKeyUp = 131072.f;
 
 // What raw scores are multiplied by besides their key's scale. The sign of a
-// negative softmax scale is in the converted keys; and it is above zero (the
-// smallest float, which no finite score makes more than 5e-7), so that -inf
-// stays -inf. NaN stays NaN.
-constexpr float kLeast = 1.4e-45f;
+// negative softmax scale is in the converted keys. NaN stays NaN.
 template <bool BF16>
 __device__ __forceinline__ float score_mult(const Fp8Args& a) {
-  const float m = fabsf(a.scale_dev ? *a.scale_dev : a.scale) * (BF16 ? kKeyUp * kLog2e : kLog2e);
-  return m < kLeast ? kLeast : m;
+  return fabsf(a.scale_dev ? *a.scale_dev : a.scale) * (BF16 ? kKeyUp * kLog2e : kLog2e);
+}
+
+// That times a key's scale, which is what the softmax warps get: above zero,
+// whatever the two are, so that -inf stays -inf (the smallest float makes no
+// finite score more than 5e-7 in size), and finite where both are.
+__device__ __forceinline__ float key_factor(float ks, float mult) {
+  constexpr float kMost = 3.4028235e38f;
+  const float f = ks * mult;
+  if (f > kMost && ks <= kMost && mult <= kMost) return kMost;
+  return f < 1.4e-45f ? 1.4e-45f : f;
 }
 
 // Eight f16 that stand for codes as bf16 times 2^-17, exact: a code has four
@@ -1105,10 +1111,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
       }
     } else if (warp == W0 + 2) {
       // ---------------------------------------------------------- scales
-      // K scales leave here between these two, so that their product with
-      // `mult` is above zero, and finite where the scale is
       const float mult = score_mult<BF16>(a);
-      const float klo = kLeast / mult, khi = 3.4e38f / mult;
       int T = 0;
       bool ok = true;
       while (ok && next_segment<NX>(a, qt, sh, g)) {
@@ -1146,7 +1149,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
             break;
           }
           if (lane < 16) {
-            meta[ms].ks[lane] = ks < klo ? klo : (ks > khi && ks <= 3.4028235e38f) ? khi : ks;
+            meta[ms].ks[lane] = key_factor(ks, mult);
             meta[ms].vs[lane] = vs;
           }
           if (lane == 0) {
@@ -1165,7 +1168,6 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
     const int x = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const int gq = r / qt, i = r - gq * qt;
-    const float mult = score_mult<BF16>(a);
     int T = 0, act = 0, TX = 0;  // tiles of the CTA; segments and tiles of this row tile
     int cont = -1, start = -1;
     bool ok = true;
@@ -1236,7 +1238,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const float* w = q + u * 8;
-            mg[u] = fmaxf(max3(max3(w[0], w[1], w[2]), w[3], w[4]), max3(w[5], w[6], w[7])) * (k4[u] * mult);
+            mg[u] = fmaxf(max3(max3(w[0], w[1], w[2]), w[3], w[4]), max3(w[5], w[6], w[7])) * k4[u];
           }
           mt = fmaxf(mt, max3(mg[0], mg[1], fmaxf(mg[2], mg[3])));
         };
@@ -1297,7 +1299,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           tmem_wait_ld32(v);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const float km = k4[u] * mult, vr = v4[u] * inv_vref;
+            const float km = k4[u], vr = v4[u] * inv_vref;
 #pragma unroll
             for (int e = 8 * u; e < 8 * u + 8; e += 2) {
               fma2(p[e], p[e + 1], km, km, nmu, nmu);
