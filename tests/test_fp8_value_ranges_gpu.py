@@ -61,3 +61,16 @@ def test_key_scales_of_zero(S, dtype):
     mask[0, 33:45:2] = False
     mask[1, 18:21] = False
     check(d, mask, rows=False)
+
+
+@pytest.mark.parametrize("name", ["ks", "vs"])
+@pytest.mark.parametrize("S,D", [(4, 128), (40, 128), (150, 64)])
+def test_parts_of_a_split_that_hold_no_number(S, D, name):
+    """NaN scales of a long run of blocks, so that some part of a split sequence holds nothing else (and, for one
+    start of the run, no part holds NaN and numbers): NaN all the same."""
+    for starts, first, n in (([6000], 8, 22), ([6000], 9, 21), ([6000], 10, 21), ([5000, 3], 8, 22)):
+        d = P.setup(starts, S, 1, 4, D, 128)
+        for j in range(first, first + n):
+            d[name][d["bt"][0, j].item()] = float("nan")
+        out = P.run(P.dev(d))
+        assert torch.isnan(out[0]).all() and not torch.isnan(out[1:]).any()

@@ -1387,6 +1387,11 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
   }
 }
 
+// Whether a part (maximum, sum) saw no key. Scores that are all NaN leave the
+// maximum at -inf too (it passes over NaN), but a sum of NaN, which the join
+// takes on.
+__device__ __forceinline__ bool no_keys(float2 ml) { return ml.x == neg_inf() && ml.y == 0.f; }
+
 // Joins the partial results of the units that several CTAs share. CTA (c, y):
 // the chain that CTA c of the attention kernel starts, in parts c, c + 1, ...
 // while those continue the same unit. 8 warps = RPC rows x KS slices of the
@@ -1456,7 +1461,7 @@ __global__ void __launch_bounds__(256) paged_attn_fp8_merge_kernel(const Fp8Args
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (ml[u].x == neg_inf()) continue;
+        if (no_keys(ml[u])) continue;
         const float mn = fmaxf(M, ml[u].x);
         const float f0 = exp2_approx(M - mn), f1 = exp2_approx(ml[u].x - mn);
         M = mn;
@@ -1472,7 +1477,7 @@ __global__ void __launch_bounds__(256) paged_attn_fp8_merge_kernel(const Fp8Args
       __syncthreads();
       for (int k = 1; slice == 0 && k < KS; ++k) {
         const float2 ml = sml[warp + k * RPC];
-        if (ml.x == neg_inf()) continue;
+        if (no_keys(ml)) continue;
         const float mn = fmaxf(M, ml.x);
         const float f0 = exp2_approx(M - mn), f1 = exp2_approx(ml.x - mn);
         M = mn;
