@@ -74,3 +74,17 @@ def test_parts_of_a_split_that_hold_no_number(S, D, name):
             d[name][d["bt"][0, j].item()] = float("nan")
         out = P.run(P.dev(d))
         assert torch.isnan(out[0]).all() and not torch.isnan(out[1:]).any()
+
+
+@pytest.mark.parametrize("S", [1, 4, 40])
+@pytest.mark.parametrize("small,large", [(-99, 60), (-40, 100)])
+@pytest.mark.parametrize("turned", [False, True])
+def test_value_scales_from_end_to_end(S, small, large, turned):
+    """Half of a sequence's blocks with V scales of one end of float32, half of the other: what is too small to count
+    is lost, nothing else is."""
+    d = P.setup([1200], S, 2, 4, 64, 16)
+    half = d["bt"][0, :38].long()
+    rest = d["bt"][0, 38:].long()
+    d["vs"][half if not turned else rest] = 2.0 ** small
+    d["vs"][rest if not turned else half] = 2.0 ** large
+    check(d, rows=False)

@@ -360,8 +360,8 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
     if (__uint_as_float(vmaxb) > vref) {
       const float now = pow2_above(__uint_as_float(vmaxb));
       const float inv = 1.f / now;  // a power of two: exact
-      const float f = vref * inv;
-      if (f > 0.f) {
+      const float f = vref * inv;  // zero where what is held is too small to count
+      if (vref > 0.f) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
