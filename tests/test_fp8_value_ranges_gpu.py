@@ -76,6 +76,18 @@ def test_parts_of_a_split_that_hold_no_number(S, D, name):
         assert torch.isnan(out[0]).all() and not torch.isnan(out[1:]).any()
 
 
+@pytest.mark.parametrize("S,G,bs,first", [(16, 1, 8, 8), (8, 2, 8, 4), (4, 4, 16, 2), (24, 1, 8, 12), (64, 2, 16, 32),
+                                          (200, 1, 8, 96), (100, 4, 16, 20)])
+@pytest.mark.parametrize("binades", [16, 20, 26, 90])
+def test_values_behind_a_row_cost_it_nothing(S, G, bs, first, binades):
+    """The chunk's tokens from `first` on, a block's first row, hold values 2^16 and more times the earlier ones': a
+    row that does not see them keeps its bits."""
+    for vstd in (0.5, 1e-5):
+        d = P.setup([(-first) % bs, (-first) % bs + 2 * bs], S, 2, G, 64, bs, vstd=vstd)
+        d["v"][:, :, :, first:] *= 2.0 ** binades
+        check(d)
+
+
 @pytest.mark.parametrize("S", [1, 4, 40])
 @pytest.mark.parametrize("small,large", [(-99, 60), (-40, 100)])
 @pytest.mark.parametrize("turned", [False, True])

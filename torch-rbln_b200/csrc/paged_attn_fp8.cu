@@ -14,10 +14,12 @@
 // its largest magnitude lies in [2^14, 2^15): exact down to 2^-28 of the row's
 // largest. Many rows: the keys go to bf16 instead, exact too.
 // The probabilities' vs is taken relative to a running power of two (vref) at
-// or above the largest scale seen, so a cache of small values keeps all of
-// f16's bits and one of large values cannot overflow; the accumulator is
-// rescaled when vref grows. A block whose scale is far below vref keeps its
-// probabilities to 2^-25 of vref, an error of 2^-25 of the largest value.
+// or above the largest scale that the row has seen, so a cache of small values
+// keeps all of f16's bits and one of large values cannot overflow; the row's
+// accumulator is rescaled when vref grows. It is each row's own: what a row may
+// not see costs it nothing (but see kFarBelow). A block whose scale is far
+// below vref keeps its probabilities to 2^-25 of vref, an error of 2^-25 of the
+// largest value.
 // The running maximum, the sums and the accumulators are float32.
 
 #include <algorithm>
@@ -89,6 +91,15 @@ __device__ __forceinline__ float pow2_above(float x) {
   x = fminf(fmaxf(x, 1e-30f), 1e30f);
   return __uint_as_float((__float_as_uint(x) + 0x007fffffu) & 0x7f800000u);
 }
+
+// Reciprocal of a power of two that pow2_above gave; 2^127 for zero, which
+// stands for no scale yet.
+__device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+
+// vref is held above this times the largest scale behind the row's limit, so
+// that the ratio of the two stays finite (and zero times it is zero). That
+// costs the row bits only where what it may not see is 2^112 times larger.
+constexpr float kFarBelow = 1.1754944e-38f;  // 2^-126
 
 // Power of two that brings a row's largest magnitude m to [2^14, 2^15), and
 // its inverse; 1 for rows of zeros, infinities or NaN.
@@ -320,7 +331,10 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
   }
   // keys below this are every live row's (their columns' limits)
   const int all_lim = a.causal ? (int)min((int64_t)pos + c0 / a.G + 1, (int64_t)t1) : t1;
-  float vref = 0.f, inv_vref = 0.f;  // power of two at or above every V scale met, and its reciprocal
+  // Each column's power of two at or above every V scale that it has seen, as
+  // its exponent in a byte (0: none yet).
+  uint32_t vexp = 0;
+  auto vref = [&](int nt, int k) { return __uint_as_float((vexp >> (16 * nt + 8 * k) & 0xffu) << 23); };
 
   auto consume = [&](int ts, int st) {
     const unsigned char* stage = ring + st * R::STAGE;
@@ -355,30 +369,47 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
         }
       }
     }
-    // V scales relative to vref; positive floats order as their bits
-    const uint32_t vmaxb = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs[lane], 0.f)));
-    if (__uint_as_float(vmaxb) > vref) {
-      const float now = pow2_above(__uint_as_float(vmaxb));
-      const float inv = 1.f / now;  // a power of two: exact
-      const float f = vref * inv;  // zero where what is held is too small to count
-      if (vref > 0.f) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o_acc[nt][mt][k] *= f;
-      }
-      vref = now;
-      inv_vref = inv;
-    }
+    const bool inside = ts + kMqTile <= all_lim;  // no key behind a live column's limit
     float ksc[4], vsc[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       ksc[r] = ks[gid + 8 * r];
-      vsc[r] = vs[gid + 8 * r] * inv_vref;
+      vsc[r] = vs[gid + 8 * r];
     }
-    const bool whole_tile = vmask == 0xffffffffu && ts + kMqTile <= all_lim;
+    // the tile's largest V scale; positive floats order as their bits
+    const float vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs[lane], 0.f))));
+    // A lane's first column is of its earliest token and sees no more than the
+    // others; while all tiles are inside, they are all alike.
+    if (__any_sync(0xffffffffu, vmax > vref(0, 0))) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float m = vmax;
+          if (!inside) {  // the largest that this column sees
+            m *= kFarBelow;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (ts + gid + 8 * r < lim[nt][k]) m = fmaxf(m, vsc[r]);
+            m = warp_max_xor_rows(m);
+          }
+          const float was = vref(nt, k), now = m > was ? pow2_above(m) : was;
+          const float f = was * pow2_inverse(now);  // zero where what is held is too small to count
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            o_acc[nt][mt][k] *= f;
+            o_acc[nt][mt][2 + k] *= f;
+          }
+          const int at = 16 * nt + 8 * k;
+          vexp = (vexp & ~(0xffu << at)) | (__float_as_uint(now) >> 23 << at);
+        }
+    }
+    {
+      const float inv = pow2_inverse(vref(0, 0));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) vsc[r] = inside ? vsc[r] * inv : 1.f;  // 1: by each column's own, below
+    }
+    const bool whole_tile = vmask == 0xffffffffu && inside;
     uint32_t pb[2][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -416,6 +447,13 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
           o_acc[nt][mt][0] *= al[0]; o_acc[nt][mt][2] *= al[0];
           o_acc[nt][mt][1] *= al[1]; o_acc[nt][mt][3] *= al[1];
         }
+      }
+      if (!inside) {
+        const float inv[2] = {pow2_inverse(vref(nt, 0)), pow2_inverse(vref(nt, 1))};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) s[nt][2 * r + k] *= vs[gid + 8 * r] * inv[k];
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -481,10 +519,10 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int d0 = gid * VSEG + 2 * mt, d1 = d0 + 1;
-      sO(warp)[c][d0] = o_acc[nt][mt][0] * vref;
-      sO(warp)[c + 1][d0] = o_acc[nt][mt][1] * vref;
-      sO(warp)[c][d1] = o_acc[nt][mt][2] * vref;
-      sO(warp)[c + 1][d1] = o_acc[nt][mt][3] * vref;
+      sO(warp)[c][d0] = o_acc[nt][mt][0] * vref(nt, 0);
+      sO(warp)[c + 1][d0] = o_acc[nt][mt][1] * vref(nt, 1);
+      sO(warp)[c][d1] = o_acc[nt][mt][2] * vref(nt, 0);
+      sO(warp)[c + 1][d1] = o_acc[nt][mt][3] * vref(nt, 1);
     }
   }
   __syncthreads();
@@ -1193,7 +1231,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
       const int lim = a.causal ? (int)min((int64_t)pos + s + 1, (int64_t)g.keys) : g.keys;
       // of the tile's first token
       const int first_lim = a.causal ? (int)min((int64_t)pos + (g.tile * NX + x) * qt + 1, (int64_t)g.keys) : g.keys;
-      float m_run = neg_inf(), l_run = 0.f, vref = 0.f, inv_vref = 0.f;
+      float m_run = neg_inf(), l_run = 0.f, vref = 0.f;
       for (int j = 0; j < nt; ++j, ++T, ++TX) {
         const int ms = T % kMetaRing, t0 = (g.j0 + j) * 128;
         const int sfb = NX == 2 ? x : (T & 1), sfp = NX == 2 ? TX & 1 : (T >> 1) & 1;
@@ -1260,11 +1298,17 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           l_run *= factor;
           m_run = m_new;
         }
-        const float vm = meta[ms].vmax;
-        if (vm > vref) {  // the same for every row
+        float vm = meta[ms].vmax;
+        if (t0 + 128 > first_lim) {  // the largest V scale that this row sees
+          const int seen = lim - t0;
+          vm *= kFarBelow;
+#pragma unroll 4
+          for (int u = 0; u < 16; ++u)
+            if (8 * u < seen) vm = fmaxf(vm, meta[ms].vs[u]);
+        }
+        if (vm > vref) {
           const float now = pow2_above(vm);
-          inv_vref = 1.f / now;
-          factor *= vref * inv_vref;
+          factor *= vref * pow2_inverse(now);
           vref = now;
         }
         if (j >= 1 && __any_sync(0xffffffffu, factor != 1.f)) {
@@ -1286,7 +1330,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           }
           tmem_wait_st();
         }
-        const float nmu = (m_run == neg_inf()) ? 0.f : -m_run;
+        const float nmu = (m_run == neg_inf()) ? 0.f : -m_run, inv_vref = pow2_inverse(vref);
         float sa0 = 0.f, sa1 = 0.f, sb0 = 0.f, sb1 = 0.f;
         // P of a chunk is 16 columns of f16 pairs over scores that are done with
 #pragma unroll 1
