@@ -89,7 +89,23 @@ def test_values_behind_a_row_cost_it_nothing(S, G, bs, first, binades):
 
 
 @pytest.mark.parametrize("S", [1, 4, 40])
-@pytest.mark.parametrize("small,large", [(-99, 60), (-40, 100)])
+@pytest.mark.parametrize("starts", [[300, 11], [5000]])
+def test_values_near_the_largest(S, starts):
+    """bf16 values up to 3e38, V scales up to 7e35: a mean of finite values is finite."""
+    check(P.setup(starts, S, 2, 4, 128, 16, vstd=6e37))
+
+
+@pytest.mark.parametrize("S", [1, 4, 40])
+@pytest.mark.parametrize("starts", [[300, 11], [5000]])
+def test_value_scales_far_below_one(S, starts):
+    """V scales of 2^-123, as a caller may make them."""
+    d = P.setup(starts, S, 2, 4, 128, 16)
+    d["vs"] *= 2.0 ** -115
+    check(d, rows=False)
+
+
+@pytest.mark.parametrize("S", [1, 4, 40])
+@pytest.mark.parametrize("small,large", [(-99, 60), (-120, 118), (-40, 100)])
 @pytest.mark.parametrize("turned", [False, True])
 def test_value_scales_from_end_to_end(S, small, large, turned):
     """Half of a sequence's blocks with V scales of one end of float32, half of the other: what is too small to count

@@ -18,9 +18,11 @@
 // keeps all of f16's bits and one of large values cannot overflow; the row's
 // accumulator is rescaled when vref grows. It is each row's own: what a row may
 // not see costs it nothing (but see kFarBelow). A block whose scale is far
-// below vref keeps its probabilities to 2^-25 of vref, an error of 2^-25 of the
-// largest value.
-// The running maximum, the sums and the accumulators are float32.
+// below vref keeps its probabilities to 2^-25 of vref each, so T keys err by T
+// 2^-25 of the largest value that the row sees at most.
+// The running maximum, the sums and the accumulators are float32, and the
+// accumulators stay relative to vref until their mean is taken: sums of values
+// near float32's largest would pass it.
 
 #include <algorithm>
 #include <atomic>
@@ -72,8 +74,8 @@ struct Fp8Args {
   // balanced: desc[2c], desc[2c + 1] = the unit that CTA c continues / starts
   // without finishing (-1: none), with its partial result in the same slot
   int* desc;
-  float* part_o;   // [2 nCTA][rows][D], relative to 2^m, times the V scales
-  float2* part_ml; // [2 nCTA][rows]: (m, l)
+  float* part_o;   // [2 nCTA][rows][D], relative to 2^m and vref
+  float4* part_ml; // [2 nCTA][rows]: (m, l, vref, 0)
   uint32_t* err;
 };
 
@@ -86,9 +88,10 @@ __device__ __forceinline__ void dependents_enter() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Smallest power of two above x / 2^1 that is >= x (x clamped to a sane range).
+// The smallest power of two at or above x, within [2^-126, 2^126]: those have a
+// normal reciprocal, and no float is over four times the largest.
 __device__ __forceinline__ float pow2_above(float x) {
-  x = fminf(fmaxf(x, 1e-30f), 1e30f);
+  x = fminf(fmaxf(x, 1.1754944e-38f), 8.5070592e37f);
   return __uint_as_float((__float_as_uint(x) + 0x007fffffu) & 0x7f800000u);
 }
 
@@ -503,9 +506,10 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
   __syncwarp();
 
   // ---- join the four warps ------------------------------------------------
-  // a warp's O lies over its own ring; the maxima and sums behind all rings
-  static_assert(NC * D * 4 <= R::WARP, "O over the ring");
+  // a warp's O and its vrefs lie over its own ring; the maxima and sums behind all rings
+  static_assert(NC * (D + 1) * 4 <= R::WARP, "O over the ring");
   auto sO = [&](int w) { return reinterpret_cast<float(*)[D]>(dsm + w * R::WARP); };
+  auto sV = [&](int w) { return reinterpret_cast<float*>(dsm + w * R::WARP + NC * D * 4); };
   auto sM = reinterpret_cast<float(*)[NC]>(dsm + kMqWarps * R::WARP);
   auto sL = reinterpret_cast<float(*)[NC]>(dsm + kMqWarps * R::WARP + kMqWarps * NC * 4);
 #pragma unroll
@@ -515,28 +519,34 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
     if (gid == 0) {
       sM[warp][c] = m_run[nt][0]; sM[warp][c + 1] = m_run[nt][1];
       sL[warp][c] = l0; sL[warp][c + 1] = l1;
+      sV(warp)[c] = vref(nt, 0); sV(warp)[c + 1] = vref(nt, 1);
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int d0 = gid * VSEG + 2 * mt, d1 = d0 + 1;
-      sO(warp)[c][d0] = o_acc[nt][mt][0] * vref(nt, 0);
-      sO(warp)[c + 1][d0] = o_acc[nt][mt][1] * vref(nt, 1);
-      sO(warp)[c][d1] = o_acc[nt][mt][2] * vref(nt, 0);
-      sO(warp)[c + 1][d1] = o_acc[nt][mt][3] * vref(nt, 1);
+      sO(warp)[c][d0] = o_acc[nt][mt][0];
+      sO(warp)[c + 1][d0] = o_acc[nt][mt][1];
+      sO(warp)[c][d1] = o_acc[nt][mt][2];
+      sO(warp)[c + 1][d1] = o_acc[nt][mt][3];
     }
   }
   __syncthreads();
   for (int idx = tid; idx < cols * (D / 4); idx += kMqThreads) {
     const int c = idx / (D / 4), d4 = (idx % (D / 4)) * 4;
-    float M = neg_inf();
+    float M = neg_inf(), up = 0.f;
 #pragma unroll
-    for (int w = 0; w < kMqWarps; ++w) M = fmaxf(M, sM[w][c]);
+    for (int w = 0; w < kMqWarps; ++w) {
+      M = fmaxf(M, sM[w][c]);
+      up = fmaxf(up, sV(w)[c]);
+    }
+    const float down = pow2_inverse(up);
     float L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kMqWarps; ++w) {
-      const float f = (sM[w][c] == neg_inf()) ? 0.f : exp2_approx(sM[w][c] - M);
+      float f = (sM[w][c] == neg_inf()) ? 0.f : exp2_approx(sM[w][c] - M);
       L += f * sL[w][c];
+      f *= sV(w)[c] * down;
       const float4 o = *reinterpret_cast<const float4*>(&sO(w)[c][d4]);
       acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
     }
@@ -544,10 +554,10 @@ __device__ __forceinline__ void mq_segment(const Fp8Args& a, unsigned char* dsm,
       const float inv = 1.f / L;  // no visible key: 0 / 0, as the softmax over nothing
       const int cg = c0 + c, s = cg / a.G, g = cg - s * a.G;
       *reinterpret_cast<uint2*>(a.out + b * a.os_b + h * a.os_h + g * a.os_g + s * a.os_s + d4 * 2) =
-          make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+          make_uint2(pack2<BF16>(acc.x * inv * up, acc.y * inv * up), pack2<BF16>(acc.z * inv * up, acc.w * inv * up));
     } else {
       *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * NC + c) * D + d4) = acc;
-      if (d4 == 0) a.part_ml[(int64_t)slot * NC + c] = make_float2(M, L);
+      if (d4 == 0) a.part_ml[(int64_t)slot * NC + c] = make_float4(M, L, up, 0.f);
     }
   }
   __syncthreads();  // the area is reused by the CTA's next segment
@@ -755,8 +765,8 @@ __device__ __forceinline__ float score_mult(const Fp8Args& a) {
 __device__ __forceinline__ float key_factor(float ks, float mult) {
   constexpr float kMost = 3.4028235e38f;
   const float f = ks * mult;
-  if (f > kMost && ks <= kMost && mult <= kMost) return kMost;
-  return f < 1.4e-45f ? 1.4e-45f : f;
+  const float g = f > kMost && fmaxf(ks, mult) <= kMost ? kMost : f;
+  return g < 1.4e-45f ? 1.4e-45f : g;
 }
 
 // Eight f16 that stand for codes as bf16 times 2^-17, exact: a code has four
@@ -1180,6 +1190,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
             ks = 1.f;
             vs = 0.f;
           }
+          ks = key_factor(ks, mult);
           const uint32_t vmax = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vs, 0.f)));
           if (T >= kMetaRing &&
               !__all_sync(0xffffffffu, wait_for(bar(T_ME + ms), ((T / kMetaRing) - 1) & 1, abort))) {
@@ -1187,7 +1198,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
             break;
           }
           if (lane < 16) {
-            meta[ms].ks[lane] = key_factor(ks, mult);
+            meta[ms].ks[lane] = ks;
             meta[ms].vs[lane] = vs;
           }
           if (lane == 0) {
@@ -1377,7 +1388,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
         break;
       }
       tc_fence_after();
-      const float up = g.whole ? vref / l_run : vref;  // a row that sees no key: 0 / 0
+      const float inv_l = 1.f / l_run;  // a row that sees no key: 0 times infinity
       const int64_t slot = ((int64_t)(2 * blockIdx.x + (g.head ? 1 : 0)) * NX + x) * 128 + r;
       char* orow = a.out + g.b * a.os_b + g.h * a.os_h + gq * a.os_g + (int64_t)s * a.os_s;
 #pragma unroll
@@ -1394,8 +1405,10 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
         if (!row_ok) continue;
         float f[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]) * up;
+        for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]);
         if (g.whole) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = f[e] * inv_l * vref;
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4)
             *reinterpret_cast<uint4*>(orow + (c * 32 + q4 * 8) * 2) =
@@ -1408,7 +1421,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
                 make_float4(f[q4 * 4], f[q4 * 4 + 1], f[q4 * 4 + 2], f[q4 * 4 + 3]);
         }
       }
-      if (!g.whole && row_ok) a.part_ml[slot] = make_float2(m_run, l_run);
+      if (!g.whole && row_ok) a.part_ml[slot] = make_float4(m_run, l_run, vref, 0.f);
       if (nt > 0) {
         tc_fence_before();
         __syncwarp();
@@ -1431,23 +1444,36 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
   }
 }
 
-// Whether a part (maximum, sum) saw no key. Scores that are all NaN leave the
-// maximum at -inf too (it passes over NaN), but a sum of NaN, which the join
-// takes on.
-__device__ __forceinline__ bool no_keys(float2 ml) { return ml.x == neg_inf() && ml.y == 0.f; }
+// Takes a part (maximum, sum, vref) of a row into the row's so far; w0 and w1
+// are what their accumulators count with. False: the part saw no key. Scores
+// that are all NaN leave a maximum of -inf too (it passes over NaN), but a sum
+// of NaN, which is taken on.
+__device__ __forceinline__ bool join(float4& row, const float4& part, float& w0, float& w1) {
+  if (part.x == neg_inf() && part.y == 0.f) return false;
+  const float m = fmaxf(row.x, part.x), v = fmaxf(row.z, part.z), down = pow2_inverse(v);
+  w0 = exp2_approx(row.x - m);
+  w1 = exp2_approx(part.x - m);
+  row.y = row.y * w0 + part.y * w1;
+  w0 *= row.z * down;
+  w1 *= part.z * down;
+  row.x = m;
+  row.z = v;
+  return true;
+}
 
 // Joins the partial results of the units that several CTAs share. CTA (c, y):
 // the chain that CTA c of the attention kernel starts, in parts c, c + 1, ...
 // while those continue the same unit. 8 warps = RPC rows x KS slices of the
 // chain, PASSES times over, a lane holding 4 (D = 128) or 2 dimensions of its
-// row; the next four parts' loads are issued before any is used. Bound by the
-// parts' bytes in L2, and by its launch where there are few.
+// row; the next four parts' loads (of each slice two; four: 109 us for 64
+// sequences of 4 tokens, against 106) are issued before any is used. Bound by
+// the parts' bytes in L2, and by its launch where there are few.
 template <int D, bool BF16, int ROWS, int RPC, int PASSES>
 __global__ void __launch_bounds__(256) paged_attn_fp8_merge_kernel(const Fp8Args a, int n_cta, int qt) {
-  constexpr int KS = 8 / RPC, E = D / 32, U = 4;
+  constexpr int KS = 8 / RPC, E = D / 32, U = KS == 1 ? 4 : 2;
   static_assert(KS == 1 || PASSES == 1, "slices meet once");
   __shared__ float so[8][D];
-  __shared__ float2 sml[8];
+  __shared__ float4 sml[8];
   __shared__ int s_len;
   dependents_enter();
   const int c = blockIdx.x;
@@ -1479,16 +1505,17 @@ __global__ void __launch_bounds__(256) paged_attn_fp8_merge_kernel(const Fp8Args
       s = (tile * (ROWS / 128) + (row >> 7)) * qt + r - g * qt;
     }
     const bool live = g < a.G && s < a.S;
-    float M = neg_inf(), L = 0.f, acc[E];
+    float4 all = make_float4(neg_inf(), 0.f, 0.f, 0.f);
+    float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
     for (int i0 = slice; live && i0 < parts; i0 += U * KS) {
-      float2 ml[U];
+      float4 ml[U];
       float o[U][E];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + u * KS;
-        ml[u] = make_float2(neg_inf(), 0.f);
+        ml[u] = make_float4(neg_inf(), 0.f, 0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[u][e] = 0.f;
         if (i < parts) {
@@ -1505,39 +1532,33 @@ __global__ void __launch_bounds__(256) paged_attn_fp8_merge_kernel(const Fp8Args
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (no_keys(ml[u])) continue;
-        const float mn = fmaxf(M, ml[u].x);
-        const float f0 = exp2_approx(M - mn), f1 = exp2_approx(ml[u].x - mn);
-        M = mn;
-        L = L * f0 + ml[u].y * f1;
+        float w0, w1;
+        if (!join(all, ml[u], w0, w1)) continue;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + o[u][e] * f1;
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + o[u][e] * w1;
       }
     }
     if (KS > 1) {
 #pragma unroll
       for (int e = 0; e < E; ++e) so[warp][lane * E + e] = acc[e];
-      if (lane == 0) sml[warp] = make_float2(M, L);
+      if (lane == 0) sml[warp] = all;
       __syncthreads();
       for (int k = 1; slice == 0 && k < KS; ++k) {
-        const float2 ml = sml[warp + k * RPC];
-        if (no_keys(ml)) continue;
-        const float mn = fmaxf(M, ml.x);
-        const float f0 = exp2_approx(M - mn), f1 = exp2_approx(ml.x - mn);
-        M = mn;
-        L = L * f0 + ml.y * f1;
+        float w0, w1;
+        if (!join(all, sml[warp + k * RPC], w0, w1)) continue;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + so[warp + k * RPC][lane * E + e] * f1;
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * w0 + so[warp + k * RPC][lane * E + e] * w1;
       }
     }
     if (!live || slice != 0) continue;
-    const float inv = 1.f / L;
+    const float inv = 1.f / all.y;  // a row that sees no key: 0 times infinity
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = acc[e] * inv * all.z;
     char* to = a.out + b * a.os_b + h * a.os_h + g * a.os_g + (int64_t)s * a.os_s + lane * E * 2;
     if constexpr (E == 4)
-      *reinterpret_cast<uint2*>(to) =
-          make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]));
     else
-      *reinterpret_cast<uint32_t*>(to) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
+      *reinterpret_cast<uint32_t*>(to) = pack2<BF16>(acc[0], acc[1]);
   }
 }
 
@@ -1597,7 +1618,7 @@ int plan_fp8(const rbln_paged_attn_params_t* p, Fp8Plan* pl) {
     pl->desc = off;
     off += round256((size_t)2 * pl->ctas * sizeof(int));
     pl->ml = off;
-    off += round256((size_t)2 * pl->ctas * pl->rows * sizeof(float2));
+    off += round256((size_t)2 * pl->ctas * pl->rows * sizeof(float4));
     pl->o = off;
     off += round256((size_t)2 * pl->ctas * pl->rows * p->head_dim * sizeof(float));
   }
@@ -1759,7 +1780,7 @@ int run_prefill_fp8(const rbln_paged_attn_params_t* p, cudaStream_t st) {
   char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(p->workspace) + 255) & ~uintptr_t(255));
   if (pl.balanced) {
     a.desc = reinterpret_cast<int*>(base + pl.desc);
-    a.part_ml = reinterpret_cast<float2*>(base + pl.ml);
+    a.part_ml = reinterpret_cast<float4*>(base + pl.ml);
     a.part_o = reinterpret_cast<float*>(base + pl.o);
   }
   a.err = p->error_flags;
