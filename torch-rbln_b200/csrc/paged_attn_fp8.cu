@@ -1595,8 +1595,9 @@ int plan_fp8(const rbln_paged_attn_params_t* p, Fp8Plan* pl) {
   // Two row tiles share a key tile's conversion where there are over 128 rows:
   // one tile against two, same sequences: 105 to 111 us at 128 rows, 169 to
   // 124 at 160, 310 to 216 at 512.
-  const int64_t pool = (int64_t)p->num_blocks * p->cache_stride[0];
-  pl->nx = rows <= 16 && pool >> 4 <= (int64_t)UINT32_MAX ? 0 : rows <= 128 ? 1 : 2;
+  const int64_t last = (p->num_blocks - 1) * p->cache_stride[0] + (p->num_kv_heads - 1) * p->cache_stride[1] +
+                       (p->block_size - 1) * p->cache_stride[2];  // where the pool's last row starts
+  pl->nx = rows <= 16 && last >> 4 <= (int64_t)UINT32_MAX ? 0 : rows <= 128 ? 1 : 2;
   pl->nt = rows <= 8 ? 1 : 2;
   pl->qt = 128 / p->group;
   pl->rows = pl->nx ? 128 * pl->nx : 8 * pl->nt;
