@@ -50,3 +50,21 @@ def test_tensors_of_another_device(name):
                 call()
                 pytest.fail(f"call {i} was taken")
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("S", [1, 5, 40])
+def test_masks_over_no_position(S):
+    """A position mask [B, 0] keeps nothing; it is refused, not taken for no mask."""
+    import torch_rbln_b200 as tr
+
+    x = P.dev(P.setup([20, 3], S, 2, 4, 64, 16))
+    mask = torch.ones([2, 0], dtype=torch.bool, device=DEV)
+    with pytest.raises(RuntimeError, match="mask covers no position"):
+        P.run(x, mask=mask)
+    new, at = (x["q"], x["k"], x["v"]), (x["seq"], x["scale"], x["bt"], x["bs"])
+    wide = [x[n].to(torch.bfloat16) for n in ("kc", "vc")]
+    with pytest.raises(RuntimeError, match="mask covers no position"):
+        tr.paged_causal_attn_prefill(*new, *wide, *at, False, mask)
+    if S == 1:
+        with pytest.raises(RuntimeError, match="mask covers no position"):
+            tr.paged_causal_attn_decode(*new, *wide, *at, mask)

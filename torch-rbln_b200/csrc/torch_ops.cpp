@@ -168,6 +168,8 @@ void fill_paged(Common& c, const char* op, const at::Tensor& q_in, const at::Ten
     TORCH_CHECK(c.mask.scalar_type() == at::kFloat || c.mask.scalar_type() == at::kHalf ||
                     c.mask.scalar_type() == at::kBFloat16 || c.mask.scalar_type() == at::kBool,
                 op, ": mask must be floating point or bool");
+    // an empty one has no pointer, which would read as no mask
+    TORCH_CHECK(c.mask.dim() > 0 && c.mask.size(-1) > 0, op, ": mask covers no position, got ", c.mask.sizes());
     if (c.mask.stride(-1) != 1) c.mask = c.mask.contiguous();
     p.mask = c.mask.data_ptr();
     p.mask_dtype = to_rbln_dtype(c.mask.scalar_type());
