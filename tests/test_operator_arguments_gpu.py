@@ -68,3 +68,15 @@ def test_masks_over_no_position(S):
     if S == 1:
         with pytest.raises(RuntimeError, match="mask covers no position"):
             tr.paged_causal_attn_decode(*new, *wide, *at, mask)
+
+
+@pytest.mark.parametrize("S", [1, 4, 40])
+def test_rows_that_are_there_cost_no_copies(S):
+    """k and v None: the call allocates its output and its workspace, nothing that would stand in for the rows."""
+    x = P.dev(P.setup([200, 90], S, 2, 4, 64, 16))
+    P.run(x)
+    for _ in range(2):
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        out = P.run(x, rows=False)
+        assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == 2
+    assert out.shape == x["q"].shape

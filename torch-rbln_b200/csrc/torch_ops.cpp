@@ -78,13 +78,15 @@ struct Common {
   rbln_paged_attn_params_t p{};
 };
 
-// Shared validation and parameter fill for the four paged ops.
+// Shared validation and parameter fill for the paged ops. k and v undefined:
+// their rows are in the cache already.
 void fill_paged(Common& c, const char* op, const at::Tensor& q_in, const at::Tensor& k_in,
                 const at::Tensor& v_in, at::Tensor& kcache, at::Tensor& vcache, const at::Tensor& seq_in,
                 const at::Tensor& scale, const at::Tensor& block_table_in, int64_t block_size,
                 const std::optional<at::Tensor>& mask_in, bool decode) {
   TORCH_CHECK(q_in.is_cuda(), op, ": expected CUDA tensors, q is on ", q_in.device());
-  TORCH_CHECK(q_in.dim() == 5 && k_in.dim() == 5 && v_in.dim() == 5, op,
+  const bool rows = k_in.defined();
+  TORCH_CHECK(q_in.dim() == 5 && (!rows || (k_in.dim() == 5 && v_in.dim() == 5)), op,
               ": q/k/v must be 5-D [B, Hkv, G, S, D] / [B, Hkv, 1, S, D]");
   TORCH_CHECK(kcache.dim() == 5 && vcache.dim() == 5, op,
               ": kcache/vcache must be 5-D [num_blocks, Hkv, 1, block_size, D]");
@@ -98,20 +100,23 @@ void fill_paged(Common& c, const char* op, const at::Tensor& q_in, const at::Ten
   // k, v or a cache of another device would be read through a pointer that q's GPU does not have
   TORCH_CHECK(kcache.device() == q_in.device() && vcache.device() == q_in.device(), op,
               ": caches must be on q's device");
-  TORCH_CHECK(k_in.device() == q_in.device() && v_in.device() == q_in.device(), op, ": k and v must be on q's device");
+  TORCH_CHECK(!rows || (k_in.device() == q_in.device() && v_in.device() == q_in.device()), op,
+              ": k and v must be on q's device");
   TORCH_CHECK(kcache.stride(-1) == 1 && kcache.size(2) == 1, op,
               ": caches must be [num_blocks, Hkv, 1, block_size, D] with a contiguous last dim");
   const auto dt = q_in.scalar_type();
   TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf, op, ": q must be bfloat16 or float16, got ", dt);
-  TORCH_CHECK(k_in.scalar_type() == dt && v_in.scalar_type() == dt, op, ": q, k, v must share a dtype");
+  TORCH_CHECK(!rows || (k_in.scalar_type() == dt && v_in.scalar_type() == dt), op, ": q, k, v must share a dtype");
 
   c.q = q_in.contiguous();
-  c.k = k_in.contiguous();
-  c.v = v_in.contiguous();
   const int64_t B = c.q.size(0), Hkv = c.q.size(1), G = c.q.size(2), S = c.q.size(3), D = c.q.size(4);
-  TORCH_CHECK(c.k.size(0) == B && c.k.size(1) == Hkv && c.k.size(2) == 1 && c.k.size(3) == S &&
-                  c.k.size(4) == D && c.v.sizes() == c.k.sizes(),
-              op, ": k/v must be [B, Hkv, 1, S, D] matching q ", c.q.sizes(), ", got ", c.k.sizes());
+  if (rows) {
+    c.k = k_in.contiguous();
+    c.v = v_in.contiguous();
+    TORCH_CHECK(c.k.size(0) == B && c.k.size(1) == Hkv && c.k.size(2) == 1 && c.k.size(3) == S &&
+                    c.k.size(4) == D && c.v.sizes() == c.k.sizes(),
+                op, ": k/v must be [B, Hkv, 1, S, D] matching q ", c.q.sizes(), ", got ", c.k.sizes());
+  }
   TORCH_CHECK(kcache.size(1) == Hkv, op, ": caches hold ", kcache.size(1), " KV heads, q has ", Hkv);
   TORCH_CHECK(D <= kcache.size(-1), op, ": head_dim ", D, " exceeds the cache's last dim ", kcache.size(-1));
   TORCH_CHECK(kcache.size(3) == block_size, op, ": block_size ", block_size,
@@ -147,10 +152,12 @@ void fill_paged(Common& c, const char* op, const at::Tensor& q_in, const at::Ten
   c.out = at::empty_like(c.q, at::MemoryFormat::Contiguous);
   p.out = c.out.data_ptr();
   for (int i = 0; i < 4; ++i) p.out_stride[i] = c.out.stride(i);
-  p.k_new = c.k.data_ptr();
-  p.v_new = c.v.data_ptr();
-  p.k_new_stride[0] = c.k.stride(0); p.k_new_stride[1] = c.k.stride(1); p.k_new_stride[2] = c.k.stride(3);
-  p.v_new_stride[0] = c.v.stride(0); p.v_new_stride[1] = c.v.stride(1); p.v_new_stride[2] = c.v.stride(3);
+  if (rows) {
+    p.k_new = c.k.data_ptr();
+    p.v_new = c.v.data_ptr();
+    p.k_new_stride[0] = c.k.stride(0); p.k_new_stride[1] = c.k.stride(1); p.k_new_stride[2] = c.k.stride(3);
+    p.v_new_stride[0] = c.v.stride(0); p.v_new_stride[1] = c.v.stride(1); p.v_new_stride[2] = c.v.stride(3);
+  }
   p.kcache = kcache.data_ptr();
   p.vcache = vcache.data_ptr();
   p.kv_dtype = to_rbln_dtype(kcache.scalar_type());
@@ -342,14 +349,11 @@ at::Tensor paged_causal_attn_prefill_kvfp8_cuda(const at::Tensor& q, const std::
   TORCH_CHECK(q.dim() == 5, op, ": q must be 5-D [B, Hkv, G, S, D]");
   check_scales(op, kcache, k_scale, v_scale);
   Common c;
-  // without k and v, q's first query heads stand in for their checks
-  const at::Tensor qk = rows ? at::Tensor() : q.slice(2, 0, 1);
-  fill_paged(c, op, q, rows ? *k : qk, rows ? *v : qk, kcache, vcache, seq, scale, block_table, block_size, mask,
-             false);
+  fill_paged(c, op, q, rows ? *k : at::Tensor(), rows ? *v : at::Tensor(), kcache, vcache, seq, scale, block_table,
+             block_size, mask, false);
   if (c.mask.defined())
     TORCH_CHECK(c.mask.dim() == 2 && (c.mask.size(0) == 1 || c.mask.size(0) == q.size(0)), op,
                 ": mask must be a position mask [B, L], got ", c.mask.sizes());
-  if (!rows) c.p.k_new = c.p.v_new = nullptr;
   c.p.k_scale = k_scale.data_ptr<float>();
   c.p.v_scale = v_scale.data_ptr<float>();
   c.p.scale_stride[0] = k_scale.stride(0);
