@@ -177,8 +177,12 @@ int rbln_paged_prefill_workspace_size(const rbln_paged_attn_params_t* p, size_t*
  * attention reads them back with the rest. The scale here is
  * max(amax, 1e-6) * (1 / 448) with the reciprocal rounded to float32, as torch
  * computes `amax / 448.0` on the GPU, so a cache filled by this call holds bit
- * for bit what one quantised by torch there holds; rbln_paged_kv_write divides,
- * and its scales differ from these by at most one unit in the last place. k_new / v_new NULL:
+ * for bit what one quantised by torch there holds; rbln_paged_kv_write divides.
+ * After one write of the same rows to empty blocks the scales of the two differ
+ * by at most one unit in the last place. A later write that leaves a block's
+ * largest value finds its scale from 448 times the old one, which moves it by a
+ * unit at a time: up by at most 6 in all here, by at most 1 with the division.
+ * The held codes stay as they are. k_new / v_new NULL:
  * the rows [seq[b], seq[b] + S_q) are in the cache already
  * (rbln_rotary_paged_kv_write). A key in a block outside the pool, at or past
  * the span, or not kept by the mask is not seen, whatever its bytes hold; a

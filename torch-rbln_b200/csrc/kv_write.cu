@@ -64,6 +64,17 @@ __device__ __forceinline__ float block_scale(const WriteArgs& a, float amax) {
   return a.reciprocal ? m * (1.f / kFp8Max) : __fdiv_rn(m, kFp8Max);
 }
 
+// Whether a block's held codes have to be found anew for its new scale. The
+// rounded reciprocal moves the scale of a block whose largest value stays by a
+// unit in the last place at a time (448 times the old scale, times 1 / 448:
+// over half of all scales move, by 6 units in all before they rest), which
+// leaves every code as it is: they lie 2^-5 of their value and more from the
+// next rounding. So up to 2^-20 of the scale they are left alone.
+__device__ __forceinline__ bool requantise(const WriteArgs& a, float scale, float old) {
+  if (a.reciprocal && fabsf(scale - old) <= fminf(scale, old) * 0x1p-20f) return false;
+  return scale != old;
+}
+
 __device__ __forceinline__ float from_e4m3(uint8_t q) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)q, __NV_E4M3);
   return __half2float(__half(h));
@@ -201,7 +212,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_kv_write_kernel(const Wri
     }
     const float scale = block_scale(a, warp_max(m));
     const float inv = __frcp_rn(scale);
-    if (held > 0 && scale != old) {
+    if (held > 0 && requantise(a, scale, old)) {
       for (int i = lane; i < held * cpr; i += 32) {
         const int r = i / cpr, c = i - r * cpr;
         uint2* q = reinterpret_cast<uint2*>(c8 + (int64_t)r * a.cs_tok + c * 8);
@@ -312,7 +323,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_kv_write_staged_kernel(co
   }
   const float scale = block_scale(a, warp_max(m));
   const float inv = __frcp_rn(scale);
-  if (held > 0 && scale != old) {
+  if (held > 0 && requantise(a, scale, old)) {
     for (int i = lane; i < held * cpr; i += 32) {
       const int r = i >> cshift, c = i & (cpr - 1);
       uint2* q = reinterpret_cast<uint2*>(c8 + (int64_t)r * a.cs_tok + c * 8);
