@@ -186,7 +186,9 @@ int rbln_paged_prefill_workspace_size(const rbln_paged_attn_params_t* p, size_t*
  * the rows [seq[b], seq[b] + S_q) are in the cache already
  * (rbln_rotary_paged_kv_write). A key in a block outside the pool, at or past
  * the span, or not kept by the mask is not seen, whatever its bytes hold; a
- * query that sees no key gives NaN. sinks are not supported. The workspace
+ * query that sees no key gives NaN. Scales are not negative (a write makes none;
+ * what one gives is not defined); zero, NaN and infinity are taken as they
+ * stand. sinks are not supported. The workspace
  * (rbln_paged_prefill_workspace_size) is required. */
 int rbln_paged_causal_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stream);
 

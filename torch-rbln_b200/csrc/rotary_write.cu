@@ -2,7 +2,8 @@
 // paged cache, in one launch (rbln_rotary_paged_kv_write): what a rotary
 // layer, and then rbln_paged_kv_write on its result, would do in three, with
 // one read of q, k and v and the rotated keys quantised from float32, not
-// from a rounded copy.
+// from a rounded copy. (The torch op copies inputs that are not contiguous
+// before that.)
 //
 // Token s of sequence b sits at position seq[b] + s. An fp8 cache follows the
 // rule of rbln_paged_kv_write (kv_write.cu): scale = max(amax, 1e-6) / 448
