@@ -88,6 +88,18 @@ def test_values_behind_a_row_cost_it_nothing(S, G, bs, first, binades):
         check(d)
 
 
+@pytest.mark.parametrize("S,G,bs,first", [(4, 4, 16, 2), (40, 4, 64, 20), (40, 1, 128, 20), (100, 2, 32, 28)])
+def test_values_behind_a_row_under_a_mask(S, G, bs, first):
+    """A block of which the mask drops the chunk's earlier tokens; its kept ones, from `first` on, hold large values.
+    A row before them sees nothing of that block, and its bits are those of the blocks before."""
+    start = 2 * bs
+    d = P.setup([start, start], S, 2, G, 64, bs)
+    d["v"][:, :, :, first:] *= 2.0 ** 20
+    mask = torch.ones([2, d["bt"].shape[1] * bs], dtype=torch.bool)
+    mask[:, start: start + first] = False
+    check(d, mask)
+
+
 @pytest.mark.parametrize("S", [1, 4, 40])
 @pytest.mark.parametrize("starts", [[300, 11], [5000]])
 def test_values_near_the_largest(S, starts):

@@ -1261,13 +1261,19 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
         uint32_t v[32];
         float* const p = reinterpret_cast<float*>(v);
         const uint4 kwv = *reinterpret_cast<const uint4*>(meta[ms].keep);
+        float vm = meta[ms].vmax;
         if ((kwv.x & kwv.y & kwv.z & kwv.w) != 0xffffffffu || t0 + 128 > first_lim) {
-          // some key is not for some row: -inf over those scores first
+          // some key is not for some row: -inf over those scores first, and
+          // the largest V scale of the groups of which the row sees a key
+          vm *= kFarBelow;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             const int n = lim - (t0 + 32 * c);  // keys of the chunk before the row's limit
             const uint32_t kw = meta[ms].keep[c] & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u);
             tmem_ld32(ts + c * 32, v);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if ((kw >> (8 * u)) & 0xffu) vm = fmaxf(vm, meta[ms].vs[4 * c + u]);
             tmem_wait_ld32(v);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
@@ -1308,14 +1314,6 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           factor = exp2_approx(m_run - m_new);
           l_run *= factor;
           m_run = m_new;
-        }
-        float vm = meta[ms].vmax;
-        if (t0 + 128 > first_lim) {  // the largest V scale that this row sees
-          const int seen = lim - t0;
-          vm *= kFarBelow;
-#pragma unroll 4
-          for (int u = 0; u < 16; ++u)
-            if (8 * u < seen) vm = fmaxf(vm, meta[ms].vs[u]);
         }
         if (vm > vref) {
           const float now = pow2_above(vm);
