@@ -187,8 +187,10 @@ int rbln_paged_prefill_workspace_size(const rbln_paged_attn_params_t* p, size_t*
  * (rbln_rotary_paged_kv_write). A key in a block outside the pool, at or past
  * the span, or not kept by the mask is not seen, whatever its bytes hold; a
  * query that sees no key gives NaN. Scales are not negative (a write makes none;
- * what one gives is not defined); zero, NaN and infinity are taken as they
- * stand. sinks are not supported. The workspace
+ * what one gives is not defined); zero and all other finite ones are taken as
+ * they stand. One that is NaN or infinite gives no number to a query that sees
+ * its block, and may give none to an earlier token of the call. sinks are not
+ * supported. The workspace
  * (rbln_paged_prefill_workspace_size) is required. */
 int rbln_paged_causal_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stream);
 

@@ -166,8 +166,11 @@ __device__ __forceinline__ void cost_prefix(const Fp8Args& a, int unit, int scal
 // shared memory. The keys of all (head, sequence) units are cut into equal
 // shares, one CTA each, three CTAs an SM (two: 110 us against 102 for 64
 // sequences of 4 tokens, G = 4, 8 KV heads, behind 128 to 4096 keys). There it
-// reads 2.7 TB/s, 42 % of the copy rate: latency of 12 warps an SM and the
-// segments' starts bound it (copies alone 82 us, products alone 77).
+// takes 107 us with its merge and reads 2.7 TB/s, 41 % of the copy rate:
+// latency of 12 warps an SM and the segments' starts bound it (copies alone 82
+// us, products alone 77). Issue slots are busy 37 % of the time; of the 7.7
+// cycles from one instruction of a warp to its next 1.7 are for the one before,
+// 1.4 for long loads, 1.2 for the next to be fetched, 0.9 for shared memory.
 // ---------------------------------------------------------------------------
 // A warp's ring of tiles in shared memory, filled by cp.async. Rows are
 // swizzled by 16-byte chunks so that the fragments' loads meet no bank twice:
@@ -659,10 +662,13 @@ __global__ void __launch_bounds__(kMqThreads, kMqCtas) paged_attn_fp8_rows_kerne
 // V and the keys of f16 queries are f16 (one instruction for two codes), the
 // keys of bf16 queries bf16. Reading codes instead of 16-bit rows halves HBM
 // and L2 traffic. Shared memory (D = 128, NX = 2): Q 64 KB, K and V 2 x 32 KB
-// each, raw 2 x 16 KB. Loops are rolled: instruction fetch bounds the kernel
-// (the chunk below took 633 us unrolled). It measures 387 us, 754 TFLOP/s, for
-// 8 sequences of 512 queries behind 512 to 7680 keys: the chain from a row
-// tile's scores through its softmax to its product bounds it.
+// each, raw 2 x 16 KB. Loops are rolled: unrolled, with the roles' code in one
+// instruction cache, the chunk below took 633 us. It measures 387 us, 754
+// TFLOP/s, for 8 sequences of 512 queries behind 512 to 7680 keys. The chain
+// from a row tile's scores through its softmax to its product bounds it: the
+// tensor pipe is busy 40 % of the time, the exponentials' 40 %, issue slots 51
+// %; of the 7.8 cycles from one instruction of a warp to its next 2.2 are for
+// long loads, 1.8 for the one before, 0.5 for the next to be fetched.
 //
 // The key tiles of all units, head-major, are cut into equal shares, one a
 // CTA, so that there is one wave without a tail however unequal the
@@ -967,7 +973,7 @@ __global__ void __launch_bounds__(TcCfg<NX>::THREADS, 1)
           const uint32_t turn = part == 0 ? flip : 0u;
           const uint8_t* src = sgen + L::R0 + rs * L::RAW + row0 * D + c16 * 16;
           uint8_t* dst = sgen + (part ? L::V0 : L::K0) + st * L::TILE + row0 * 128 + dst_panel;
-          // two steps a turn: instruction fetch bounds this kernel (one, two, four steps:
+          // two steps a turn, for the instruction cache that the roles share (one, two, four steps:
           // 386, 387, 404 us for 8 sequences of 512 queries behind 512 to 7680 keys, 251, 250,
           // 257 for 4 of 48 queries behind some 18000 to 31000; eight: a third slower than two)
 #pragma unroll 2
