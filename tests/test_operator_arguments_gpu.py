@@ -80,3 +80,17 @@ def test_rows_that_are_there_cost_no_copies(S):
         out = P.run(x, rows=False)
         assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == 2
     assert out.shape == x["q"].shape
+
+
+@pytest.mark.parametrize("which", ["key", "value", "grad_out", "out", "logsumexp"])
+def test_sdpa_backward_of_another_device(which):
+    """A tensor of the backward call left on the host: refused before any launch."""
+    q, k, v = (torch.randn(1, 2, 16, 64, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+    out, lse, cq, ck, mq, mk, seed, off, _ = torch.ops.aten._scaled_dot_product_fused_attention_overrideable(
+        q, k, v, None, 0.0, True)
+    t = dict(grad_out=torch.ones_like(out), query=q, key=k, value=v, out=out, logsumexp=lse)
+    t[which] = t[which].cpu()
+    with pytest.raises(RuntimeError, match="must be on query's device"):
+        torch.ops.aten._scaled_dot_product_fused_attention_overrideable_backward(
+            t["grad_out"], t["query"], t["key"], t["value"], torch.empty(0, device=DEV), [True, True, True, False],
+            t["out"], t["logsumexp"], cq, ck, mq, mk, 0.0, True, seed, off)

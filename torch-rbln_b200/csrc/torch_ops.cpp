@@ -942,6 +942,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> sdpa_overrideable_bac
   TORCH_CHECK(key.scalar_type() == dt && value.scalar_type() == dt && grad_out.scalar_type() == dt &&
                   out.scalar_type() == dt,
               op, ": q, k, v, out and grad_out must share a dtype");
+  for (const at::Tensor* t : {&key, &value, &grad_out, &out, &logsumexp, &attn_bias})
+    TORCH_CHECK(!t->defined() || t->numel() == 0 || t->device() == query.device(), op,
+                ": all tensors must be on query's device, got ", t->device(), " beside ", query.device());
   c10::cuda::CUDAGuard guard(query.device());
   // last dim contiguous and 16-byte aligned rows
   auto rows16 = [](const at::Tensor& t) {
