@@ -268,6 +268,73 @@ int rbln_rotary_paged_kv_write(const rbln_paged_attn_params_t* p, const rbln_rot
 int rbln_paged_kv_read(const rbln_paged_attn_params_t* p, void* k_out, void* v_out, const int64_t* out_stride,
                        cudaStream_t stream);
 
+/* Pages that several sequences share. One block table serves the caches of
+ * all layers; refs[p] counts the table entries that hold page p, and a page
+ * with a count of 0 or less is free. A table entry outside [0, num_blocks)
+ * holds no page. The caches of all layers are alike in shape, strides and
+ * type. Calls on one table or pool are ordered by the stream; each call's
+ * result is that of one thread going through rows and columns in order.
+ * No reference counterpart. */
+typedef struct {
+  int32_t batch, max_blocks; /* block_table [batch, max_blocks]; max_blocks * block_size < 2^31 */
+  int32_t num_blocks, block_size;
+  void* block_table;
+  int32_t block_table_dtype; /* I16 (num_blocks <= 32768), I32 or I64 */
+  int64_t block_table_stride[2];
+  int32_t* refs;             /* [num_blocks], contiguous */
+  const void* lengths;       /* [batch]: see each call */
+  int32_t lengths_dtype;     /* I16, I32 or I64 */
+  int64_t lengths_stride;
+  /* reserve and compact: host arrays [num_layers] of device pointers */
+  int32_t num_layers, num_kv_heads, head_dim;
+  int32_t kv_dtype;          /* F16, BF16 or FP8_E4M3 */
+  void* const* kcaches;      /* each [num_blocks, num_kv_heads, block_size, head_dim] */
+  void* const* vcaches;
+  int64_t cache_stride[3];   /* block, head, token */
+  float* const* k_scales;    /* fp8: each [num_blocks, num_kv_heads]; else NULL */
+  float* const* v_scales;
+  int64_t scale_stride[2];   /* block, head */
+  void* workspace;           /* rbln_paged_kv_pages_workspace_size bytes */
+  size_t workspace_bytes;
+} rbln_pages_params_t;
+
+size_t rbln_pages_params_sizeof(void);
+
+/* Forks row parents[i] into row i of table_out [forks, max_blocks] (the
+ * table's type, columns contiguous) and lengths_out [forks] (the lengths'
+ * type): the entries that hold the parent's positions [0, lengths[parent])
+ * are taken over and their counts go up; the others are -1. Lengths are cut
+ * to [0, span]. A parent outside [0, batch) gives an empty row. */
+int rbln_paged_kv_fork(const rbln_pages_params_t* p, const void* parents, int32_t parents_dtype,
+                       int64_t parents_stride, int32_t forks, void* table_out, int64_t table_out_stride,
+                       void* lengths_out, cudaStream_t stream);
+
+/* Gives the positions from lengths[b] (none below 0) on: every entry from
+ * position ceil(lengths[b] / block_size) * block_size on becomes -1 and its
+ * page's count goes down, never below 0. */
+int rbln_paged_kv_free(const rbln_pages_params_t* p, cudaStream_t stream);
+
+/* Scratch for reserve (new_tokens >= 0) and compact (new_tokens < 0). */
+int rbln_paged_kv_pages_workspace_size(const rbln_pages_params_t* p, int32_t new_tokens, size_t* bytes);
+
+/* Makes positions [lengths[b], lengths[b] + new_tokens) of every row with
+ * lengths[b] >= 0 writable, as far as the span goes: an entry without a page
+ * gets the lowest free one, and one whose page others hold too gets the
+ * lowest free one with a copy, in every layer, of the rows that the sequence
+ * holds there (and of the page's scales). Rows in order, so of a page that
+ * only rows of this call hold the last one keeps it. granted[b]: how many
+ * positions from lengths[b] on may be written, fewer than asked for where
+ * free pages or the span ran out (those entries are left as they were).
+ * Rows of a page that was not copied, and its scales, are left as they are. */
+int rbln_paged_kv_reserve(const rbln_pages_params_t* p, int32_t new_tokens, int32_t* granted, cudaStream_t stream);
+
+/* Moves the pages in use to the front of the pool: with *live of them, the
+ * i-th free page below *live takes the i-th page in use from there on, in
+ * every layer, with scales and counts, and the table's entries follow.
+ * moved[p]: where page p is now, -1 for one that was free. p->lengths is not
+ * read. */
+int rbln_paged_kv_compact(const rbln_pages_params_t* p, int32_t* moved, int32_t* live, cudaStream_t stream);
+
 /* Dense scaled dot-product attention, forward. */
 typedef struct {
   int32_t batch, num_heads, num_kv_heads, q_len, kv_len, head_dim; /* GQA: num_heads % num_kv_heads == 0 */

@@ -14,6 +14,7 @@
 #include <ATen/SDPBackend.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/_fused_sdp_choice_native.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
@@ -28,6 +29,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <string>
+#include <vector>
 
 #include "rbln_attn.h"
 
@@ -714,6 +716,201 @@ void paged_kv_write_cuda(const at::Tensor& k_in, const at::Tensor& v_in, at::Ten
 }
 
 // ---------------------------------------------------------------------------
+// Pages that several sequences share (pages.cu): the caller's state is one
+// block table for all layers and refs, how many of its entries hold each page.
+// ---------------------------------------------------------------------------
+bool is_index(at::ScalarType t) { return t == at::kShort || t == at::kInt || t == at::kLong; }
+
+// A table that the call writes must hold every entry at a place of its own.
+rbln_pages_params_t check_pages(const char* op, const at::Tensor& block_table, const at::Tensor& refs,
+                                int64_t block_size, bool written) {
+  TORCH_CHECK(block_table.is_cuda(), op, ": expected CUDA tensors, block_table is on ", block_table.device());
+  TORCH_CHECK(block_table.dim() == 2 && is_index(block_table.scalar_type()), op,
+              ": block_table must be [B, max_blocks] of int16/int32/int64, got ", block_table.sizes(), " of ",
+              block_table.scalar_type());
+  TORCH_CHECK(!written || at::has_internal_overlap(block_table) != at::MemOverlap::Yes, op,
+              ": block_table is written and must not be expanded");
+  TORCH_CHECK(refs.dim() == 1 && refs.scalar_type() == at::kInt && refs.is_contiguous(), op,
+              ": refs must be contiguous int32 [num_blocks], got ", refs.sizes(), " of ", refs.scalar_type());
+  TORCH_CHECK(refs.device() == block_table.device(), op, ": refs must be on block_table's device");
+  TORCH_CHECK(block_size > 0 && block_size <= INT32_MAX, op, ": block_size must be positive, got ", block_size);
+  TORCH_CHECK(block_table.size(0) <= INT32_MAX && refs.numel() <= INT32_MAX &&
+                  block_table.size(1) <= INT32_MAX / block_size,
+              op, ": block_table spans 2^31 positions or more");
+  TORCH_CHECK(block_table.scalar_type() != at::kShort || refs.numel() <= 32768, op,
+              ": an int16 block_table cannot name ", refs.numel(), " blocks");
+  rbln_pages_params_t p{};
+  p.batch = (int32_t)block_table.size(0);
+  p.max_blocks = (int32_t)block_table.size(1);
+  p.num_blocks = (int32_t)refs.numel();
+  p.block_size = (int32_t)block_size;
+  p.block_table = block_table.data_ptr();
+  p.block_table_dtype = to_rbln_dtype(block_table.scalar_type());
+  p.block_table_stride[0] = block_table.stride(0);
+  p.block_table_stride[1] = block_table.stride(1);
+  p.refs = refs.data_ptr<int32_t>();
+  p.lengths_dtype = RBLN_DT_I32;
+  return p;
+}
+
+// One whole number a row of the table, kept alive by the caller.
+at::Tensor check_lengths(const char* op, const char* name, const at::Tensor& lengths_in, const at::Tensor& block_table,
+                         rbln_pages_params_t& p) {
+  at::Tensor n = on_device(lengths_in, block_table).reshape({-1});
+  TORCH_CHECK(is_index(n.scalar_type()), op, ": ", name, " must be int16/int32/int64, got ", n.scalar_type());
+  TORCH_CHECK(n.numel() == block_table.size(0), op, ": ", name, " must hold one entry per row, got ",
+              lengths_in.sizes(), " for ", block_table.sizes());
+  p.lengths = n.data_ptr();
+  p.lengths_dtype = to_rbln_dtype(n.scalar_type());
+  p.lengths_stride = n.stride(0);
+  return n;
+}
+
+struct LayerPointers {
+  std::vector<void*> k, v;
+  std::vector<float*> ks, vs;
+};
+using TensorLists = std::optional<std::vector<at::Tensor>>;
+
+// The caches of all layers, alike, [num_blocks, Hkv, 1, block_size, D]; their
+// number of blocks is refs'. Scales go with float8_e4m3fn caches only.
+void check_layers(const char* op, at::TensorList kcaches, at::TensorList vcaches, const TensorLists& k_scales,
+                  const TensorLists& v_scales, const at::Tensor& block_table, rbln_pages_params_t& p,
+                  LayerPointers& ptrs) {
+  TORCH_CHECK(!kcaches.empty() && kcaches.size() == vcaches.size(), op,
+              ": kcaches and vcaches must hold one cache for each layer, got ", kcaches.size(), " and ",
+              vcaches.size());
+  const at::Tensor& c = kcaches[0];
+  const auto ct = c.scalar_type();
+  const bool fp8 = ct == at::kFloat8_e4m3fn;
+  TORCH_CHECK(c.dim() == 5 && c.size(2) == 1 && c.stride(-1) == 1, op,
+              ": caches must be [num_blocks, Hkv, 1, block_size, D] with a contiguous last dim, got ", c.sizes());
+  TORCH_CHECK(fp8 || ct == at::kBFloat16 || ct == at::kHalf, op,
+              ": caches must be bfloat16, float16 or float8_e4m3fn, got ", ct);
+  TORCH_CHECK(c.size(0) == p.num_blocks, op, ": caches hold ", c.size(0), " blocks, refs ", p.num_blocks);
+  TORCH_CHECK(c.size(1) > 0 && c.size(-1) > 0 && c.size(-1) % 64 == 0, op,
+              ": the last dimension of a cache must be a multiple of 64, but got shape ", c.sizes());
+  TORCH_CHECK(at::has_internal_overlap(c) != at::MemOverlap::Yes, op, ": caches are written and must not be expanded");
+  for (const at::TensorList list : {kcaches, vcaches})
+    for (const at::Tensor& t : list) {
+      TORCH_CHECK(t.device() == block_table.device(), op, ": caches must be on block_table's device");
+      TORCH_CHECK(t.sizes() == c.sizes() && t.strides() == c.strides() && t.scalar_type() == ct, op,
+                  ": all caches must match in shape, strides and dtype");
+    }
+  TORCH_CHECK(k_scales.has_value() == fp8 && v_scales.has_value() == fp8, op,
+              ": k_scales and v_scales go with float8_e4m3fn caches, and only with them");
+  p.num_layers = (int32_t)kcaches.size();
+  p.num_kv_heads = (int32_t)c.size(1);
+  p.head_dim = (int32_t)c.size(-1);
+  p.kv_dtype = to_rbln_dtype(ct);
+  p.block_size = (int32_t)c.size(3);
+  p.cache_stride[0] = c.stride(0);
+  p.cache_stride[1] = c.stride(1);
+  p.cache_stride[2] = c.stride(3);
+  for (size_t i = 0; i < kcaches.size(); ++i) {
+    ptrs.k.push_back(kcaches[i].data_ptr());
+    ptrs.v.push_back(vcaches[i].data_ptr());
+  }
+  p.kcaches = ptrs.k.data();
+  p.vcaches = ptrs.v.data();
+  if (!fp8) return;
+  TORCH_CHECK(k_scales->size() == kcaches.size() && v_scales->size() == kcaches.size(), op,
+              ": k_scales and v_scales must hold one tensor for each layer");
+  for (size_t i = 0; i < kcaches.size(); ++i) {
+    check_scales(op, c, (*k_scales)[i], (*v_scales)[i]);
+    TORCH_CHECK((*k_scales)[i].strides() == (*k_scales)[0].strides(), op, ": all scales must match in strides");
+    ptrs.ks.push_back((*k_scales)[i].data_ptr<float>());
+    ptrs.vs.push_back((*v_scales)[i].data_ptr<float>());
+  }
+  p.k_scales = ptrs.ks.data();
+  p.v_scales = ptrs.vs.data();
+  p.scale_stride[0] = (*k_scales)[0].stride(0);
+  p.scale_stride[1] = (*k_scales)[0].stride(1);
+}
+
+at::Tensor pages_workspace(const char* op, rbln_pages_params_t& p, int64_t new_tokens, const at::Tensor& like) {
+  size_t bytes = 0;
+  check_rc(rbln_paged_kv_pages_workspace_size(&p, (int32_t)new_tokens, &bytes), op);
+  at::Tensor w = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+  p.workspace = w.data_ptr();
+  p.workspace_bytes = bytes;
+  return w;
+}
+
+cudaStream_t stream_of(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// rbln_attn::paged_kv_fork: rows parents[i] of the table as rows of a new one,
+// their pages shared and counted.
+std::tuple<at::Tensor, at::Tensor> paged_kv_fork_cuda(const at::Tensor& block_table, const at::Tensor& lengths_in,
+                                                      const at::Tensor& parents_in, at::Tensor& refs,
+                                                      int64_t block_size) {
+  const char* op = "paged_kv_fork";
+  rbln_pages_params_t p = check_pages(op, block_table, refs, block_size, false);
+  c10::cuda::CUDAGuard guard(block_table.device());
+  const at::Tensor lengths = check_lengths(op, "lengths", lengths_in, block_table, p);
+  const at::Tensor parents = on_device(parents_in, block_table);
+  TORCH_CHECK(parents.dim() == 1 && is_index(parents.scalar_type()), op,
+              ": parents must be 1-D of int16/int32/int64, got ", parents.sizes(), " of ", parents.scalar_type());
+  const int64_t N = parents.numel();
+  TORCH_CHECK(N + p.batch <= INT32_MAX, op, ": too many forks");
+  at::Tensor table = at::empty({N, block_table.size(1)}, block_table.options());
+  at::Tensor out_lengths = at::empty({N}, lengths.options());
+  check_rc(rbln_paged_kv_fork(&p, parents.data_ptr(), to_rbln_dtype(parents.scalar_type()),
+                              N > 0 ? parents.stride(0) : 1, (int32_t)N, table.data_ptr(), table.stride(0),
+                              out_lengths.data_ptr(), stream_of(block_table)),
+           op);
+  return {table, out_lengths};
+}
+
+// rbln_attn::paged_kv_free: the pages behind the first keep[b] positions of
+// every row go back.
+void paged_kv_free_cuda(at::Tensor& block_table, const at::Tensor& keep_in, at::Tensor& refs, int64_t block_size) {
+  const char* op = "paged_kv_free";
+  rbln_pages_params_t p = check_pages(op, block_table, refs, block_size, true);
+  c10::cuda::CUDAGuard guard(block_table.device());
+  const at::Tensor keep = check_lengths(op, "keep", keep_in, block_table, p);
+  check_rc(rbln_paged_kv_free(&p, stream_of(block_table)), op);
+}
+
+// rbln_attn::paged_kv_reserve: pages of their own for every row's next
+// new_tokens positions; returns how many of them may be written.
+at::Tensor paged_kv_reserve_cuda(at::TensorList kcaches, at::TensorList vcaches, at::Tensor& block_table,
+                                 const at::Tensor& seq_in, at::Tensor& refs, int64_t block_size, int64_t new_tokens,
+                                 const TensorLists& k_scales, const TensorLists& v_scales) {
+  const char* op = "paged_kv_reserve";
+  rbln_pages_params_t p = check_pages(op, block_table, refs, block_size, true);
+  LayerPointers ptrs;
+  check_layers(op, kcaches, vcaches, k_scales, v_scales, block_table, p, ptrs);
+  TORCH_CHECK(p.block_size == block_size, op, ": block_size ", block_size,
+              " does not match the cache's block dimension ", p.block_size);
+  TORCH_CHECK(new_tokens >= 0 && new_tokens <= INT32_MAX, op, ": new_tokens must be in [0, 2^31), got ", new_tokens);
+  c10::cuda::CUDAGuard guard(block_table.device());
+  const at::Tensor seq = check_lengths(op, "seq", seq_in, block_table, p);
+  at::Tensor granted = at::empty({block_table.size(0)}, block_table.options().dtype(at::kInt));
+  const at::Tensor workspace = pages_workspace(op, p, new_tokens, block_table);
+  check_rc(rbln_paged_kv_reserve(&p, (int32_t)new_tokens, granted.data_ptr<int32_t>(), stream_of(block_table)), op);
+  return granted;
+}
+
+// rbln_attn::paged_kv_compact: pages in use moved to the front of the pool;
+// returns where each went and how many there are.
+std::tuple<at::Tensor, at::Tensor> paged_kv_compact_cuda(at::TensorList kcaches, at::TensorList vcaches,
+                                                         at::Tensor& block_table, at::Tensor& refs,
+                                                         const TensorLists& k_scales, const TensorLists& v_scales) {
+  const char* op = "paged_kv_compact";
+  TORCH_CHECK(!kcaches.empty() && kcaches[0].dim() == 5, op, ": kcaches must hold [num_blocks, Hkv, 1, block_size, D]");
+  rbln_pages_params_t p = check_pages(op, block_table, refs, kcaches[0].size(3), true);
+  LayerPointers ptrs;
+  check_layers(op, kcaches, vcaches, k_scales, v_scales, block_table, p, ptrs);
+  c10::cuda::CUDAGuard guard(block_table.device());
+  at::Tensor moved = at::empty_like(refs);
+  at::Tensor live = at::empty({1}, refs.options());
+  const at::Tensor workspace = pages_workspace(op, p, -1, block_table);
+  check_rc(rbln_paged_kv_compact(&p, moved.data_ptr<int32_t>(), live.data_ptr<int32_t>(), stream_of(block_table)), op);
+  return {moved, live};
+}
+
+// ---------------------------------------------------------------------------
 // flash_attention_naive_{prefill,decode}: the unified-cache form of the paged
 // ops (torch_rbln/_internal/register_custom_ops.py:453-560; CPU semantics in
 // test/rbln/test_custom_kernel.py:546-573). kv_cache [2, num_blocks, Hkv, 1,
@@ -1054,6 +1251,17 @@ TORCH_LIBRARY(rbln_attn, m) {
   m.def(
       "paged_kv_read(Tensor kcache, Tensor vcache, Tensor lengths, Tensor block_table, SymInt block_size, "
       "SymInt max_len, Tensor? k_scale=None, Tensor? v_scale=None, ScalarType? dtype=None) -> (Tensor, Tensor)");
+  m.def(
+      "paged_kv_fork(Tensor block_table, Tensor lengths, Tensor parents, Tensor(a!) refs, SymInt block_size) -> "
+      "(Tensor, Tensor)");
+  m.def("paged_kv_free(Tensor(a!) block_table, Tensor keep, Tensor(b!) refs, SymInt block_size) -> ()");
+  m.def(
+      "paged_kv_reserve(Tensor(a!)[] kcaches, Tensor(b!)[] vcaches, Tensor(c!) block_table, Tensor seq, "
+      "Tensor(d!) refs, SymInt block_size, SymInt new_tokens, Tensor(e!)[]? k_scales=None, "
+      "Tensor(f!)[]? v_scales=None) -> Tensor");
+  m.def(
+      "paged_kv_compact(Tensor(a!)[] kcaches, Tensor(b!)[] vcaches, Tensor(c!) block_table, Tensor(d!) refs, "
+      "Tensor(e!)[]? k_scales=None, Tensor(f!)[]? v_scales=None) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(rbln_attn, CUDA, m) {
@@ -1061,6 +1269,10 @@ TORCH_LIBRARY_IMPL(rbln_attn, CUDA, m) {
   m.impl("rotary", &rotary_cuda);
   m.impl("rotary_paged_kv_write", &rotary_paged_kv_write_cuda);
   m.impl("paged_kv_read", &paged_kv_read_cuda);
+  m.impl("paged_kv_fork", &paged_kv_fork_cuda);
+  m.impl("paged_kv_free", &paged_kv_free_cuda);
+  m.impl("paged_kv_reserve", &paged_kv_reserve_cuda);
+  m.impl("paged_kv_compact", &paged_kv_compact_cuda);
 }
 
 TORCH_LIBRARY_IMPL(rbln_attn, AutogradCUDA, m) { m.impl("rotary", &rotary_autograd); }

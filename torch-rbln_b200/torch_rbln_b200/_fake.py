@@ -55,3 +55,22 @@ def _paged_kv_read(kcache, vcache, lengths, block_table, block_size, max_len, k_
         dtype = torch.bfloat16 if kcache.dtype == torch.float8_e4m3fn else kcache.dtype
     shape = [lengths.numel(), kcache.shape[1], 1, max_len, kcache.shape[-1]]
     return kcache.new_empty(shape, dtype=dtype), kcache.new_empty(shape, dtype=dtype)
+
+
+@torch.library.register_fake("rbln_attn::paged_kv_fork")
+def _paged_kv_fork(block_table, lengths, parents, refs, block_size):
+    n = parents.shape[0]
+    return block_table.new_empty([n, block_table.shape[1]]), lengths.new_empty([n], device=block_table.device)
+
+
+torch.library.register_fake("rbln_attn::paged_kv_free", _writes_only)
+
+
+@torch.library.register_fake("rbln_attn::paged_kv_reserve")
+def _paged_kv_reserve(kcaches, vcaches, block_table, *args, **kwargs):
+    return block_table.new_empty([block_table.shape[0]], dtype=torch.int32)
+
+
+@torch.library.register_fake("rbln_attn::paged_kv_compact")
+def _paged_kv_compact(kcaches, vcaches, block_table, refs, *args, **kwargs):
+    return torch.empty_like(refs), refs.new_empty([1])

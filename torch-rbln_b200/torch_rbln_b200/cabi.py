@@ -115,6 +115,19 @@ class RotaryParams(ctypes.Structure):
     ]
 
 
+class PagesParams(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("max_blocks", c_i32), ("num_blocks", c_i32), ("block_size", c_i32),
+        ("block_table", c_vp), ("block_table_dtype", c_i32), ("block_table_stride", c_i64 * 2),
+        ("refs", c_vp),
+        ("lengths", c_vp), ("lengths_dtype", c_i32), ("lengths_stride", c_i64),
+        ("num_layers", c_i32), ("num_kv_heads", c_i32), ("head_dim", c_i32), ("kv_dtype", c_i32),
+        ("kcaches", ctypes.POINTER(c_vp)), ("vcaches", ctypes.POINTER(c_vp)), ("cache_stride", c_i64 * 3),
+        ("k_scales", ctypes.POINTER(c_vp)), ("v_scales", ctypes.POINTER(c_vp)), ("scale_stride", c_i64 * 2),
+        ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class PeerOut(ctypes.Structure):
     """rbln_peer_out_t: every rank's output buffer and flag array, as mapped on this GPU."""
     _fields_ = [("out", c_vp), ("flags", c_vp), ("n", c_i32), ("rank", c_i32), ("head0", c_i32),
@@ -141,6 +154,14 @@ ENTRY_POINTS = {
     "rbln_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryParams), c_vp]),
     "rbln_rotary_paged_kv_write": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), ctypes.POINTER(RotaryParams), c_vp]),
     "rbln_paged_kv_read": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), c_vp, c_vp, ctypes.POINTER(c_i64), c_vp]),
+    "rbln_pages_params_sizeof": (ctypes.c_size_t, []),
+    "rbln_paged_kv_fork": (ctypes.c_int, [ctypes.POINTER(PagesParams), c_vp, c_i32, c_i64, c_i32, c_vp, c_i64, c_vp,
+                                          c_vp]),
+    "rbln_paged_kv_free": (ctypes.c_int, [ctypes.POINTER(PagesParams), c_vp]),
+    "rbln_paged_kv_pages_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagesParams), c_i32,
+                                                          ctypes.POINTER(ctypes.c_size_t)]),
+    "rbln_paged_kv_reserve": (ctypes.c_int, [ctypes.POINTER(PagesParams), c_i32, c_vp, c_vp]),
+    "rbln_paged_kv_compact": (ctypes.c_int, [ctypes.POINTER(PagesParams), c_vp, c_vp, c_vp]),
     "rbln_sdpa_fwd": (ctypes.c_int, [ctypes.POINTER(SdpaParams), c_vp]),
     "rbln_sdpa_bwd_workspace_size": (ctypes.c_int, [ctypes.POINTER(SdpaBwdParams), ctypes.POINTER(ctypes.c_size_t)]),
     "rbln_sdpa_bwd": (ctypes.c_int, [ctypes.POINTER(SdpaBwdParams), c_vp]),
@@ -173,6 +194,8 @@ def lib() -> ctypes.CDLL:
             raise RuntimeError("rbln_peer_out_t layout mismatch between ctypes and the library")
         if L.rbln_rotary_params_sizeof() != ctypes.sizeof(RotaryParams):
             raise RuntimeError("rbln_rotary_params_t layout mismatch between ctypes and the library")
+        if L.rbln_pages_params_sizeof() != ctypes.sizeof(PagesParams):
+            raise RuntimeError("rbln_pages_params_t layout mismatch between ctypes and the library")
         _lib = L
     return _lib
 
@@ -303,6 +326,33 @@ def rotary_params(q, k, q_out, k_out, positions, inv_freq, interleaved=False, ms
     p.inv_freq = inv_freq.data_ptr()
     p.interleaved, p.inverse, p.mscale = int(interleaved), int(inverse), mscale
     return p
+
+
+def pages_params(block_table, refs, block_size, lengths=None, kcaches=(), vcaches=(), k_scales=None, v_scales=None):
+    """Fills PagesParams; returns (params, keepalive): the layers' pointer arrays must outlive the call."""
+    p = PagesParams()
+    p.batch, p.max_blocks = block_table.shape
+    p.num_blocks, p.block_size = refs.numel(), block_size
+    p.block_table, p.block_table_dtype = block_table.data_ptr(), _DT[block_table.dtype]
+    p.block_table_stride[0], p.block_table_stride[1] = block_table.stride()
+    p.refs = refs.data_ptr()
+    p.lengths_dtype = DT_I32
+    if lengths is not None:
+        p.lengths, p.lengths_dtype, p.lengths_stride = lengths.data_ptr(), _DT[lengths.dtype], lengths.stride(0)
+    keep = {}
+    if kcaches:
+        c = kcaches[0]
+        p.num_layers, p.num_kv_heads, p.head_dim, p.kv_dtype = len(kcaches), c.shape[1], c.shape[-1], _DT[c.dtype]
+        for i, d in enumerate((0, 1, 3)):
+            p.cache_stride[i] = c.stride(d)
+        for name, tensors in (("kcaches", kcaches), ("vcaches", vcaches), ("k_scales", k_scales),
+                              ("v_scales", v_scales)):
+            if tensors is not None:
+                keep[name] = (c_vp * len(tensors))(*[t.data_ptr() for t in tensors])
+                setattr(p, name, ctypes.cast(keep[name], ctypes.POINTER(c_vp)))
+        if k_scales is not None:
+            p.scale_stride[0], p.scale_stride[1] = k_scales[0].stride()
+    return p, keep
 
 
 def call(name: str, p: PagedAttnParams, stream: Optional[torch.cuda.Stream] = None) -> int:
