@@ -201,6 +201,32 @@ int rbln_paged_causal_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream
  * mask[b, s, t] > 0 (p->mask required, mask_stride = {batch, query row}). */
 int rbln_paged_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stream);
 
+/* rbln_paged_causal_attn_decode for a batch in which groups of sequences share
+ * their first positions: group g is the sequences [group_starts[g],
+ * group_starts[g + 1]), which share positions [0, shared_lens[g]). Those are
+ * read once for the group, through the block table of its first sequence; the
+ * rest of each sequence, its new token included, through its own. A sequence
+ * whose new position is below its group's shared length, and one outside all
+ * groups, is read through its own table alone. Values of group_starts are cut
+ * to [0, batch] and to no less than the ones before them, shared lengths to
+ * [0, span]. Of p: as for rbln_paged_causal_attn_decode, with kv_dtype equal to
+ * q_dtype, no mask, sinks, num_splits or prof_events; block_size in {8, 16, 32,
+ * 64, 128} or a multiple of 128; group <= 16; batch <= 4096, num_groups <= 1024.
+ * A position in a block outside the pool is not seen. The workspace
+ * (rbln_paged_decode_shared_workspace_size) is required.
+ * No reference counterpart. */
+typedef struct {
+  int32_t num_groups;
+  const int32_t* group_starts; /* [num_groups + 1] */
+  const int32_t* shared_lens;  /* [num_groups] */
+} rbln_shared_prefix_t;
+
+size_t rbln_shared_prefix_sizeof(void);
+int rbln_paged_decode_shared_workspace_size(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s,
+                                            size_t* bytes);
+int rbln_paged_causal_attn_decode_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s,
+                                         cudaStream_t stream);
+
 /* Paged KV-cache write on its own: k_new/v_new [B, Hkv, S = q_len, D]
  * (strides b, h, s in k_new_stride / v_new_stride) written at positions
  * [seq[b], seq[b] + S) through the block table -- the append step of the

@@ -6,7 +6,7 @@ import copy
 import pytest
 import torch
 
-import page_refs as ref
+from tests import page_refs as ref
 
 pytestmark = pytest.mark.gpu
 

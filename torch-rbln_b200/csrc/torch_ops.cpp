@@ -291,6 +291,44 @@ at::Tensor paged_causal_attn_decode_kvfp8_cuda(const at::Tensor& q, const at::Te
   return run_decode(c, kcache, op, false);
 }
 
+// rbln_custom_ops::paged_causal_attn_decode_shared: paged_causal_attn_decode
+// for a batch in which group g, the sequences [group_starts[g],
+// group_starts[g + 1]), shares its first shared_lens[g] positions. No
+// counterpart in the reference's op set.
+at::Tensor paged_causal_attn_decode_shared_cuda(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                at::Tensor& kcache, at::Tensor& vcache, const at::Tensor& seq,
+                                                const at::Tensor& scale, const at::Tensor& block_table,
+                                                int64_t block_size, const at::Tensor& group_starts,
+                                                const at::Tensor& shared_lens) {
+  const char* op = "paged_causal_attn_decode_shared";
+  TORCH_CHECK(kcache.scalar_type() == q.scalar_type(), op, ": cache dtype must equal q dtype");
+  auto whole = [&](const at::Tensor& t, const char* name) {
+    TORCH_CHECK(t.dim() == 1 && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong), op, ": ", name,
+                " must be 1-D of int32/int64, got ", t.sizes(), " of ", t.scalar_type());
+    return on_device(t, q).to(at::kInt).contiguous();
+  };
+  TORCH_CHECK(q.is_cuda(), op, ": expected CUDA tensors, q is on ", q.device());
+  c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor starts = whole(group_starts, "group_starts"), lens = whole(shared_lens, "shared_lens");
+  TORCH_CHECK(starts.numel() == lens.numel() + 1, op, ": group_starts must hold one entry more than shared_lens, got ",
+              starts.numel(), " and ", lens.numel());
+  Common c;
+  fill_paged(c, op, q, k, v, kcache, vcache, seq, scale, block_table, block_size, std::nullopt, true);
+  rbln_shared_prefix_t s{};
+  s.num_groups = (int32_t)lens.numel();
+  s.group_starts = starts.data_ptr<int32_t>();
+  s.shared_lens = lens.data_ptr<int32_t>();
+  size_t ws = 0;
+  check_rc(rbln_paged_decode_shared_workspace_size(&c.p, &s, &ws), op);
+  const at::Tensor workspace = at::empty({(int64_t)ws}, c.q.options().dtype(at::kByte));
+  c.p.workspace = workspace.data_ptr();
+  c.p.workspace_bytes = ws;
+  check_rc(rbln_paged_causal_attn_decode_shared(&c.p, &s, at::cuda::getCurrentCUDAStream(c.q.device().index()).stream()),
+           op);
+  check_device_flags(c, op);
+  return c.out;
+}
+
 at::Tensor run_prefill(Common& c, const char* op, bool keep_mask) {
   c10::cuda::CUDAGuard guard(c.q.device());
   size_t ws = 0;
@@ -1307,6 +1345,10 @@ TORCH_LIBRARY(rbln_custom_ops, m) {
       "paged_causal_attn_decode(Tensor q, Tensor k, Tensor v, Tensor(a3!) kcache, Tensor(a4!) vcache, "
       "Tensor seq, Tensor scale, Tensor block_table, SymInt block_size, Tensor? mask=None) -> Tensor");
   m.def(
+      "paged_causal_attn_decode_shared(Tensor q, Tensor k, Tensor v, Tensor(a3!) kcache, Tensor(a4!) vcache, "
+      "Tensor seq, Tensor scale, Tensor block_table, SymInt block_size, Tensor group_starts, Tensor shared_lens) -> "
+      "Tensor");
+  m.def(
       "paged_causal_attn_decode_kvfp8(Tensor q, Tensor k, Tensor v, Tensor(a3!) kcache, Tensor(a4!) vcache, "
       "Tensor k_scale, Tensor v_scale, Tensor seq, Tensor scale, Tensor block_table, SymInt block_size, "
       "Tensor? mask=None) -> Tensor");
@@ -1324,6 +1366,7 @@ TORCH_LIBRARY_IMPL(rbln_custom_ops, CUDA, m) {
   m.impl("paged_causal_attn_prefill_kvfp8", &paged_causal_attn_prefill_kvfp8_cuda);
   m.impl("paged_attn_decode", &paged_attn_decode_cuda);
   m.impl("paged_causal_attn_decode", &paged_causal_attn_decode_cuda);
+  m.impl("paged_causal_attn_decode_shared", &paged_causal_attn_decode_shared_cuda);
   m.impl("paged_causal_attn_decode_kvfp8", &paged_causal_attn_decode_kvfp8_cuda);
   m.impl("flash_attention_naive_prefill", &flash_attention_naive_prefill_cuda);
   m.impl("flash_attention_naive_decode", &flash_attention_naive_decode_cuda);

@@ -42,6 +42,7 @@ from .ops import (  # noqa: E402,F401
     paged_attn_prefill,
     paged_causal_attn_decode,
     paged_causal_attn_decode_kvfp8,
+    paged_causal_attn_decode_shared,
     paged_causal_attn_prefill,
     paged_causal_attn_prefill_kvfp8,
 )
@@ -54,6 +55,7 @@ __all__ = [
     "paged_attn_prefill",
     "paged_causal_attn_decode",
     "paged_causal_attn_decode_kvfp8",
+    "paged_causal_attn_decode_shared",
     "paged_causal_attn_prefill",
     "paged_causal_attn_prefill_kvfp8",
     "rotary_frequencies",

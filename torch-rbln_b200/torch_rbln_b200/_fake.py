@@ -13,6 +13,7 @@ _NAMES = (
     "paged_causal_attn_prefill_kvfp8",
     "paged_causal_attn_decode",
     "paged_causal_attn_decode_kvfp8",
+    "paged_causal_attn_decode_shared",
     "flash_attention_naive_prefill",
     "flash_attention_naive_decode",
 )

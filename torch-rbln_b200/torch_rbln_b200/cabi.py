@@ -128,6 +128,11 @@ class PagesParams(ctypes.Structure):
     ]
 
 
+class SharedPrefix(ctypes.Structure):
+    """rbln_shared_prefix_t: group_starts int32 [num_groups + 1] and shared_lens int32 [num_groups], on the device."""
+    _fields_ = [("num_groups", c_i32), ("group_starts", c_vp), ("shared_lens", c_vp)]
+
+
 class PeerOut(ctypes.Structure):
     """rbln_peer_out_t: every rank's output buffer and flag array, as mapped on this GPU."""
     _fields_ = [("out", c_vp), ("flags", c_vp), ("n", c_i32), ("rank", c_i32), ("head0", c_i32),
@@ -154,6 +159,12 @@ ENTRY_POINTS = {
     "rbln_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryParams), c_vp]),
     "rbln_rotary_paged_kv_write": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), ctypes.POINTER(RotaryParams), c_vp]),
     "rbln_paged_kv_read": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams), c_vp, c_vp, ctypes.POINTER(c_i64), c_vp]),
+    "rbln_shared_prefix_sizeof": (ctypes.c_size_t, []),
+    "rbln_paged_decode_shared_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams),
+                                                               ctypes.POINTER(SharedPrefix),
+                                                               ctypes.POINTER(ctypes.c_size_t)]),
+    "rbln_paged_causal_attn_decode_shared": (ctypes.c_int, [ctypes.POINTER(PagedAttnParams),
+                                                            ctypes.POINTER(SharedPrefix), c_vp]),
     "rbln_pages_params_sizeof": (ctypes.c_size_t, []),
     "rbln_paged_kv_fork": (ctypes.c_int, [ctypes.POINTER(PagesParams), c_vp, c_i32, c_i64, c_i32, c_vp, c_i64, c_vp,
                                           c_vp]),
@@ -194,6 +205,8 @@ def lib() -> ctypes.CDLL:
             raise RuntimeError("rbln_peer_out_t layout mismatch between ctypes and the library")
         if L.rbln_rotary_params_sizeof() != ctypes.sizeof(RotaryParams):
             raise RuntimeError("rbln_rotary_params_t layout mismatch between ctypes and the library")
+        if L.rbln_shared_prefix_sizeof() != ctypes.sizeof(SharedPrefix):
+            raise RuntimeError("rbln_shared_prefix_t layout mismatch between ctypes and the library")
         if L.rbln_pages_params_sizeof() != ctypes.sizeof(PagesParams):
             raise RuntimeError("rbln_pages_params_t layout mismatch between ctypes and the library")
         _lib = L

@@ -51,6 +51,15 @@ def paged_causal_attn_decode_kvfp8(*args):
     return _ops.paged_causal_attn_decode_kvfp8(*args)
 
 
+def paged_causal_attn_decode_shared(*args):
+    """paged_causal_attn_decode for a batch whose sequences share their first positions in groups:
+    paged_causal_attn_decode's first nine arguments, then group_starts [n + 1] and shared_lens [n]. Sequences
+    [group_starts[g], group_starts[g + 1]) share positions [0, shared_lens[g]), which are read once for all of them
+    through the block table of the first."""
+    _count("paged_causal_attn_decode_shared", args, 11, 11)
+    return _ops.paged_causal_attn_decode_shared(*args)
+
+
 def flash_attention_naive_prefill(*args):
     _count("flash_attention_naive_prefill", args, 9, 10)
     return _ops.flash_attention_naive_prefill(*args)
