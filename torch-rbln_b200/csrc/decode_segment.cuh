@@ -191,12 +191,9 @@ __host__ __device__ constexpr int segment_smem() {
 // LA (block-table lookahead): false = look up each tile's block where it is
 // fetched; true = load the next tile's entry into registers one tile early,
 // so that the lookup is off the tile's critical path.
-// SHARED: positions below `shared` are looked up in row `lead` of the block
-// table instead of row b.
-template <int D, int KV, bool Q_BF16, int NT, bool LA, bool SHARED = false>
+template <int D, int KV, bool Q_BF16, int NT, bool LA>
 __device__ __forceinline__ void decode_segment(const DecodeArgs& a, unsigned char* dsm, int b, int h, int t0,
-                                               int t1, bool append, bool whole, int64_t slot, int lead = 0,
-                                               int shared = 0) {
+                                               int t1, bool append, bool whole, int64_t slot) {
   using C = Cfg<D, KV>;
   constexpr bool MB = C::MMA_BF16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -218,8 +215,7 @@ __device__ __forceinline__ void decode_segment(const DecodeArgs& a, unsigned cha
     const int tpos = ts + (lane & 15);
     const bool in = tpos < t1;
     e.keep = in && (a.mask == nullptr || load_keep(a.mask, a.mask_dtype, b * a.mask_stride + tpos));
-    const int64_t bt_row = SHARED && tpos < shared ? lead : b;
-    const int64_t blk = in ? load_index(a.bt, a.bt_dtype, bt_row * a.bt_stride + tpos / a.bs) : -1;
+    const int64_t blk = in ? load_index(a.bt, a.bt_dtype, b * a.bt_stride + tpos / a.bs) : -1;
     e.blk = (blk >= 0 && blk < a.num_blocks) ? (int)blk : -1;
   };
   TileEntry ent;

@@ -3,79 +3,826 @@
 //   out[b] = softmax(scale q[b] K^T) V over positions [0, min(seq[b] + 1, span)),
 // positions below the group's shared length read through the table of its
 // first sequence, the others through the sequence's own.
+//
+// The softmax over a union of positions is joined from its parts: part i
+// gives O_i = sum_t e^{s_t - m_i} v_t / l_i and lse_i = m_i + log l_i, and
+// O = sum_i e^{lse_i} O_i / sum_i e^{lse_i}. Four launches, each a
+// programmatic dependent of the one before:
+//  * shared_plan_kernel (one CTA): every row's group, the units of work and
+//    where each CTA starts in them;
+//  * shared_prefix_kernel (tcgen05): the query heads of a KV head of up to
+//    2 x 128 rows of a group against the shared keys, so that the tensor
+//    cores work on rows that a batch without a shared prefix would bring one
+//    by one, and a key is read once for them;
+//  * shared_own_kernel: each sequence's own positions with the decode
+//    kernels' segments (mma.sync, one sequence and KV head at a time), and
+//    the append of the new token;
+//  * shared_merge_kernel: the parts of every row.
 
 #include <algorithm>
 
 #include "decode_segment.cuh"
+#include "sm100.cuh"
+#include "tma_map.cuh"
 
 namespace rbln {
 namespace {
 
+using namespace sm100;
+
 constexpr int kMaxBatch = 4096, kMaxGroups = 1024;
 constexpr int kPlanThreads = 1024;
+constexpr int kPerRow = kMaxBatch / kPlanThreads;
+constexpr int kKeys = 128;            // keys a tile
+constexpr int kRows = 128;            // query rows a tile
+constexpr int kPanel = 128 * 128;     // bytes: 128 rows of 64 elements
+constexpr int kPrefixThreads = 384;   // softmax warpgroups 0-3 and 4-7, producer 8, MMA 9
+constexpr int kUnitCost = 1;          // key tiles charged to a unit's start
+constexpr int kSegCost = 128;         // keys charged to the start of a sequence's own part
+constexpr int kMinOwn = 256;          // smallest share of a CTA of own positions
+// Registers a thread after the split (launch: 168 each): a softmax thread
+// holds its whole row of 128 scores.
+constexpr uint32_t kRegsSoftmax = 216, kRegsOther = 64;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kPrefixThreads * 168, "register split exceeds the launch");
+
+// What the plan leaves for the other kernels.
+struct Totals {
+  int cost;         // of all units of a KV head, in key tiles of 128 rows
+  int share;        // of a CTA of the prefix kernel
+  int rows;         // rows that a KV head's units store for each CTA that works on them
+  int own_share;    // own positions of a CTA
+};
 
 struct SharedArgs {
   int groups;
   const int32_t* starts;
   const int32_t* lens;
-  int* row_shared;  // [B] positions that are read through row_lead's table
-  int* row_lead;    // [B]
+  int seqs;            // sequences a row tile holds: 128 / G
+  int ctas;            // of the prefix kernel
+  Totals* totals;
+  int* row_shared;     // [B] positions that are read through the group's table
+  int* row_group;      // [B] that group, -1: none
+  int* own;            // [B + 1] prefix of the rows' own positions, as in the decode kernels
+  int* own_first;      // [nchunk] first sequence of a chunk
+  int4* group;         // [groups] first sequence, sequences, shared positions, stored rows before it
+  int* before;         // [groups + 1] cost of the groups before it, in one KV head
+  int* cta_group;      // [ctas] group that a CTA starts in, -1: none
+  float* part_o;       // parts of the shared positions, see Unit
+  float* part_lse;
 };
 
-// One CTA: every row's group and the positions that it shares.
+// ------------------------------------------------------------------- plan
+// Exclusive scan over the CTA's threads (sum or maximum); *all: of all.
+template <bool MAX, typename T>
+__device__ __forceinline__ T scan_before(T v, T zero, T* all) {
+  __shared__ T warps[kPlanThreads / 32];
+  auto join = [](T a, T b) { return MAX ? (a > b ? a : b) : a + b; };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  T x = v;
+  for (int o = 1; o < 32; o <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x = join(x, y);
+  }
+  __syncthreads();  // the last call's sums have been read
+  if (lane == 31) warps[warp] = x;
+  __syncthreads();
+  T w = warps[lane];
+  for (int o = 1; o < 32; o <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w = join(w, y);
+  }
+  *all = __shfl_sync(0xffffffffu, w, 31);
+  const T wb = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+  const T up = __shfl_up_sync(0xffffffffu, x, 1);
+  return join(warp > 0 ? wb : zero, lane > 0 ? up : zero);
+}
+
+__host__ __device__ __forceinline__ int tiles_of(int positions) { return (positions + kKeys - 1) / kKeys; }
+
+// A group's units: `full` of 2 x seqs sequences, whose key tiles cost 2 (two
+// row tiles), and one of the rest: 1 where those fit in one row tile.
+struct GroupUnits {
+  int full, rest, tiles, full_cost, rest_cost;
+  __device__ __forceinline__ GroupUnits(int n, int len, int seqs) {
+    full = n / (2 * seqs);
+    rest = n - full * 2 * seqs;
+    tiles = tiles_of(len);
+    full_cost = 2 * tiles + kUnitCost;
+    rest_cost = rest == 0 ? 0 : (rest > seqs ? 2 * tiles : tiles) + kUnitCost;
+  }
+};
+
 __global__ void __launch_bounds__(kPlanThreads, 1) shared_plan_kernel(const DecodeArgs a, const SharedArgs s) {
   __shared__ int start[kMaxGroups + 1];
-  for (int g = threadIdx.x; g <= s.groups; g += kPlanThreads) start[g] = min(max(s.starts[g], 0), a.B);
+  __shared__ int before[kMaxGroups + 1];
+  __shared__ int active[kMaxGroups];
+  pdl_enter();
+  const int tid = threadIdx.x;
+  // the groups' starts, none before the one before it
+  {
+    int v[2], m = 0, all;
+    for (int k = 0; k < 2; ++k) {
+      const int g = 2 * tid + k;
+      if (g <= s.groups) m = max(m, min(max(s.starts[g], 0), a.B));
+      v[k] = m;
+    }
+    const int up = scan_before<true>(m, 0, &all);
+    for (int k = 0; k < 2; ++k)
+      if (2 * tid + k <= s.groups) start[2 * tid + k] = max(v[k], up);
+    if (tid < kMaxGroups) active[tid] = 0;
+  }
   __syncthreads();
-  if (threadIdx.x == 0)
-    for (int g = 1; g <= s.groups; ++g) start[g] = max(start[g], start[g - 1]);
-  __syncthreads();
-  for (int b = threadIdx.x; b < a.B; b += kPlanThreads) {
-    int lo = -1, hi = s.groups;  // the last group that starts at or before b
+  // rows: group, shared positions, own positions
+  int own[kPerRow], sum = 0, all;
+  for (int k = 0; k < kPerRow; ++k) {
+    const int b = kPerRow * tid + k;
+    own[k] = 0;
+    if (b >= a.B) continue;
+    int lo = -1, hi = s.groups;  // the last start at or before b
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (start[mid] <= b) lo = mid; else hi = mid - 1;
     }
-    int n = 0;
+    int pos, n = 0;
+    const int L = seq_len(a, b, pos);
     if (lo >= 0 && lo < s.groups) {
       n = min(max(s.lens[lo], 0), a.span);
-      if (a.seq[b * a.seq_stride] < n) n = 0;
+      if (pos < n) n = 0;
     }
+    if (n > 0) active[lo] = 1;
     s.row_shared[b] = n;
-    s.row_lead[b] = n > 0 ? start[lo] : b;
+    s.row_group[b] = n > 0 ? lo : -1;
+    own[k] = ((L - n + 15) & ~15) + kSegCost;
+    sum += own[k];
+  }
+  int run = scan_before<false>(sum, 0, &all);
+  const int W = max(kMinOwn, ((all + a.nchunk - 1) / a.nchunk + 15) & ~15);
+  for (int k = 0; k < kPerRow; ++k) {
+    const int b = kPerRow * tid + k;
+    if (b >= a.B) continue;
+    s.own[b] = run;
+    for (int c = (run + W - 1) / W; c * W < run + own[k]; ++c) s.own_first[c] = b;
+    run += own[k];
+  }
+  if (tid == 0) s.own[a.B] = all;
+  // groups: cost and stored rows
+  __syncthreads();
+  int cost = 0, rows = 0, total, all_rows, len = 0, n = 0;
+  if (tid < s.groups) {
+    n = start[tid + 1] - start[tid];
+    len = active[tid] ? min(max(s.lens[tid], 0), a.span) : 0;
+    if (len == 0) n = 0;
+    const GroupUnits u(n, len, s.seqs);
+    cost = u.full * u.full_cost + u.rest_cost;
+    rows = (2 * s.seqs * u.full + (u.rest > s.seqs ? u.rest : 2 * u.rest)) * a.G;
+  }
+  const int cb = scan_before<false>(cost, 0, &total);
+  const int rb = scan_before<false>(rows, 0, &all_rows);
+  if (tid < s.groups) {
+    s.group[tid] = make_int4(start[tid], n, len, rb);
+    s.before[tid] = before[tid] = cb;
+  }
+  // the line is below 2^30 long. A share of 2 at least: so every CTA between a unit's first and last has a tile of it
+  const int share = max(2, (total * a.Hkv + s.ctas - 1) / s.ctas);
+  if (tid == 0) {
+    s.before[s.groups] = total;
+    *s.totals = Totals{total, share, all_rows, W};
+  }
+  __syncthreads();
+  if (tid < s.ctas) {
+    const int at = tid * share;
+    int g = -1;
+    if (at < total * a.Hkv) {
+      const int x = at % total;
+      int lo = 0, hi = s.groups - 1;  // the last group that starts at or before x: it has a cost
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (before[mid] <= x) lo = mid; else hi = mid - 1;
+      }
+      g = lo;
+    }
+    s.cta_group[tid] = g;
   }
 }
 
-// CTA (h, b): the whole context of one (sequence, KV head).
+// ----------------------------------------------------------------- prefix
+// The units of all KV heads, head by head, group by group, stand end to end
+// on a line, each unit's start charged kUnitCost, each key tile its cost; CTA
+// c takes [c share, (c + 1) share), a tile by where it starts. A unit's rows
+// as CTA c sees them are stored from row c 256 + R on, with R the rows that
+// the units before it store: no two of them overlap, since a unit stores 256
+// rows at most, and neither does one unit's with another's in one CTA.
+struct Unit {
+  int h, b0, n;     // KV head, sequences [b0, b0 + n)
+  int lead, len;    // row of the block table, shared positions
+  bool wide;        // two row tiles, each against all keys; else one, its key tiles in turn by two warpgroups
+  int t0, t1;       // this CTA's key tiles
+  int64_t row0;     // first stored row
+};
+
+struct Walk {
+  const SharedArgs& s;
+  const int Hkv, G;
+  const int cost, rows;
+  int lo, hi, g;
+  __device__ __forceinline__ Walk(const SharedArgs& s_, int Hkv_, int G_)
+      : s(s_), Hkv(Hkv_), G(G_), cost(s_.totals->cost), rows(s_.totals->rows) {
+    const int share = s.totals->share;
+    lo = blockIdx.x * share;
+    hi = min(lo + share, cost * Hkv);
+    g = s.cta_group[blockIdx.x];
+  }
+  __device__ __forceinline__ bool next(Unit& u) {
+    while (lo < hi) {
+      const int h = lo / cost, x = lo - h * cost;
+      if (x < s.before[g] || x >= s.before[g + 1]) {
+        int l = 0, r = s.groups - 1;
+        while (l < r) {
+          const int mid = (l + r + 1) >> 1;
+          if (s.before[mid] <= x) l = mid; else r = mid - 1;
+        }
+        g = l;
+      }
+      const int4 gr = s.group[g];
+      const GroupUnits gu(gr.y, gr.z, s.seqs);
+      const int y = x - s.before[g], k = min(y / gu.full_cost, gu.full);
+      const bool whole = k < gu.full;
+      const int base = lo - y + k * gu.full_cost, end = base + (whole ? gu.full_cost : gu.rest_cost);
+      u.wide = whole || gu.rest > s.seqs;
+      const int w = u.wide ? 2 : 1;
+      const int first = base + kUnitCost, stop = min(hi, end);
+      u.t0 = (max(lo, first) - first + w - 1) / w;
+      u.t1 = (max(stop, first) - first + w - 1) / w;
+      lo = stop;
+      if (u.t0 >= u.t1) continue;
+      u.h = h;
+      u.b0 = gr.x + k * 2 * s.seqs;
+      u.n = whole ? 2 * s.seqs : gu.rest;
+      u.lead = gr.x;
+      u.len = gr.z;
+      u.row0 = (int64_t)blockIdx.x * 2 * kRows + (int64_t)h * rows + gr.w + k * 2 * s.seqs * G;
+      return true;
+    }
+    return false;
+  }
+};
+
+template <int D>
+struct PrefixSmem {
+  static constexpr int NP = D / 64;
+  static constexpr int STAGES = D == 128 ? 2 : 3;  // of K and of V
+  static constexpr int TILE = NP * kPanel;
+  static constexpr int Q = 0;  // two row tiles
+  static constexpr int K = Q + 2 * TILE;
+  static constexpr int V = K + STAGES * TILE;
+  static constexpr int BAR = V + STAGES * TILE;
+  static constexpr int TMEM = BAR + 32 * 8;
+  static constexpr int ABORT = TMEM + 8;
+  static constexpr int TOTAL = ABORT + 8 + 1024;
+  // above half an SM's shared memory: one CTA an SM, which takes all of its TMEM
+  static constexpr int ALLOC = TOTAL > 120 * 1024 ? TOTAL : 120 * 1024;
+};
+
+enum PrefixBar {
+  B_QF, B_QE,                    // a unit's queries are there; their last product is done
+  B_KF, B_KE = B_KF + 3,         // a stage of K is filled, free
+  B_VF = B_KE + 3, B_VE = B_VF + 3,
+  B_SF = B_VE + 3,               // scores of x computed, and every product before them
+  B_PF = B_SF + 2,               // probabilities of x written (4 warps)
+  B_OF = B_PF + 2,               // a unit's last product of x is done
+  B_OE = B_OF + 2,               // its result is read (4 warps)
+  B_DONE = B_OE + 2, B_COUNT
+};
+
+// Roles as in the chunked prefill's 128-key kernel: two softmax warpgroups x
+// = 0, 1, each with a score buffer (128 columns of TMEM, the probabilities
+// written over its first half) and an accumulator (D columns). In a wide
+// unit they hold a row tile each and both work on every key tile; in the
+// others they share the one row tile and take the key tiles in turn, so that
+// up to 128 rows keep both of them and the copies busy too.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kPrefixThreads, 1)
+    shared_prefix_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const DecodeArgs a, const SharedArgs s) {
+  using L = PrefixSmem<D>;
+  constexpr int NP = L::NP, ST = L::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* sgen = smem_raw + (sbase - smem_u32(smem_raw));
+  volatile int* abort = reinterpret_cast<volatile int*>(sgen + L::ABORT);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + L::TMEM);
+  auto bar = [&](int i) { return sbase + L::BAR + 8u * i; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    *abort = 0;
+    for (int i = 0; i < B_COUNT; ++i)
+      mbar_init(bar(i), (i >= B_PF && i < B_PF + 2) || (i >= B_OE && i < B_OE + 2) ? 4u : 1u);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_enter();  // the set-up above overlaps the plan
+  const uint32_t tmem = *tmem_slot;
+  auto t_s = [&](int x) { return tmem + x * 128; };
+  auto t_o = [&](int x) { return tmem + 256 + x * 128; };
+  const int rpb = min(a.bs, kKeys), boxes = kKeys / rpb;  // <= 16 boxes a tile
+  // lane's box of key tile t: its block (num_blocks: none), first row there
+  auto block_of = [&](const Unit& u, int t, int& row) {
+    int blk = a.num_blocks;
+    row = 0;
+    const int key = t * kKeys + lane * rpb;
+    if (lane < boxes && key < u.len) {
+      const int bi = key / a.bs;
+      row = key - bi * a.bs;
+      const int64_t v = load_index(a.bt, a.bt_dtype, u.lead * a.bt_stride + bi);
+      if (v >= 0 && v < a.num_blocks) blk = (int)v;
+    }
+    return blk;
+  };
+
+  if (warp >= 8) {
+   setmaxnreg_dec<kRegsOther>();
+   if (warp == 8) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+    }
+    int T = 0, act = 0, k_issued = 0, v_issued = 0;
+    bool ok = true;
+    Unit u;
+    for (Walk w(s, a.Hkv, a.G); ok && w.next(u);) {
+      if (act >= 1 && !__all_sync(0xffffffffu, mbar_wait(bar(B_QE), (act - 1) & 1, abort))) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar(B_QF), (u.wide ? 2 : 1) * NP * s.seqs * a.G * 128);
+        for (int x = 0; x < (u.wide ? 2 : 1); ++x)
+          for (int p = 0; p < NP; ++p)
+            tma_load_4d(sbase + L::Q + x * L::TILE + p * kPanel, &tm_q, bar(B_QF), p * 64, 0, u.h, u.b0 + x * s.seqs);
+      }
+      for (int t = u.t0; t < u.t1; ++t, ++T) {
+        int row;
+        const int blk = block_of(u, t, row);
+        if (blk == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < u.len)
+          flag_error(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
+        const int st = T % ST;
+        if (T >= ST && !__all_sync(0xffffffffu, mbar_wait(bar(B_KE + st), (T / ST - 1) & 1, abort))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(bar(B_KF + st), NP * kPanel);
+        __syncwarp();
+        if (lane < boxes)
+          for (int p = 0; p < NP; ++p)
+            tma_load_4d(sbase + L::K + st * L::TILE + p * kPanel + lane * rpb * 128, &tm_k, bar(B_KF + st), p * 64, row,
+                        u.h, blk);
+        k_issued = T + 1;
+        if (T >= ST && !__all_sync(0xffffffffu, mbar_wait(bar(B_VE + st), (T / ST - 1) & 1, abort))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(bar(B_VF + st), NP * kPanel);
+        __syncwarp();
+        if (lane < boxes)
+          for (int p = 0; p < NP; ++p)
+            tma_load_4d(sbase + L::V + st * L::TILE + p * kPanel + lane * rpb * 128, &tm_v, bar(B_VF + st), p * 64, row,
+                        u.h, blk);
+        v_issued = T + 1;
+      }
+      ++act;
+    }
+    if (*abort) {
+      // let the copies in flight land before the CTA exits
+      const long long t0 = clock64();
+      for (int j = max(0, k_issued - ST); j < k_issued; ++j)
+        while (!mbar_try_wait(bar(B_KF + j % ST), (j / ST) & 1) && clock64() - t0 < 4000000) {
+        }
+      for (int j = max(0, v_issued - ST); j < v_issued; ++j)
+        while (!mbar_try_wait(bar(B_VF + j % ST), (j / ST) & 1) && clock64() - t0 < 8000000) {
+        }
+    }
+   } else if (warp == 9 && lane == 0) {
+    // ----------------------------------------------------------------- MMA
+    // Step j of a unit, for x = 0, 1: the product with V of x's tile of step
+    // j - 1, then the scores of its tile of step j. x's tile of step j is
+    // t0 + j in a wide unit, t0 + 2 j + x in another.
+    const uint32_t id_qk = idesc_f16(BF16, kRows, kKeys, false), id_pv = idesc_f16(BF16, kRows, D, true);
+    int T = 0, act = 0, n_s[2] = {0, 0}, n_o[2] = {0, 0};
+    bool ok = true;
+    Unit u;
+    for (Walk w(s, a.Hkv, a.G); ok && w.next(u);) {
+      const int nt = u.t1 - u.t0, steps = u.wide ? nt : (nt + 1) / 2;
+      if (!mbar_wait(bar(B_QF), act & 1, abort)) break;
+      for (int j = 0; ok && j <= steps; ++j) {
+        for (int x = 0; x < 2; ++x) {
+          const int i1 = u.wide ? j : 2 * j + x, i0 = u.wide ? j - 1 : i1 - 2;
+          if (j >= 1 && i0 < nt) {
+            const int Ti = T + i0, st = Ti % ST;
+            if (!mbar_wait(bar(B_VF + st), (Ti / ST) & 1, abort) ||
+                !mbar_wait(bar(B_PF + x), (n_s[x] - 1) & 1, abort) ||
+                (j == 1 && n_o[x] >= 1 && !mbar_wait(bar(B_OE + x), (n_o[x] - 1) & 1, abort))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t vb = sbase + L::V + st * L::TILE;
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              umma_f16_ts(t_o(x), t_s(x) + kk * 8, sw128_desc(vb + kk * 16 * 128, kPanel, 1024), id_pv,
+                          (j > 1 || kk > 0) ? 1u : 0u);
+            if (i1 >= nt) {  // x's last tile of the unit
+              umma_commit(bar(B_OF + x));
+              ++n_o[x];
+            }
+            if (!u.wide || x == 1) umma_commit(bar(B_VE + st));
+          }
+          if (i1 < nt) {
+            const int Ti = T + i1, st = Ti % ST;
+            if (!mbar_wait(bar(B_KF + st), (Ti / ST) & 1, abort)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t qb = sbase + L::Q + (u.wide ? x * L::TILE : 0), kb = sbase + L::K + st * L::TILE;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_f16_ss(t_s(x), sw128_desc(qb + (kk >> 2) * kPanel + (kk & 3) * 32, 16, 1024),
+                          sw128_desc(kb + (kk >> 2) * kPanel + (kk & 3) * 32, 16, 1024), id_qk, kk > 0 ? 1u : 0u);
+            umma_commit(bar(B_SF + x));
+            ++n_s[x];
+            if (!u.wide || x == 1) umma_commit(bar(B_KE + st));
+            if (i1 == nt - 1 && (!u.wide || x == 1)) umma_commit(bar(B_QE));
+          }
+        }
+      }
+      T += nt;
+      ++act;
+    }
+    if (*abort) {
+      umma_commit(bar(B_DONE));
+      const long long t0 = clock64();
+      while (!mbar_try_wait(bar(B_DONE), 0) && clock64() - t0 < 4000000) {
+      }
+    }
+   }
+  } else {
+    setmaxnreg_inc<kRegsSoftmax>();
+    // ------------------------------------------------------------- softmax
+    const int x = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const int bl = r / a.G, g = r - bl * a.G;  // the row's sequence in its tile, and query head
+    const float scale = a.scale_dev ? *a.scale_dev : a.scale;
+    const float qk_mult = scale * kLog2e;
+    const float mult = qk_mult > 0.f ? qk_mult : 1.f;
+    int T = 0, n_s = 0, n_o = 0;
+    bool ok = true;
+    Unit u;
+    for (Walk w(s, a.Hkv, a.G); ok && w.next(u); T += u.t1 - u.t0) {
+      const int i = (u.wide ? x * s.seqs : 0) + bl;
+      const bool row_ok = bl < s.seqs && i < u.n;
+      const int lim = row_ok ? s.row_shared[u.b0 + i] : 0;
+      float m_run = neg_inf(), l_run = 0.f;
+      int done = 0;
+      for (int t = u.t0 + (u.wide ? 0 : x); t < u.t1; t += u.wide ? 1 : 2, ++done) {
+        // keys in blocks outside the pool
+        int row;
+        const bool none = block_of(u, t, row) == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < u.len;
+        const uint32_t bad = __ballot_sync(0xffffffffu, none);
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_SF + x), n_s & 1, abort))) {
+          ok = false;
+          break;
+        }
+        ++n_s;
+        tc_fence_after();
+        __syncwarp();
+        float xv[kKeys];
+        {
+          uint32_t r0[32], r1[32], r2[32], r3[32];
+          tmem_ld32(t_s(x) + lane_off + 0, r0);
+          tmem_ld32(t_s(x) + lane_off + 32, r1);
+          tmem_ld32(t_s(x) + lane_off + 64, r2);
+          tmem_ld32(t_s(x) + lane_off + 96, r3);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            xv[e] = __uint_as_float(r0[e]);
+            xv[32 + e] = __uint_as_float(r1[e]);
+            xv[64 + e] = __uint_as_float(r2[e]);
+            xv[96 + e] = __uint_as_float(r3[e]);
+          }
+        }
+        // The maximum is taken on raw scores (a positive factor keeps the
+        // order), the scale folded into the exponent's multiply-add.
+        if (!(qk_mult > 0.f)) {
+#pragma unroll
+          for (int e = 0; e < kKeys; e += 2) mul2(xv[e], xv[e + 1], qk_mult, qk_mult);
+        }
+        const int seen = lim - t * kKeys;  // of this tile's keys
+        if (seen < kKeys || bad) {
+          const int per = __ffs(rpb) - 4;  // a box has 8 << per keys
+#pragma unroll
+          for (int z = 0; z < kKeys / 8; ++z) {
+            const int n = (bad >> (z >> per)) & 1u ? 0 : seen - 8 * z;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e >= n) xv[8 * z + e] = neg_inf();
+          }
+        }
+        float mx0 = neg_inf(), mx1 = neg_inf(), mx2 = neg_inf(), mx3 = neg_inf();
+#pragma unroll
+        for (int e = 0; e < kKeys; e += 8) {
+          mx0 = max3(mx0, xv[e], xv[e + 1]);
+          mx1 = max3(mx1, xv[e + 2], xv[e + 3]);
+          mx2 = max3(mx2, xv[e + 4], xv[e + 5]);
+          mx3 = max3(mx3, xv[e + 6], xv[e + 7]);
+        }
+        const float m_new = fmaxf(m_run, max3(mx0, mx1, fmaxf(mx2, mx3)) * mult);
+        // O is rescaled only when the maximum grows by more than 2^8
+        const bool grow = m_new > m_run + 8.f;
+        float factor = 1.f;
+        if (grow) {
+          factor = exp2_approx(m_run - m_new);
+          l_run *= factor;
+          m_run = m_new;
+        }
+        // x's last product with V is done (its scores' barrier says so)
+        if (done > 0 && __any_sync(0xffffffffu, grow && factor != 1.f)) {
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o(x) + lane_off + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st32(t_o(x) + lane_off + c * 32, o);
+          }
+          tmem_wait_st();
+        }
+        const float nmu = (m_run == neg_inf()) ? 0.f : -m_run;
+#pragma unroll
+        for (int e = 0; e < kKeys; e += 2) fma2(xv[e], xv[e + 1], mult, mult, nmu, nmu);
+        // one pair of exponentials in eight runs on the FMA pipe
+#pragma unroll
+        for (int e = 0; e < kKeys; e += 2) {
+          if ((e / 2) % 8 == 7) {
+            exp2_poly2(xv[e], xv[e + 1]);
+          } else {
+            xv[e] = exp2_approx(xv[e]);
+            xv[e + 1] = exp2_approx(xv[e + 1]);
+          }
+        }
+        float sa0 = 0.f, sa1 = 0.f, sb0 = 0.f, sb1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < kKeys; e += 4) {
+          add2(sa0, sa1, xv[e], xv[e + 1]);
+          add2(sb0, sb1, xv[e + 2], xv[e + 3]);
+        }
+        l_run += (sa0 + sa1) + (sb0 + sb1);
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = pack2<BF16>(xv[32 * c + 2 * e], xv[32 * c + 2 * e + 1]);
+          tmem_st16(t_s(x) + lane_off + c * 16, pk);
+        }
+        tmem_wait_st();
+        // rows of V behind the shared positions may hold anything: zeros
+        // before the probabilities are released (in a wide unit by x = 0,
+        // whose product comes first)
+        if (t * kKeys + kKeys > u.len && (x == 0 || !u.wide)) {
+          const int Ti = T + t - u.t0, st = Ti % ST;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(B_VF + st), (Ti / ST) & 1, abort))) {
+            ok = false;
+            break;
+          }
+          if (t * kKeys + r >= u.len) {
+            uint8_t* vrow = sgen + L::V + st * L::TILE + r * 128;
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(vrow + p * kPanel + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_PF + x));
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      // x = 1 stores behind x = 0: other rows in a wide unit, the same ones of other keys else
+      const int64_t at = u.row0 + (x == 0 ? 0 : (int64_t)(u.wide ? s.seqs : u.n) * a.G) + bl * a.G + g;
+      if (done == 0) {
+        if (row_ok) s.part_lse[at] = neg_inf();
+        continue;
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(B_OF + x), n_o & 1, abort))) {
+        ok = false;
+        break;
+      }
+      ++n_o;
+      tc_fence_after();
+      const float inv = 1.f / l_run;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        tmem_ld32(t_o(x) + lane_off + c * 32, o);
+        tmem_wait_ld();
+        if (row_ok) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(s.part_o + at * D + c * 32 + e) =
+                make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                            __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+        }
+      }
+      if (row_ok) s.part_lse[at] = m_run == neg_inf() ? neg_inf() : m_run + __log2f(l_run);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_OE + x));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort && threadIdx.x == 0) flag_error(a.err, RBLN_DEVERR_TIMEOUT);
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// -------------------------------------------------------------------- own
+// As paged_decode_balanced_kernel, over the positions that a sequence does
+// not share: chunk c of KV head h, list positions [c W, (c + 1) W).
 template <int D, int KV, bool Q_BF16, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) shared_decode_kernel(const DecodeArgs a, const SharedArgs s) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) shared_own_kernel(const DecodeArgs a, const SharedArgs s) {
   extern __shared__ __align__(16) unsigned char dsm[];
+  pdl_enter();
+  const int c = blockIdx.x, h = blockIdx.y;
+  const int W = s.totals->own_share, all = s.own[a.B];
+  int lo = c * W;
+  if (lo >= all) return;
+  const int hi = min(lo + W, all);
+  for (int b = s.own_first[c]; b < a.B && lo < hi; ++b) {
+    const int pb = s.own[b] + kSegCost, pe = s.own[b + 1];  // b's own positions: [pb, pe)
+    const int seg_hi = min(hi, pe), seg_lo = max(lo, pb);
+    lo = seg_hi;
+    if (seg_lo >= seg_hi) continue;  // only the charge of b's start falls in this chunk
+    const int shared = s.row_shared[b];
+    int pos;
+    const int L = seq_len(a, b, pos);
+    const int t0 = shared + seg_lo - pb, t1 = min(shared + seg_hi - pb, L);
+    const bool append = pos < a.span && pos >= t0 && pos < t1;
+    decode_segment<D, KV, Q_BF16, NT, false>(a, dsm, b, h, t0, t1, append, seg_lo == pb && seg_hi == pe && shared == 0,
+                                             ((int64_t)h * (a.nchunk + a.B) + c + b) * a.G);
+  }
+}
+
+// ------------------------------------------------------------------ merge
+// CTA (h, b, z): the parts of one (KV head, sequence), a slice of its query
+// heads. Thread = (query head, 4 dims), eight parts at once; parts of the
+// shared positions first, then of the sequence's own.
+template <int D, bool Q_BF16>
+__global__ void __launch_bounds__(kThreads) shared_merge_kernel(const DecodeArgs a, const SharedArgs s) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int h = blockIdx.x, b = blockIdx.y;
+  const int gn = a.G / (int)gridDim.z, g0 = (int)blockIdx.z * gn;
   int pos;
-  const int L = seq_len(a, b, pos);
-  if (pos < 0 && h == 0 && threadIdx.x == 0) flag_error(a.err, RBLN_DEVERR_SEQ_RANGE);
-  decode_segment<D, KV, Q_BF16, NT, false, true>(a, dsm, b, h, 0, L, pos >= 0 && pos < a.span, true, 0, s.row_lead[b],
-                                                 s.row_shared[b]);
+  const int L = seq_len(a, b, pos), shared = s.row_shared[b];
+  if (pos < 0 && h == 0 && blockIdx.z == 0 && threadIdx.x == 0) flag_error(a.err, RBLN_DEVERR_SEQ_RANGE);
+  const Totals tot = *s.totals;
+  // own parts
+  const int pb = s.own[b] + kSegCost, pe = s.own[b + 1];
+  const int cf = pb / tot.own_share, own = pe > pb ? (pe - 1) / tot.own_share - cf + 1 : 0;
+  if (L > 0 && shared == 0 && own == 1) return;  // one chunk held the whole sequence and wrote the output
+  const int64_t own_slot = ((int64_t)h * (a.nchunk + a.B) + cf + b) * a.G;
+  // shared parts: of every CTA that has tiles of the row's unit, two where x = 0, 1 took the tiles in turn
+  int parts = 0, turn = 1;
+  int64_t row = 0, turn_rows = 0;
+  if (shared > 0) {
+    const int grp = s.row_group[b];
+    const int4 gr = s.group[grp];
+    const GroupUnits gu(gr.y, gr.z, s.seqs);
+    const int k = (b - gr.x) / (2 * s.seqs), i = b - gr.x - k * 2 * s.seqs;
+    const bool wide = k < gu.full || gu.rest > s.seqs;
+    const int first = h * tot.cost + s.before[grp] + k * gu.full_cost + kUnitCost;
+    const int c0 = first / tot.share, c1 = (first + (gu.tiles - 1) * (wide ? 2 : 1)) / tot.share;
+    turn = wide ? 1 : 2;
+    turn_rows = (int64_t)gu.rest * a.G;
+    parts = (c1 - c0 + 1) * turn;
+    row = (int64_t)c0 * 2 * kRows + (int64_t)h * tot.rows + gr.w + (k * 2 * s.seqs + i) * a.G;
+  }
+  constexpr int kBatch = 8;
+  for (int idx = threadIdx.x; idx < gn * (D / 4); idx += kThreads) {
+    const int g = g0 + idx / (D / 4), d4 = (idx % (D / 4)) * 4;
+    float M = neg_inf(), S = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < parts + own; s0 += kBatch) {
+      float l[kBatch];
+      float4 o[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = s0 + u;
+        l[u] = neg_inf();
+        o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i >= parts + own) continue;
+        const bool mine = i >= parts;
+        const int64_t at = mine ? own_slot + (int64_t)(i - parts) * a.G + g
+                                : row + (int64_t)(i / turn) * 2 * kRows + (i % turn) * turn_rows + g;
+        l[u] = (mine ? a.part_lse : s.part_lse)[at];
+        o[u] = *reinterpret_cast<const float4*>((mine ? a.part_o : s.part_o) + at * D + d4);
+      }
+      float mb = M;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) mb = fmaxf(mb, l[u]);
+      if (mb != M) {  // M == -inf: S and acc are still 0
+        const float c = (M == neg_inf()) ? 0.f : exp2_approx(M - mb);
+        S *= c;
+        acc.x *= c; acc.y *= c; acc.z *= c; acc.w *= c;
+        M = mb;
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (l[u] != neg_inf()) {  // a part with nothing visible carries no weight
+          const float w = exp2_approx(l[u] - M);
+          S += w;
+          acc.x += w * o[u].x; acc.y += w * o[u].y; acc.z += w * o[u].z; acc.w += w * o[u].w;
+        }
+    }
+    // no position visible: NaN, as softmax of all -inf
+    const float inv = (M == neg_inf()) ? pos_nan() : 1.f / S;
+    acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+    store_out(a, b, h, g, d4, make_uint2(pack2<Q_BF16>(acc.x, acc.y), pack2<Q_BF16>(acc.z, acc.w)));
+  }
+}
+
+// -------------------------------------------------------------- host side
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
 }
 
 template <int D, int KV, bool QB, int NT>
-int launch(const DecodeArgs& a, const SharedArgs& s, cudaStream_t st) {
-  shared_plan_kernel<<<1, kPlanThreads, 0, st>>>(a, s);
-  static SmemOptIn done;
-  if (!allow_smem(reinterpret_cast<const void*>(shared_decode_kernel<D, KV, QB, NT>), segment_smem<D, NT>(), done))
+int launch(const DecodeArgs& a, const SharedArgs& s, const Maps& m, cudaStream_t st) {
+  // the register split assumes 168 registers a thread at launch: with fewer
+  // it would never be granted
+  static const bool regs_ok = [] {
+    cudaFuncAttributes fa{};
+    return cudaFuncGetAttributes(&fa, shared_prefix_kernel<D, QB>) == cudaSuccess &&
+           2 * 128 * kRegsSoftmax + 128 * kRegsOther <= (uint32_t)fa.numRegs * kPrefixThreads;
+  }();
+  if (!regs_ok) return RBLN_ERR_LAUNCH;
+  static SmemOptIn prefix_smem, own_smem;
+  if (!allow_smem(reinterpret_cast<const void*>(shared_prefix_kernel<D, QB>), PrefixSmem<D>::ALLOC, prefix_smem) ||
+      !allow_smem(reinterpret_cast<const void*>(shared_own_kernel<D, KV, QB, NT>), segment_smem<D, NT>(), own_smem))
     return RBLN_ERR_LAUNCH;
-  shared_decode_kernel<D, KV, QB, NT><<<dim3(a.Hkv, a.B), kThreads, segment_smem<D, NT>(), st>>>(a, s);
-  return cudaGetLastError() == cudaSuccess ? RBLN_OK : RBLN_ERR_LAUNCH;
+  int rc = launch_after(shared_plan_kernel, dim3(1), kPlanThreads, 0, st, a, s);
+  if (rc == RBLN_OK && s.groups > 0)
+    rc = launch_after(shared_prefix_kernel<D, QB>, dim3(s.ctas), kPrefixThreads, PrefixSmem<D>::ALLOC, st, m.q, m.k, m.v,
+                      a, s);
+  if (rc == RBLN_OK)
+    rc = launch_after(shared_own_kernel<D, KV, QB, NT>, dim3(a.nchunk, a.Hkv), kThreads, segment_smem<D, NT>(), st, a, s);
+  if (rc == RBLN_OK)
+    rc = launch_after(shared_merge_kernel<D, QB>, dim3(a.Hkv, a.B, merge_head_split(a.Hkv, a.B, a.G)), kThreads, 0, st, a,
+                      s);
+  return rc;
 }
 
 template <int D>
-int launch_any(const DecodeArgs& a, const SharedArgs& s, bool bf16, cudaStream_t st) {
-  if (bf16) return a.G > 8 ? launch<D, KV_BF16, true, 2>(a, s, st) : launch<D, KV_BF16, true, 1>(a, s, st);
-  return a.G > 8 ? launch<D, KV_F16, false, 2>(a, s, st) : launch<D, KV_F16, false, 1>(a, s, st);
+int launch_any(const DecodeArgs& a, const SharedArgs& s, const Maps& m, bool bf16, cudaStream_t st) {
+  if (bf16) return a.G > 8 ? launch<D, KV_BF16, true, 2>(a, s, m, st) : launch<D, KV_BF16, true, 1>(a, s, m, st);
+  return a.G > 8 ? launch<D, KV_F16, false, 2>(a, s, m, st) : launch<D, KV_F16, false, 1>(a, s, m, st);
 }
 
+constexpr int kSms = 148;  // a persistent CTA on each
+
 struct Plan {
-  size_t row_shared, row_lead, total;
+  int nchunk;
+  size_t totals, row_shared, row_group, own, own_first, group, before, cta_group, own_o, own_lse, part_o, part_lse, total;
 };
 
 int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s, Plan* pl) {
@@ -88,22 +835,55 @@ int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s
   if ((int64_t)p->max_blocks * p->block_size > (1 << 30)) return RBLN_ERR_UNSUPPORTED;
   const bool tiles = p->block_size % 128 == 0 || (p->block_size >= 8 && 128 % p->block_size == 0);
   if (!tiles) return RBLN_ERR_UNSUPPORTED;
+  if ((int64_t)p->batch * ((int64_t)p->max_blocks * p->block_size + 15 + kSegCost) >= (int64_t)1 << 30)
+    return RBLN_ERR_UNSUPPORTED;
+  // the units' line, with room for a CTA's share past its end, is counted in 32 bits
+  const int64_t units = (int64_t)p->batch / (2 * (kRows / p->group)) + s->num_groups + 1;
+  if (p->num_kv_heads * units * (2 * tiles_of(p->max_blocks * p->block_size) + kUnitCost) >= (int64_t)1 << 30)
+    return RBLN_ERR_UNSUPPORTED;
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t start = at;
     at += (n + 255) / 256 * 256;
     return start;
   };
-  pl->row_shared = take(p->batch * sizeof(int));
-  pl->row_lead = take(p->batch * sizeof(int));
+  // one wave of CTAs of the own positions: 4 an SM for up to 8 query heads a KV head, 2 above
+  pl->nchunk = std::max(1, kSms * (p->group <= 8 ? 4 : 2) / p->num_kv_heads);
+  const size_t B = p->batch, N = s->num_groups, D = p->head_dim;
+  const size_t own = (size_t)p->num_kv_heads * (pl->nchunk + B) * p->group;
+  // a row of the shared parts is stored once for each CTA that has keys of it: 256 rows a CTA at most, and a unit's
+  // rows (twice them where its key tiles are taken in turn) for its first one
+  const size_t part = N == 0 ? 0 : (size_t)kSms * 2 * kRows + 2 * B * p->group * p->num_kv_heads;
+  pl->totals = take(sizeof(Totals));
+  pl->row_shared = take(B * sizeof(int));
+  pl->row_group = take(B * sizeof(int));
+  pl->own = take((B + 1) * sizeof(int));
+  pl->own_first = take(pl->nchunk * sizeof(int));
+  pl->group = take(N * sizeof(int4));
+  pl->before = take((N + 1) * sizeof(int));
+  pl->cta_group = take(kSms * sizeof(int));
+  pl->own_o = take(own * D * sizeof(float));
+  pl->own_lse = take(own * sizeof(float));
+  pl->part_o = take(part * D * sizeof(float));
+  pl->part_lse = take(part * sizeof(float));
   pl->total = at + 256;
   return RBLN_OK;
 }
 
-int run_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s, cudaStream_t st) {
+int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t* s, cudaStream_t st) {
   Plan pl;
-  const int rc = plan_shared(p, s, &pl);
+  const int rc = plan_shared(p_in, s, &pl);
   if (rc != RBLN_OK) return rc;
+  // a dimension of one entry has any stride: one that the tensor maps take
+  rbln_paged_attn_params_t q = *p_in;
+  const rbln_paged_attn_params_t* p = &q;
+  if (q.batch == 1) q.q_stride[0] = q.out_stride[0] = q.k_new_stride[0] = q.v_new_stride[0] = q.head_dim;
+  if (q.num_kv_heads == 1) {
+    q.q_stride[1] = q.out_stride[1] = q.k_new_stride[1] = q.v_new_stride[1] = q.head_dim;
+    q.cache_stride[1] = q.head_dim;
+  }
+  if (q.group == 1) q.q_stride[2] = q.out_stride[2] = q.head_dim;
+  if (q.num_blocks == 1) q.cache_stride[0] = q.head_dim;
   if (p->q_len != 1) return RBLN_ERR_INVALID_ARGUMENT;
   if (p->mask || p->sinks || p->num_splits || p->prof_events[0] || p->prof_events[1]) return RBLN_ERR_UNSUPPORTED;
   if ((p->q_dtype != RBLN_DT_BF16 && p->q_dtype != RBLN_DT_F16) || p->kv_dtype != p->q_dtype)
@@ -151,14 +931,41 @@ int run_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s,
   a.B = p->batch; a.Hkv = p->num_kv_heads; a.G = p->group; a.num_blocks = p->num_blocks;
   a.bs = p->block_size; a.span = p->max_blocks * p->block_size;
   a.err = p->error_flags;
+  a.nchunk = pl.nchunk;
+  a.part_o = reinterpret_cast<float*>(ws + pl.own_o);
+  a.part_lse = reinterpret_cast<float*>(ws + pl.own_lse);
   SharedArgs x{};
   x.groups = s->num_groups;
   x.starts = s->group_starts;
   x.lens = s->shared_lens;
+  x.seqs = kRows / p->group;
+  x.ctas = kSms;
+  x.totals = reinterpret_cast<Totals*>(ws + pl.totals);
   x.row_shared = reinterpret_cast<int*>(ws + pl.row_shared);
-  x.row_lead = reinterpret_cast<int*>(ws + pl.row_lead);
+  x.row_group = reinterpret_cast<int*>(ws + pl.row_group);
+  x.own = reinterpret_cast<int*>(ws + pl.own);
+  x.own_first = reinterpret_cast<int*>(ws + pl.own_first);
+  x.group = reinterpret_cast<int4*>(ws + pl.group);
+  x.before = reinterpret_cast<int*>(ws + pl.before);
+  x.cta_group = reinterpret_cast<int*>(ws + pl.cta_group);
+  x.part_o = reinterpret_cast<float*>(ws + pl.part_o);
+  x.part_lse = reinterpret_cast<float*>(ws + pl.part_lse);
+  Maps m;
+  if (x.groups > 0) {
+    // queries [B, Hkv, G, D] in boxes of `seqs` sequences of one KV head, rows in order (sequence, query head)
+    const uint64_t dims[4] = {(uint64_t)p->head_dim, (uint64_t)p->group, (uint64_t)p->num_kv_heads, (uint64_t)p->batch};
+    const uint64_t strides[3] = {(uint64_t)q.q_stride[2] * 2, (uint64_t)q.q_stride[1] * 2, (uint64_t)q.q_stride[0] * 2};
+    const uint32_t box[4] = {64, (uint32_t)p->group, 1, (uint32_t)x.seqs};
+    const int rpb = std::min(p->block_size, kKeys);
+    if (!make_map(&m.q, tmap_dtype(p->q_dtype), 4, const_cast<void*>(p->q), dims, strides, box) ||
+        !map_kv(&m.k, p->kcache, p->kv_dtype, p->num_blocks, p->num_kv_heads, p->block_size, p->head_dim,
+                q.cache_stride[0], q.cache_stride[1], q.cache_stride[2], rpb) ||
+        !map_kv(&m.v, p->vcache, p->kv_dtype, p->num_blocks, p->num_kv_heads, p->block_size, p->head_dim,
+                q.cache_stride[0], q.cache_stride[1], q.cache_stride[2], rpb))
+      return RBLN_ERR_INVALID_ARGUMENT;
+  }
   const bool bf16 = p->q_dtype == RBLN_DT_BF16;
-  return p->head_dim == 128 ? launch_any<128>(a, x, bf16, st) : launch_any<64>(a, x, bf16, st);
+  return p->head_dim == 128 ? launch_any<128>(a, x, m, bf16, st) : launch_any<64>(a, x, m, bf16, st);
 }
 
 }  // namespace
