@@ -36,10 +36,14 @@ constexpr int kPerRow = kMaxBatch / kPlanThreads;
 constexpr int kKeys = 128;            // keys a tile
 constexpr int kRows = 128;            // query rows a tile
 constexpr int kPanel = 128 * 128;     // bytes: 128 rows of 64 elements
-constexpr int kPrefixThreads = 384;   // softmax warpgroups 0-3 and 4-7, producer 8, MMA 9
+constexpr int kPrefixThreads = 384;   // softmax warpgroups 0-3 and 4-7, producers 8 and 10, MMA 9
 constexpr int kUnitCost = 1;          // key tiles charged to a unit's start
 constexpr int kSegCost = 128;         // keys charged to the start of a sequence's own part
 constexpr int kMinOwn = 256;          // smallest share of a CTA of own positions
+constexpr int kSms = 148;
+// Own positions that keep an SM as long as a key tile of 128 rows does: the
+// SMs are divided between the two kernels, which run side by side, by it.
+constexpr int kOwnPerTile = 128;
 // Registers a thread after the split (launch: 168 each): a softmax thread
 // holds its whole row of 128 scores.
 constexpr uint32_t kRegsSoftmax = 216, kRegsOther = 64;
@@ -58,7 +62,8 @@ struct SharedArgs {
   const int32_t* starts;
   const int32_t* lens;
   int seqs;            // sequences a row tile holds: 128 / G
-  int ctas;            // of the prefix kernel
+  int ctas;            // of the prefix kernel, one an SM
+  int own_ctas;        // of the own kernel on an SM
   Totals* totals;
   int* row_shared;     // [B] positions that are read through the group's table
   int* row_group;      // [B] that group, -1: none
@@ -156,17 +161,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) shared_plan_kernel(const Deco
     sum += own[k];
   }
   int run = scan_before<false>(sum, 0, &all);
-  const int W = max(kMinOwn, ((all + a.nchunk - 1) / a.nchunk + 15) & ~15);
-  for (int k = 0; k < kPerRow; ++k) {
-    const int b = kPerRow * tid + k;
-    if (b >= a.B) continue;
-    s.own[b] = run;
-    for (int c = (run + W - 1) / W; c * W < run + own[k]; ++c) s.own_first[c] = b;
-    run += own[k];
-  }
-  if (tid == 0) s.own[a.B] = all;
   // groups: cost and stored rows
-  __syncthreads();
   int cost = 0, rows = 0, total, all_rows, len = 0, n = 0;
   if (tid < s.groups) {
     n = start[tid + 1] - start[tid];
@@ -182,9 +177,25 @@ __global__ void __launch_bounds__(kPlanThreads, 1) shared_plan_kernel(const Deco
     s.group[tid] = make_int4(start[tid], n, len, rb);
     s.before[tid] = before[tid] = cb;
   }
-  // the line is below 2^30 long. A share of 2 at least: so every CTA between a unit's first and last has a tile of it
-  const int share = max(2, (total * a.Hkv + s.ctas - 1) / s.ctas);
+  // SMs for the shared positions, the others are left to the own ones. The
+  // line is below 2^30 long. A share of 2 at least: so every CTA between a
+  // unit's first and last has a tile of it.
+  const int line = total * a.Hkv;
+  const float own_line = (float)all * a.Hkv / kOwnPerTile;
+  const int sms = max(1, min(s.ctas - 2, (int)(s.ctas * (line / (line + own_line)))));
+  const int share = max(2, (line + sms - 1) / sms);
+  const int left = s.ctas - (line + share - 1) / share;
+  const int chunks = max(1, min(a.nchunk, left * s.own_ctas / a.Hkv));
+  const int W = max(kMinOwn, ((all + chunks - 1) / chunks + 15) & ~15);
+  for (int k = 0; k < kPerRow; ++k) {
+    const int b = kPerRow * tid + k;
+    if (b >= a.B) continue;
+    s.own[b] = run;
+    for (int c = (run + W - 1) / W; c * W < run + own[k]; ++c) s.own_first[c] = b;
+    run += own[k];
+  }
   if (tid == 0) {
+    s.own[a.B] = all;
     s.before[s.groups] = total;
     *s.totals = Totals{total, share, all_rows, W};
   }
@@ -192,7 +203,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) shared_plan_kernel(const Deco
   if (tid < s.ctas) {
     const int at = tid * share;
     int g = -1;
-    if (at < total * a.Hkv) {
+    if (at < line) {
       const int x = at % total;
       int lo = 0, hi = s.groups - 1;  // the last group that starts at or before x: it has a cost
       while (lo < hi) {
@@ -294,6 +305,17 @@ enum PrefixBar {
   B_DONE = B_OE + 2, B_COUNT
 };
 
+// Eight floats times f, one whole sector of memory: a thread holds a row, so
+// that narrower stores of a warp would each touch 32 sectors in part.
+__device__ __forceinline__ void store_sector(float* to, const uint32_t* o, float f) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[i]) * f;
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
 // Roles as in the chunked prefill's 128-key kernel: two softmax warpgroups x
 // = 0, 1, each with a score buffer (128 columns of TMEM, the probabilities
 // written over its first half) and an accumulator (D columns). In a wide
@@ -326,7 +348,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_enter();  // the set-up above overlaps the plan
+  // The set-up above overlaps the plan. Behind it the own kernel may start on
+  // the SMs that are left: it needs the plan and what ran before, all complete
+  // here, and not this grid.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __threadfence();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   auto t_s = [&](int x) { return tmem + x * 128; };
   auto t_o = [&](int x) { return tmem + 256 + x * 128; };
@@ -347,63 +374,54 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 
   if (warp >= 8) {
    setmaxnreg_dec<kRegsOther>();
-   if (warp == 8) {
-    // ------------------------------------------------------------ producer
+   if (warp == 8 || warp == 10) {
+    // ----------------------------------------------------------- producers
+    // warp 8: queries and K, warp 10: V. A stage of V is freed by a product
+    // that waits for the softmax, one of K long before: in one queue the next
+    // K tiles would stand behind it.
+    const bool keys = warp == 8;
+    const CUtensorMap* tm = keys ? &tm_k : &tm_v;
+    const int full = keys ? B_KF : B_VF, empty = keys ? B_KE : B_VE;
+    const uint32_t ring = sbase + (keys ? L::K : L::V);
     if (lane == 0) {
-      prefetch_tmap(&tm_q);
-      prefetch_tmap(&tm_k);
-      prefetch_tmap(&tm_v);
+      if (keys) prefetch_tmap(&tm_q);
+      prefetch_tmap(tm);
     }
-    int T = 0, act = 0, k_issued = 0, v_issued = 0;
+    int T = 0, act = 0;
     bool ok = true;
     Unit u;
-    for (Walk w(s, a.Hkv, a.G); ok && w.next(u);) {
-      if (act >= 1 && !__all_sync(0xffffffffu, mbar_wait(bar(B_QE), (act - 1) & 1, abort))) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar(B_QF), (u.wide ? 2 : 1) * NP * s.seqs * a.G * 128);
-        for (int x = 0; x < (u.wide ? 2 : 1); ++x)
-          for (int p = 0; p < NP; ++p)
-            tma_load_4d(sbase + L::Q + x * L::TILE + p * kPanel, &tm_q, bar(B_QF), p * 64, 0, u.h, u.b0 + x * s.seqs);
+    for (Walk w(s, a.Hkv, a.G); ok && w.next(u); ++act) {
+      if (keys) {
+        if (act >= 1 && !__all_sync(0xffffffffu, mbar_wait(bar(B_QE), (act - 1) & 1, abort))) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar(B_QF), (u.wide ? 2 : 1) * NP * s.seqs * a.G * 128);
+          for (int x = 0; x < (u.wide ? 2 : 1); ++x)
+            for (int p = 0; p < NP; ++p)
+              tma_load_4d(sbase + L::Q + x * L::TILE + p * kPanel, &tm_q, bar(B_QF), p * 64, 0, u.h, u.b0 + x * s.seqs);
+        }
       }
       for (int t = u.t0; t < u.t1; ++t, ++T) {
         int row;
         const int blk = block_of(u, t, row);
-        if (blk == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < u.len)
+        if (keys && blk == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < u.len)
           flag_error(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
         const int st = T % ST;
-        if (T >= ST && !__all_sync(0xffffffffu, mbar_wait(bar(B_KE + st), (T / ST - 1) & 1, abort))) {
+        if (T >= ST && !__all_sync(0xffffffffu, mbar_wait(bar(empty + st), (T / ST - 1) & 1, abort))) {
           ok = false;
           break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(bar(B_KF + st), NP * kPanel);
+        if (lane == 0) mbar_arrive_expect_tx(bar(full + st), NP * kPanel);
         __syncwarp();
         if (lane < boxes)
           for (int p = 0; p < NP; ++p)
-            tma_load_4d(sbase + L::K + st * L::TILE + p * kPanel + lane * rpb * 128, &tm_k, bar(B_KF + st), p * 64, row,
-                        u.h, blk);
-        k_issued = T + 1;
-        if (T >= ST && !__all_sync(0xffffffffu, mbar_wait(bar(B_VE + st), (T / ST - 1) & 1, abort))) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(bar(B_VF + st), NP * kPanel);
-        __syncwarp();
-        if (lane < boxes)
-          for (int p = 0; p < NP; ++p)
-            tma_load_4d(sbase + L::V + st * L::TILE + p * kPanel + lane * rpb * 128, &tm_v, bar(B_VF + st), p * 64, row,
-                        u.h, blk);
-        v_issued = T + 1;
+            tma_load_4d(ring + st * L::TILE + p * kPanel + lane * rpb * 128, tm, bar(full + st), p * 64, row, u.h, blk);
       }
-      ++act;
     }
     if (*abort) {
       // let the copies in flight land before the CTA exits
       const long long t0 = clock64();
-      for (int j = max(0, k_issued - ST); j < k_issued; ++j)
-        while (!mbar_try_wait(bar(B_KF + j % ST), (j / ST) & 1) && clock64() - t0 < 4000000) {
-        }
-      for (int j = max(0, v_issued - ST); j < v_issued; ++j)
-        while (!mbar_try_wait(bar(B_VF + j % ST), (j / ST) & 1) && clock64() - t0 < 8000000) {
+      for (int j = max(0, T - ST); j < T; ++j)
+        while (!mbar_try_wait(bar(full + j % ST), (j / ST) & 1) && clock64() - t0 < 4000000) {
         }
     }
    } else if (warp == 9 && lane == 0) {
@@ -639,10 +657,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         tmem_wait_ld();
         if (row_ok) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(s.part_o + at * D + c * 32 + e) =
-                make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                            __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+          for (int e = 0; e < 32; e += 8) store_sector(s.part_o + at * D + c * 32 + e, o + e, inv);
         }
       }
       if (row_ok) s.part_lse[at] = m_run == neg_inf() ? neg_inf() : m_run + __log2f(l_run);
@@ -665,9 +680,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 // As paged_decode_balanced_kernel, over the positions that a sequence does
 // not share: chunk c of KV head h, list positions [c W, (c + 1) W).
 template <int D, int KV, bool Q_BF16, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) shared_own_kernel(const DecodeArgs a, const SharedArgs s) {
-  extern __shared__ __align__(16) unsigned char dsm[];
-  pdl_enter();
+__device__ __forceinline__ void own_chunk(const DecodeArgs& a, const SharedArgs& s, unsigned char* dsm) {
   const int c = blockIdx.x, h = blockIdx.y;
   const int W = s.totals->own_share, all = s.own[a.B];
   int lo = c * W;
@@ -686,6 +699,20 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) shared_own_kernel(c
     decode_segment<D, KV, Q_BF16, NT, false>(a, dsm, b, h, t0, t1, append, seg_lo == pb && seg_hi == pe && shared == 0,
                                              ((int64_t)h * (a.nchunk + a.B) + c + b) * a.G);
   }
+}
+
+// Runs beside the prefix kernel, whose CTAs have all begun, so that the plan
+// and everything before it is complete. It ends only when that kernel has, by
+// its first CTA (the others leave their SMs to those that wait to start): the
+// merge waits for this grid, and so for both.
+template <int D, int KV, bool Q_BF16, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) shared_own_kernel(const DecodeArgs a, const SharedArgs s) {
+  extern __shared__ __align__(16) unsigned char dsm[];
+  if (s.groups == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // there is no prefix kernel
+  __threadfence();  // nothing is read from a cache line older than the plan
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  own_chunk<D, KV, Q_BF16, NT>(a, s, dsm);
+  if (blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ merge
@@ -818,8 +845,6 @@ int launch_any(const DecodeArgs& a, const SharedArgs& s, const Maps& m, bool bf1
   return a.G > 8 ? launch<D, KV_F16, false, 2>(a, s, m, st) : launch<D, KV_F16, false, 1>(a, s, m, st);
 }
 
-constexpr int kSms = 148;  // a persistent CTA on each
-
 struct Plan {
   int nchunk;
   size_t totals, row_shared, row_group, own, own_first, group, before, cta_group, own_o, own_lse, part_o, part_lse, total;
@@ -940,6 +965,7 @@ int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t*
   x.lens = s->shared_lens;
   x.seqs = kRows / p->group;
   x.ctas = kSms;
+  x.own_ctas = p->group <= 8 ? 4 : 2;
   x.totals = reinterpret_cast<Totals*>(ws + pl.totals);
   x.row_shared = reinterpret_cast<int*>(ws + pl.row_shared);
   x.row_group = reinterpret_cast<int*>(ws + pl.row_group);
