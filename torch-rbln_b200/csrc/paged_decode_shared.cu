@@ -30,20 +30,18 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kMaxBatch = 4096, kMaxGroups = 1024;
-constexpr int kPlanThreads = 1024;
-constexpr int kPerRow = kMaxBatch / kPlanThreads;
+constexpr int kMaxBatch = 4096, kMaxGroups = 1024;  // what the plan's CTA takes
+constexpr int kPlanRows = 4;          // rows a thread of the plan
 constexpr int kKeys = 128;            // keys a tile
 constexpr int kRows = 128;            // query rows a tile
 constexpr int kPanel = 128 * 128;     // bytes: 128 rows of 64 elements
 constexpr int kPrefixThreads = 384;   // softmax warpgroups 0-3 and 4-7, producers 8 and 10, MMA 9
-constexpr int kUnitCost = 1;          // key tiles charged to a unit's start
 constexpr int kSegCost = 128;         // keys charged to the start of a sequence's own part
 constexpr int kMinOwn = 256;          // smallest share of a CTA of own positions
 constexpr int kSms = 148;
-// Own positions that keep an SM as long as a key tile of 128 rows does: the
-// SMs are divided between the two kernels, which run side by side, by it.
-constexpr int kOwnPerTile = 128;
+// What a key tile costs a CTA with two row tiles and with one (whose two
+// warpgroups take the tiles in turn), and a unit's start.
+constexpr int kWideCost = 4, kTurnCost = 3, kUnitCost = 2;
 // Registers a thread after the split (launch: 168 each): a softmax thread
 // holds its whole row of 128 scores.
 constexpr uint32_t kRegsSoftmax = 216, kRegsOther = 64;
@@ -51,10 +49,20 @@ static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kPrefixThreads * 168,
 
 // What the plan leaves for the other kernels.
 struct Totals {
-  int cost;         // of all units of a KV head, in key tiles of 128 rows
-  int share;        // of a CTA of the prefix kernel
-  int rows;         // rows that a KV head's units store for each CTA that works on them
-  int own_share;    // own positions of a CTA
+  int cost;       // of all units of a KV head
+  int share;      // of a CTA of the prefix kernel
+  int rows;       // rows that a KV head's units store for each CTA that works on them
+  int own_share;  // own positions of a CTA
+};
+
+// A CTA's key tiles of a unit of the prefix kernel.
+struct Unit {
+  int h, b0, n;   // KV head, sequences [b0, b0 + n)
+  int lead, len;  // row of the block table, shared positions
+  int wide;       // two row tiles, each against all keys; else one, its key tiles in turn by two warpgroups
+  int t0, t1;     // this CTA's key tiles
+  int row0;       // first stored row
+  int group, next;  // the group, and where on the line the CTA goes on
 };
 
 struct SharedArgs {
@@ -64,215 +72,248 @@ struct SharedArgs {
   int seqs;            // sequences a row tile holds: 128 / G
   int ctas;            // of the prefix kernel, one an SM
   int own_ctas;        // of the own kernel on an SM
+  float tile_us;       // time of a key tile of cost 1, and of an own position, on an SM
+  float own_us;
   Totals* totals;
   int* row_shared;     // [B] positions that are read through the group's table
-  int* row_group;      // [B] that group, -1: none
+  int4* row_parts;     // [B] the row's unit: its first key tile on KV head 0's line, the last one less that (-1: no
+                       // shared part), its stored row, the stored rows of x = 0 where tiles are taken in turn
   int* own;            // [B + 1] prefix of the rows' own positions, as in the decode kernels
   int* own_first;      // [nchunk] first sequence of a chunk
   int4* group;         // [groups] first sequence, sequences, shared positions, stored rows before it
   int* before;         // [groups + 1] cost of the groups before it, in one KV head
-  int* cta_group;      // [ctas] group that a CTA starts in, -1: none
-  float* part_o;       // parts of the shared positions, see Unit
+  Unit* first;         // [ctas] the first unit of each CTA, t0 = t1: none
+  float* part_o;       // parts of the shared positions, see unit_at
   float* part_lse;
 };
 
-// ------------------------------------------------------------------- plan
-// Exclusive scan over the CTA's threads (sum or maximum); *all: of all.
-template <bool MAX, typename T>
-__device__ __forceinline__ T scan_before(T v, T zero, T* all) {
-  __shared__ T warps[kPlanThreads / 32];
-  auto join = [](T a, T b) { return MAX ? (a > b ? a : b) : a + b; };
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T x = v;
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x = join(x, y);
-  }
-  __syncthreads();  // the last call's sums have been read
-  if (lane == 31) warps[warp] = x;
-  __syncthreads();
-  T w = warps[lane];
-  for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w = join(w, y);
-  }
-  *all = __shfl_sync(0xffffffffu, w, 31);
-  const T wb = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
-  const T up = __shfl_up_sync(0xffffffffu, x, 1);
-  return join(warp > 0 ? wb : zero, lane > 0 ? up : zero);
-}
-
 __host__ __device__ __forceinline__ int tiles_of(int positions) { return (positions + kKeys - 1) / kKeys; }
 
-// A group's units: `full` of 2 x seqs sequences, whose key tiles cost 2 (two
-// row tiles), and one of the rest: 1 where those fit in one row tile.
+// A group's units: `full` of 2 x seqs sequences and one of the rest, which
+// takes its tiles in turn where those fit in one row tile.
 struct GroupUnits {
   int full, rest, tiles, full_cost, rest_cost;
   __device__ __forceinline__ GroupUnits(int n, int len, int seqs) {
     full = n / (2 * seqs);
     rest = n - full * 2 * seqs;
     tiles = tiles_of(len);
-    full_cost = 2 * tiles + kUnitCost;
-    rest_cost = rest == 0 ? 0 : (rest > seqs ? 2 * tiles : tiles) + kUnitCost;
+    full_cost = kWideCost * tiles + kUnitCost;
+    rest_cost = rest == 0 ? 0 : (rest > seqs ? kWideCost : kTurnCost) * tiles + kUnitCost;
   }
 };
 
-__global__ void __launch_bounds__(kPlanThreads, 1) shared_plan_kernel(const DecodeArgs a, const SharedArgs s) {
-  __shared__ int start[kMaxGroups + 1];
-  __shared__ int before[kMaxGroups + 1];
-  __shared__ int active[kMaxGroups];
-  pdl_enter();
-  const int tid = threadIdx.x;
-  // the groups' starts, none before the one before it
-  {
-    int v[2], m = 0, all;
-    for (int k = 0; k < 2; ++k) {
-      const int g = 2 * tid + k;
-      if (g <= s.groups) m = max(m, min(max(s.starts[g], 0), a.B));
-      v[k] = m;
+// The units of all KV heads, head by head, group by group, stand end to end
+// on a line, each unit's start charged kUnitCost, each key tile its cost; CTA
+// c takes [c share, (c + 1) share), a tile by where it starts. A unit's rows
+// as CTA c sees them are stored from row 256 c + R on, with R the rows that
+// the units before it store: no two of them overlap, since a unit stores 256
+// rows at most, and neither does one unit's with another's in one CTA.
+//
+// The unit at `lo` of the line, in group g of head h, as a CTA sees it that
+// ends at `hi`; gr: the group, before: its start on the head's line.
+__device__ __forceinline__ Unit unit_at(int lo, int hi, int cta, int h, int g, int4 gr, int before, int head_cost,
+                                        int head_rows, int seqs, int G) {
+  const GroupUnits gu(gr.y, gr.z, seqs);
+  const int y = lo - h * head_cost - before, k = min(y / gu.full_cost, gu.full);
+  const bool whole = k < gu.full;
+  const int base = lo - y + k * gu.full_cost, end = base + (whole ? gu.full_cost : gu.rest_cost);
+  Unit u;
+  u.wide = whole || gu.rest > seqs;
+  const int w = u.wide ? kWideCost : kTurnCost;
+  const int first = base + kUnitCost;
+  u.next = min(hi, end);
+  u.t0 = (max(lo, first) - first + w - 1) / w;
+  u.t1 = (max(u.next, first) - first + w - 1) / w;
+  u.h = h;
+  u.b0 = gr.x + k * 2 * seqs;
+  u.n = whole ? 2 * seqs : gu.rest;
+  u.lead = gr.x;
+  u.len = gr.z;
+  u.row0 = cta * 2 * kRows + h * head_rows + gr.w + k * 2 * seqs * G;
+  u.group = g;
+  return u;
+}
+
+// ------------------------------------------------------------------- plan
+// Exclusive scan over the CTA's threads of N values (sum or maximum) at once;
+// all[i]: of all threads.
+template <int THREADS, bool MAX, int N>
+__device__ __forceinline__ void scan_before(int (&v)[N], int (&all)[N]) {
+  constexpr int W = THREADS / 32;
+  __shared__ int warps[N][32];
+  auto join = [](int a, int b) { return MAX ? max(a, b) : a + b; };  // of values from 0 up
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = v[i];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x[i], o);
+      if (lane >= o) x[i] = join(x[i], y);
     }
-    const int up = scan_before<true>(m, 0, &all);
-    for (int k = 0; k < 2; ++k)
-      if (2 * tid + k <= s.groups) start[2 * tid + k] = max(v[k], up);
-    if (tid < kMaxGroups) active[tid] = 0;
+    if (lane == 31) warps[i][warp] = x[i];
   }
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    int w = lane < W ? warps[i][lane] : 0;
+    for (int o = 1; o < W; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w = join(w, y);
+    }
+    all[i] = __shfl_sync(0xffffffffu, w, W - 1);
+    const int wb = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    const int up = __shfl_up_sync(0xffffffffu, x[i], 1);
+    v[i] = join(warp > 0 ? wb : 0, lane > 0 ? up : 0);
+  }
+}
+
+// The last i of [-1, n] (0 <= i where `at` starts at 0) with at[i] <= x.
+__device__ __forceinline__ int last_at_most(const int* at, int lo, int hi, int x) {
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (at[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// One CTA of 256 threads for up to 1024 rows and 256 groups, else of 1024.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) shared_plan_kernel(const DecodeArgs a, const SharedArgs s) {
+  constexpr int GROUPS = THREADS;
+  __shared__ int start[GROUPS + 1], before[GROUPS + 1], len[GROUPS], stored[GROUPS];
+  pdl_enter();
+  const int tid = threadIdx.x;
+  int cut[2], seq[kPlanRows];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) cut[k] = 2 * tid + k <= s.groups ? min(max(s.starts[2 * tid + k], 0), a.B) : 0;
+#pragma unroll
+  for (int k = 0; k < kPlanRows; ++k)
+    seq[k] = kPlanRows * tid + k < a.B ? a.seq[(kPlanRows * tid + k) * a.seq_stride] : -1;
+  const int mine = tid < s.groups ? min(max(s.lens[tid], 0), a.span) : 0;
+  // the groups' starts, none before the one before it
+  cut[1] = max(cut[0], cut[1]);
+  int top[1] = {cut[1]}, most[1];
+  scan_before<THREADS, true>(top, most);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (2 * tid + k <= s.groups) start[2 * tid + k] = max(cut[k], top[0]);
+  len[tid] = mine;
+  stored[tid] = 0;
+  __syncthreads();
   // rows: group, shared positions, own positions
-  int own[kPerRow], sum = 0, all;
-  for (int k = 0; k < kPerRow; ++k) {
-    const int b = kPerRow * tid + k;
+  int own[kPlanRows], group[kPlanRows], shared[kPlanRows], sum = 0;
+#pragma unroll
+  for (int k = 0; k < kPlanRows; ++k) {
+    const int b = kPlanRows * tid + k;
     own[k] = 0;
+    group[k] = -1;
+    shared[k] = 0;
     if (b >= a.B) continue;
-    int lo = -1, hi = s.groups;  // the last start at or before b
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (start[mid] <= b) lo = mid; else hi = mid - 1;
+    const int g = last_at_most(start, -1, s.groups, b);
+    if (g >= 0 && g < s.groups && len[g] > 0 && seq[k] >= len[g]) {
+      group[k] = g;
+      shared[k] = len[g];
+      stored[g] = 1;  // some row of it has a shared part
     }
-    int pos, n = 0;
-    const int L = seq_len(a, b, pos);
-    if (lo >= 0 && lo < s.groups) {
-      n = min(max(s.lens[lo], 0), a.span);
-      if (pos < n) n = 0;
-    }
-    if (n > 0) active[lo] = 1;
-    s.row_shared[b] = n;
-    s.row_group[b] = n > 0 ? lo : -1;
-    own[k] = ((L - n + 15) & ~15) + kSegCost;
+    const int L = seq[k] < 0 ? 0 : min(seq[k] + 1, a.span);
+    own[k] = ((L - shared[k] + 15) & ~15) + kSegCost;
     sum += own[k];
+    s.row_shared[b] = shared[k];
   }
-  int run = scan_before<false>(sum, 0, &all);
-  // groups: cost and stored rows
-  int cost = 0, rows = 0, total, all_rows, len = 0, n = 0;
+  __syncthreads();
+  // own positions before this thread's rows; cost and stored rows of the groups before this thread's
+  int n = 0;
+  if (tid < s.groups && stored[tid]) n = start[tid + 1] - start[tid];
+  const GroupUnits gu(n, n > 0 ? mine : 0, s.seqs);
+  int v[3] = {sum, gu.full * gu.full_cost + gu.rest_cost,
+              (2 * s.seqs * gu.full + (gu.rest > s.seqs ? gu.rest : 2 * gu.rest)) * a.G};
+  int all[3];
+  scan_before<THREADS, false>(v, all);
+  const int total = all[1];
   if (tid < s.groups) {
-    n = start[tid + 1] - start[tid];
-    len = active[tid] ? min(max(s.lens[tid], 0), a.span) : 0;
-    if (len == 0) n = 0;
-    const GroupUnits u(n, len, s.seqs);
-    cost = u.full * u.full_cost + u.rest_cost;
-    rows = (2 * s.seqs * u.full + (u.rest > s.seqs ? u.rest : 2 * u.rest)) * a.G;
+    before[tid] = s.before[tid] = v[1];
+    stored[tid] = v[2];
+    len[tid] = n > 0 ? mine : 0;
+    s.group[tid] = make_int4(start[tid], n, n > 0 ? mine : 0, v[2]);
   }
-  const int cb = scan_before<false>(cost, 0, &total);
-  const int rb = scan_before<false>(rows, 0, &all_rows);
-  if (tid < s.groups) {
-    s.group[tid] = make_int4(start[tid], n, len, rb);
-    s.before[tid] = before[tid] = cb;
-  }
-  // SMs for the shared positions, the others are left to the own ones. The
-  // line is below 2^30 long. A share of 2 at least: so every CTA between a
-  // unit's first and last has a tile of it.
+  // The SMs are divided so that both kernels end together: with m of N SMs,
+  //   line / m + late = own / (N - m),
+  // `late` what the first has to do besides, all in microseconds.
   const int line = total * a.Hkv;
-  const float own_line = (float)all * a.Hkv / kOwnPerTile;
-  const int sms = max(1, min(s.ctas - 2, (int)(s.ctas * (line / (line + own_line)))));
-  const int share = max(2, (line + sms - 1) / sms);
+  const float N = (float)s.ctas, late = 4.f, P = line * s.tile_us, O = (float)all[0] * a.Hkv * s.own_us;
+  const float half = 0.5f * (late * N - P - O);
+  const int sms = min(s.ctas - 2, max(1, (int)((half + sqrtf(half * half + late * P * N)) / late + 0.5f)));
+  // The line is below 2^30 long. A share of a wide tile at least: so every
+  // CTA between a unit's first and last has a tile of it.
+  const int share = max(kWideCost, (line + sms - 1) / sms);
   const int left = s.ctas - (line + share - 1) / share;
   const int chunks = max(1, min(a.nchunk, left * s.own_ctas / a.Hkv));
-  const int W = max(kMinOwn, ((all + chunks - 1) / chunks + 15) & ~15);
-  for (int k = 0; k < kPerRow; ++k) {
-    const int b = kPerRow * tid + k;
+  const int W = max(kMinOwn, ((all[0] + chunks - 1) / chunks + 15) & ~15);
+  if (tid == 0) {
+    s.own[a.B] = all[0];
+    s.before[s.groups] = before[s.groups] = total;
+    *s.totals = Totals{total, share, all[2], W};
+  }
+  __syncthreads();
+  int run = v[0];
+#pragma unroll
+  for (int k = 0; k < kPlanRows; ++k) {
+    const int b = kPlanRows * tid + k;
     if (b >= a.B) continue;
     s.own[b] = run;
     for (int c = (run + W - 1) / W; c * W < run + own[k]; ++c) s.own_first[c] = b;
     run += own[k];
-  }
-  if (tid == 0) {
-    s.own[a.B] = all;
-    s.before[s.groups] = total;
-    *s.totals = Totals{total, share, all_rows, W};
-  }
-  __syncthreads();
-  if (tid < s.ctas) {
-    const int at = tid * share;
-    int g = -1;
-    if (at < line) {
-      const int x = at % total;
-      int lo = 0, hi = s.groups - 1;  // the last group that starts at or before x: it has a cost
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (before[mid] <= x) lo = mid; else hi = mid - 1;
-      }
-      g = lo;
+    int4 parts = make_int4(0, -1, 0, 0);
+    if (group[k] >= 0) {
+      const int g = group[k], i = b - start[g];
+      const GroupUnits u(start[g + 1] - start[g], len[g], s.seqs);
+      const int unit = i / (2 * s.seqs);
+      const bool wide = unit < u.full || u.rest > s.seqs;
+      parts.x = before[g] + unit * u.full_cost + kUnitCost;
+      parts.y = (u.tiles - 1) * (wide ? kWideCost : kTurnCost);
+      parts.z = stored[g] + i * a.G;
+      parts.w = wide ? 0 : u.rest * a.G;
     }
-    s.cta_group[tid] = g;
+    s.row_parts[b] = parts;
+  }
+  for (int c = tid; c < s.ctas; c += THREADS) {
+    const int lo = c * share, hi = min(lo + share, line);
+    Unit u{};
+    if (lo < hi) {
+      const int h = lo / total, g = last_at_most(before, 0, s.groups - 1, lo - h * total);
+      u = unit_at(lo, hi, c, h, g, make_int4(start[g], start[g + 1] - start[g], len[g], stored[g]), before[g], total,
+                  all[2], s.seqs, a.G);
+    } else {
+      u.next = hi;
+    }
+    s.first[c] = u;
   }
 }
 
 // ----------------------------------------------------------------- prefix
-// The units of all KV heads, head by head, group by group, stand end to end
-// on a line, each unit's start charged kUnitCost, each key tile its cost; CTA
-// c takes [c share, (c + 1) share), a tile by where it starts. A unit's rows
-// as CTA c sees them are stored from row c 256 + R on, with R the rows that
-// the units before it store: no two of them overlap, since a unit stores 256
-// rows at most, and neither does one unit's with another's in one CTA.
-struct Unit {
-  int h, b0, n;     // KV head, sequences [b0, b0 + n)
-  int lead, len;    // row of the block table, shared positions
-  bool wide;        // two row tiles, each against all keys; else one, its key tiles in turn by two warpgroups
-  int t0, t1;       // this CTA's key tiles
-  int64_t row0;     // first stored row
-};
-
+// A CTA's units, one after the other.
 struct Walk {
   const SharedArgs& s;
   const int Hkv, G;
-  const int cost, rows;
-  int lo, hi, g;
-  __device__ __forceinline__ Walk(const SharedArgs& s_, int Hkv_, int G_)
-      : s(s_), Hkv(Hkv_), G(G_), cost(s_.totals->cost), rows(s_.totals->rows) {
-    const int share = s.totals->share;
-    lo = blockIdx.x * share;
-    hi = min(lo + share, cost * Hkv);
-    g = s.cta_group[blockIdx.x];
+  Unit u;
+  bool begun = false;
+  __device__ __forceinline__ Walk(const SharedArgs& s_, int Hkv_, int G_) : s(s_), Hkv(Hkv_), G(G_) {
+    u = s.first[blockIdx.x];
   }
-  __device__ __forceinline__ bool next(Unit& u) {
-    while (lo < hi) {
-      const int h = lo / cost, x = lo - h * cost;
-      if (x < s.before[g] || x >= s.before[g + 1]) {
-        int l = 0, r = s.groups - 1;
-        while (l < r) {
-          const int mid = (l + r + 1) >> 1;
-          if (s.before[mid] <= x) l = mid; else r = mid - 1;
-        }
-        g = l;
-      }
-      const int4 gr = s.group[g];
-      const GroupUnits gu(gr.y, gr.z, s.seqs);
-      const int y = x - s.before[g], k = min(y / gu.full_cost, gu.full);
-      const bool whole = k < gu.full;
-      const int base = lo - y + k * gu.full_cost, end = base + (whole ? gu.full_cost : gu.rest_cost);
-      u.wide = whole || gu.rest > s.seqs;
-      const int w = u.wide ? 2 : 1;
-      const int first = base + kUnitCost, stop = min(hi, end);
-      u.t0 = (max(lo, first) - first + w - 1) / w;
-      u.t1 = (max(stop, first) - first + w - 1) / w;
-      lo = stop;
-      if (u.t0 >= u.t1) continue;
-      u.h = h;
-      u.b0 = gr.x + k * 2 * s.seqs;
-      u.n = whole ? 2 * s.seqs : gu.rest;
-      u.lead = gr.x;
-      u.len = gr.z;
-      u.row0 = (int64_t)blockIdx.x * 2 * kRows + (int64_t)h * rows + gr.w + k * 2 * s.seqs * G;
-      return true;
+  __device__ __forceinline__ bool next() {
+    if (!begun) {
+      begun = true;
+      if (u.t0 < u.t1) return true;
+    }
+    const Totals t = *s.totals;
+    const int hi = min(((int)blockIdx.x + 1) * t.share, t.cost * Hkv);
+    while (u.next < hi) {
+      const int lo = u.next, h = lo / t.cost, x = lo - h * t.cost;
+      int g = u.group;
+      if (x < s.before[g] || x >= s.before[g + 1]) g = last_at_most(s.before, 0, s.groups - 1, x);
+      u = unit_at(lo, hi, blockIdx.x, h, g, s.group[g], s.before[g], t.cost, t.rows, s.seqs, G);
+      if (u.t0 < u.t1) return true;
     }
     return false;
   }
@@ -389,8 +430,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     }
     int T = 0, act = 0;
     bool ok = true;
-    Unit u;
-    for (Walk w(s, a.Hkv, a.G); ok && w.next(u); ++act) {
+    Walk w(s, a.Hkv, a.G);
+    const Unit& u = w.u;
+    for (; ok && w.next(); ++act) {
       if (keys) {
         if (act >= 1 && !__all_sync(0xffffffffu, mbar_wait(bar(B_QE), (act - 1) & 1, abort))) break;
         if (lane == 0) {
@@ -432,8 +474,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const uint32_t id_qk = idesc_f16(BF16, kRows, kKeys, false), id_pv = idesc_f16(BF16, kRows, D, true);
     int T = 0, act = 0, n_s[2] = {0, 0}, n_o[2] = {0, 0};
     bool ok = true;
-    Unit u;
-    for (Walk w(s, a.Hkv, a.G); ok && w.next(u);) {
+    Walk w(s, a.Hkv, a.G);
+    const Unit& u = w.u;
+    for (; ok && w.next();) {
       const int nt = u.t1 - u.t0, steps = u.wide ? nt : (nt + 1) / 2;
       if (!mbar_wait(bar(B_QF), act & 1, abort)) break;
       for (int j = 0; ok && j <= steps; ++j) {
@@ -499,8 +542,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const float mult = qk_mult > 0.f ? qk_mult : 1.f;
     int T = 0, n_s = 0, n_o = 0;
     bool ok = true;
-    Unit u;
-    for (Walk w(s, a.Hkv, a.G); ok && w.next(u); T += u.t1 - u.t0) {
+    Walk w(s, a.Hkv, a.G);
+    const Unit& u = w.u;
+    for (; ok && w.next(); T += u.t1 - u.t0) {
       const int i = (u.wide ? x * s.seqs : 0) + bl;
       const bool row_ok = bl < s.seqs && i < u.n;
       const int lim = row_ok ? s.row_shared[u.b0 + i] : 0;
@@ -637,7 +681,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       // x = 1 stores behind x = 0: other rows in a wide unit, the same ones of other keys else
-      const int64_t at = u.row0 + (x == 0 ? 0 : (int64_t)(u.wide ? s.seqs : u.n) * a.G) + bl * a.G + g;
+      const int64_t at = u.row0 + (x == 0 ? 0 : (u.wide ? s.seqs : u.n) * a.G) + bl * a.G + g;
       if (done == 0) {
         if (row_ok) s.part_lse[at] = neg_inf();
         continue;
@@ -681,7 +725,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 // not share: chunk c of KV head h, list positions [c W, (c + 1) W).
 template <int D, int KV, bool Q_BF16, int NT>
 __device__ __forceinline__ void own_chunk(const DecodeArgs& a, const SharedArgs& s, unsigned char* dsm) {
-  const int c = blockIdx.x, h = blockIdx.y;
+  const int c = blockIdx.x / a.Hkv, h = blockIdx.x - c * a.Hkv;  // the CTAs without work come last
   const int W = s.totals->own_share, all = s.own[a.B];
   int lo = c * W;
   if (lo >= all) return;
@@ -712,60 +756,61 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) shared_own_kernel(c
   __threadfence();  // nothing is read from a cache line older than the plan
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   own_chunk<D, KV, Q_BF16, NT>(a, s, dsm);
-  if (blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ merge
 // CTA (h, b, z): the parts of one (KV head, sequence), a slice of its query
-// heads. Thread = (query head, 4 dims), eight parts at once; parts of the
-// shared positions first, then of the sequence's own.
+// heads; parts of the shared positions first, then of the sequence's own.
+// Thread = (query head, 4 dims), eight parts at once; where the heads leave
+// threads over, `ways` of them share a row's parts and are joined in shared
+// memory. Where the parts are is known from the plan, before the wait.
 template <int D, bool Q_BF16>
 __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const DecodeArgs a, const SharedArgs s) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int kBatch = 8, kLanes = D / 4, kSlots = kThreads / kLanes;
+  __shared__ float4 s_acc[kSlots][kLanes];
+  __shared__ float2 s_ml[kSlots];
+  __threadfence();  // as in the own kernel
   const int h = blockIdx.x, b = blockIdx.y;
   const int gn = a.G / (int)gridDim.z, g0 = (int)blockIdx.z * gn;
   int pos;
-  const int L = seq_len(a, b, pos), shared = s.row_shared[b];
-  if (pos < 0 && h == 0 && blockIdx.z == 0 && threadIdx.x == 0) flag_error(a.err, RBLN_DEVERR_SEQ_RANGE);
+  const int L = seq_len(a, b, pos);
   const Totals tot = *s.totals;
-  // own parts
+  const int4 rp = s.row_parts[b];
   const int pb = s.own[b] + kSegCost, pe = s.own[b + 1];
   const int cf = pb / tot.own_share, own = pe > pb ? (pe - 1) / tot.own_share - cf + 1 : 0;
-  if (L > 0 && shared == 0 && own == 1) return;  // one chunk held the whole sequence and wrote the output
   const int64_t own_slot = ((int64_t)h * (a.nchunk + a.B) + cf + b) * a.G;
-  // shared parts: of every CTA that has tiles of the row's unit, two where x = 0, 1 took the tiles in turn
-  int parts = 0, turn = 1;
-  int64_t row = 0, turn_rows = 0;
-  if (shared > 0) {
-    const int grp = s.row_group[b];
-    const int4 gr = s.group[grp];
-    const GroupUnits gu(gr.y, gr.z, s.seqs);
-    const int k = (b - gr.x) / (2 * s.seqs), i = b - gr.x - k * 2 * s.seqs;
-    const bool wide = k < gu.full || gu.rest > s.seqs;
-    const int first = h * tot.cost + s.before[grp] + k * gu.full_cost + kUnitCost;
-    const int c0 = first / tot.share, c1 = (first + (gu.tiles - 1) * (wide ? 2 : 1)) / tot.share;
-    turn = wide ? 1 : 2;
-    turn_rows = (int64_t)gu.rest * a.G;
-    parts = (c1 - c0 + 1) * turn;
-    row = (int64_t)c0 * 2 * kRows + (int64_t)h * tot.rows + gr.w + (k * 2 * s.seqs + i) * a.G;
+  // of every CTA that has tiles of the row's unit, two where x = 0, 1 took the tiles in turn
+  int parts = 0;
+  const int turn = rp.w > 0 ? 1 : 0;
+  int64_t row = 0;
+  if (rp.y >= 0) {
+    const int first = h * tot.cost + rp.x, c0 = first / tot.share, c1 = (first + rp.y) / tot.share;
+    parts = (c1 - c0 + 1) << turn;
+    row = (int64_t)c0 * 2 * kRows + h * tot.rows + rp.z;
   }
-  constexpr int kBatch = 8;
-  for (int idx = threadIdx.x; idx < gn * (D / 4); idx += kThreads) {
-    const int g = g0 + idx / (D / 4), d4 = (idx % (D / 4)) * 4;
+  const int slot = threadIdx.x / kLanes, d4 = (threadIdx.x % kLanes) * 4;
+  const int ways = max(1, kSlots / gn), way = slot % ways;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (pos < 0 && h == 0 && blockIdx.z == 0 && threadIdx.x == 0) flag_error(a.err, RBLN_DEVERR_SEQ_RANGE);
+  if (L > 0 && rp.y < 0 && own == 1) return;  // one chunk held the whole sequence and wrote the output
+  for (int r0 = 0; r0 < gn; r0 += kSlots / ways) {
+    const int r = r0 + slot / ways, g = g0 + r;
+    const bool live = r < gn;
     float M = neg_inf(), S = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < parts + own; s0 += kBatch) {
+    for (int s0 = way; live && s0 < parts + own; s0 += kBatch * ways) {
       float l[kBatch];
       float4 o[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const int i = s0 + u;
+        const int i = s0 + u * ways;
         l[u] = neg_inf();
         o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i >= parts + own) continue;
         const bool mine = i >= parts;
         const int64_t at = mine ? own_slot + (int64_t)(i - parts) * a.G + g
-                                : row + (int64_t)(i / turn) * 2 * kRows + (i % turn) * turn_rows + g;
+                                : row + (int64_t)(i >> turn) * 2 * kRows + (i & turn) * rp.w + g;
         l[u] = (mine ? a.part_lse : s.part_lse)[at];
         o[u] = *reinterpret_cast<const float4*>((mine ? a.part_o : s.part_o) + at * D + d4);
       }
@@ -786,6 +831,26 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const DecodeArgs
           acc.x += w * o[u].x; acc.y += w * o[u].y; acc.z += w * o[u].z; acc.w += w * o[u].w;
         }
     }
+    if (ways > 1) {  // the same for all threads; then one pass takes all rows
+      s_acc[slot][d4 / 4] = acc;
+      if (d4 == 0) s_ml[slot] = make_float2(M, S);
+      __syncthreads();
+      if (way != 0) return;
+      float top = neg_inf();
+      for (int w = 0; w < ways; ++w) top = fmaxf(top, s_ml[slot + w].x);
+      S = 0.f;
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < ways; ++w) {
+        const float2 ml = s_ml[slot + w];
+        if (ml.x == neg_inf()) continue;
+        const float f = exp2_approx(ml.x - top);
+        const float4 o = s_acc[slot + w][d4 / 4];
+        S += f * ml.y;
+        acc.x += f * o.x; acc.y += f * o.y; acc.z += f * o.z; acc.w += f * o.w;
+      }
+      M = top;
+    }
+    if (!live) continue;
     // no position visible: NaN, as softmax of all -inf
     const float inv = (M == neg_inf()) ? pos_nan() : 1.f / S;
     acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
@@ -827,12 +892,14 @@ int launch(const DecodeArgs& a, const SharedArgs& s, const Maps& m, cudaStream_t
   if (!allow_smem(reinterpret_cast<const void*>(shared_prefix_kernel<D, QB>), PrefixSmem<D>::ALLOC, prefix_smem) ||
       !allow_smem(reinterpret_cast<const void*>(shared_own_kernel<D, KV, QB, NT>), segment_smem<D, NT>(), own_smem))
     return RBLN_ERR_LAUNCH;
-  int rc = launch_after(shared_plan_kernel, dim3(1), kPlanThreads, 0, st, a, s);
+  int rc = a.B <= 256 * kPlanRows && s.groups <= 256
+               ? launch_after(shared_plan_kernel<256>, dim3(1), 256, 0, st, a, s)
+               : launch_after(shared_plan_kernel<1024>, dim3(1), 1024, 0, st, a, s);
   if (rc == RBLN_OK && s.groups > 0)
     rc = launch_after(shared_prefix_kernel<D, QB>, dim3(s.ctas), kPrefixThreads, PrefixSmem<D>::ALLOC, st, m.q, m.k, m.v,
                       a, s);
   if (rc == RBLN_OK)
-    rc = launch_after(shared_own_kernel<D, KV, QB, NT>, dim3(a.nchunk, a.Hkv), kThreads, segment_smem<D, NT>(), st, a, s);
+    rc = launch_after(shared_own_kernel<D, KV, QB, NT>, dim3(a.nchunk * a.Hkv), kThreads, segment_smem<D, NT>(), st, a, s);
   if (rc == RBLN_OK)
     rc = launch_after(shared_merge_kernel<D, QB>, dim3(a.Hkv, a.B, merge_head_split(a.Hkv, a.B, a.G)), kThreads, 0, st, a,
                       s);
@@ -847,7 +914,7 @@ int launch_any(const DecodeArgs& a, const SharedArgs& s, const Maps& m, bool bf1
 
 struct Plan {
   int nchunk;
-  size_t totals, row_shared, row_group, own, own_first, group, before, cta_group, own_o, own_lse, part_o, part_lse, total;
+  size_t totals, row_shared, row_parts, own, own_first, group, before, first, own_o, own_lse, part_o, part_lse, total;
 };
 
 int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s, Plan* pl) {
@@ -864,7 +931,7 @@ int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s
     return RBLN_ERR_UNSUPPORTED;
   // the units' line, with room for a CTA's share past its end, is counted in 32 bits
   const int64_t units = (int64_t)p->batch / (2 * (kRows / p->group)) + s->num_groups + 1;
-  if (p->num_kv_heads * units * (2 * tiles_of(p->max_blocks * p->block_size) + kUnitCost) >= (int64_t)1 << 30)
+  if (p->num_kv_heads * units * (kWideCost * tiles_of(p->max_blocks * p->block_size) + kUnitCost) >= (int64_t)1 << 30)
     return RBLN_ERR_UNSUPPORTED;
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -881,12 +948,12 @@ int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s
   const size_t part = N == 0 ? 0 : (size_t)kSms * 2 * kRows + 2 * B * p->group * p->num_kv_heads;
   pl->totals = take(sizeof(Totals));
   pl->row_shared = take(B * sizeof(int));
-  pl->row_group = take(B * sizeof(int));
+  pl->row_parts = take(B * sizeof(int4));
   pl->own = take((B + 1) * sizeof(int));
   pl->own_first = take(pl->nchunk * sizeof(int));
   pl->group = take(N * sizeof(int4));
   pl->before = take((N + 1) * sizeof(int));
-  pl->cta_group = take(kSms * sizeof(int));
+  pl->first = take(kSms * sizeof(Unit));
   pl->own_o = take(own * D * sizeof(float));
   pl->own_lse = take(own * sizeof(float));
   pl->part_o = take(part * D * sizeof(float));
@@ -966,14 +1033,16 @@ int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t*
   x.seqs = kRows / p->group;
   x.ctas = kSms;
   x.own_ctas = p->group <= 8 ? 4 : 2;
+  x.tile_us = 0.56f;
+  x.own_us = p->head_dim == 128 ? 0.0092f : 0.0067f;
   x.totals = reinterpret_cast<Totals*>(ws + pl.totals);
   x.row_shared = reinterpret_cast<int*>(ws + pl.row_shared);
-  x.row_group = reinterpret_cast<int*>(ws + pl.row_group);
+  x.row_parts = reinterpret_cast<int4*>(ws + pl.row_parts);
   x.own = reinterpret_cast<int*>(ws + pl.own);
   x.own_first = reinterpret_cast<int*>(ws + pl.own_first);
   x.group = reinterpret_cast<int4*>(ws + pl.group);
   x.before = reinterpret_cast<int*>(ws + pl.before);
-  x.cta_group = reinterpret_cast<int*>(ws + pl.cta_group);
+  x.first = reinterpret_cast<Unit*>(ws + pl.first);
   x.part_o = reinterpret_cast<float*>(ws + pl.part_o);
   x.part_lse = reinterpret_cast<float*>(ws + pl.part_lse);
   Maps m;
