@@ -52,7 +52,8 @@ struct Totals {
   int cost;       // of all units of a KV head
   int share;      // of a CTA of the prefix kernel
   int rows;       // rows that a KV head's units store for each CTA that works on them
-  int own_share;  // own positions of a CTA
+  int own;        // own positions of a KV head, with what the sequences' starts are charged
+  int own_share;  // of a CTA
 };
 
 // A CTA's key tiles of a unit of the prefix kernel.
@@ -63,6 +64,15 @@ struct Unit {
   int t0, t1;     // this CTA's key tiles
   int row0;       // first stored row
   int group, next;  // the group, and where on the line the CTA goes on
+};
+
+// A CTA's segment of a sequence's own positions.
+struct OwnPart {
+  int h, b;
+  int t0, t1;      // positions
+  int append;      // the new token's position is among them
+  int whole;       // they are all that the sequence sees
+  long long next;  // where on the line the CTA goes on
 };
 
 struct SharedArgs {
@@ -79,7 +89,6 @@ struct SharedArgs {
   int4* row_parts;     // [B] the row's unit: its first key tile on KV head 0's line, the last one less that (-1: no
                        // shared part), its stored row, the stored rows of x = 0 where tiles are taken in turn
   int* own;            // [B + 1] prefix of the rows' own positions, as in the decode kernels
-  int* own_first;      // [nchunk] first sequence of a chunk
   int4* group;         // [groups] first sequence, sequences, shared positions, stored rows before it
   int* before;         // [groups + 1] cost of the groups before it, in one KV head
   Unit* first;         // [ctas] the first unit of each CTA, t0 = t1: none
@@ -132,6 +141,26 @@ __device__ __forceinline__ Unit unit_at(int lo, int hi, int cta, int h, int g, i
   u.row0 = cta * 2 * kRows + h * head_rows + gr.w + k * 2 * seqs * G;
   u.group = g;
   return u;
+}
+
+// The own positions of all KV heads and sequences, each sequence's rounded up
+// to 16 and its start charged kSegCost, stand on another line, cut likewise:
+// the segment at `lo` of a CTA that ends at `hi`, in sequence b, whose range
+// of a KV head's line is [from, to).
+__device__ __forceinline__ OwnPart own_at(long long lo, long long hi, int h, int b, int all, int from, int to, int shared,
+                                          int seq, int span) {
+  const long long pb = (long long)h * all + from + kSegCost, pe = (long long)h * all + to;
+  const long long seg_lo = max(lo, pb), seg_hi = min(hi, pe);
+  OwnPart p;
+  p.h = h;
+  p.b = b;
+  p.next = seg_hi;
+  const int L = seq < 0 ? 0 : min(seq + 1, span);
+  p.t0 = shared + (int)(seg_lo - pb);
+  p.t1 = seg_lo < seg_hi ? min(shared + (int)(seg_hi - pb), L) : p.t0;
+  p.append = seq < span && seq >= p.t0 && seq < p.t1;
+  p.whole = seg_lo == pb && seg_hi == pe && shared == 0;
+  return p;
 }
 
 // ------------------------------------------------------------------- plan
@@ -247,13 +276,13 @@ __global__ void __launch_bounds__(THREADS, 1) shared_plan_kernel(const DecodeArg
   // The line is below 2^30 long. A share of a wide tile at least: so every
   // CTA between a unit's first and last has a tile of it.
   const int share = max(kWideCost, (line + sms - 1) / sms);
-  const int left = s.ctas - (line + share - 1) / share;
-  const int chunks = max(1, min(a.nchunk, left * s.own_ctas / a.Hkv));
-  const int W = max(kMinOwn, ((all[0] + chunks - 1) / chunks + 15) & ~15);
+  const int own_ctas = (s.ctas - (line + share - 1) / share) * s.own_ctas;
+  const long long own_line = (long long)all[0] * a.Hkv;
+  const int W = max(kMinOwn, (int)((own_line + own_ctas - 1) / own_ctas + 15) & ~15);
   if (tid == 0) {
     s.own[a.B] = all[0];
     s.before[s.groups] = before[s.groups] = total;
-    *s.totals = Totals{total, share, all[2], W};
+    *s.totals = Totals{total, share, all[2], all[0], W};
   }
   __syncthreads();
   int run = v[0];
@@ -262,7 +291,6 @@ __global__ void __launch_bounds__(THREADS, 1) shared_plan_kernel(const DecodeArg
     const int b = kPlanRows * tid + k;
     if (b >= a.B) continue;
     s.own[b] = run;
-    for (int c = (run + W - 1) / W; c * W < run + own[k]; ++c) s.own_first[c] = b;
     run += own[k];
     int4 parts = make_int4(0, -1, 0, 0);
     if (group[k] >= 0) {
@@ -722,26 +750,37 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 
 // -------------------------------------------------------------------- own
 // As paged_decode_balanced_kernel, over the positions that a sequence does
-// not share: chunk c of KV head h, list positions [c W, (c + 1) W).
+// not share; segments of CTA c in sequence b of KV head h are stored in slot
+// c + h B + b.
 template <int D, int KV, bool Q_BF16, int NT>
 __device__ __forceinline__ void own_chunk(const DecodeArgs& a, const SharedArgs& s, unsigned char* dsm) {
-  const int c = blockIdx.x / a.Hkv, h = blockIdx.x - c * a.Hkv;  // the CTAs without work come last
-  const int W = s.totals->own_share, all = s.own[a.B];
-  int lo = c * W;
-  if (lo >= all) return;
-  const int hi = min(lo + W, all);
-  for (int b = s.own_first[c]; b < a.B && lo < hi; ++b) {
-    const int pb = s.own[b] + kSegCost, pe = s.own[b + 1];  // b's own positions: [pb, pe)
-    const int seg_hi = min(hi, pe), seg_lo = max(lo, pb);
-    lo = seg_hi;
-    if (seg_lo >= seg_hi) continue;  // only the charge of b's start falls in this chunk
-    const int shared = s.row_shared[b];
-    int pos;
-    const int L = seq_len(a, b, pos);
-    const int t0 = shared + seg_lo - pb, t1 = min(shared + seg_hi - pb, L);
-    const bool append = pos < a.span && pos >= t0 && pos < t1;
-    decode_segment<D, KV, Q_BF16, NT, false>(a, dsm, b, h, t0, t1, append, seg_lo == pb && seg_hi == pe && shared == 0,
-                                             ((int64_t)h * (a.nchunk + a.B) + c + b) * a.G);
+  __shared__ int before[kWarps];
+  const int c = blockIdx.x;
+  const int W = s.totals->own_share, all = s.totals->own;
+  const long long lo = (long long)c * W, hi = min(lo + W, (long long)all * a.Hkv);
+  if (lo >= hi) return;
+  // the sequence at `lo`: all threads count those that start at or before it
+  const int h = (int)(lo / all), x = (int)(lo - (long long)h * all);
+  int n = 0;
+  for (int i = threadIdx.x; i < a.B; i += kThreads) n += s.own[i] <= x;
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) before[threadIdx.x >> 5] = n;
+  __syncthreads();
+  OwnPart p;
+  p.h = h;
+  p.b = before[0] + before[1] + before[2] + before[3] - 1;
+  p.next = lo;
+  while (true) {
+    p = own_at(p.next, hi, p.h, p.b, all, s.own[p.b], s.own[p.b + 1], s.row_shared[p.b], a.seq[p.b * a.seq_stride],
+               a.span);
+    if (p.t0 < p.t1)
+      decode_segment<D, KV, Q_BF16, NT, false>(a, dsm, p.b, p.h, p.t0, p.t1, p.append, p.whole,
+                                               ((int64_t)c + (int64_t)p.h * a.B + p.b) * a.G);
+    if (p.next >= hi) return;
+    if (++p.b == a.B) {
+      p.b = 0;
+      ++p.h;
+    }
   }
 }
 
@@ -778,8 +817,9 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const DecodeArgs
   const Totals tot = *s.totals;
   const int4 rp = s.row_parts[b];
   const int pb = s.own[b] + kSegCost, pe = s.own[b + 1];
-  const int cf = pb / tot.own_share, own = pe > pb ? (pe - 1) / tot.own_share - cf + 1 : 0;
-  const int64_t own_slot = ((int64_t)h * (a.nchunk + a.B) + cf + b) * a.G;
+  const long long own0 = (long long)h * tot.own + pb;
+  const int cf = (int)(own0 / tot.own_share), own = pe > pb ? (int)((own0 + pe - pb - 1) / tot.own_share) - cf + 1 : 0;
+  const int64_t own_slot = ((int64_t)cf + (int64_t)h * a.B + b) * a.G;
   // of every CTA that has tiles of the row's unit, two where x = 0, 1 took the tiles in turn
   int parts = 0;
   const int turn = rp.w > 0 ? 1 : 0;
@@ -899,7 +939,7 @@ int launch(const DecodeArgs& a, const SharedArgs& s, const Maps& m, cudaStream_t
     rc = launch_after(shared_prefix_kernel<D, QB>, dim3(s.ctas), kPrefixThreads, PrefixSmem<D>::ALLOC, st, m.q, m.k, m.v,
                       a, s);
   if (rc == RBLN_OK)
-    rc = launch_after(shared_own_kernel<D, KV, QB, NT>, dim3(a.nchunk * a.Hkv), kThreads, segment_smem<D, NT>(), st, a, s);
+    rc = launch_after(shared_own_kernel<D, KV, QB, NT>, dim3(s.ctas * s.own_ctas), kThreads, segment_smem<D, NT>(), st, a, s);
   if (rc == RBLN_OK)
     rc = launch_after(shared_merge_kernel<D, QB>, dim3(a.Hkv, a.B, merge_head_split(a.Hkv, a.B, a.G)), kThreads, 0, st, a,
                       s);
@@ -913,8 +953,8 @@ int launch_any(const DecodeArgs& a, const SharedArgs& s, const Maps& m, bool bf1
 }
 
 struct Plan {
-  int nchunk;
-  size_t totals, row_shared, row_parts, own, own_first, group, before, first, own_o, own_lse, part_o, part_lse, total;
+  int own_ctas;
+  size_t totals, row_shared, row_parts, own, group, before, first, own_o, own_lse, part_o, part_lse, total;
 };
 
 int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s, Plan* pl) {
@@ -939,10 +979,9 @@ int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s
     at += (n + 255) / 256 * 256;
     return start;
   };
-  // one wave of CTAs of the own positions: 4 an SM for up to 8 query heads a KV head, 2 above
-  pl->nchunk = std::max(1, kSms * (p->group <= 8 ? 4 : 2) / p->num_kv_heads);
+  pl->own_ctas = p->group <= 8 ? 4 : 2;  // an SM holds
   const size_t B = p->batch, N = s->num_groups, D = p->head_dim;
-  const size_t own = (size_t)p->num_kv_heads * (pl->nchunk + B) * p->group;
+  const size_t own = (size_t)(kSms * pl->own_ctas + p->num_kv_heads * B) * p->group;
   // a row of the shared parts is stored once for each CTA that has keys of it: 256 rows a CTA at most, and a unit's
   // rows (twice them where its key tiles are taken in turn) for its first one
   const size_t part = N == 0 ? 0 : (size_t)kSms * 2 * kRows + 2 * B * p->group * p->num_kv_heads;
@@ -950,7 +989,6 @@ int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s
   pl->row_shared = take(B * sizeof(int));
   pl->row_parts = take(B * sizeof(int4));
   pl->own = take((B + 1) * sizeof(int));
-  pl->own_first = take(pl->nchunk * sizeof(int));
   pl->group = take(N * sizeof(int4));
   pl->before = take((N + 1) * sizeof(int));
   pl->first = take(kSms * sizeof(Unit));
@@ -1023,7 +1061,6 @@ int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t*
   a.B = p->batch; a.Hkv = p->num_kv_heads; a.G = p->group; a.num_blocks = p->num_blocks;
   a.bs = p->block_size; a.span = p->max_blocks * p->block_size;
   a.err = p->error_flags;
-  a.nchunk = pl.nchunk;
   a.part_o = reinterpret_cast<float*>(ws + pl.own_o);
   a.part_lse = reinterpret_cast<float*>(ws + pl.own_lse);
   SharedArgs x{};
@@ -1032,14 +1069,13 @@ int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t*
   x.lens = s->shared_lens;
   x.seqs = kRows / p->group;
   x.ctas = kSms;
-  x.own_ctas = p->group <= 8 ? 4 : 2;
+  x.own_ctas = pl.own_ctas;
   x.tile_us = 0.56f;
   x.own_us = p->head_dim == 128 ? 0.0092f : 0.0067f;
   x.totals = reinterpret_cast<Totals*>(ws + pl.totals);
   x.row_shared = reinterpret_cast<int*>(ws + pl.row_shared);
   x.row_parts = reinterpret_cast<int4*>(ws + pl.row_parts);
   x.own = reinterpret_cast<int*>(ws + pl.own);
-  x.own_first = reinterpret_cast<int*>(ws + pl.own_first);
   x.group = reinterpret_cast<int4*>(ws + pl.group);
   x.before = reinterpret_cast<int*>(ws + pl.before);
   x.first = reinterpret_cast<Unit*>(ws + pl.first);
