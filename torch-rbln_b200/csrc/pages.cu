@@ -107,34 +107,44 @@ __global__ void __launch_bounds__(256) paged_kv_fork_kernel(const ForkArgs a) {
 // ------------------------------------------------------------------- free
 constexpr int kFreeRows = 16;
 
-// refs[id] goes down by n, never below 0: what a decrement takes too much it
-// puts back, and no decrement sees a count above the true one.
-__device__ __forceinline__ void give_back(int* refs, int64_t id, int n) {
-  const int old = atomicSub(refs + id, n);
-  if (old < n) atomicAdd(refs + id, n - max(old, 0));
-}
-
-// CTA (x, y): 16 rows of 256 columns, a thread a column. Forks of one parent
-// hold the same page in a column: a run of equal entries is one atomic.
+// CTA (x, y): 16 rows of 256 columns, a thread a column, all its loads at
+// once. Forks of one parent hold the same page in a column: a run of equal
+// entries is one atomic. A count goes down by n, never below 0: what a
+// decrement takes too much it puts back, and none sees a count above the true
+// one.
 __global__ void __launch_bounds__(256) paged_kv_free_kernel(const Table t, const Lengths keep, int span) {
   const int col = blockIdx.y * 256 + threadIdx.x;
   if (col >= t.cols) return;
-  const int r0 = blockIdx.x * kFreeRows, r1 = min(r0 + kFreeRows, t.rows);
-  int64_t run = -1;
-  int n = 0;
-  for (int r = r0; r < r1; ++r) {
-    if ((int64_t)col * t.bs < length_of(keep, r, span)) continue;
-    const int64_t id = entry(t, r, col);
-    store_index(t.ids, t.dtype, r * t.s_row + col * t.s_col, -1);
-    if (!is_page(t, id)) continue;
-    if (id != run) {
-      if (n) give_back(t.refs, run, n);
-      run = id;
-      n = 0;
+  const int r0 = blockIdx.x * kFreeRows;
+  int64_t id[kFreeRows];
+#pragma unroll
+  for (int i = 0; i < kFreeRows; ++i) id[i] = r0 + i < t.rows ? entry(t, r0 + i, col) : -1;
+  bool gone[kFreeRows];
+#pragma unroll
+  for (int i = 0; i < kFreeRows; ++i)
+    gone[i] = r0 + i < t.rows && (int64_t)col * t.bs >= length_of(keep, r0 + i, span);
+  int page[kFreeRows], n[kFreeRows];  // runs: the page, how many entries end here
+  int last = -1, run = 0;
+#pragma unroll
+  for (int i = 0; i < kFreeRows; ++i) {
+    if (gone[i] && id[i] != -1) store_index(t.ids, t.dtype, (int64_t)(r0 + i) * t.s_row + col * t.s_col, -1);
+    const int p = gone[i] && is_page(t, id[i]) ? (int)id[i] : -1;
+    const bool same = p == last;
+    page[i] = last;
+    n[i] = p < 0 || same ? 0 : run;  // a page behind another one ends that one's run
+    if (p >= 0) {
+      run = same ? run + 1 : 1;
+      last = p;
     }
-    ++n;
   }
-  if (n) give_back(t.refs, run, n);
+  int old[kFreeRows + 1];
+#pragma unroll
+  for (int i = 0; i < kFreeRows; ++i) old[i] = n[i] > 0 ? atomicSub(t.refs + page[i], n[i]) : 0;
+  old[kFreeRows] = run > 0 ? atomicSub(t.refs + last, run) : 0;
+#pragma unroll
+  for (int i = 0; i < kFreeRows; ++i)
+    if (old[i] < n[i]) atomicAdd(t.refs + page[i], n[i] - max(old[i], 0));
+  if (old[kFreeRows] < run) atomicAdd(t.refs + last, run - max(old[kFreeRows], 0));
 }
 
 // --------------------------------------------------------------- planning
@@ -308,6 +318,73 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_kv_reserve_kernel(const
   }
 }
 
+constexpr int kSmallEntries = kPlanThreads;  // one a thread
+constexpr int kSmallPages = 64 * kPlanThreads;
+constexpr int kSlots = 2 * kSmallEntries;    // of the table of shared pages, a power of two
+
+// The same for one entry a thread: one CTA, in which an entry is looked up
+// once, and what the entries share is in shared memory. Three dependent
+// reads (length, entry, count) beside the search for free pages.
+__global__ void __launch_bounds__(kPlanThreads, 1) paged_kv_reserve_small_kernel(const ReserveArgs a) {
+  __shared__ int key[kSlots], here[kSlots], last[kSlots];  // shared pages of this call's entries
+  __shared__ int given[kSmallEntries];
+  const int i = threadIdx.x, n = (int)a.entries;
+  Want w{};
+  if (i < n) w = want_of(a, i);
+  for (int k = i; k < kSlots; k += kPlanThreads) {
+    key[k] = here[k] = last[k] = -1;
+  }
+  for (int b = i; b < a.t.rows; b += kPlanThreads) {
+    const int seq = length_of(a.seq, b, a.span);
+    a.granted[b] = seq < 0 ? 0 : (int)min((int64_t)a.fresh_tokens, (int64_t)a.span - seq);
+  }
+  const int p_per = (a.t.num_blocks + kPlanThreads - 1) / kPlanThreads;
+  const int p0 = min(i * p_per, a.t.num_blocks), p1 = min(p0 + p_per, a.t.num_blocks);
+  uint64_t free_mask = 0;  // p_per <= 64
+#pragma unroll 8
+  for (int p = p0; p < p1; ++p) free_mask |= (uint64_t)(a.t.refs[p] <= 0) << (p - p0);
+  const int count = w.page ? a.t.refs[w.id] : 0;
+  const bool held = count > 1;
+  __syncthreads();
+  int slot = 0;
+  if (held) {
+    slot = (int)(((uint32_t)w.id * 2654435761u) >> 16) & (kSlots - 1);
+    while (true) {  // at most as many pages as threads: half of the slots
+      const int was = atomicCAS(key + slot, -1, (int)w.id);
+      if (was == -1 || was == (int)w.id) break;
+      slot = (slot + 1) & (kSlots - 1);
+    }
+    atomicAdd(here + slot, 1);  // from -1
+    atomicMax(last + slot, i);
+  }
+  __syncthreads();
+  const bool keeps = held && here[slot] + 1 >= count && last[slot] == i;
+  const bool need = w.want && (!w.page || (held && !keeps));
+  int all_need, all_unused;
+  const int rank = block_before(need, &all_need);
+  int page_rank = block_before(__popcll(free_mask), &all_unused);
+  for (uint64_t m = free_mask; m && page_rank < all_need; m &= m - 1) given[page_rank++] = p0 + __ffsll((long long)m) - 1;
+  here[i] = here[i + kSmallEntries] = 0;  // from here on: entries that moved
+  __syncthreads();
+  const bool got = need && rank < all_unused;
+  if (got) {
+    const int page = given[rank];
+    store_index(a.t.ids, a.t.dtype, w.row * a.t.s_row + w.col * a.t.s_col, page);
+    a.t.refs[page] = 1;
+    if (held) {
+      atomicSub(a.t.refs + w.id, 1);
+      atomicAdd(here + slot, 1);
+    }
+  }
+  const bool copies = got && held && w.seq > w.col * a.t.bs;
+  int all_copies;
+  const int move = block_before(copies, &all_copies);  // its barriers order the counts in `here`, too
+  if (copies) a.moves[move] = Move{(int)w.id, given[rank], w.seq - w.col * a.t.bs};
+  if (i == 0) *a.count = all_copies;
+  if (w.want && !got && !(w.page && count - (held ? here[slot] : 0) <= 1))
+    atomicMin(a.granted + w.row, max(w.col * a.t.bs - w.seq, 0));
+}
+
 struct CompactArgs {
   int* refs;
   int num_blocks, bs;
@@ -327,15 +404,24 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_kv_compact_kernel(const
   const int threads = gridDim.x * kPlanThreads, g = blockIdx.x * kPlanThreads + threadIdx.x;
   const int64_t p_per = ((int64_t)a.num_blocks + threads - 1) / threads;
   const int p0 = (int)min(g * p_per, (int64_t)a.num_blocks), p1 = (int)min(p0 + p_per, (int64_t)a.num_blocks);
+  // this thread's pages in use, kept as bits where 64 hold them
+  uint64_t mask = 0;
+  const bool bits = p_per <= 64;
   int used = 0, cta_used, live;
-  for (int p = p0; p < p1; ++p) used += a.refs[p] > 0;
-  int before = block_before(used, &cta_used);
+#pragma unroll 8
+  for (int p = p0; p < p1; ++p) {
+    const bool in = a.refs[p] > 0;
+    used += in;
+    if (bits) mask |= (uint64_t)in << (p - p0);
+  }
+  auto in_use = [&](int p) { return bits ? (mask >> (p - p0)) & 1 : a.refs[p] > 0; };
+  block_before(used, &cta_used);
   if (threadIdx.x == 0) a.ctas[2 * blockIdx.x] = cta_used;
   cluster_sync();
   ctas_before(a.ctas, 0, &live);
   int holes = 0, movers = 0, n;
   for (int p = p0; p < p1; ++p) {
-    const bool in = a.refs[p] > 0;
+    const bool in = in_use(p);
     holes += p < live && !in;
     movers += p >= live && in;
   }
@@ -348,7 +434,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) paged_kv_compact_kernel(const
   hole += ctas_before(ctas, 0, &all);
   mover += ctas_before(ctas, 1, &all);
   for (int p = p0; p < p1; ++p) {
-    const bool in = a.refs[p] > 0;
+    const bool in = in_use(p);
     if (p < live && !in) a.dst[hole++] = p;
     if (p >= live && in) a.src[mover++] = p;
     a.moved[p] = in ? p : -1;
@@ -662,7 +748,12 @@ int rbln_paged_kv_reserve(const rbln_pages_params_t* p, int32_t new_tokens, int3
   a.take = reinterpret_cast<int*>(ws + w.take);
   a.moves = reinterpret_cast<Move*>(ws + w.moves);
   a.entries = entries;
-  rc = launch_plan(paged_kv_reserve_kernel, plan_ctas(std::max<int64_t>(entries, p->batch), p->num_blocks), stream, a);
+  if (entries <= kSmallEntries && p->num_blocks <= kSmallPages) {
+    paged_kv_reserve_small_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+    rc = launched();
+  } else {
+    rc = launch_plan(paged_kv_reserve_kernel, plan_ctas(std::max<int64_t>(entries, p->batch), p->num_blocks), stream, a);
+  }
   if (rc != RBLN_OK || entries == 0) return rc;
   return launch_copies(p, a.moves, a.count, p->batch, nullptr, stream);
 }
