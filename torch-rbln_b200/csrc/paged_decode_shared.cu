@@ -575,14 +575,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     for (; ok && w.next(); T += u.t1 - u.t0) {
       const int i = (u.wide ? x * s.seqs : 0) + bl;
       const bool row_ok = bl < s.seqs && i < u.n;
-      const int lim = row_ok ? s.row_shared[u.b0 + i] : 0;
+      // rows that are none are not masked: nothing reads what they give
+      const int lim = row_ok ? s.row_shared[u.b0 + i] : u.len + kKeys;
+      const bool rows = __any_sync(0xffffffffu, row_ok);  // a warp without any only keeps the barriers' count
       float m_run = neg_inf(), l_run = 0.f;
       int done = 0;
-      for (int t = u.t0 + (u.wide ? 0 : x); t < u.t1; t += u.wide ? 1 : 2, ++done) {
-        // keys in blocks outside the pool
+      const int step = u.wide ? 1 : 2;
+      // keys in blocks outside the pool: looked up a tile ahead
+      auto none_of = [&](int t) {
         int row;
-        const bool none = block_of(u, t, row) == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < u.len;
+        return t < u.t1 && block_of(u, t, row) == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < u.len;
+      };
+      int t = u.t0 + (u.wide ? 0 : x);
+      bool none = none_of(t);
+      for (; t < u.t1; t += step, ++done) {
         const uint32_t bad = __ballot_sync(0xffffffffu, none);
+        none = none_of(t + step);
         if (!__all_sync(0xffffffffu, mbar_wait(bar(B_SF + x), n_s & 1, abort))) {
           ok = false;
           break;
@@ -590,6 +598,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         ++n_s;
         tc_fence_after();
         __syncwarp();
+       if (rows) {
         float xv[kKeys];
         {
           uint32_t r0[32], r1[32], r2[32], r3[32];
@@ -683,6 +692,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           tmem_st16(t_s(x) + lane_off + c * 16, pk);
         }
         tmem_wait_st();
+       }
         // rows of V behind the shared positions may hold anything: zeros
         // before the probabilities are released (in a wide unit by x = 0,
         // whose product comes first)
