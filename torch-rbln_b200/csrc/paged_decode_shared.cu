@@ -6,17 +6,17 @@
 //
 // The softmax over a union of positions is joined from its parts: part i
 // gives O_i = sum_t e^{s_t - m_i} v_t / l_i and lse_i = m_i + log l_i, and
-// O = sum_i e^{lse_i} O_i / sum_i e^{lse_i}. Four launches, each a
+// O = sum_i e^{lse_i} O_i / sum_i e^{lse_i}. Three launches, each a
 // programmatic dependent of the one before:
-//  * shared_plan_kernel (one CTA): every row's group, the units of work and
-//    where each CTA starts in them;
-//  * shared_prefix_kernel (tcgen05): the query heads of a KV head of up to
-//    2 x 128 rows of a group against the shared keys, so that the tensor
-//    cores work on rows that a batch without a shared prefix would bring one
-//    by one, and a key is read once for them;
-//  * shared_own_kernel: each sequence's own positions with the decode
-//    kernels' segments (mma.sync, one sequence and KV head at a time), and
-//    the append of the new token;
+//  * shared_prefix_kernel (tcgen05, one CTA an SM): first the plan, made by
+//    every CTA for itself: the rows' groups, the units of work, where each CTA
+//    starts in them, how many SMs this kernel takes. Then the query heads of a
+//    KV head of up to 2 x 128 rows of a group against the shared keys, so that
+//    the tensor cores work on rows that a batch without a shared prefix would
+//    bring one by one, and a key is read once for them;
+//  * shared_own_kernel, beside it on the other SMs: each sequence's own
+//    positions with the decode kernels' segments (mma.sync, one sequence and
+//    KV head at a time), and the append of the new token;
 //  * shared_merge_kernel: the parts of every row.
 
 #include <algorithm>
@@ -31,7 +31,6 @@ namespace {
 using namespace sm100;
 
 constexpr int kMaxBatch = 4096, kMaxGroups = 1024;  // what the plan's CTA takes
-constexpr int kPlanRows = 4;          // rows a thread of the plan
 constexpr int kKeys = 128;            // keys a tile
 constexpr int kRows = 128;            // query rows a tile
 constexpr int kPanel = 128 * 128;     // bytes: 128 rows of 64 elements
@@ -89,9 +88,6 @@ struct SharedArgs {
   int4* row_parts;     // [B] the row's unit: its first key tile on KV head 0's line, the last one less that (-1: no
                        // shared part), its stored row, the stored rows of x = 0 where tiles are taken in turn
   int* own;            // [B + 1] prefix of the rows' own positions, as in the decode kernels
-  int4* group;         // [groups] first sequence, sequences, shared positions, stored rows before it
-  int* before;         // [groups + 1] cost of the groups before it, in one KV head
-  Unit* first;         // [ctas] the first unit of each CTA, t0 = t1: none
   float* part_o;       // parts of the shared positions, see unit_at
   float* part_lse;
 };
@@ -206,73 +202,90 @@ __device__ __forceinline__ int last_at_most(const int* at, int lo, int hi, int x
   return lo;
 }
 
-// One CTA of 256 threads for up to 1024 rows and 256 groups, else of 1024.
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS, 1) shared_plan_kernel(const DecodeArgs a, const SharedArgs s) {
-  constexpr int GROUPS = THREADS;
-  __shared__ int start[GROUPS + 1], before[GROUPS + 1], len[GROUPS], stored[GROUPS];
-  pdl_enter();
-  const int tid = threadIdx.x;
-  int cut[2], seq[kPlanRows];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) cut[k] = 2 * tid + k <= s.groups ? min(max(s.starts[2 * tid + k], 0), a.B) : 0;
-#pragma unroll
-  for (int k = 0; k < kPlanRows; ++k)
-    seq[k] = kPlanRows * tid + k < a.B ? a.seq[(kPlanRows * tid + k) * a.seq_stride] : -1;
-  const int mine = tid < s.groups ? min(max(s.lens[tid], 0), a.span) : 0;
+// What a CTA of the prefix kernel knows of the plan.
+struct PlanSmem {
+  int start[kMaxGroups + 1], before[kMaxGroups + 1];  // first sequence; cost of the groups before it, in one KV head
+  int len[kMaxGroups], stored[kMaxGroups];            // shared positions; rows that the groups before it store
+  Totals totals;
+  Unit first, at[kPrefixThreads / 32];  // of this CTA; where each warp is
+  __device__ __forceinline__ int4 group(int g) const {
+    return make_int4(start[g], len[g] > 0 ? start[g + 1] - start[g] : 0, len[g], stored[g]);
+  }
+};
+
+// The plan, made by every CTA of the prefix kernel for itself: that takes less
+// time than a launch of its own. What the other kernels read is stored by all
+// of them, a row by one. own, group: scratch for all rows.
+__device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs& s, PlanSmem& P, int* own, short* group) {
+  constexpr int T = kPrefixThreads, PG = (kMaxGroups + T) / T;  // starts a thread
+  const int tid = threadIdx.x, cta = blockIdx.x;
   // the groups' starts, none before the one before it
-  cut[1] = max(cut[0], cut[1]);
-  int top[1] = {cut[1]}, most[1];
-  scan_before<THREADS, true>(top, most);
+  int cut[PG], top[1] = {0}, most[1];
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (2 * tid + k <= s.groups) start[2 * tid + k] = max(cut[k], top[0]);
-  len[tid] = mine;
-  stored[tid] = 0;
+  for (int k = 0; k < PG; ++k) {
+    const int g = PG * tid + k;
+    if (g <= s.groups) top[0] = max(top[0], min(max(s.starts[g], 0), a.B));
+    cut[k] = top[0];
+    if (g < s.groups) {
+      P.len[g] = min(max(s.lens[g], 0), a.span);
+      P.stored[g] = 0;
+    }
+  }
+  scan_before<T, true>(top, most);
+#pragma unroll
+  for (int k = 0; k < PG; ++k)
+    if (PG * tid + k <= s.groups) P.start[PG * tid + k] = max(cut[k], top[0]);
   __syncthreads();
   // rows: group, shared positions, own positions
-  int own[kPlanRows], group[kPlanRows], shared[kPlanRows], sum = 0;
-#pragma unroll
-  for (int k = 0; k < kPlanRows; ++k) {
-    const int b = kPlanRows * tid + k;
-    own[k] = 0;
-    group[k] = -1;
-    shared[k] = 0;
-    if (b >= a.B) continue;
-    const int g = last_at_most(start, -1, s.groups, b);
-    if (g >= 0 && g < s.groups && len[g] > 0 && seq[k] >= len[g]) {
-      group[k] = g;
-      shared[k] = len[g];
-      stored[g] = 1;  // some row of it has a shared part
-    }
-    const int L = seq[k] < 0 ? 0 : min(seq[k] + 1, a.span);
-    own[k] = ((L - shared[k] + 15) & ~15) + kSegCost;
-    sum += own[k];
-    s.row_shared[b] = shared[k];
+  for (int b = tid; b < a.B; b += T) {
+    const int seq = a.seq[b * a.seq_stride], g = last_at_most(P.start, -1, s.groups, b);
+    int shared = 0;
+    if (g >= 0 && g < s.groups && seq >= P.len[g]) shared = P.len[g];
+    if (shared > 0) P.stored[g] = 1;  // some row of the group has a shared part
+    const int L = seq < 0 ? 0 : min(seq + 1, a.span);
+    own[b] = ((L - shared + 15) & ~15) + kSegCost;
+    group[b] = (short)(shared > 0 ? g : -1);
   }
   __syncthreads();
   // own positions before this thread's rows; cost and stored rows of the groups before this thread's
-  int n = 0;
-  if (tid < s.groups && stored[tid]) n = start[tid + 1] - start[tid];
-  const GroupUnits gu(n, n > 0 ? mine : 0, s.seqs);
-  int v[3] = {sum, gu.full * gu.full_cost + gu.rest_cost,
-              (2 * s.seqs * gu.full + (gu.rest > s.seqs ? gu.rest : 2 * gu.rest)) * a.G};
-  int all[3];
-  scan_before<THREADS, false>(v, all);
-  const int total = all[1];
-  if (tid < s.groups) {
-    before[tid] = s.before[tid] = v[1];
-    stored[tid] = v[2];
-    len[tid] = n > 0 ? mine : 0;
-    s.group[tid] = make_int4(start[tid], n, n > 0 ? mine : 0, v[2]);
+  const int per = (a.B + T - 1) / T, b0 = min(per * tid, a.B), b1 = min(b0 + per, a.B);
+  int v[3] = {0, 0, 0}, all[3], cost[PG], rows[PG];
+  for (int b = b0; b < b1; ++b) v[0] += own[b];
+#pragma unroll
+  for (int k = 0; k < PG; ++k) {
+    const int g = PG * tid + k;
+    cost[k] = rows[k] = 0;
+    if (g < s.groups && P.stored[g]) {
+      const GroupUnits u(P.start[g + 1] - P.start[g], P.len[g], s.seqs);
+      cost[k] = u.full * u.full_cost + u.rest_cost;
+      rows[k] = (2 * s.seqs * u.full + (u.rest > s.seqs ? u.rest : 2 * u.rest)) * a.G;
+    }
+    v[1] += cost[k];
+    v[2] += rows[k];
+  }
+  scan_before<T, false>(v, all);
+  for (int b = b0, run = v[0]; b < b1; ++b) {
+    const int n = own[b];
+    own[b] = run;
+    run += n;
+  }
+#pragma unroll
+  for (int k = 0; k < PG; ++k) {
+    const int g = PG * tid + k;
+    if (g >= s.groups) break;
+    if (cost[k] == 0) P.len[g] = 0;
+    P.before[g] = v[1];
+    P.stored[g] = v[2];
+    v[1] += cost[k];
+    v[2] += rows[k];
   }
   // The SMs are divided so that both kernels end together: with m of N SMs,
   //   line / m + late = own / (N - m),
   // `late` what the first has to do besides, all in microseconds.
-  const int line = total * a.Hkv;
-  const float N = (float)s.ctas, late = 4.f, P = line * s.tile_us, O = (float)all[0] * a.Hkv * s.own_us;
-  const float half = 0.5f * (late * N - P - O);
-  const int sms = min(s.ctas - 2, max(1, (int)((half + sqrtf(half * half + late * P * N)) / late + 0.5f)));
+  const int total = all[1], line = total * a.Hkv;
+  const float N = (float)s.ctas, late = 4.f, p = line * s.tile_us, o = (float)all[0] * a.Hkv * s.own_us;
+  const float half = 0.5f * (late * N - p - o);
+  const int sms = min(s.ctas - 2, max(1, (int)((half + sqrtf(half * half + late * p * N)) / late + 0.5f)));
   // The line is below 2^30 long. A share of a wide tile at least: so every
   // CTA between a unit's first and last has a tile of it.
   const int share = max(kWideCost, (line + sms - 1) / sms);
@@ -280,72 +293,71 @@ __global__ void __launch_bounds__(THREADS, 1) shared_plan_kernel(const DecodeArg
   const long long own_line = (long long)all[0] * a.Hkv;
   const int W = max(kMinOwn, (int)((own_line + own_ctas - 1) / own_ctas + 15) & ~15);
   if (tid == 0) {
-    s.own[a.B] = all[0];
-    s.before[s.groups] = before[s.groups] = total;
-    *s.totals = Totals{total, share, all[2], all[0], W};
+    P.before[s.groups] = total;
+    P.totals = Totals{total, share, all[2], all[0], W};
+    if (cta == 0) {
+      *s.totals = P.totals;
+      s.own[a.B] = all[0];
+    }
   }
   __syncthreads();
-  int run = v[0];
-#pragma unroll
-  for (int k = 0; k < kPlanRows; ++k) {
-    const int b = kPlanRows * tid + k;
-    if (b >= a.B) continue;
-    s.own[b] = run;
-    run += own[k];
+  for (int b = cta + tid * s.ctas; b < a.B; b += T * s.ctas) {
+    const int g = group[b];
     int4 parts = make_int4(0, -1, 0, 0);
-    if (group[k] >= 0) {
-      const int g = group[k], i = b - start[g];
-      const GroupUnits u(start[g + 1] - start[g], len[g], s.seqs);
-      const int unit = i / (2 * s.seqs);
+    if (g >= 0) {
+      const int i = b - P.start[g], unit = i / (2 * s.seqs);
+      const GroupUnits u(P.start[g + 1] - P.start[g], P.len[g], s.seqs);
       const bool wide = unit < u.full || u.rest > s.seqs;
-      parts.x = before[g] + unit * u.full_cost + kUnitCost;
+      parts.x = P.before[g] + unit * u.full_cost + kUnitCost;
       parts.y = (u.tiles - 1) * (wide ? kWideCost : kTurnCost);
-      parts.z = stored[g] + i * a.G;
+      parts.z = P.stored[g] + i * a.G;
       parts.w = wide ? 0 : u.rest * a.G;
     }
+    s.own[b] = own[b];
+    s.row_shared[b] = g >= 0 ? P.len[g] : 0;
     s.row_parts[b] = parts;
   }
-  for (int c = tid; c < s.ctas; c += THREADS) {
-    const int lo = c * share, hi = min(lo + share, line);
+  if (tid == T - 1) {
+    const int lo = cta * share, hi = min(lo + share, line);
     Unit u{};
+    u.next = hi;
     if (lo < hi) {
-      const int h = lo / total, g = last_at_most(before, 0, s.groups - 1, lo - h * total);
-      u = unit_at(lo, hi, c, h, g, make_int4(start[g], start[g + 1] - start[g], len[g], stored[g]), before[g], total,
-                  all[2], s.seqs, a.G);
-    } else {
-      u.next = hi;
+      const int h = lo / total, g = last_at_most(P.before, 0, s.groups - 1, lo - h * total);
+      u = unit_at(lo, hi, cta, h, g, P.group(g), P.before[g], total, all[2], s.seqs, a.G);
     }
-    s.first[c] = u;
+    P.first = u;
   }
 }
 
 // ----------------------------------------------------------------- prefix
-// A CTA's units, one after the other.
-struct Walk {
-  const SharedArgs& s;
-  const int Hkv, G;
-  Unit u;
-  bool begun = false;
-  __device__ __forceinline__ Walk(const SharedArgs& s_, int Hkv_, int G_) : s(s_), Hkv(Hkv_), G(G_) {
-    u = s.first[blockIdx.x];
+// Goes on to the CTA's next unit with key tiles: u, which is P.first at first
+// (begun false). One thread of a role does this for all of it, in shared
+// memory, so that the unit takes no registers of the softmax's.
+__device__ __forceinline__ bool next_unit(const PlanSmem& P, const SharedArgs& s, const DecodeArgs& a, Unit& u,
+                                          bool begun) {
+  if (!begun) {
+    u = P.first;
+    if (u.t0 < u.t1) return true;
   }
-  __device__ __forceinline__ bool next() {
-    if (!begun) {
-      begun = true;
-      if (u.t0 < u.t1) return true;
-    }
-    const Totals t = *s.totals;
-    const int hi = min(((int)blockIdx.x + 1) * t.share, t.cost * Hkv);
-    while (u.next < hi) {
-      const int lo = u.next, h = lo / t.cost, x = lo - h * t.cost;
-      int g = u.group;
-      if (x < s.before[g] || x >= s.before[g + 1]) g = last_at_most(s.before, 0, s.groups - 1, x);
-      u = unit_at(lo, hi, blockIdx.x, h, g, s.group[g], s.before[g], t.cost, t.rows, s.seqs, G);
-      if (u.t0 < u.t1) return true;
-    }
-    return false;
+  const int cost = P.totals.cost, hi = min(((int)blockIdx.x + 1) * P.totals.share, cost * a.Hkv);
+  while (u.next < hi) {
+    const int lo = u.next, h = lo / cost, x = lo - h * cost;
+    int g = u.group;
+    if (x < P.before[g] || x >= P.before[g + 1]) g = last_at_most(P.before, 0, s.groups - 1, x);
+    u = unit_at(lo, hi, blockIdx.x, h, g, P.group(g), P.before[g], cost, P.totals.rows, s.seqs, a.G);
+    if (u.t0 < u.t1) return true;
   }
-};
+  return false;
+}
+// The same for all lanes of a warp.
+__device__ __forceinline__ bool warp_next_unit(const PlanSmem& P, const SharedArgs& s, const DecodeArgs& a, Unit& u,
+                                               bool begun) {
+  __syncwarp();
+  bool more = false;
+  if ((threadIdx.x & 31) == 0) more = next_unit(P, s, a, u, begun);
+  __syncwarp();
+  return __shfl_sync(0xffffffffu, (int)more, 0) != 0;
+}
 
 template <int D>
 struct PrefixSmem {
@@ -358,7 +370,10 @@ struct PrefixSmem {
   static constexpr int BAR = V + STAGES * TILE;
   static constexpr int TMEM = BAR + 32 * 8;
   static constexpr int ABORT = TMEM + 8;
-  static constexpr int TOTAL = ABORT + 8 + 1024;
+  static constexpr int PLAN = ABORT + 8;
+  static constexpr int TOTAL = PLAN + (int)sizeof(PlanSmem) + 1024;
+  // the plan's scratch lies where the queries come later
+  static_assert(2 * TILE >= kMaxBatch * 6, "scratch of the plan");
   // above half an SM's shared memory: one CTA an SM, which takes all of its TMEM
   static constexpr int ALLOC = TOTAL > 120 * 1024 ? TOTAL : 120 * 1024;
 };
@@ -417,25 +432,30 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // The set-up above overlaps the plan. Behind it the own kernel may start on
-  // the SMs that are left: it needs the plan and what ran before, all complete
-  // here, and not this grid.
+  // The set-up above overlaps what ran before. Behind the plan the own kernel
+  // may start on the SMs that are left: it needs the plan and what ran before,
+  // and not the rest of this grid.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  PlanSmem& P = *reinterpret_cast<PlanSmem*>(sgen + L::PLAN);
+  make_plan(a, s, P, reinterpret_cast<int*>(sgen + L::Q), reinterpret_cast<short*>(sgen + L::Q + kMaxBatch * 4));
   __threadfence();
+  fence_proxy_async_smem();  // the scratch is written by copies next
+  __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  Unit& u = P.at[warp];
   const uint32_t tmem = *tmem_slot;
   auto t_s = [&](int x) { return tmem + x * 128; };
   auto t_o = [&](int x) { return tmem + 256 + x * 128; };
   const int rpb = min(a.bs, kKeys), boxes = kKeys / rpb;  // <= 16 boxes a tile
   // lane's box of key tile t: its block (num_blocks: none), first row there
-  auto block_of = [&](const Unit& u, int t, int& row) {
+  auto block_of = [&](int lead, int len, int t, int& row) {
     int blk = a.num_blocks;
     row = 0;
     const int key = t * kKeys + lane * rpb;
-    if (lane < boxes && key < u.len) {
+    if (lane < boxes && key < len) {
       const int bi = key / a.bs;
       row = key - bi * a.bs;
-      const int64_t v = load_index(a.bt, a.bt_dtype, u.lead * a.bt_stride + bi);
+      const int64_t v = load_index(a.bt, a.bt_dtype, lead * a.bt_stride + bi);
       if (v >= 0 && v < a.num_blocks) blk = (int)v;
     }
     return blk;
@@ -458,9 +478,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     }
     int T = 0, act = 0;
     bool ok = true;
-    Walk w(s, a.Hkv, a.G);
-    const Unit& u = w.u;
-    for (; ok && w.next(); ++act) {
+    for (; ok && warp_next_unit(P, s, a, u, act > 0); ++act) {
       if (keys) {
         if (act >= 1 && !__all_sync(0xffffffffu, mbar_wait(bar(B_QE), (act - 1) & 1, abort))) break;
         if (lane == 0) {
@@ -470,10 +488,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
               tma_load_4d(sbase + L::Q + x * L::TILE + p * kPanel, &tm_q, bar(B_QF), p * 64, 0, u.h, u.b0 + x * s.seqs);
         }
       }
-      for (int t = u.t0; t < u.t1; ++t, ++T) {
+      const int t1 = u.t1, lead = u.lead, len = u.len, h = u.h;
+      for (int t = u.t0; t < t1; ++t, ++T) {
         int row;
-        const int blk = block_of(u, t, row);
-        if (keys && blk == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < u.len)
+        const int blk = block_of(lead, len, t, row);
+        if (keys && blk == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < len)
           flag_error(a.err, RBLN_DEVERR_BLOCK_ID_RANGE);
         const int st = T % ST;
         if (T >= ST && !__all_sync(0xffffffffu, mbar_wait(bar(empty + st), (T / ST - 1) & 1, abort))) {
@@ -484,7 +503,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         __syncwarp();
         if (lane < boxes)
           for (int p = 0; p < NP; ++p)
-            tma_load_4d(ring + st * L::TILE + p * kPanel + lane * rpb * 128, tm, bar(full + st), p * 64, row, u.h, blk);
+            tma_load_4d(ring + st * L::TILE + p * kPanel + lane * rpb * 128, tm, bar(full + st), p * 64, row, h, blk);
       }
     }
     if (*abort) {
@@ -502,14 +521,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const uint32_t id_qk = idesc_f16(BF16, kRows, kKeys, false), id_pv = idesc_f16(BF16, kRows, D, true);
     int T = 0, act = 0, n_s[2] = {0, 0}, n_o[2] = {0, 0};
     bool ok = true;
-    Walk w(s, a.Hkv, a.G);
-    const Unit& u = w.u;
-    for (; ok && w.next();) {
-      const int nt = u.t1 - u.t0, steps = u.wide ? nt : (nt + 1) / 2;
+    for (; ok && next_unit(P, s, a, u, act > 0);) {
+      const bool wide = u.wide;
+      const int nt = u.t1 - u.t0, steps = wide ? nt : (nt + 1) / 2;
       if (!mbar_wait(bar(B_QF), act & 1, abort)) break;
       for (int j = 0; ok && j <= steps; ++j) {
         for (int x = 0; x < 2; ++x) {
-          const int i1 = u.wide ? j : 2 * j + x, i0 = u.wide ? j - 1 : i1 - 2;
+          const int i1 = wide ? j : 2 * j + x, i0 = wide ? j - 1 : i1 - 2;
           if (j >= 1 && i0 < nt) {
             const int Ti = T + i0, st = Ti % ST;
             if (!mbar_wait(bar(B_VF + st), (Ti / ST) & 1, abort) ||
@@ -528,7 +546,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
               umma_commit(bar(B_OF + x));
               ++n_o[x];
             }
-            if (!u.wide || x == 1) umma_commit(bar(B_VE + st));
+            if (!wide || x == 1) umma_commit(bar(B_VE + st));
           }
           if (i1 < nt) {
             const int Ti = T + i1, st = Ti % ST;
@@ -537,15 +555,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
               break;
             }
             tc_fence_after();
-            const uint32_t qb = sbase + L::Q + (u.wide ? x * L::TILE : 0), kb = sbase + L::K + st * L::TILE;
+            const uint32_t qb = sbase + L::Q + (wide ? x * L::TILE : 0), kb = sbase + L::K + st * L::TILE;
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
               umma_f16_ss(t_s(x), sw128_desc(qb + (kk >> 2) * kPanel + (kk & 3) * 32, 16, 1024),
                           sw128_desc(kb + (kk >> 2) * kPanel + (kk & 3) * 32, 16, 1024), id_qk, kk > 0 ? 1u : 0u);
             umma_commit(bar(B_SF + x));
             ++n_s[x];
-            if (!u.wide || x == 1) umma_commit(bar(B_KE + st));
-            if (i1 == nt - 1 && (!u.wide || x == 1)) umma_commit(bar(B_QE));
+            if (!wide || x == 1) umma_commit(bar(B_KE + st));
+            if (i1 == nt - 1 && (!wide || x == 1)) umma_commit(bar(B_QE));
           }
         }
       }
@@ -570,25 +588,25 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const float mult = qk_mult > 0.f ? qk_mult : 1.f;
     int T = 0, n_s = 0, n_o = 0;
     bool ok = true;
-    Walk w(s, a.Hkv, a.G);
-    const Unit& u = w.u;
-    for (; ok && w.next(); T += u.t1 - u.t0) {
-      const int i = (u.wide ? x * s.seqs : 0) + bl;
+    for (bool begun = false; ok && warp_next_unit(P, s, a, u, begun); begun = true, T += u.t1 - u.t0) {
+      const bool wide = u.wide;
+      const int t1 = u.t1, len = u.len, lead = u.lead;
+      const int i = (wide ? x * s.seqs : 0) + bl;
       const bool row_ok = bl < s.seqs && i < u.n;
       // rows that are none are not masked: nothing reads what they give
-      const int lim = row_ok ? s.row_shared[u.b0 + i] : u.len + kKeys;
+      const int lim = row_ok ? s.row_shared[u.b0 + i] : len + kKeys;
       const bool rows = __any_sync(0xffffffffu, row_ok);  // a warp without any only keeps the barriers' count
       float m_run = neg_inf(), l_run = 0.f;
       int done = 0;
-      const int step = u.wide ? 1 : 2;
+      const int step = wide ? 1 : 2;
       // keys in blocks outside the pool: looked up a tile ahead
       auto none_of = [&](int t) {
         int row;
-        return t < u.t1 && block_of(u, t, row) == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < u.len;
+        return t < t1 && block_of(lead, len, t, row) == a.num_blocks && lane < boxes && t * kKeys + lane * rpb < len;
       };
-      int t = u.t0 + (u.wide ? 0 : x);
+      int t = u.t0 + (wide ? 0 : x);
       bool none = none_of(t);
-      for (; t < u.t1; t += step, ++done) {
+      for (; t < t1; t += step, ++done) {
         const uint32_t bad = __ballot_sync(0xffffffffu, none);
         none = none_of(t + step);
         if (!__all_sync(0xffffffffu, mbar_wait(bar(B_SF + x), n_s & 1, abort))) {
@@ -696,13 +714,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         // rows of V behind the shared positions may hold anything: zeros
         // before the probabilities are released (in a wide unit by x = 0,
         // whose product comes first)
-        if (t * kKeys + kKeys > u.len && (x == 0 || !u.wide)) {
+        if (t * kKeys + kKeys > len && (x == 0 || !wide)) {
           const int Ti = T + t - u.t0, st = Ti % ST;
           if (!__all_sync(0xffffffffu, mbar_wait(bar(B_VF + st), (Ti / ST) & 1, abort))) {
             ok = false;
             break;
           }
-          if (t * kKeys + r >= u.len) {
+          if (t * kKeys + r >= len) {
             uint8_t* vrow = sgen + L::V + st * L::TILE + r * 128;
 #pragma unroll
             for (int p = 0; p < NP; ++p)
@@ -719,7 +737,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       // x = 1 stores behind x = 0: other rows in a wide unit, the same ones of other keys else
-      const int64_t at = u.row0 + (x == 0 ? 0 : (u.wide ? s.seqs : u.n) * a.G) + bl * a.G + g;
+      const int64_t at = u.row0 + (x == 0 ? 0 : (wide ? s.seqs : u.n) * a.G) + bl * a.G + g;
       if (done == 0) {
         if (row_ok) s.part_lse[at] = neg_inf();
         continue;
@@ -801,7 +819,6 @@ __device__ __forceinline__ void own_chunk(const DecodeArgs& a, const SharedArgs&
 template <int D, int KV, bool Q_BF16, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) shared_own_kernel(const DecodeArgs a, const SharedArgs s) {
   extern __shared__ __align__(16) unsigned char dsm[];
-  if (s.groups == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // there is no prefix kernel
   __threadfence();  // nothing is read from a cache line older than the plan
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   own_chunk<D, KV, Q_BF16, NT>(a, s, dsm);
@@ -938,16 +955,25 @@ int launch(const DecodeArgs& a, const SharedArgs& s, const Maps& m, cudaStream_t
            2 * 128 * kRegsSoftmax + 128 * kRegsOther <= (uint32_t)fa.numRegs * kPrefixThreads;
   }();
   if (!regs_ok) return RBLN_ERR_LAUNCH;
+  // The own kernel starts on SMs that the prefix kernel has just left, with
+  // nearly all of their memory given to shared memory. Its loads in flight
+  // need L1: it asks for the shared memory that its CTAs take and no more
+  // (317 us against 443 beside 32768 shared positions).
+  static SmemOptIn carved;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return RBLN_ERR_LAUNCH;
+  if (carved.bytes[dev].load(std::memory_order_relaxed) == 0) {
+    if (cudaFuncSetAttribute(shared_own_kernel<D, KV, QB, NT>, cudaFuncAttributePreferredSharedMemoryCarveout, 40) !=
+        cudaSuccess)
+      return RBLN_ERR_LAUNCH;
+    carved.bytes[dev].store(1, std::memory_order_relaxed);
+  }
   static SmemOptIn prefix_smem, own_smem;
   if (!allow_smem(reinterpret_cast<const void*>(shared_prefix_kernel<D, QB>), PrefixSmem<D>::ALLOC, prefix_smem) ||
       !allow_smem(reinterpret_cast<const void*>(shared_own_kernel<D, KV, QB, NT>), segment_smem<D, NT>(), own_smem))
     return RBLN_ERR_LAUNCH;
-  int rc = a.B <= 256 * kPlanRows && s.groups <= 256
-               ? launch_after(shared_plan_kernel<256>, dim3(1), 256, 0, st, a, s)
-               : launch_after(shared_plan_kernel<1024>, dim3(1), 1024, 0, st, a, s);
-  if (rc == RBLN_OK && s.groups > 0)
-    rc = launch_after(shared_prefix_kernel<D, QB>, dim3(s.ctas), kPrefixThreads, PrefixSmem<D>::ALLOC, st, m.q, m.k, m.v,
-                      a, s);
+  int rc = launch_after(shared_prefix_kernel<D, QB>, dim3(s.ctas), kPrefixThreads, PrefixSmem<D>::ALLOC, st, m.q,
+                        m.k, m.v, a, s);
   if (rc == RBLN_OK)
     rc = launch_after(shared_own_kernel<D, KV, QB, NT>, dim3(s.ctas * s.own_ctas), kThreads, segment_smem<D, NT>(), st, a, s);
   if (rc == RBLN_OK)
@@ -964,7 +990,7 @@ int launch_any(const DecodeArgs& a, const SharedArgs& s, const Maps& m, bool bf1
 
 struct Plan {
   int own_ctas;
-  size_t totals, row_shared, row_parts, own, group, before, first, own_o, own_lse, part_o, part_lse, total;
+  size_t totals, row_shared, row_parts, own, own_o, own_lse, part_o, part_lse, total;
 };
 
 int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s, Plan* pl) {
@@ -999,9 +1025,6 @@ int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s
   pl->row_shared = take(B * sizeof(int));
   pl->row_parts = take(B * sizeof(int4));
   pl->own = take((B + 1) * sizeof(int));
-  pl->group = take(N * sizeof(int4));
-  pl->before = take((N + 1) * sizeof(int));
-  pl->first = take(kSms * sizeof(Unit));
   pl->own_o = take(own * D * sizeof(float));
   pl->own_lse = take(own * sizeof(float));
   pl->part_o = take(part * D * sizeof(float));
@@ -1080,19 +1103,18 @@ int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t*
   x.seqs = kRows / p->group;
   x.ctas = kSms;
   x.own_ctas = pl.own_ctas;
-  x.tile_us = 0.56f;
-  x.own_us = p->head_dim == 128 ? 0.0092f : 0.0067f;
+  // Measured with both kernels at work: a wide tile 2.3 us, an own position (of up to four CTAs) 9 and 7 ns. From 7.8
+  // to 12 ns the largest case took 409, 385, 385, 366, 371, 379, 392 us, smaller ones the same within a tenth.
+  x.tile_us = 0.58f;
+  x.own_us = p->head_dim == 128 ? 0.0092f : 0.0073f;
   x.totals = reinterpret_cast<Totals*>(ws + pl.totals);
   x.row_shared = reinterpret_cast<int*>(ws + pl.row_shared);
   x.row_parts = reinterpret_cast<int4*>(ws + pl.row_parts);
   x.own = reinterpret_cast<int*>(ws + pl.own);
-  x.group = reinterpret_cast<int4*>(ws + pl.group);
-  x.before = reinterpret_cast<int*>(ws + pl.before);
-  x.first = reinterpret_cast<Unit*>(ws + pl.first);
   x.part_o = reinterpret_cast<float*>(ws + pl.part_o);
   x.part_lse = reinterpret_cast<float*>(ws + pl.part_lse);
   Maps m;
-  if (x.groups > 0) {
+  {
     // queries [B, Hkv, G, D] in boxes of `seqs` sequences of one KV head, rows in order (sequence, query head)
     const uint64_t dims[4] = {(uint64_t)p->head_dim, (uint64_t)p->group, (uint64_t)p->num_kv_heads, (uint64_t)p->batch};
     const uint64_t strides[3] = {(uint64_t)q.q_stride[2] * 2, (uint64_t)q.q_stride[1] * 2, (uint64_t)q.q_stride[0] * 2};

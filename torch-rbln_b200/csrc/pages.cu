@@ -492,6 +492,12 @@ __global__ void __launch_bounds__(kCopyThreads) paged_kv_pages_copy_kernel(const
     const int64_t item = y / a.layers;
     const int layer = (int)(y - item * a.layers);
     const Move m = a.moves[item];
+    float* scale = nullptr;
+    float old = 0.f;
+    if (lane == 0 && a.ks[0] != nullptr) {
+      scale = (part ? a.vs : a.ks)[layer] + h * a.ss_head;
+      old = scale[m.src * a.ss_block];  // on its way while the rows are copied
+    }
     char* base = (part ? a.v : a.k)[layer] + h * a.cs_head;
     const char* from = base + m.src * a.cs_block;
     char* to = base + m.dst * a.cs_block;
@@ -512,10 +518,7 @@ __global__ void __launch_bounds__(kCopyThreads) paged_kv_pages_copy_kernel(const
       for (int u = 0; u < kCopyLoads; ++u)
         if (i0 + 32 * u < vecs) *reinterpret_cast<uint4*>(to + at[u]) = w[u];
     }
-    if (lane == 0 && a.ks[0] != nullptr) {
-      float* s = (part ? a.vs : a.ks)[layer] + h * a.ss_head;
-      s[m.dst * a.ss_block] = s[m.src * a.ss_block];
-    }
+    if (scale != nullptr) scale[m.dst * a.ss_block] = old;
   }
 }
 
