@@ -320,6 +320,39 @@ def test_strided_table_and_lengths(ops):
     assert (base.cpu()[:, 1::2] == 77).all()
 
 
+def test_pool_beyond_32_bits(ops):
+    """Pages at byte offsets that 32 bits do not hold, and more pages than one CTA searches."""
+    D, bs, Hkv = 128, 16, 8
+    blocks = 5 * 2 ** 30 // (Hkv * bs * D * 2)
+    k, v = (torch.empty(blocks, Hkv, 1, bs, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    last = blocks - 1
+    k[last], v[last] = torch.randn_like(k[last]), torch.randn_like(v[last])
+    refs = torch.ones(blocks, dtype=torch.int32, device="cuda")
+    refs[last], refs[blocks - 5] = 2, 0
+    k[blocks - 5], v[blocks - 5] = 0, 0
+    t = torch.full([2, 2], last, dtype=torch.int32, device="cuda")
+    t[:, 1] = -1
+    assert ops.paged_kv_reserve([k], [v], t, dev([7, 7]), refs, bs, 1).tolist() == [1, 1]
+    assert t[:, 0].tolist() == [blocks - 5, last] and refs[blocks - 5] == 1 and refs[last] == 1
+    for c in (k, v):
+        assert torch.equal(c[blocks - 5, :, :, :7], c[last, :, :, :7]) and (c[blocks - 5, :, :, 7:] == 0).all()
+    refs.zero_()
+    refs[last] = 3
+    moved, live = ops.paged_kv_compact([k], [v], t, refs)
+    assert live.item() == 1 and moved[last] == 0 and refs[0] == 3 and refs[last] == 0 and t[1, 0] == 0
+    assert torch.equal(k[0], k[last]) and torch.equal(v[0], v[last])
+
+
+def test_schemas_fakes_and_traces(ops):
+    table, refs = ref.pool(3, 4, [30, 20, 50], 16, 9)
+    t, r, n = table_of(table, 4), dev(refs), dev([30, 20, 50])
+    k, v = ([torch.randn(len(refs), 1, 1, 16, 64).to(torch.bfloat16).cuda() for _ in range(2)] for _ in range(2))
+    torch.library.opcheck(ops.paged_kv_fork.default, (t, n, dev([0, 2, 2]), r, 16))
+    torch.library.opcheck(ops.paged_kv_free.default, (t, n, r, 16))
+    torch.library.opcheck(ops.paged_kv_reserve.default, (k, v, t, n, r, 16, 3))
+    torch.library.opcheck(ops.paged_kv_compact.default, (k, v, t, r))
+
+
 def test_refusals(ops):
     bs = 16
     table, refs = ref.pool(2, 4, [30, 20], bs, 4)

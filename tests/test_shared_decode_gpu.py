@@ -142,6 +142,42 @@ def test_strided_inputs_and_heads_outermost_pools():
     assert torch.equal(y["kcache"].cpu().contiguous().view(torch.int16), x["kcache"].view(torch.int16))
 
 
+def test_cache_rows_longer_than_the_head():
+    """A cache whose last dimension is larger than the queries': its first D elements are the head."""
+    x = ref.inputs(64, 16, BF, 2, 4, 40, [0, 33, 40], [300, 140], [1 + b for b in range(40)])
+    for n in ("kcache", "vcache"):
+        x[n] = torch.cat([x[n], torch.full_like(x[n], float("nan"))], dim=-1).contiguous()
+    ref.check(x)
+
+
+def test_the_most_sequences_and_groups():
+    """4096 sequences in 1024 groups, some empty, some of one sequence, some of many."""
+    sizes = [(i * 7) % 9 for i in range(1023)]
+    sizes.append(4096 - sum(sizes))
+    starts = [sum(sizes[:i]) for i in range(1025)]
+    lens = [(i * 37) % 200 for i in range(1024)]
+    own = [None if b % 11 == 3 else 1 + b % 21 for b in range(4096)]
+    ref.check(ref.inputs(64, 16, BF, 1, 2, 4096, starts, lens, own))
+
+
+def test_pool_beyond_32_bits():
+    """Pages at byte offsets that 32 bits do not hold."""
+    D, bs, Hkv = 128, 16, 8
+    blocks = 5 * 2 ** 30 // (Hkv * bs * D * 2)
+    x = ref.inputs(D, bs, BF, Hkv, 2, 9, [0, 9], [200], [1 + 5 * b for b in range(9)])
+    used = x["kcache"].shape[0]
+    y = ref.gpu(x)
+    for n in ("kcache", "vcache"):
+        big = torch.empty(blocks, Hkv, 1, bs, D, dtype=BF, device="cuda")
+        big[blocks - used:] = y[n]
+        y[n] = big
+    y["block_table"] = torch.where(y["block_table"] >= 0, y["block_table"] + blocks - used, y["block_table"])
+    got = ref.call(y)
+    want, bound = ref.decode(x)
+    ref.within(got, want, bound)
+    assert torch.equal(y["kcache"][blocks - used:].cpu().view(torch.int16), x["kcache"].view(torch.int16))
+
+
 def test_no_sequences():
     x = ref.gpu(ref.inputs(64, 16, BF, 1, 2, 1, [0, 1], [3], [4]))
     for n in ("q", "k", "v", "seq", "block_table"):
@@ -238,6 +274,12 @@ def test_pages_forked_reserved_attended_and_freed():
         seq += 1
     ops.paged_kv_free(rows, torch.zeros_like(seq), r, bs)
     assert (r == 0).all() and (rows == -1).all()
+
+
+def test_schema_fake_and_trace():
+    x = ref.gpu(ref.inputs(64, 16, BF, 2, 4, 4, [0, 4], [40], [3] * 4, poison=False))
+    torch.library.opcheck(torch.ops.rbln_custom_ops.paged_causal_attn_decode_shared.default,
+                          tuple(x[n] for n in ref.ORDER))
 
 
 def test_error_flags():

@@ -794,7 +794,8 @@ rbln_pages_params_t check_pages(const char* op, const at::Tensor& block_table, c
 // One whole number a row of the table, kept alive by the caller.
 at::Tensor check_lengths(const char* op, const char* name, const at::Tensor& lengths_in, const at::Tensor& block_table,
                          rbln_pages_params_t& p) {
-  at::Tensor n = on_device(lengths_in, block_table).reshape({-1});
+  at::Tensor n = on_device(lengths_in, block_table);
+  if (n.dim() != 1) n = n.reshape({-1});
   TORCH_CHECK(is_index(n.scalar_type()), op, ": ", name, " must be int16/int32/int64, got ", n.scalar_type());
   TORCH_CHECK(n.numel() == block_table.size(0), op, ": ", name, " must hold one entry per row, got ",
               lengths_in.sizes(), " for ", block_table.sizes());
@@ -845,6 +846,8 @@ void check_layers(const char* op, at::TensorList kcaches, at::TensorList vcaches
   p.cache_stride[0] = c.stride(0);
   p.cache_stride[1] = c.stride(1);
   p.cache_stride[2] = c.stride(3);
+  ptrs.k.reserve(kcaches.size());
+  ptrs.v.reserve(kcaches.size());
   for (size_t i = 0; i < kcaches.size(); ++i) {
     ptrs.k.push_back(kcaches[i].data_ptr());
     ptrs.v.push_back(vcaches[i].data_ptr());
