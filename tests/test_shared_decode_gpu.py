@@ -192,6 +192,24 @@ def test_same_bits_every_time():
         assert torch.equal(ref.call(x).view(torch.int16), first.view(torch.int16))
 
 
+def test_calls_back_to_back():
+    """Many different calls without a pause, each over the workspace that another left behind: every one gives what
+    it gives alone."""
+    cases = []
+    for i in range(24):
+        D, bs, Hkv, G = (64, 128)[i % 2], (16, 64, 32)[i % 3], (1, 2, 4)[i // 2 % 3], (1, 4, 8, 2)[i // 3 % 4]
+        sizes = [(13, 32, 5)[i % 3]] * (1 + i % 2)
+        starts = [sum(sizes[:j]) for j in range(len(sizes) + 1)]
+        x = ref.inputs(D, bs, BF if i % 4 else F16, Hkv, G, sum(sizes), starts, [(700, 128, 3001)[i // 4 % 3]] * len(sizes),
+                       [1 + (b * 7 + i) % 60 for b in range(sum(sizes))])
+        cases.append((ref.gpu(x), ref.decode(x)))
+    for i in range(12):
+        outs = [ref.call(cases[k][0]) for k in torch.randperm(24, generator=torch.Generator().manual_seed(i)).tolist()]
+        order = torch.randperm(24, generator=torch.Generator().manual_seed(i)).tolist()
+        for k, got in zip(order, outs):
+            ref.within(got, *cases[k][1], f"pass {i}, case {k}")
+
+
 def test_graphs_and_streams():
     """Two captured graphs and eager calls on other streams, interleaved."""
     xs = [ref.inputs(128, 16, BF, 2, 4, 24, [0, 10, 24], [500, 130], [1 + (7 + i) * b % 90 for b in range(24)])

@@ -215,7 +215,8 @@ struct PlanSmem {
 
 // The plan, made by every CTA of the prefix kernel for itself: that takes less
 // time than a launch of its own. What the other kernels read is stored by all
-// of them, a row by one. own, group: scratch for all rows.
+// of them, a row by one; it is not read in this grid, whose CTAs do not wait
+// for one another. own, group: scratch for all rows.
 __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs& s, PlanSmem& P, int* own, short* group) {
   constexpr int T = kPrefixThreads, PG = (kMaxGroups + T) / T;  // starts a thread
   const int tid = threadIdx.x, cta = blockIdx.x;
@@ -594,7 +595,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const int i = (wide ? x * s.seqs : 0) + bl;
       const bool row_ok = bl < s.seqs && i < u.n;
       // rows that are none are not masked: nothing reads what they give
-      const int lim = row_ok ? s.row_shared[u.b0 + i] : len + kKeys;
+      // (a row whose new position is below the shared ones sees none of them)
+      const int lim = !row_ok ? len + kKeys : a.seq[(u.b0 + i) * a.seq_stride] >= len ? len : 0;
       const bool rows = __any_sync(0xffffffffu, row_ok);  // a warp without any only keeps the barriers' count
       float m_run = neg_inf(), l_run = 0.f;
       int done = 0;
