@@ -36,7 +36,7 @@ constexpr int kRows = 128;            // query rows a tile
 constexpr int kPanel = 128 * 128;     // bytes: 128 rows of 64 elements
 constexpr int kPrefixThreads = 384;   // softmax warpgroups 0-3 and 4-7, producers 8 and 10, MMA 9
 constexpr int kSegCost = 128;         // keys charged to the start of a sequence's own part
-constexpr int kMinOwn = 256;          // smallest share of a CTA of own positions
+constexpr int kMinOwn = kSegCost + 16;  // smallest share of a CTA of own positions (256: 16.3 us for four sequences, 14.4)
 constexpr int kSms = 148;
 // What a key tile costs a CTA with two row tiles and with one (whose two
 // warpgroups take the tiles in turn), and a unit's start.
