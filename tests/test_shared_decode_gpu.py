@@ -113,6 +113,29 @@ def test_far_apart_scores():
         ref.check(ref.inputs(128, 16, BF, 2, 4, 40, [0, 40], [1000], [1 + b for b in range(40)], std=std))
 
 
+def test_nan_in_seen_places():
+    """Scores that are all NaN in one CTA's part, or in a row's own, give that row NaN."""
+    for D, bs, G, n in ((128, 16, 4, 40), (64, 64, 2, 5)):
+        x = ref.inputs(D, bs, BF, 2, G, n, [0, n], [6000], [1 + 3 * b for b in range(n)], poison=False)
+        y = {m: c.clone() if isinstance(c, torch.Tensor) else c for m, c in x.items()}
+        x["k"][3] = float("nan")
+        x["q"][n - 1, 1, 0] = float("nan")
+        ref.check(x)
+        y["kcache"][y["block_table"][0, 1024 // bs: 2048 // bs].long(), 1] = float("nan")
+        ref.check(y)
+
+
+def test_groups_given_in_64_bits():
+    x = ref.inputs(64, 16, BF, 1, 4, 6, [0, 6], [64], [16] * 6, poison=False)
+    x["group_starts"], x["shared_lens"] = torch.tensor([-2 ** 40, 2 ** 40]), torch.tensor([2 ** 33])
+    x["seq"][:] = 200  # past the span of 80: all 80 positions are shared
+    y = ref.gpu(x)
+    got = ref.call(y)
+    x["group_starts"], x["shared_lens"] = torch.tensor([0, 6]), torch.tensor([10 ** 6])
+    want, bound = ref.decode(x)
+    ref.within(got, want, bound)
+
+
 def test_long_context():
     """Prefixes whose parts are joined over many CTAs, with few rows and with many."""
     ref.check(ref.inputs(128, 16, BF, 1, 1, 2, [0, 2], [20001], [1, 90]))
@@ -204,8 +227,8 @@ def test_calls_back_to_back():
                        [1 + (b * 7 + i) % 60 for b in range(sum(sizes))])
         cases.append((ref.gpu(x), ref.decode(x)))
     for i in range(12):
-        outs = [ref.call(cases[k][0]) for k in torch.randperm(24, generator=torch.Generator().manual_seed(i)).tolist()]
         order = torch.randperm(24, generator=torch.Generator().manual_seed(i)).tolist()
+        outs = [ref.call(cases[k][0]) for k in order]
         for k, got in zip(order, outs):
             ref.within(got, *cases[k][1], f"pass {i}, case {k}")
 

@@ -762,7 +762,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           for (int e = 0; e < 32; e += 8) store_sector(s.part_o + at * D + c * 32 + e, o + e, inv);
         }
       }
-      if (row_ok) s.part_lse[at] = m_run == neg_inf() ? neg_inf() : m_run + __log2f(l_run);
+      // (a row that saw nothing has l = 0; one whose scores are all NaN stays NaN)
+      if (row_ok) s.part_lse[at] = l_run == 0.f ? neg_inf() : m_run + __log2f(l_run);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_OE + x));
@@ -804,7 +805,7 @@ __device__ __forceinline__ void own_chunk(const DecodeArgs& a, const SharedArgs&
     p = own_at(p.next, hi, p.h, p.b, all, s.own[p.b], s.own[p.b + 1], s.row_shared[p.b], a.seq[p.b * a.seq_stride],
                a.span);
     if (p.t0 < p.t1)
-      decode_segment<D, KV, Q_BF16, NT, false>(a, dsm, p.b, p.h, p.t0, p.t1, p.append, p.whole,
+      decode_segment<D, KV, Q_BF16, NT, false, true>(a, dsm, p.b, p.h, p.t0, p.t1, p.append, p.whole,
                                                ((int64_t)c + (int64_t)p.h * a.B + p.b) * a.G);
     if (p.next >= hi) return;
     if (++p.b == a.B) {

@@ -305,7 +305,9 @@ at::Tensor paged_causal_attn_decode_shared_cuda(const at::Tensor& q, const at::T
   auto whole = [&](const at::Tensor& t, const char* name) {
     TORCH_CHECK(t.dim() == 1 && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong), op, ": ", name,
                 " must be 1-D of int32/int64, got ", t.sizes(), " of ", t.scalar_type());
-    return on_device(t, q).to(at::kInt).contiguous();
+    const at::Tensor x = on_device(t, q);
+    // values that 32 bits do not hold are cut as all others are
+    return (x.scalar_type() == at::kLong ? x.clamp(-1, INT32_MAX).to(at::kInt) : x).contiguous();
   };
   TORCH_CHECK(q.is_cuda(), op, ": expected CUDA tensors, q is on ", q.device());
   c10::cuda::CUDAGuard guard(q.device());
