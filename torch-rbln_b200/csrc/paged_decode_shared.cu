@@ -83,6 +83,7 @@ struct SharedArgs {
   int own_ctas;        // of the own kernel on an SM
   float tile_us;       // time of a key tile of cost 1, and of an own position, on an SM
   float own_us;
+  float late_us;       // what the prefix kernel has to do besides its tiles
   Totals* totals;
   int* row_shared;     // [B] positions that are read through the group's table
   int4* row_parts;     // [B] the row's unit: its first key tile on KV head 0's line, the last one less that (-1: no
@@ -282,9 +283,9 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
   }
   // The SMs are divided so that both kernels end together: with m of N SMs,
   //   line / m + late = own / (N - m),
-  // `late` what the first has to do besides, all in microseconds.
+  // all in microseconds.
   const int total = all[1], line = total * a.Hkv;
-  const float N = (float)s.ctas, late = 4.f, p = line * s.tile_us, o = (float)all[0] * a.Hkv * s.own_us;
+  const float N = (float)s.ctas, late = s.late_us, p = line * s.tile_us, o = (float)all[0] * a.Hkv * s.own_us;
   const float half = 0.5f * (late * N - p - o);
   const int sms = min(s.ctas - 2, max(1, (int)((half + sqrtf(half * half + late * p * N)) / late + 0.5f)));
   // The line is below 2^30 long. A share of a wide tile at least: so every
@@ -1110,6 +1111,9 @@ int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t*
   // to 12 ns the largest case took 409, 385, 385, 366, 371, 379, 392 us, smaller ones the same within a tenth.
   x.tile_us = 0.58f;
   x.own_us = p->head_dim == 128 ? 0.0092f : 0.0073f;
+  // the merge is released sooner where the prefix kernel ends first: 2, 4, 6, 8, 10 us here gave 35.1, 33.4, 31.8, 32.2,
+  // 33.0 us for 64 sequences behind 4096 positions
+  x.late_us = p->head_dim == 128 ? 6.f : 4.f;
   x.totals = reinterpret_cast<Totals*>(ws + pl.totals);
   x.row_shared = reinterpret_cast<int*>(ws + pl.row_shared);
   x.row_parts = reinterpret_cast<int4*>(ws + pl.row_parts);
