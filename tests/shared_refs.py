@@ -83,10 +83,10 @@ def decode(x):
         p = torch.softmax(Q @ K.transpose(1, 2) * scale, dim=-1)
         e = (Q.abs() @ K.abs().transpose(1, 2) * abs(scale)).amax(-1, keepdim=True)
         o, size, T = p @ V, p @ V.abs(), len(at)
-        # A probability is rounded once to the inputs' type. Its exponential is off by under 2^-13 (a cubic, one pair
-        # in eight; the others by 2^-22), a score by under 2^-20 of e, which moves numerator and denominator. The
-        # product is summed in float32 sixteen keys at a time, each step off by a unit at most.
-        inner = size * (rounding + 2.0 ** -13 + 2 * e * 2.0 ** -20 + (T / 16 + 40) * 2.0 ** -23)
+        # A probability is rounded once to the inputs' type. Its exponential is off by under 2^-20 (the function 2^-22,
+        # and the parts' weights), a score by under 2^-20 of e, which moves numerator and denominator. The product is
+        # summed in float32 sixteen keys at a time, each step off by a unit at most.
+        inner = size * (rounding + 2.0 ** -20 + 2 * e * 2.0 ** -20 + (T / 16 + 40) * 2.0 ** -23)
         if q.dtype == torch.float16:  # below 2^-14 of the largest, half a subnormal step
             inner = inner + T * 2.0 ** -25 * V.abs().amax()
         out[b, :, :, 0] = o

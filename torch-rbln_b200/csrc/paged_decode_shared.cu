@@ -36,7 +36,8 @@ constexpr int kRows = 128;            // query rows a tile
 constexpr int kPanel = 128 * 128;     // bytes: 128 rows of 64 elements
 constexpr int kPrefixThreads = 384;   // softmax warpgroups 0-3 and 4-7, producers 8 and 10, MMA 9
 constexpr int kSegCost = 128;         // keys charged to the start of a sequence's own part
-constexpr int kMinOwn = kSegCost + 16;  // smallest share of a CTA of own positions (256: 16.3 us for four sequences, 14.4)
+// smallest share of a CTA of own positions (256: 16.3 us for four sequences behind 500, now 14.4)
+constexpr int kMinOwn = kSegCost + 16;
 constexpr int kSms = 148;
 // What a key tile costs a CTA with two row tiles and with one (whose two
 // warpgroups take the tiles in turn), and a unit's start.
@@ -685,33 +686,31 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           tmem_wait_st();
         }
         const float nmu = (m_run == neg_inf()) ? 0.f : -m_run;
-#pragma unroll
-        for (int e = 0; e < kKeys; e += 2) fma2(xv[e], xv[e + 1], mult, mult, nmu, nmu);
-        // one pair of exponentials in eight runs on the FMA pipe
-#pragma unroll
-        for (int e = 0; e < kKeys; e += 2) {
-          if ((e / 2) % 8 == 7) {
-            exp2_poly2(xv[e], xv[e + 1]);
-          } else {
-            xv[e] = exp2_approx(xv[e]);
-            xv[e + 1] = exp2_approx(xv[e + 1]);
-          }
-        }
+        // Exponents, sums and stores 32 keys at a time, so that the stores of
+        // one part overlap the exponentials of the next. All exponentials on
+        // the SFU: some of them on the FMA pipe, by a polynomial, measured no
+        // faster (every 4th pair 374 us for the largest case, every 8th and
+        // none 364; 430 with every 8th under the power cap, 422 with none).
         float sa0 = 0.f, sa1 = 0.f, sb0 = 0.f, sb1 = 0.f;
-#pragma unroll
-        for (int e = 0; e < kKeys; e += 4) {
-          add2(sa0, sa1, xv[e], xv[e + 1]);
-          add2(sb0, sb1, xv[e + 2], xv[e + 3]);
-        }
-        l_run += (sa0 + sa1) + (sb0 + sb1);
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) {
           uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) pk[e] = pack2<BF16>(xv[32 * c + 2 * e], xv[32 * c + 2 * e + 1]);
+          for (int e = 32 * c; e < 32 * c + 32; e += 2) {
+            fma2(xv[e], xv[e + 1], mult, mult, nmu, nmu);
+            xv[e] = exp2_approx(xv[e]);
+            xv[e + 1] = exp2_approx(xv[e + 1]);
+            if ((e / 2) & 1) {
+              add2(sb0, sb1, xv[e], xv[e + 1]);
+            } else {
+              add2(sa0, sa1, xv[e], xv[e + 1]);
+            }
+            pk[(e - 32 * c) / 2] = pack2<BF16>(xv[e], xv[e + 1]);
+          }
           tmem_st16(t_s(x) + lane_off + c * 16, pk);
         }
+        l_run += (sa0 + sa1) + (sb0 + sb1);
         tmem_wait_st();
        }
         // rows of V behind the shared positions may hold anything: zeros
@@ -979,7 +978,8 @@ int launch(const DecodeArgs& a, const SharedArgs& s, const Maps& m, cudaStream_t
   int rc = launch_after(shared_prefix_kernel<D, QB>, dim3(s.ctas), kPrefixThreads, PrefixSmem<D>::ALLOC, st, m.q,
                         m.k, m.v, a, s);
   if (rc == RBLN_OK)
-    rc = launch_after(shared_own_kernel<D, KV, QB, NT>, dim3(s.ctas * s.own_ctas), kThreads, segment_smem<D, NT>(), st, a, s);
+    rc = launch_after(shared_own_kernel<D, KV, QB, NT>, dim3(s.ctas * s.own_ctas), kThreads, segment_smem<D, NT>(), st,
+                      a, s);
   if (rc == RBLN_OK)
     rc = launch_after(shared_merge_kernel<D, QB>, dim3(a.Hkv, a.B, merge_head_split(a.Hkv, a.B, a.G)), kThreads, 0, st, a,
                       s);
@@ -1074,7 +1074,8 @@ int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t*
       if (p->k_new_stride[i] * 2 % 16 != 0 || p->v_new_stride[i] * 2 % 16 != 0) return RBLN_ERR_INVALID_ARGUMENT;
   }
   // rows are addressed as 32-bit counts of 16 bytes
-  const int64_t reach = ((int64_t)(p->num_blocks - 1) * p->cache_stride[0] + (int64_t)(p->num_kv_heads - 1) * p->cache_stride[1] +
+  const int64_t reach = ((int64_t)(p->num_blocks - 1) * p->cache_stride[0] +
+                         (int64_t)(p->num_kv_heads - 1) * p->cache_stride[1] +
                          (int64_t)(p->block_size - 1) * p->cache_stride[2] + p->head_dim) * 2;
   if (reach / 16 > (int64_t)UINT32_MAX) return RBLN_ERR_UNSUPPORTED;
   if (!p->workspace || p->workspace_bytes < pl.total) return RBLN_ERR_WORKSPACE;

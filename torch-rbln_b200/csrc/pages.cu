@@ -545,7 +545,8 @@ int check_table(const rbln_pages_params_t* p, bool lengths = true) {
 int check_caches(const rbln_pages_params_t* p) {
   if (p->num_layers < 1 || p->num_kv_heads < 1 || p->head_dim < 1 || !p->kcaches || !p->vcaches)
     return RBLN_ERR_INVALID_ARGUMENT;
-  const int size = p->kv_dtype == RBLN_DT_FP8_E4M3 ? 1 : p->kv_dtype == RBLN_DT_F16 || p->kv_dtype == RBLN_DT_BF16 ? 2 : 0;
+  const bool half = p->kv_dtype == RBLN_DT_F16 || p->kv_dtype == RBLN_DT_BF16;
+  const int size = p->kv_dtype == RBLN_DT_FP8_E4M3 ? 1 : half ? 2 : 0;
   if (size == 0) return RBLN_ERR_UNSUPPORTED;
   if ((p->k_scales == nullptr) != (p->v_scales == nullptr) || (size == 1) != (p->k_scales != nullptr))
     return RBLN_ERR_INVALID_ARGUMENT;
@@ -608,7 +609,9 @@ Workspace workspace_of(const rbln_pages_params_t* p, int64_t entries) {
 }
 
 // One CTA where a thread has few entries and pages, else a cluster of eight.
-int plan_ctas(int64_t entries, int64_t pages) { return entries <= kPlanThreads && pages <= 4 * kPlanThreads ? 1 : kPlanCtas; }
+int plan_ctas(int64_t entries, int64_t pages) {
+  return entries <= kPlanThreads && pages <= 4 * kPlanThreads ? 1 : kPlanCtas;
+}
 
 template <typename A>
 int launch_plan(void (*kernel)(A), int ctas, cudaStream_t st, const A& a) {
