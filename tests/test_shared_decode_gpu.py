@@ -151,6 +151,16 @@ def test_one_table_row_for_all():
     ref.check(x)
 
 
+def test_table_wider_than_the_lengths_need():
+    """The batch's spans add up to more positions than 31 bits hold; the lengths do not."""
+    x = ref.inputs(64, 16, BF, 2, 4, 40, [0, 40], [100], [1] * 40, poison=False)
+    wide = torch.full([1, 2 ** 22], -1, dtype=torch.int32)
+    wide[:, : x["block_table"].shape[1]] = x["block_table"][:1]
+    x["block_table"] = wide
+    x["k"], x["v"] = x["k"][:1].expand_as(x["k"]).clone(), x["v"][:1].expand_as(x["v"]).clone()
+    ref.check(x)
+
+
 def test_strided_inputs_and_heads_outermost_pools():
     x = ref.inputs(128, 16, BF, 3, 4, 18, [0, 18], [333], [1 + b for b in range(18)])
     y = ref.gpu(x)

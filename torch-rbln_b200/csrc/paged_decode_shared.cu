@@ -35,9 +35,10 @@ constexpr int kKeys = 128;            // keys a tile
 constexpr int kRows = 128;            // query rows a tile
 constexpr int kPanel = 128 * 128;     // bytes: 128 rows of 64 elements
 constexpr int kPrefixThreads = 384;   // softmax warpgroups 0-3 and 4-7, producers 8 and 10, MMA 9
-constexpr int kSegCost = 128;         // keys charged to the start of a sequence's own part
-// smallest share of a CTA of own positions (256: 16.3 us for four sequences behind 500, now 14.4)
-constexpr int kMinOwn = kSegCost + 16;
+// Own positions are counted in sixteens: what the start of a sequence's own
+// part is charged, and the smallest share of a CTA (16 of them: 16.3 us for
+// four sequences behind 500 positions, now 14.4).
+constexpr int kSegCost = 8, kMinOwn = kSegCost + 1;
 constexpr int kSms = 148;
 // What a key tile costs a CTA with two row tiles and with one (whose two
 // warpgroups take the tiles in turn), and a unit's start.
@@ -52,7 +53,7 @@ struct Totals {
   int cost;       // of all units of a KV head
   int share;      // of a CTA of the prefix kernel
   int rows;       // rows that a KV head's units store for each CTA that works on them
-  int own;        // own positions of a KV head, with what the sequences' starts are charged
+  int own;        // sixteens of own positions of a KV head, with what the sequences' starts are charged
   int own_share;  // of a CTA
 };
 
@@ -89,7 +90,7 @@ struct SharedArgs {
   int* row_shared;     // [B] positions that are read through the group's table
   int4* row_parts;     // [B] the row's unit: its first key tile on KV head 0's line, the last one less that (-1: no
                        // shared part), its stored row, the stored rows of x = 0 where tiles are taken in turn
-  int* own;            // [B + 1] prefix of the rows' own positions, as in the decode kernels
+  int* own;            // [B + 1] prefix of the rows' own positions in sixteens, their starts' charge included
   float* part_o;       // parts of the shared positions, see unit_at
   float* part_lse;
 };
@@ -142,9 +143,9 @@ __device__ __forceinline__ Unit unit_at(int lo, int hi, int cta, int h, int g, i
 }
 
 // The own positions of all KV heads and sequences, each sequence's rounded up
-// to 16 and its start charged kSegCost, stand on another line, cut likewise:
-// the segment at `lo` of a CTA that ends at `hi`, in sequence b, whose range
-// of a KV head's line is [from, to).
+// to sixteens and its start charged kSegCost, stand on another line, cut
+// likewise: the segment at `lo` of a CTA that ends at `hi`, in sequence b,
+// whose range of a KV head's line is [from, to).
 __device__ __forceinline__ OwnPart own_at(long long lo, long long hi, int h, int b, int all, int from, int to, int shared,
                                           int seq, int span) {
   const long long pb = (long long)h * all + from + kSegCost, pe = (long long)h * all + to;
@@ -154,8 +155,8 @@ __device__ __forceinline__ OwnPart own_at(long long lo, long long hi, int h, int
   p.b = b;
   p.next = seg_hi;
   const int L = seq < 0 ? 0 : min(seq + 1, span);
-  p.t0 = shared + (int)(seg_lo - pb);
-  p.t1 = seg_lo < seg_hi ? min(shared + (int)(seg_hi - pb), L) : p.t0;
+  p.t0 = shared + 16 * (int)(seg_lo - pb);
+  p.t1 = seg_lo < seg_hi ? min(shared + 16 * (int)(seg_hi - pb), L) : p.t0;
   p.append = seq < span && seq >= p.t0 && seq < p.t1;
   p.whole = seg_lo == pb && seg_hi == pe && shared == 0;
   return p;
@@ -246,7 +247,7 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
     if (g >= 0 && g < s.groups && seq >= P.len[g]) shared = P.len[g];
     if (shared > 0) P.stored[g] = 1;  // some row of the group has a shared part
     const int L = seq < 0 ? 0 : min(seq + 1, a.span);
-    own[b] = ((L - shared + 15) & ~15) + kSegCost;
+    own[b] = (L - shared + 15) / 16 + kSegCost;
     group[b] = (short)(shared > 0 ? g : -1);
   }
   __syncthreads();
@@ -286,7 +287,7 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
   //   line / m + late = own / (N - m),
   // all in microseconds.
   const int total = all[1], line = total * a.Hkv;
-  const float N = (float)s.ctas, late = s.late_us, p = line * s.tile_us, o = (float)all[0] * a.Hkv * s.own_us;
+  const float N = (float)s.ctas, late = s.late_us, p = line * s.tile_us, o = 16.f * (float)all[0] * a.Hkv * s.own_us;
   const float half = 0.5f * (late * N - p - o);
   const int sms = min(s.ctas - 2, max(1, (int)((half + sqrtf(half * half + late * p * N)) / late + 0.5f)));
   // The line is below 2^30 long. A share of a wide tile at least: so every
@@ -294,7 +295,7 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
   const int share = max(kWideCost, (line + sms - 1) / sms);
   const int own_ctas = (s.ctas - (line + share - 1) / share) * s.own_ctas;
   const long long own_line = (long long)all[0] * a.Hkv;
-  const int W = max(kMinOwn, (int)((own_line + own_ctas - 1) / own_ctas + 15) & ~15);
+  const int W = max(kMinOwn, (int)((own_line + own_ctas - 1) / own_ctas));
   if (tid == 0) {
     P.before[s.groups] = total;
     P.totals = Totals{total, share, all[2], all[0], W};
@@ -1007,7 +1008,8 @@ int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s
   if ((int64_t)p->max_blocks * p->block_size > (1 << 30)) return RBLN_ERR_UNSUPPORTED;
   const bool tiles = p->block_size % 128 == 0 || (p->block_size >= 8 && 128 % p->block_size == 0);
   if (!tiles) return RBLN_ERR_UNSUPPORTED;
-  if ((int64_t)p->batch * ((int64_t)p->max_blocks * p->block_size + 15 + kSegCost) >= (int64_t)1 << 30)
+  // a KV head's own positions are counted in 32 bits, in sixteens
+  if ((int64_t)p->batch * ((int64_t)p->max_blocks * p->block_size / 16 + 1 + kSegCost) >= (int64_t)1 << 30)
     return RBLN_ERR_UNSUPPORTED;
   // the units' line, with room for a CTA's share past its end, is counted in 32 bits
   const int64_t units = (int64_t)p->batch / (2 * (kRows / p->group)) + s->num_groups + 1;
