@@ -797,13 +797,14 @@ template <int D, int KV, bool Q_BF16, int NT>
 __device__ __forceinline__ void own_chunk(const DecodeArgs& a, const SharedArgs& s, unsigned char* dsm) {
   __shared__ int before[kWarps];
   const int c = blockIdx.x;
-  const int W = s.totals->own_share, all = s.totals->own;
+  // (the plan is read past L1: it was made while this grid could already be on its way)
+  const int W = __ldcg(&s.totals->own_share), all = __ldcg(&s.totals->own);
   const long long lo = (long long)c * W, hi = min(lo + W, (long long)all * a.Hkv);
   if (lo >= hi) return;
   // the sequence at `lo`: all threads count those that start at or before it
   const int h = (int)(lo / all), x = (int)(lo - (long long)h * all);
   int n = 0;
-  for (int i = threadIdx.x; i < a.B; i += kThreads) n += s.own[i] <= x;
+  for (int i = threadIdx.x; i < a.B; i += kThreads) n += __ldcg(s.own + i) <= x;
   n = __reduce_add_sync(0xffffffffu, n);
   if ((threadIdx.x & 31) == 0) before[threadIdx.x >> 5] = n;
   __syncthreads();
@@ -812,8 +813,8 @@ __device__ __forceinline__ void own_chunk(const DecodeArgs& a, const SharedArgs&
   p.b = before[0] + before[1] + before[2] + before[3] - 1;
   p.next = lo;
   while (true) {
-    p = own_at(p.next, hi, p.h, p.b, all, s.own[p.b], s.own[p.b + 1], s.row_shared[p.b], a.seq[p.b * a.seq_stride],
-               a.span);
+    p = own_at(p.next, hi, p.h, p.b, all, __ldcg(s.own + p.b), __ldcg(s.own + p.b + 1), __ldcg(s.row_shared + p.b),
+               a.seq[p.b * a.seq_stride], a.span);
     if (p.t0 < p.t1)
       decode_segment<D, KV, Q_BF16, NT, false, true>(a, dsm, p.b, p.h, p.t0, p.t1, p.append, p.whole,
                                                ((int64_t)c + (int64_t)p.h * a.B + p.b) * a.G);
@@ -858,9 +859,14 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const DecodeArgs
   const int gn = a.G / (int)gridDim.z, g0 = (int)blockIdx.z * gn;
   int pos;
   const int L = seq_len(a, b, pos);
-  const Totals tot = *s.totals;
-  const int4 rp = s.row_parts[b];
-  const int pb = s.own[b] + kSegCost, pe = s.own[b + 1];
+  Totals tot;
+  tot.cost = __ldcg(&s.totals->cost);
+  tot.share = __ldcg(&s.totals->share);
+  tot.rows = __ldcg(&s.totals->rows);
+  tot.own = __ldcg(&s.totals->own);
+  tot.own_share = __ldcg(&s.totals->own_share);
+  const int4 rp = __ldcg(s.row_parts + b);
+  const int pb = __ldcg(s.own + b) + kSegCost, pe = __ldcg(s.own + b + 1);
   const long long own0 = (long long)h * tot.own + pb;
   const int cf = (int)(own0 / tot.own_share), own = pe > pb ? (int)((own0 + pe - pb - 1) / tot.own_share) - cf + 1 : 0;
   const int64_t own_slot = ((int64_t)cf + (int64_t)h * a.B + b) * a.G;
