@@ -125,6 +125,20 @@ def test_nan_in_seen_places():
         ref.check(y)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shared", [1, 100, 129])
+@pytest.mark.parametrize("B", [1, 4])
+@pytest.mark.parametrize("G", [1, 4, 8])
+def test_nan_alone_in_a_part(D, shared, B, G):
+    """One of few parts holds nothing but NaN: that of the new token, or those of the shared positions."""
+    x = ref.inputs(D, 16, BF, 8, G, B, [0, B], [shared], [1] * B, poison=False)
+    y = {m: c.clone() if isinstance(c, torch.Tensor) else c for m, c in x.items()}
+    x["k"][B - 1] = float("nan")
+    ref.check(x, "new key")
+    y["kcache"][y["block_table"][0, : -(-shared // 16)].long(), 1] = float("nan")
+    ref.check(y, "shared keys")
+
+
 def test_groups_given_in_64_bits():
     x = ref.inputs(64, 16, BF, 1, 4, 6, [0, 6], [64], [16] * 6, poison=False)
     x["group_starts"], x["shared_lens"] = torch.tensor([-2 ** 40, 2 ** 40]), torch.tensor([2 ** 33])

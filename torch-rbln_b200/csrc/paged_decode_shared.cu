@@ -932,7 +932,7 @@ __global__ void __launch_bounds__(kThreads) shared_merge_kernel(const DecodeArgs
       acc = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int w = 0; w < ways; ++w) {
         const float2 ml = s_ml[slot + w];
-        if (ml.x == neg_inf()) continue;
+        if (ml.y == 0.f) continue;  // saw nothing (where all parts are NaN, S is, and the maximum is -inf too)
         const float f = exp2_approx(ml.x - top);
         const float4 o = s_acc[slot + w][d4 / 4];
         S += f * ml.y;
