@@ -309,3 +309,15 @@ def test_decode_negative_seq_sets_flag():
                block_table=d["block_table"][keep])
     ref = oracle(sub)
     check((got[0][keep], got[1], got[2]), ref)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "fp8", "masked", "one split a 64 tokens"])
+@pytest.mark.parametrize("G,D", [(4, 128), (1, 64), (12, 64)])
+def test_nan_alone_in_a_part(kind, G, D):
+    """The 129th token is a part of its own behind 128 others: where its key is NaN, so is every output."""
+    d = make_decode(1, 2, G, D, 16, [129], dtype=torch.float16 if kind == "f16" else torch.bfloat16, fp8=kind == "fp8")
+    d["k"][:, 1] = float("nan")
+    span = d["block_table"].shape[1] * 16
+    mask = (torch.arange(span) < 129).float().reshape(1, 1, 1, 1, span) if kind == "masked" else None
+    out = run_cabi(d, num_splits=span // 64)[0] if kind == "one split a 64 tokens" else run_op(d, mask)[0]
+    assert torch.isnan(out[:, 1]).all() and torch.isfinite(out[:, 0].float()).all()

@@ -191,9 +191,7 @@ __host__ __device__ constexpr int segment_smem() {
 // LA (block-table lookahead): false = look up each tile's block where it is
 // fetched; true = load the next tile's entry into registers one tile early,
 // so that the lookup is off the tile's critical path.
-// NAN_PART: a partial whose scores are all NaN keeps a NaN log-sum-exp, where
-// it would else read as one that saw nothing.
-template <int D, int KV, bool Q_BF16, int NT, bool LA, bool NAN_PART = false>
+template <int D, int KV, bool Q_BF16, int NT, bool LA>
 __device__ __forceinline__ void decode_segment(const DecodeArgs& a, unsigned char* dsm, int b, int h, int t0,
                                                int t1, bool append, bool whole, int64_t slot) {
   using C = Cfg<D, KV>;
@@ -515,8 +513,8 @@ __device__ __forceinline__ void decode_segment(const DecodeArgs& a, unsigned cha
       acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
       const int64_t ps = slot + g;
       *reinterpret_cast<float4*>(a.part_o + ps * D + d4) = acc;
-      if (d4 == 0)
-        a.part_lse[ps] = (M == neg_inf() && !(NAN_PART && Lsum != Lsum)) ? neg_inf() : M + __log2f(Lsum);
+      // -inf for a part that saw nothing; one whose scores are all NaN has no maximum either, and stays NaN
+      if (d4 == 0) a.part_lse[ps] = Lsum == 0.f ? neg_inf() : M + __log2f(Lsum);
     }
   }
   if (a.out_peers && final_out) __threadfence_system();  // peer stores before the epoch exchange

@@ -816,7 +816,7 @@ __device__ __forceinline__ void own_chunk(const DecodeArgs& a, const SharedArgs&
     p = own_at(p.next, hi, p.h, p.b, all, __ldcg(s.own + p.b), __ldcg(s.own + p.b + 1), __ldcg(s.row_shared + p.b),
                a.seq[p.b * a.seq_stride], a.span);
     if (p.t0 < p.t1)
-      decode_segment<D, KV, Q_BF16, NT, false, true>(a, dsm, p.b, p.h, p.t0, p.t1, p.append, p.whole,
+      decode_segment<D, KV, Q_BF16, NT, false>(a, dsm, p.b, p.h, p.t0, p.t1, p.append, p.whole,
                                                ((int64_t)c + (int64_t)p.h * a.B + p.b) * a.G);
     if (p.next >= hi) return;
     if (++p.b == a.B) {
