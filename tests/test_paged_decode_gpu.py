@@ -321,3 +321,14 @@ def test_nan_alone_in_a_part(kind, G, D):
     mask = (torch.arange(span) < 129).float().reshape(1, 1, 1, 1, span) if kind == "masked" else None
     out = run_cabi(d, num_splits=span // 64)[0] if kind == "one split a 64 tokens" else run_op(d, mask)[0]
     assert torch.isnan(out[:, 1]).all() and torch.isfinite(out[:, 0].float()).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("splits", [0, 3])
+def test_the_largest_position(fp8, splits):
+    """A position of 2^31 - 1 is past the span as any other: nothing is written and all positions are seen."""
+    d = make_decode(5, 2, 4, 128, 16, [900, 1, 300, 17, 640], fp8=fp8, seed=splits)
+    d["seq"][[0, 3]] = d["block_table"].shape[1] * 16
+    want = oracle(d)
+    d["seq"][[0, 3]] = 2 ** 31 - 1
+    check(run_cabi(d, num_splits=splits), want)

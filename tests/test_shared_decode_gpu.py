@@ -74,6 +74,19 @@ def test_shared_length_zero_negative_and_past_the_span():
         ref.check(x, f"{n} {seq}")
 
 
+@pytest.mark.parametrize("D,bs,dtype,Hkv,G", SHAPES[:3])
+def test_the_largest_position(D, bs, dtype, Hkv, G):
+    """A position of 2^31 - 1, past the span as any other: nothing is written, all positions are seen, and the rows
+    beside it are as they were."""
+    for starts, lens in (([0, 12], [300]), ([0], []), ([3, 8], [129])):
+        x = ref.inputs(D, bs, dtype, Hkv, G, 12, starts, lens, [1 + 17 * b for b in range(12)], poison=False)
+        x["seq"][[0, 4, 11]] = 2 ** 31 - 1
+        t = x["block_table"]
+        spare = next(p for p in range(len(x["kcache"])) if not (t == p).any())  # no row writes it
+        x["block_table"] = torch.where(t < 0, spare, t)
+        ref.check(x, str(starts))
+
+
 def test_starts_that_do_not_ascend():
     for starts in ([0, 6, 3, 9], [5, 5, 5, 2], [-4, 3, 100, 7], [9, 0, 0, 0]):
         x = ref.inputs(128, 16, BF, 1, 4, 9, [0, 3, 6, 9], [64, 64, 64], [20] * 9)

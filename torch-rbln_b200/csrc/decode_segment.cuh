@@ -6,6 +6,7 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "ranges.cuh"
 
 namespace rbln {
 namespace {
@@ -106,7 +107,7 @@ __device__ __forceinline__ void decode_extent(const DecodeArgs& a, int b, int& p
   if (a.mask) {
     L = min(a.span, a.mask_len);
   } else {
-    L = pos < 0 ? 0 : min(pos + 1, a.span);
+    L = positions_seen(pos, a.span);
   }
   nsplit = max(1, (L + a.chunk - 1) / a.chunk);
 }
@@ -524,7 +525,7 @@ __device__ __forceinline__ void decode_segment(const DecodeArgs& a, unsigned cha
 // Context length seen by sequence b (see decode_extent).
 __device__ __forceinline__ int seq_len(const DecodeArgs& a, int b, int& pos) {
   pos = a.seq[b * a.seq_stride];
-  return a.mask ? min(a.span, a.mask_len) : (pos < 0 ? 0 : min(pos + 1, a.span));
+  return a.mask ? min(a.span, a.mask_len) : positions_seen(pos, a.span);
 }
 
 // host side

@@ -158,7 +158,7 @@ __device__ __forceinline__ OwnPart own_at(long long lo, long long hi, int h, int
   p.h = h;
   p.b = b;
   p.next = seg_hi;
-  const int L = seq < 0 ? 0 : min(seq + 1, span);
+  const int L = positions_seen(seq, span);
   p.t0 = shared + 16 * (int)(seg_lo - pb);
   p.t1 = seg_lo < seg_hi ? min(shared + 16 * (int)(seg_hi - pb), L) : p.t0;
   p.append = seq < span && seq >= p.t0 && seq < p.t1;
@@ -250,7 +250,7 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
     int shared = 0;
     if (g >= 0 && g < s.groups && seq >= P.len[g]) shared = P.len[g];
     if (shared > 0) P.stored[g] = 1;  // some row of the group has a shared part
-    const int L = seq < 0 ? 0 : min(seq + 1, a.span);
+    const int L = positions_seen(seq, a.span);
     own[b] = (L - shared + 15) / 16 + kSegCost;
     group[b] = (short)(shared > 0 ? g : -1);
   }
