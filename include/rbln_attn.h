@@ -219,8 +219,8 @@ int rbln_paged_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stre
  * No reference counterpart. */
 typedef struct {
   int32_t num_groups;
-  const int32_t* group_starts; /* [num_groups + 1] */
-  const int32_t* shared_lens;  /* [num_groups] */
+  const int32_t* group_starts; /* [num_groups + 1]; not read where num_groups is 0, and may be NULL then */
+  const int32_t* shared_lens;  /* [num_groups], likewise */
 } rbln_shared_prefix_t;
 
 size_t rbln_shared_prefix_sizeof(void);

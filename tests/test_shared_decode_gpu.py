@@ -360,6 +360,25 @@ def test_schema_fake_and_trace():
                           tuple(x[n] for n in ref.ORDER))
 
 
+def test_no_groups_and_no_arrays_of_them():
+    """Through the C entry point, as it may be called without any group: the arrays are NULL."""
+    from torch_rbln_b200 import cabi
+
+    x = ref.inputs(128, 16, BF, 2, 4, 6, [0], [], [3, 40, 300, 1, 17, 130])
+    y = ref.gpu(x)
+    p, keep = cabi.paged_params(y["q"], y["k"], y["v"], y["kcache"], y["vcache"], y["seq"], y["block_table"], 16,
+                                float(x["scale"]))
+    s, n = cabi.SharedPrefix(0, None, None), ctypes.c_size_t(0)
+    assert cabi.lib().rbln_paged_decode_shared_workspace_size(ctypes.byref(p), ctypes.byref(s), ctypes.byref(n)) == 0
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
+    assert cabi.lib().rbln_paged_causal_attn_decode_shared(ctypes.byref(p), ctypes.byref(s),
+                                                           ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    want, bound = ref.decode(x)
+    ref.within(keep["out"], want, bound)
+    assert torch.equal(y["kcache"].cpu().view(torch.int16), x["kcache"].view(torch.int16))
+
+
 def test_error_flags():
     from torch_rbln_b200 import cabi
 

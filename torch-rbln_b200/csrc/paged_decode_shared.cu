@@ -232,7 +232,8 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
 #pragma unroll
   for (int k = 0; k < PG; ++k) {
     const int g = PG * tid + k;
-    if (g <= s.groups) top[0] = max(top[0], min(max(s.starts[g], 0), a.B));
+    // (without groups there need not be any starts: P.start[0] = 0 then)
+    if (s.groups > 0 && g <= s.groups) top[0] = max(top[0], min(max(s.starts[g], 0), a.B));
     cut[k] = top[0];
     if (g < s.groups) {
       P.len[g] = min(max(s.lens[g], 0), a.span);
