@@ -207,7 +207,10 @@ int rbln_paged_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stre
  * read once for the group, through the block table of its first sequence; the
  * rest of each sequence, its new token included, through its own. A sequence
  * whose new position is below its group's shared length, and one outside all
- * groups, is read through its own table alone. Values of group_starts are cut
+ * groups, is read through its own table alone. A new token below its group's
+ * shared length is written before any shared position is read. No other new
+ * token may go to a place that another sequence of the call reads, nor two
+ * different ones to one place. Values of group_starts are cut
  * to [0, batch] and to no less than the ones before them, shared lengths to
  * [0, span]. Of p: as for rbln_paged_causal_attn_decode, with kv_dtype equal to
  * q_dtype, no mask, sinks, num_splits or prof_events; block_size in {8, 16, 32,

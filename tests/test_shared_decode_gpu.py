@@ -74,6 +74,19 @@ def test_shared_length_zero_negative_and_past_the_span():
         ref.check(x, f"{n} {seq}")
 
 
+@pytest.mark.parametrize("D,bs,shared,B", [(64, 16, 200, 6), (128, 16, 700, 40), (128, 128, 6000, 70), (64, 8, 3000, 300)])
+def test_new_positions_in_shared_pages(D, bs, shared, B):
+    """New tokens that go to pages of the group's shared positions, the first sequence's own among them: all of its
+    sequences see them, and so do those of a second group over the same pages."""
+    for again in range(4):
+        n = B - B // 4
+        x = ref.inputs(D, bs, BF, 3, 4, B, [0, n, B], [shared, shared], [1 + b % 30 for b in range(B)], poison=False)
+        whole = shared // bs
+        x["block_table"][n:, :whole] = x["block_table"][0, :whole]
+        x["seq"][0], x["seq"][2], x["seq"][n] = 50 + again, 16, whole * bs - 1
+        ref.check(x, str(again))
+
+
 @pytest.mark.parametrize("D,bs,dtype,Hkv,G", SHAPES[:3])
 def test_the_largest_position(D, bs, dtype, Hkv, G):
     """A position of 2^31 - 1, past the span as any other: nothing is written, all positions are seen, and the rows

@@ -214,16 +214,20 @@ struct PlanSmem {
   int start[kMaxGroups + 1], before[kMaxGroups + 1];  // first sequence; cost of the groups before it, in one KV head
   int len[kMaxGroups], stored[kMaxGroups];            // shared positions; rows that the groups before it store
   Totals totals;
+  int below;  // whether group[b] is kBelow for any row
   Unit first, at[kPrefixThreads / 32];  // of this CTA; where each warp is
   __device__ __forceinline__ int4 group(int g) const {
     return make_int4(start[g], len[g] > 0 ? start[g + 1] - start[g] : 0, len[g], stored[g]);
   }
 };
 
+constexpr short kBelow = -2;
+
 // The plan, made by every CTA of the prefix kernel for itself: that takes less
 // time than a launch of its own. What the other kernels read is stored by all
 // of them, a row by one; it is not read in this grid, whose CTAs do not wait
-// for one another. own, group: scratch for all rows.
+// for one another. own, group: scratch for all rows; group[b] is kBelow for a
+// row whose new position lies below its group's shared length.
 __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs& s, PlanSmem& P, int* own, short* group) {
   constexpr int T = kPrefixThreads, PG = (kMaxGroups + T) / T;  // starts a thread
   const int tid = threadIdx.x, cta = blockIdx.x;
@@ -240,6 +244,7 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
       P.stored[g] = 0;
     }
   }
+  if (tid == 0) P.below = 0;
   scan_before<T, true>(top, most);
 #pragma unroll
   for (int k = 0; k < PG; ++k)
@@ -248,12 +253,13 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
   // rows: group, shared positions, own positions
   for (int b = tid; b < a.B; b += T) {
     const int seq = a.seq[b * a.seq_stride], g = last_at_most(P.start, -1, s.groups, b);
-    int shared = 0;
-    if (g >= 0 && g < s.groups && seq >= P.len[g]) shared = P.len[g];
+    const int len = g >= 0 && g < s.groups ? P.len[g] : 0, shared = seq >= len ? len : 0;
+    const bool early = seq >= 0 && seq < len;
+    if (early) P.below = 1;
     if (shared > 0) P.stored[g] = 1;  // some row of the group has a shared part
     const int L = positions_seen(seq, a.span);
     own[b] = (L - shared + 15) / 16 + kSegCost;
-    group[b] = (short)(shared > 0 ? g : -1);
+    group[b] = (short)(shared > 0 ? g : early ? kBelow : -1);
   }
   __syncthreads();
   // own positions before this thread's rows; cost and stored rows of the groups before this thread's
@@ -336,6 +342,37 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
     }
     P.first = u;
   }
+}
+
+// The new tokens of rows that lie below their group's shared length: they may
+// go to a page that the group's shared positions are read from (its first
+// row's own, above all), so every CTA writes them, for the KV heads that it
+// reads, before its first copy. The others write the same bytes, at any time,
+// as the own kernel does, which reports pages outside the pool. Kept small:
+// the code alone, which hardly any call runs, costs 0.2 us of a call (two
+// nested loops around append_token 0.3 to 2).
+template <int D>
+__device__ __forceinline__ void append_below(const DecodeArgs& a, const PlanSmem& P, const short* group) {
+  const int total = P.totals.cost, lo = (int)blockIdx.x * P.totals.share, hi = min(lo + P.totals.share, total * a.Hkv);
+  if (lo < hi && a.k_new != nullptr) {
+    const int h0 = lo / total, pieces = ((hi - 1) / total - h0 + 1) * (D / 8);
+    const bool key = threadIdx.x % 2 == 0;
+#pragma unroll 1
+    for (int b = 0; b < a.B; ++b) {
+      if (group[b] != kBelow) continue;
+      const int pos = a.seq[b * a.seq_stride], bi = pos / a.bs;
+      const int64_t blk = load_index(a.bt, a.bt_dtype, b * a.bt_stride + bi);
+      if (blk < 0 || blk >= a.num_blocks) continue;
+#pragma unroll 1
+      for (int i = threadIdx.x / 2; i < pieces; i += kPrefixThreads / 2) {
+        const int h = h0 + i / (D / 8), d = i % (D / 8) * 8;
+        const int64_t at = blk * a.cs_block + h * a.cs_head + (pos - bi * a.bs) * a.cs_tok + d;
+        const char* from = (key ? a.k_new + b * a.kn_b + h * a.kn_h : a.v_new + b * a.vn_b + h * a.vn_h) + d * 2;
+        *reinterpret_cast<uint4*>((key ? a.kcache : a.vcache) + at * 2) = *reinterpret_cast<const uint4*>(from);
+      }
+    }
+  }
+  fence_proxy_async_global();
 }
 
 // ----------------------------------------------------------------- prefix
@@ -451,7 +488,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   // and not the rest of this grid.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   PlanSmem& P = *reinterpret_cast<PlanSmem*>(sgen + L::PLAN);
-  make_plan(a, s, P, reinterpret_cast<int*>(sgen + L::Q), reinterpret_cast<short*>(sgen + L::Q + kMaxBatch * 4));
+  short* group = reinterpret_cast<short*>(sgen + L::Q + kMaxBatch * 4);
+  make_plan(a, s, P, reinterpret_cast<int*>(sgen + L::Q), group);
+  if (P.below) append_below<D>(a, P, group);
   __threadfence();
   fence_proxy_async_smem();  // the scratch is written by copies next
   __syncthreads();
