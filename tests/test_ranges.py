@@ -30,3 +30,11 @@ def test_positions_seen(tmp_path):
              for p in (-MOST - 1, -1, 0, 1, 62, 63, 64, 65, 2 ** 30 - 1, 2 ** 30, MOST - 1, MOST)]
     got = values(tmp_path, [f"rbln::positions_seen({'-2147483647 - 1' if p == -MOST - 1 else p}, {s})" for p, s in cases])
     assert got == [0 if p < 0 else min(p + 1, s) for p, s in cases]
+
+
+def test_share_start(tmp_path):
+    lines = [(4, 0), (4, 1), (4, 590), (9, 1000), (7_300_000, 2 ** 30 - 1), (14_700_000, 14_700_000), (2 ** 29, 2 ** 30 - 1),
+             (2 ** 30 - 1, 2 ** 30 - 1)]
+    cases = [(c, share, line) for share, line in lines for c in (0, 1, 2, 100, 146, 147, 148)]
+    got = values(tmp_path, [f"rbln::share_start({c}, {share}, {line})" for c, share, line in cases])
+    assert got == [min(c * share, line) for c, share, line in cases]

@@ -333,7 +333,7 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
     s.row_parts[b] = parts;
   }
   if (tid == T - 1) {
-    const int lo = cta * share, hi = min(lo + share, line);
+    const int lo = share_start(cta, share, line), hi = share_start(cta + 1, share, line);
     Unit u{};
     u.next = hi;
     if (lo < hi) {
@@ -353,7 +353,8 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
 // nested loops around append_token 0.3 to 2).
 template <int D>
 __device__ __forceinline__ void append_below(const DecodeArgs& a, const PlanSmem& P, const short* group) {
-  const int total = P.totals.cost, lo = (int)blockIdx.x * P.totals.share, hi = min(lo + P.totals.share, total * a.Hkv);
+  const int total = P.totals.cost, share = P.totals.share, line = total * a.Hkv;
+  const int lo = share_start(blockIdx.x, share, line), hi = share_start(blockIdx.x + 1, share, line);
   if (lo < hi && a.k_new != nullptr) {
     const int h0 = lo / total, pieces = ((hi - 1) / total - h0 + 1) * (D / 8);
     const bool key = threadIdx.x % 2 == 0;
@@ -385,7 +386,7 @@ __device__ __forceinline__ bool next_unit(const PlanSmem& P, const SharedArgs& s
     u = P.first;
     if (u.t0 < u.t1) return true;
   }
-  const int cost = P.totals.cost, hi = min(((int)blockIdx.x + 1) * P.totals.share, cost * a.Hkv);
+  const int cost = P.totals.cost, hi = share_start(blockIdx.x + 1, P.totals.share, cost * a.Hkv);
   while (u.next < hi) {
     const int lo = u.next, h = lo / cost, x = lo - h * cost;
     int g = u.group;
@@ -1070,7 +1071,8 @@ int plan_shared(const rbln_paged_attn_params_t* p, const rbln_shared_prefix_t* s
   // a KV head's own positions are counted in 32 bits, in sixteens
   if ((int64_t)p->batch * ((int64_t)p->max_blocks * p->block_size / 16 + 1 + kSegCost) >= (int64_t)1 << 30)
     return RBLN_ERR_UNSUPPORTED;
-  // the units' line, with room for a CTA's share past its end, is counted in 32 bits
+  // the units' line, and a place up to a share past its end, are counted in 32 bits; the bound also keeps a share of
+  // the own positions' line below 2^31
   const int64_t units = (int64_t)p->batch / (2 * (kRows / p->group)) + s->num_groups + 1;
   if (p->num_kv_heads * units * (kWideCost * tiles_of(p->max_blocks * p->block_size) + kUnitCost) >= (int64_t)1 << 30)
     return RBLN_ERR_UNSUPPORTED;
