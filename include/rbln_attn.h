@@ -316,7 +316,7 @@ typedef struct {
   const void* lengths;       /* [batch]: see each call */
   int32_t lengths_dtype;     /* I16, I32 or I64 */
   int64_t lengths_stride;
-  /* reserve and compact: host arrays [num_layers] of device pointers */
+  /* reserve and compact: host arrays [num_layers] of device pointers; a page of one KV head is below 32 GiB */
   int32_t num_layers, num_kv_heads, head_dim;
   int32_t kv_dtype;          /* F16, BF16 or FP8_E4M3 */
   void* const* kcaches;      /* each [num_blocks, num_kv_heads, block_size, head_dim] */

@@ -76,6 +76,18 @@ def test_caches_are_refused(changes, rc):
     assert cabi.lib().rbln_paged_kv_compact(ctypes.byref(p), 1, 1, None) == rc
 
 
+@pytest.mark.parametrize("head_dim,block_size,rc", [(128, 2 ** 27, -2), (64, 2 ** 28 - 1, -2), (128, 2 ** 27 - 17, -3),
+                                                    (64, 2 ** 27, -3)])
+def test_pages_whose_rows_pass_31_bits_are_refused(head_dim, block_size, rc):
+    """A page is copied in 16-byte pieces, counted in 32 bits by lanes that step 256 at a time; -3: only the workspace is
+    missing."""
+    from torch_rbln_b200 import cabi
+
+    p, keep = params(head_dim=head_dim, block_size=block_size, max_blocks=2)
+    assert reserve(p) == rc
+    assert cabi.lib().rbln_paged_kv_compact(ctypes.byref(p), 1, 1, None) == rc
+
+
 def test_other_refusals():
     from torch_rbln_b200 import cabi
 

@@ -551,6 +551,8 @@ int check_caches(const rbln_pages_params_t* p) {
   if ((p->k_scales == nullptr) != (p->v_scales == nullptr) || (size == 1) != (p->k_scales != nullptr))
     return RBLN_ERR_INVALID_ARGUMENT;
   if (p->head_dim * size % 16 != 0) return RBLN_ERR_INVALID_ARGUMENT;
+  // a page's rows are counted in 16-byte pieces, in 32 bits, with room for a step of the copy past their end
+  if (p->block_size * ((int64_t)p->head_dim * size / 16) > INT32_MAX - 32 * kCopyLoads) return RBLN_ERR_UNSUPPORTED;
   for (int i = 0; i < 3; ++i)
     if (p->cache_stride[i] * size % 16 != 0) return RBLN_ERR_INVALID_ARGUMENT;
   if (p->num_blocks == 0) return RBLN_OK;
