@@ -180,6 +180,35 @@ def test_reserve_large(ops):
                 index=torch.int16)
 
 
+@pytest.mark.parametrize("B,new", [(7, 3), (600, 25)])
+@pytest.mark.parametrize("order", ["heads outermost", "every second"])
+def test_scales_of_other_strides(ops, B, new, order):
+    """Scales that are not contiguous [blocks, heads], through both reservations and a compaction; what lies between
+    them is left alone."""
+    bs, width = 8, 14
+    lengths = torch.randint(0, 80, [B]).tolist()
+    table, refs = ref.pool(B, width, lengths, bs, 8 * B)
+    rows, seq = ref.fork(table, lengths, torch.randint(0, B, [B]).tolist(), refs, bs)
+    ref.free(table, [0] * B, refs, bs)
+    n = len(refs)
+    k, v = (ref.caches(2, n, 2, bs, 64, FP8) for _ in range(2))
+    shape, view = ([2, n], torch.t) if order == "heads outermost" else ([n, 4], lambda c: c[:, ::2])
+    cells = [torch.rand(shape) for _ in range(4)]
+    on_gpu = [c.cuda() for c in cells]
+    scales, got = [view(c) for c in cells], [view(c) for c in on_gpu]
+    gk, gv, t, r = to_gpu(k), to_gpu(v), table_of(rows, width), dev(refs)
+    granted = ops.paged_kv_reserve(gk, gv, t, dev(seq), r, bs, new, got[:2], got[2:])
+    want, moves = ref.reserve(rows, seq, refs, bs, new)
+    ref.copy(k + v, scales, moves)
+    assert moves and granted.cpu().tolist() == want and t.cpu().tolist() == rows and r.cpu().tolist() == refs
+    same_caches(gk + gv + on_gpu, k + v + cells)
+    ops.paged_kv_compact(gk, gv, t, r, got[:2], got[2:])
+    _, _, pairs = ref.compact(rows, refs)
+    ref.copy(k + v, scales, [(p, h, bs) for p, h in pairs])
+    assert pairs and t.cpu().tolist() == rows and r.cpu().tolist() == refs
+    same_caches(gk + gv + on_gpu, k + v + cells)
+
+
 def test_reserve_same_page_twice_in_a_row(ops):
     bs = 16
     table, refs = [[2, 2, 2], [2, 5, 2]], [0, 0, 5, 0, 0, 1, 0, 0, 0, 0]
