@@ -610,11 +610,6 @@ Workspace workspace_of(const rbln_pages_params_t* p, int64_t entries) {
   return w;
 }
 
-// One CTA where a thread has few entries and pages, else a cluster of eight.
-int plan_ctas(int64_t entries, int64_t pages) {
-  return entries <= kPlanThreads && pages <= 4 * kPlanThreads ? 1 : kPlanCtas;
-}
-
 template <typename A>
 int launch_plan(void (*kernel)(A), int ctas, cudaStream_t st, const A& a) {
   cudaLaunchConfig_t cfg = {};
@@ -764,7 +759,7 @@ int rbln_paged_kv_reserve(const rbln_pages_params_t* p, int32_t new_tokens, int3
     paged_kv_reserve_small_kernel<<<1, kPlanThreads, 0, stream>>>(a);
     rc = launched();
   } else {
-    rc = launch_plan(paged_kv_reserve_kernel, plan_ctas(std::max<int64_t>(entries, p->batch), p->num_blocks), stream, a);
+    rc = launch_plan(paged_kv_reserve_kernel, kPlanCtas, stream, a);
   }
   if (rc != RBLN_OK || entries == 0) return rc;
   return launch_copies(p, a.moves, a.count, p->batch, nullptr, stream);
@@ -789,7 +784,8 @@ int rbln_paged_kv_compact(const rbln_pages_params_t* p, int32_t* moved, int32_t*
   a.src = reinterpret_cast<int*>(ws + w.here);
   a.dst = reinterpret_cast<int*>(ws + w.last);
   a.moves = reinterpret_cast<Move*>(ws + w.moves);
-  rc = launch_plan(paged_kv_compact_kernel, plan_ctas(0, p->num_blocks), stream, a);
+  // one CTA where a thread has few pages, else a cluster of eight
+  rc = launch_plan(paged_kv_compact_kernel, p->num_blocks <= 4 * kPlanThreads ? 1 : kPlanCtas, stream, a);
   if (rc != RBLN_OK || p->num_blocks == 0) return rc;
   return launch_copies(p, a.moves, a.count, p->num_blocks / 2, moved, stream);
 }
