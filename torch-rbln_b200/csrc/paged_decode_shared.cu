@@ -356,17 +356,18 @@ __device__ __forceinline__ void append_below(const DecodeArgs& a, const PlanSmem
   const int total = P.totals.cost, share = P.totals.share, line = total * a.Hkv;
   const int lo = share_start(blockIdx.x, share, line), hi = share_start(blockIdx.x + 1, share, line);
   if (lo < hi && a.k_new != nullptr) {
-    const int h0 = lo / total, pieces = ((hi - 1) / total - h0 + 1) * (D / 8);
-    const bool key = threadIdx.x % 2 == 0;
+    // a warp a row; of a KV head's D / 4 pieces, K's half comes first
+    const int h0 = lo / total, pieces = ((hi - 1) / total - h0 + 1) * (D / 4);
 #pragma unroll 1
-    for (int b = 0; b < a.B; ++b) {
+    for (int b = threadIdx.x / 32; b < a.B; b += kPrefixThreads / 32) {
       if (group[b] != kBelow) continue;
       const int pos = a.seq[b * a.seq_stride], bi = pos / a.bs;
       const int64_t blk = load_index(a.bt, a.bt_dtype, b * a.bt_stride + bi);
       if (blk < 0 || blk >= a.num_blocks) continue;
 #pragma unroll 1
-      for (int i = threadIdx.x / 2; i < pieces; i += kPrefixThreads / 2) {
-        const int h = h0 + i / (D / 8), d = i % (D / 8) * 8;
+      for (int i = threadIdx.x % 32; i < pieces; i += 32) {
+        const int h = h0 + i / (D / 4), d = i % (D / 8) * 8;
+        const bool key = i % (D / 4) < D / 8;
         const int64_t at = blk * a.cs_block + h * a.cs_head + (pos - bi * a.bs) * a.cs_tok + d;
         const char* from = (key ? a.k_new + b * a.kn_b + h * a.kn_h : a.v_new + b * a.vn_b + h * a.vn_h) + d * 2;
         *reinterpret_cast<uint4*>((key ? a.kcache : a.vcache) + at * 2) = *reinterpret_cast<const uint4*>(from);
