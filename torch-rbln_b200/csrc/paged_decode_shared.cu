@@ -16,12 +16,18 @@
 //    bring one by one, and a key is read once for them;
 //  * shared_own_kernel, beside it on the other SMs: each sequence's own
 //    positions with the decode kernels' segments (mma.sync, one sequence and
-//    KV head at a time), and the append of the new token;
+//    KV head at a time), and the append of the new token (of one below the
+//    shared length after the first kernel has written it, see append_below);
 //  * shared_merge_kernel: the parts of every row.
 // GPU time, heads of 128, pages of 16, bf16: 4 sequences x 4 query heads x 8
 // KV heads behind 500 positions 14 us; 64 behind 4096, with 264 of their own
 // on average, 32; 256 x 8 query heads behind 32768, with 512 of their own,
-// 364 (a kernel that reads the prefix once for each sequence: 19, 148, 3980).
+// 365. paged_causal_attn_decode, which reads the prefix once for each sequence,
+// is the faster op behind short prefixes: with 8 KV heads of 4 query heads and
+// 64 own positions on average, 4 sequences behind 512 positions 13.8 us here
+// and 13.0 there, behind 8192 21.8 and 24.9; 64 behind 128 18.8 and 17.6,
+// behind 512 20.2 and 27.9, behind 8192 34.9 and 226; 256 behind 128 68 and 46,
+// behind 512 55 and 86.
 
 #include <algorithm>
 
@@ -738,6 +744,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           tmem_wait_st();
         }
         const float nmu = (m_run == neg_inf()) ? 0.f : -m_run;
+        // A probability is rounded once to the inputs' type, as the product's
+        // operands have to be of one type; its sum is of the unrounded ones.
         // Exponents, sums and stores 32 keys at a time, so that the stores of
         // one part overlap the exponentials of the next. All exponentials on
         // the SFU: some of them on the FMA pipe, by a polynomial, measured no
@@ -1173,7 +1181,9 @@ int run_shared(const rbln_paged_attn_params_t* p_in, const rbln_shared_prefix_t*
   x.ctas = kSms;
   x.own_ctas = pl.own_ctas;
   // Measured with both kernels at work: a wide tile 2.3 us, an own position (of up to four CTAs) 9 and 7 ns. From 7.8
-  // to 12 ns the largest case took 409, 385, 385, 366, 371, 379, 392 us, smaller ones the same within a tenth.
+  // to 12 ns the largest case took 409, 385, 385, 366, 371, 379, 392 us, smaller ones the same within a tenth. All of
+  // it with up to 8 query heads a KV head: with more, two CTAs of the own kernel share an SM, for which none of these
+  // times was measured.
   x.tile_us = 0.58f;
   x.own_us = p->head_dim == 128 ? 0.0092f : 0.0073f;
   // the merge is released sooner where the prefix kernel ends first: 2, 4, 6, 8, 10 us here gave 35.1, 33.4, 31.8, 32.2,

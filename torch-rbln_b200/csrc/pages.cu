@@ -11,9 +11,12 @@
 // The tables and counts are small, so those kernels are bound by the latency
 // of their dependent look-ups: free, fork, reserve and the copies of 64 forks
 // of 16 prompts through 24 layers take 14 us of GPU time, for 256 forks of one
-// prompt of 2048 pages 17. What is copied is bound by HBM: 980 pages of 16
-// layers, 2.05 GB read and written, 336 us with the ranking before it, 93 %
-// of the copy rate.
+// prompt of 2048 pages 18. A reservation alone takes 6 us for 128 entries among
+// 4096 pages and 42 among 65536, all of which one CTA searches for free ones;
+// the cluster that takes larger calls 18 among 65537, 22 for 2048 entries among
+// 20000 and 53 for 12000 among 400000. What is copied is bound by HBM: 980
+// pages of 16 layers, 2.05 GB read and written, 336 us with the ranking before
+// it, 93 % of the copy rate.
 
 #include <algorithm>
 
