@@ -208,15 +208,15 @@ int rbln_paged_attn_prefill(const rbln_paged_attn_params_t* p, cudaStream_t stre
  * rest of each sequence, its new token included, through its own. A sequence
  * whose new position is below its group's shared length, and one outside all
  * groups, is read through its own table alone. A new token below its group's
- * shared length is written before any shared position is read. No other new
- * token may go to a place that another sequence of the call reads, nor two
- * different ones to one place. Values of group_starts are cut
- * to [0, batch] and to no less than the ones before them, shared lengths to
- * [0, span]. Of p: as for rbln_paged_causal_attn_decode, with kv_dtype equal to
- * q_dtype, no mask, sinks, num_splits or prof_events; block_size in {8, 16, 32,
- * 64, 128} or a multiple of 128; group <= 16; batch <= 4096, num_groups <= 1024;
- * batch x span below 2^34 and, with U = batch group / 256 + num_groups,
- * num_kv_heads x U x span below 2^35 or so (RBLN_ERR_UNSUPPORTED past these).
+ * shared length is written before anything is read. No other new token may go
+ * to a place that another sequence of the call reads, nor two different ones
+ * to one place. Values of group_starts are cut to [0, batch] and to no less
+ * than the ones before them, shared lengths to [0, span]. Of p: as for
+ * rbln_paged_causal_attn_decode, with kv_dtype equal to q_dtype, no mask, sinks,
+ * num_splits or prof_events; block_size in {8, 16, 32, 64, 128} or a multiple of
+ * 128; group <= 16; batch <= 4096, num_groups <= 1024; batch x span below
+ * 2^34 and, with U = batch group / 256 + num_groups, num_kv_heads x U x span
+ * below 2^35 or so (RBLN_ERR_UNSUPPORTED past these).
  * A position in a block outside the pool is not seen. The workspace
  * (rbln_paged_decode_shared_workspace_size) is required.
  * No reference counterpart. */

@@ -87,6 +87,17 @@ def test_new_positions_in_shared_pages(D, bs, shared, B):
         ref.check(x, str(again))
 
 
+@pytest.mark.parametrize("Hkv", [1, 5, 150])
+def test_all_new_positions_in_shared_pages(Hkv):
+    """Every sequence of a group below its shared length, over the same pages: each sees the new tokens of those before
+    it, and none is read through another's table."""
+    B, n = (60, 700) if Hkv < 100 else (9, 90)
+    x = ref.inputs(64, 16, BF, Hkv, 2, B, [0, B], [n], [4] * B, poison=False)
+    x["block_table"][:] = x["block_table"][0]
+    x["seq"][:] = torch.randperm(n)[:B]
+    ref.check(x)
+
+
 @pytest.mark.parametrize("D,bs,dtype,Hkv,G", SHAPES[:3])
 def test_the_largest_position(D, bs, dtype, Hkv, G):
     """A position of 2^31 - 1, past the span as any other: nothing is written, all positions are seen, and the rows

@@ -354,16 +354,21 @@ __device__ __forceinline__ void make_plan(const DecodeArgs& a, const SharedArgs&
 // go to a page that the group's shared positions are read from (its first
 // row's own, above all), so every CTA writes them, for the KV heads that it
 // reads, before its first copy. The others write the same bytes, at any time,
-// as the own kernel does, which reports pages outside the pool. Kept small:
+// as the own kernel does, which reports pages outside the pool. Where no row
+// has a shared part, the CTAs divide the heads: the own kernel, which starts
+// behind this, reads those tokens through any row's table. Kept small:
 // the code alone, which hardly any call runs, costs 0.2 us of a call (two
 // nested loops around append_token 0.3 to 2).
 template <int D>
 __device__ __forceinline__ void append_below(const DecodeArgs& a, const PlanSmem& P, const short* group) {
   const int total = P.totals.cost, share = P.totals.share, line = total * a.Hkv;
   const int lo = share_start(blockIdx.x, share, line), hi = share_start(blockIdx.x + 1, share, line);
-  if (lo < hi && a.k_new != nullptr) {
+  const int ctas = gridDim.x, cta = blockIdx.x;
+  const int h0 = line > 0 ? lo / total : cta * a.Hkv / ctas;
+  const int h1 = line > 0 ? (lo < hi ? (hi - 1) / total + 1 : h0) : (cta + 1) * a.Hkv / ctas;
+  if (h0 < h1 && a.k_new != nullptr) {
     // a warp a row; of a KV head's D / 4 pieces, K's half comes first
-    const int h0 = lo / total, pieces = ((hi - 1) / total - h0 + 1) * (D / 4);
+    const int pieces = (h1 - h0) * (D / 4);
 #pragma unroll 1
     for (int b = threadIdx.x / 32; b < a.B; b += kPrefixThreads / 32) {
       if (group[b] != kBelow) continue;
